@@ -1,0 +1,93 @@
+// 8-bit integer activations and weights (W8A8): what the launches share.
+//
+// A row v of activations becomes codes and a scale,
+//
+//   m = max(max|v|, 2^-40),   s = m / 127,   q = rint(127 v / m)  (ties to even),
+//
+// and the product with weights that were quantised per output channel is out[i][n] = (sum_k q[i][k] w[n][k]) s[i] w_scale[n].
+// The sums are 32-bit integers: exact, and the same in any order, for K < 2^17.  A row that holds an infinity or a NaN has the scale NaN.
+#pragma once
+#include "qlinear_common.hpp"
+
+namespace qlin {
+
+typedef __attribute__((ext_vector_type(4))) float f32v4;
+
+constexpr int kInt8MaxK = (1 << 17) - 16;             // |sum| <= 2^14 K < 2^31
+constexpr float kInt8Floor = 0x1p-40f;
+
+__device__ __forceinline__ uint32_t umax32(uint32_t a, uint32_t b) { return a > b ? a : b; }
+// |v| as an ordered integer: NaN above infinity above every number
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
+  return umax32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+  v = dpp_umax<0xB1>(v);
+  v = dpp_umax<0x4E>(v);
+  v = dpp_umax<0x141>(v);
+  v = dpp_umax<0x140>(v);
+  uint32_t r = (uint32_t)__builtin_amdgcn_readlane((int)v, 0);
+  r = umax32(r, (uint32_t)__builtin_amdgcn_readlane((int)v, 16));
+  r = umax32(r, (uint32_t)__builtin_amdgcn_readlane((int)v, 32));
+  return umax32(r, (uint32_t)__builtin_amdgcn_readlane((int)v, 48));
+}
+
+// What a row's largest |v| gives: the factor that makes codes (0 where the row has none) and the scale.
+struct RowScale {
+  float inv, scale;
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t largest) {
+  if (largest >= 0x7F800000u) return {0.0f, __builtin_nanf("")};
+  const float m = fmaxf(__builtin_bit_cast(float, largest), kInt8Floor);
+  return {127.0f / m, m / 127.0f};
+}
+
+// The code of v.  EXACT, for a v and an m of 11 significant bits: v inv is off by less than 2^-22 of itself, a quotient that is no tie is at
+// least 2^-19 of itself away from one (2 * 127 v - (2 n + 1) m is a multiple of v's last place), so the quotient rounded to 21 bits
+// is on the right side of every tie or on it.
+template <bool EXACT>
+__device__ __forceinline__ int code_of(float v, float inv) {
+#pragma clang fp contract(off)
+  float t = v * inv;
+  if constexpr (EXACT) {
+    const float c = t * 9.0f;
+    const float d = c - t;
+    t = c - d;
+  }
+  t = inv == 0.0f ? 0.0f : t;                          // the row of an infinity or a NaN
+  return (int)__builtin_rintf(t);
+}
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+  return ((uint32_t)a & 0xFFu) | (((uint32_t)b & 0xFFu) << 8) | (((uint32_t)c & 0xFFu) << 16) | ((uint32_t)d << 24);
+}
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+// Where a row comes from.
+enum : int { kFromAct = 0, kFromNorm = 1, kFromSilu = 2, kFromF32 = 3, kFromCodes = 4 };
+
+// K a multiple of 16 that the integer sums hold; the sizes of one call in 64 bits.
+static inline bool int8_sizes(int M, int N, int K) {
+  return M >= 0 && N >= 0 && K > 0 && K % 16 == 0 && K <= kInt8MaxK;
+}
+static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Codes and scales of `rows` rows: from 16-bit activations (kFromAct), residual add and RMS norm (kFromNorm), SiLU(gate) x up of 16-bit
+// rows of 2 K (kFromSilu) or fp32 rows (kFromF32).
+struct QuantArgs {
+  const void* x;
+  const void* residual;
+  void* residual_out;
+  const void* norm_weight;
+  int8_t* q;
+  float* scale;
+  long long rows;
+  int K;
+  float eps;
+};
+int launch_int8_quant(int from, const QuantArgs& p, int act_dtype, hipStream_t st);
+
+}  // namespace qlin

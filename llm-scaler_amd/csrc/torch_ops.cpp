@@ -8,7 +8,8 @@
 // operator (registered as mi355x_checked::<name>), which runs it or raises, so that accepted calls, results and
 // error messages are those of that implementation.  Only the checks decide that, before anything is enqueued: once an
 // entry of the C ABI has been called, a status other than 0 is raised.  Running the call again would hide a launch that
-// failed and would add to an in-place operand twice (the residual of the norm operators).
+// failed and would add to an in-place operand twice (the residual of the norm operators).  The operators on 8-bit integers have no
+// other implementation: their checks, all of them, are here.
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/stack.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -405,6 +406,197 @@ Tensor moe_forward_full_fp8_block(const Tensor& x, const Tensor& logits, const T
   CHECKED("moe_forward_full_fp8_block", x, logits, out, w13, s13, sw13, ss13, w2, s2, sw2, ss2, gw, k, shared, E);
 }
 
+// ---------------------------------------------------------------------------------------- 8-bit integers (W8A8)
+// These operators are written here alone: every check is made below, nothing is handed to Python.
+#define REFUSE_UNLESS(cond, ...) TORCH_CHECK(cond, who, ": ", __VA_ARGS__)
+
+void int8_device(const char* who, const Tensor& x, const Tensor& t, const char* name) {
+  REFUSE_UNLESS(t.is_cuda() && t.device() == x.device(), name, " must be on the same ROCm device as the input, got ", t.device());
+  REFUSE_UNLESS(t.is_contiguous(), name, " must be contiguous");
+}
+void int8_aligned(const char* who, const Tensor& t, const char* name) {
+  REFUSE_UNLESS(((uintptr_t)t.data_ptr() & 15) == 0, name, " must start on a 16-byte boundary");
+}
+bool overlap(const Tensor& a, const Tensor& b) {
+  const char *p = (const char*)a.data_ptr(), *q = (const char*)b.data_ptr();
+  return p && q && p < q + b.nbytes() && q < p + a.nbytes();
+}
+void int8_apart(const char* who, const Tensor& out, const char* out_name, const Tensor& t, const char* name) {
+  REFUSE_UNLESS(!overlap(out, t), out_name, " must not overlap ", name);
+}
+
+// weight [N, K] with its scales and the optional bias, output M x N
+struct Int8Linear { int M, N, K, adt; };
+Int8Linear int8_linear(const char* who, const Tensor& x, int64_t per_row, const Tensor& w, const Tensor& ws, const c10::optional<Tensor>& bias,
+                       const Tensor& out) {
+  REFUSE_UNLESS(x.is_cuda(), "the input must be on a ROCm device, got ", x.device());
+  REFUSE_UNLESS(x.is_contiguous(), "the input must be contiguous");
+  int8_device(who, x, w, "weight");
+  int8_device(who, x, ws, "weight_scale");
+  int8_device(who, x, out, "output");
+  REFUSE_UNLESS(w.scalar_type() == at::kChar && w.dim() == 2, "weight must be int8 [N, K], got ", w.scalar_type(), " ", w.sizes());
+  const int64_t N = w.size(0), K = w.size(1);
+  REFUSE_UNLESS(K > 0 && K % 16 == 0 && K < 131072, "K=", K, " must be a multiple of 16 below 131072");
+  REFUSE_UNLESS(x.dim() >= 1 && x.size(-1) == per_row * K, "the input's rows must have ", per_row * K, " elements, got ", x.sizes());
+  const int64_t M = x.numel() / (per_row * K);
+  REFUSE_UNLESS(M <= INT_MAX && N <= INT_MAX, "more than 2^31 - 1 rows");
+  REFUSE_UNLESS(ws.scalar_type() == at::kFloat && ws.numel() == N, "weight_scale must be fp32 with N=", N, " entries");
+  REFUSE_UNLESS(is16(out), "output must be fp16 or bf16, got ", out.scalar_type());
+  REFUSE_UNLESS(out.numel() == M * N, "output has ", out.numel(), " elements, expected M*N=", M * N);
+  if (bias.has_value()) {
+    int8_device(who, x, *bias, "bias");
+    REFUSE_UNLESS(bias->scalar_type() == out.scalar_type() && bias->numel() == N, "bias must have N=", N, " entries in the output's type");
+    int8_apart(who, out, "output", *bias, "bias");
+  }
+  int8_aligned(who, x, "the input");
+  int8_aligned(who, w, "weight");
+  int8_apart(who, out, "output", x, "the input");
+  int8_apart(who, out, "output", w, "weight");
+  int8_apart(who, out, "output", ws, "weight_scale");
+  return {(int)M, (int)N, (int)K, act(out)};
+}
+const void* data_or_null(const c10::optional<Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+
+Tensor int8_workspace(const Tensor& x, const Int8Linear& l, long long& bytes) {
+  CALL(mi_gemm_int8_workspace, l.M, l.N, l.K, &bytes);
+  return buffer(x, bytes);
+}
+
+Tensor gemm_int8(const Tensor& x, const c10::optional<Tensor>& x_scale, const Tensor& w, const Tensor& ws,
+                 const c10::optional<Tensor>& bias, const Tensor& out) {
+  const char* who = "gemm_int8";
+  if (x_scale.has_value()) {
+    REFUSE_UNLESS(x.scalar_type() == at::kChar, "an input with scales must be int8, got ", x.scalar_type());
+  } else {
+    REFUSE_UNLESS(is16(x) && x.scalar_type() == out.scalar_type(), "an input without scales must be fp16 or bf16 like the output, got ",
+                  x.scalar_type(), " and ", out.scalar_type());
+  }
+  const Int8Linear l = int8_linear(who, x, 1, w, ws, bias, out);
+  if (x_scale.has_value()) {
+    int8_device(who, x, *x_scale, "x_scale");
+    REFUSE_UNLESS(x_scale->scalar_type() == at::kFloat && x_scale->numel() == l.M, "x_scale must be fp32 with M=", l.M, " entries");
+    int8_apart(who, out, "output", *x_scale, "x_scale");
+  }
+  if (!l.M) return out;
+  const On on(x);
+  long long bytes = 0;
+  const Tensor buf = int8_workspace(x, l, bytes);
+  CALL(mi_gemm_int8_ws, x.data_ptr(), (const float*)data_or_null(x_scale), w.data_ptr(), ws.data_ptr<float>(), data_or_null(bias),
+       out.data_ptr(), buf.data_ptr(), bytes, l.M, l.N, l.K, l.adt, on.stream);
+  return out;
+}
+
+Tensor resadd_norm_gemm_int8(const Tensor& x, const Tensor& res, const Tensor& res_out, const Tensor& nw, const Tensor& w, const Tensor& ws,
+                             const c10::optional<Tensor>& bias, const Tensor& out, double eps) {
+  const char* who = "resadd_norm_gemm_int8";
+  REFUSE_UNLESS(is16(x) && x.scalar_type() == out.scalar_type(), "hidden_states must be fp16 or bf16 like the output, got ", x.scalar_type(),
+                " and ", out.scalar_type());
+  const Int8Linear l = int8_linear(who, x, 1, w, ws, bias, out);
+  for (const auto& t : {std::make_pair(&res, "residual"), std::make_pair(&res_out, "residual_out"), std::make_pair(&nw, "norm_weight")}) {
+    int8_device(who, x, *t.first, t.second);
+    REFUSE_UNLESS(t.first->scalar_type() == x.scalar_type(), t.second, " must have the input's type, got ", t.first->scalar_type());
+    int8_aligned(who, *t.first, t.second);
+    int8_apart(who, out, "output", *t.first, t.second);
+  }
+  REFUSE_UNLESS(res.numel() == x.numel() && res_out.numel() == x.numel(), "residual and residual_out must have the input's size");
+  REFUSE_UNLESS(nw.numel() == l.K, "norm_weight must have K=", l.K, " entries");
+  int8_apart(who, res_out, "residual_out", x, "hidden_states");
+  int8_apart(who, res_out, "residual_out", nw, "norm_weight");
+  int8_apart(who, res_out, "residual_out", w, "weight");
+  int8_apart(who, res_out, "residual_out", ws, "weight_scale");
+  if (bias.has_value()) int8_apart(who, res_out, "residual_out", *bias, "bias");
+  REFUSE_UNLESS(res_out.data_ptr() == res.data_ptr() || !overlap(res_out, res), "residual_out must be residual or not overlap it");
+  if (!l.M) return out;
+  const On on(x);
+  long long bytes = 0;
+  const Tensor buf = int8_workspace(x, l, bytes);
+  CALL(mi_resadd_norm_gemm_int8_ws, x.data_ptr(), res.data_ptr(), res_out.data_ptr(), nw.data_ptr(), (float)eps, w.data_ptr(),
+       ws.data_ptr<float>(), data_or_null(bias), out.data_ptr(), buf.data_ptr(), bytes, l.M, l.N, l.K, l.adt, on.stream);
+  return out;
+}
+
+Tensor silu_mul_gemm_int8(const Tensor& gate_up, const Tensor& w, const Tensor& ws, const c10::optional<Tensor>& bias, const Tensor& out) {
+  const char* who = "silu_mul_gemm_int8";
+  REFUSE_UNLESS(is16(gate_up) && gate_up.scalar_type() == out.scalar_type(), "gate_up must be fp16 or bf16 like the output, got ",
+                gate_up.scalar_type(), " and ", out.scalar_type());
+  const Int8Linear l = int8_linear(who, gate_up, 2, w, ws, bias, out);
+  if (!l.M) return out;
+  const On on(gate_up);
+  long long bytes = 0;
+  const Tensor buf = int8_workspace(gate_up, l, bytes);
+  CALL(mi_silu_mul_gemm_int8_ws, gate_up.data_ptr(), w.data_ptr(), ws.data_ptr<float>(), data_or_null(bias), out.data_ptr(), buf.data_ptr(),
+       bytes, l.M, l.N, l.K, l.adt, on.stream);
+  return out;
+}
+
+Tensor moe_forward_full_int8(const Tensor& x, const Tensor& logits, const Tensor& out, const Tensor& w13, const Tensor& s13,
+                             const c10::optional<Tensor>& sw13, const c10::optional<Tensor>& ss13, const Tensor& w2, const Tensor& s2,
+                             const c10::optional<Tensor>& sw2, const c10::optional<Tensor>& ss2, const c10::optional<Tensor>& gw, int64_t k,
+                             int64_t shared, int64_t E) {
+  const char* who = "moe_forward_full_int8";
+  REFUSE_UNLESS(x.is_cuda(), "x must be on a ROCm device, got ", x.device());
+  REFUSE_UNLESS(x.dim() == 2 && x.is_contiguous() && is16(x), "x must be contiguous fp16 or bf16 [T, H]");
+  REFUSE_UNLESS(shared == 0 || shared == 1, "num_shared_experts must be 0 or 1, got ", shared);
+  REFUSE_UNLESS(E >= 1 && E <= 1024 && k >= 1 && k <= 64 && k <= E, "top_k=", k, " of ", E, " experts is not supported");
+  const int64_t T = x.size(0), H = x.size(1);
+  const auto dt = x.scalar_type();
+  REFUSE_UNLESS(w13.dim() == 3 && w13.size(1) % 2 == 0, "gate_up_weight must be [E, 2I, H]");
+  const int64_t I = w13.size(1) / 2;
+  REFUSE_UNLESS(H > 0 && H % 16 == 0 && H < 131072 && I > 0 && I % 16 == 0 && I < 131072,
+                "hidden and intermediate sizes must be multiples of 16 below 131072, got ", H, " and ", I);
+  // present exactly when a shared expert is asked for
+  auto opt = [&](const c10::optional<Tensor>& t, const char* name) {
+    REFUSE_UNLESS(t.has_value() == (shared == 1), name, shared ? " is missing" : " is given without a shared expert");
+  };
+  opt(sw13, "shared_gate_up_weight");
+  opt(ss13, "shared_gate_up_scale");
+  opt(sw2, "shared_down_weight");
+  opt(ss2, "shared_down_scale");
+  opt(gw, "shared_expert_gate_weight");
+  auto take = [&](const Tensor& t, at::ScalarType type, at::IntArrayRef shape, const char* name) {
+    REFUSE_UNLESS(t.scalar_type() == type && t.sizes() == shape, name, " must be ", type, " ", shape, ", got ", t.scalar_type(), " ", t.sizes());
+    int8_device(who, x, t, name);
+  };
+  auto weight = [&](const Tensor& t, at::IntArrayRef shape, const char* name) {
+    take(t, at::kChar, shape, name);
+    int8_aligned(who, t, name);
+    int8_apart(who, out, "output", t, name);
+  };
+  auto scale = [&](const Tensor& t, at::IntArrayRef shape, const char* name) {
+    take(t, at::kFloat, shape, name);
+    int8_apart(who, out, "output", t, name);
+  };
+  take(logits, dt, {T, E}, "logits");
+  take(out, dt, {T, H}, "output");
+  weight(w13, {E, 2 * I, H}, "gate_up_weight");
+  scale(s13, {E, 2 * I}, "gate_up_scale");
+  weight(w2, {E, H, I}, "down_weight");
+  scale(s2, {E, H}, "down_scale");
+  if (shared) {
+    weight(*sw13, {2 * I, H}, "shared_gate_up_weight");
+    scale(*ss13, {2 * I}, "shared_gate_up_scale");
+    weight(*sw2, {H, I}, "shared_down_weight");
+    scale(*ss2, {H}, "shared_down_scale");
+    take(*gw, dt, {1, H}, "shared_expert_gate_weight");
+    int8_aligned(who, *gw, "shared_expert_gate_weight");
+    int8_apart(who, out, "output", *gw, "shared_expert_gate_weight");
+  }
+  int8_aligned(who, x, "x");
+  int8_aligned(who, out, "output");
+  int8_apart(who, out, "output", x, "x");
+  int8_apart(who, out, "output", logits, "logits");
+  REFUSE_UNLESS(T <= INT_MAX, "more than 2^31 - 1 tokens");
+  if (!T) return out;
+  const On on(x);
+  long long bytes = 0;
+  CALL(mi_moe_forward_full_int8_workspace, (int)T, (int)k, (int)E, (int)H, (int)I, (int)shared, &bytes);
+  const Tensor buf = buffer(x, bytes);
+  CALL(mi_moe_forward_full_int8_ws, x.data_ptr(), logits.data_ptr(), out.data_ptr(), w13.data_ptr(), s13.data_ptr<float>(),
+       data_or_null(sw13), (const float*)data_or_null(ss13), w2.data_ptr(), s2.data_ptr<float>(), data_or_null(sw2),
+       (const float*)data_or_null(ss2), data_or_null(gw), buf.data_ptr(), bytes, (int)T, (int)k, (int)E, (int)H, (int)I, act(x), on.stream);
+  return out;
+}
+
 }  // namespace
 
 #define IMPL(name) m.impl(#name, &name)
@@ -417,11 +609,14 @@ Tensor moe_forward_full_fp8_block(const Tensor& x, const Tensor& logits, const T
   IMPL(esimd_gemm_int4_pgrp); IMPL(esimd_gemm_int4_pgrp_zp); IMPL(esimd_gemm_fp8_pert);                      \
   IMPL(esimd_gemm_fp8_blockscale); IMPL(esimd_gemv_fp8_blockscale_fused2)
 
-TORCH_LIBRARY_IMPL(custom_esimd_kernels_vllm, CUDA, m) { DECODE_OPS(); GEMM_OPS(); }
+TORCH_LIBRARY_IMPL(custom_esimd_kernels_vllm, CUDA, m) {
+  DECODE_OPS(); GEMM_OPS();
+  IMPL(gemm_int8); IMPL(resadd_norm_gemm_int8); IMPL(silu_mul_gemm_int8);
+}
 TORCH_LIBRARY_IMPL(custom_esimd_kernels, CUDA, m) { GEMM_OPS(); }
 TORCH_LIBRARY_IMPL(custom_esimd_kernels_sglang, CUDA, m) {
   DECODE_OPS();
   IMPL(esimd_gemv_q4_k); IMPL(esimd_gemv_q4_0); IMPL(esimd_gemm_q4_0); IMPL(esimd_gemv_q8_0); IMPL(esimd_gemv_q8_0_m);
   IMPL(esimd_gemv_q5_k); IMPL(esimd_gemv_q6_k); IMPL(esimd_gemv_q6_k_m);
 }
-TORCH_LIBRARY_IMPL(moe_ops, CUDA, m) { IMPL(moe_forward_full_fp8_block); }
+TORCH_LIBRARY_IMPL(moe_ops, CUDA, m) { IMPL(moe_forward_full_fp8_block); IMPL(moe_forward_full_int8); }

@@ -40,12 +40,15 @@ _CHECKED = {}        # operators with a native host path -> their Python impleme
 
 def _define(ns: str, schema: str, impl, meta=None):
     """Declares an operator.  Where the native host path implements it (csrc/torch_ops.cpp), `impl` is what that hands
-    the calls it does not take to, under the name mi355x_checked::<name>."""
+    the calls it does not take to, under the name mi355x_checked::<name>; None where it takes every call or refuses it."""
     lib = _library(ns)
     lib.define(schema)
     name = schema.split("(", 1)[0]
     _DEFINED.setdefault(ns, []).append(name)
-    if not torch._C._dispatch_has_kernel_for_dispatch_key(f"{ns}::{name}", "CUDA"):
+    native = torch._C._dispatch_has_kernel_for_dispatch_key(f"{ns}::{name}", "CUDA")
+    if impl is None:
+        _chk(native, f"mi355x_qlinear: the native host path does not implement {ns}::{name}")
+    elif not native:
         lib.impl(name, impl, "CUDA")
     elif name not in _CHECKED:
         _CHECKED[name] = impl
@@ -2445,6 +2448,17 @@ def register():
     _define(_V, "moe_forward_fp8_block(Tensor x, Tensor logits, Tensor gate_up_weight, Tensor gate_up_scale, "
                 "Tensor down_weight, Tensor down_scale, Tensor(a!) output, int top_k, bool act_quant) -> Tensor(a!)",
             moe_forward_fp8_block, _ret(6))
+    # 8-bit integer activations and weights: no counterpart in the reference
+    _define(_V, "gemm_int8(Tensor x, Tensor? x_scale, Tensor weight, Tensor weight_scale, Tensor? bias, Tensor(a!) output) "
+                "-> Tensor(a!)", None, _ret(5))
+    _define(_V, "resadd_norm_gemm_int8(Tensor hidden_states, Tensor residual, Tensor(b!) residual_out, Tensor norm_weight, "
+                "Tensor weight, Tensor weight_scale, Tensor? bias, Tensor(a!) output, float eps) -> Tensor(a!)", None, _ret(7))
+    _define(_V, "silu_mul_gemm_int8(Tensor gate_up, Tensor weight, Tensor weight_scale, Tensor? bias, Tensor(a!) output) "
+                "-> Tensor(a!)", None, _ret(4))
+    _define("moe_ops", "moe_forward_full_int8(Tensor x, Tensor logits, Tensor(a!) output, Tensor gate_up_weight, Tensor gate_up_scale, "
+                       "Tensor? shared_gate_up_weight, Tensor? shared_gate_up_scale, Tensor down_weight, Tensor down_scale, "
+                       "Tensor? shared_down_weight, Tensor? shared_down_scale, Tensor? shared_expert_gate_weight, int top_k, "
+                       "int num_shared_experts, int n_routed_experts) -> Tensor(a!)", None, _ret(2))
 
 
 register()
