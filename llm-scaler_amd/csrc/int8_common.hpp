@@ -9,6 +9,8 @@
 #pragma once
 #include "qlinear_common.hpp"
 
+#include <atomic>
+
 namespace qlin {
 
 typedef __attribute__((ext_vector_type(4))) float f32v4;
@@ -72,6 +74,30 @@ enum : int { kFromAct = 0, kFromNorm = 1, kFromSilu = 2, kFromF32 = 3, kFromCode
 // K a multiple of 16 that the integer sums hold; the sizes of one call in 64 bits.
 static inline bool int8_sizes(int M, int N, int K) {
   return M >= 0 && N >= 0 && K > 0 && K % 16 == 0 && K <= kInt8MaxK;
+}
+static inline int int8_cu_count() {
+  static int cus = 0;
+  if (!cus) {
+    int dev = 0;
+    hipDeviceProp_t prop;
+    if (hipGetDevice(&dev) == hipSuccess && hipGetDeviceProperties(&prop, dev) == hipSuccess) cus = prop.multiProcessorCount;
+    if (cus <= 0) cus = 256;
+  }
+  return cus;
+}
+// A kernel that asks for more LDS than a launch gets unasked: once per device.
+template <class Kernel>
+static inline int int8_raise_lds(Kernel* kernel, std::atomic<unsigned long long>& raised, size_t bytes) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return MI_ERR_LAUNCH;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (raised.load(std::memory_order_relaxed) & bit)) return MI_OK;
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess) {
+    (void)hipGetLastError();
+    return MI_ERR_LAUNCH;
+  }
+  if (dev < 64) raised.fetch_or(bit, std::memory_order_relaxed);
+  return MI_OK;
 }
 static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 

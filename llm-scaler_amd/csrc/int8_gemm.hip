@@ -1,5 +1,6 @@
 // The linears of a W8A8 layer: rows of activations to codes (int8_quant.hip), then the product (int8_gemm.hpp).
 #include "int8_gemm.hpp"
+#include "int8_rows.hpp"
 #include "../../include/mi355x_qlinear.h"
 
 namespace qlin {
@@ -37,6 +38,10 @@ static int run_linear(Linear l, const void* w, const float* w_scale, const void*
   if (!l.q.x || (N && (!w || !w_scale || !out))) return MI_ERR_ARG;
   if (!aligned16(l.q.x) || !aligned16(w)) return MI_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
+  Int8RowsArgs r{l.q.x, l.x_scale, l.q.residual, l.q.residual_out, l.q.norm_weight, (const int8_t*)w, w_scale, bias, out, M, N, K, 0, l.q.eps};
+  // one launch; the new residual must not be what other workgroups still read
+  if (l.from != kFromCodes && N && int8_rows_quantise(M, K) && (l.from != kFromNorm || l.q.residual_out != l.q.residual))
+    return launch_int8_rows(l.from, r, act_dtype, st);
   Int8GemmArgs p{};
   if (l.from == kFromCodes) {
     p.a = (const int8_t*)l.q.x;
@@ -56,6 +61,11 @@ static int run_linear(Linear l, const void* w, const float* w_scale, const void*
     p.a_scale = l.q.scale;
   }
   if (!N) return MI_OK;
+  if (M <= kInt8Rows) {
+    r.x = p.a;
+    r.x_scale = p.a_scale;
+    return launch_int8_rows(kFromCodes, r, act_dtype, st);
+  }
   p.w = (const int8_t*)w;
   p.w_scale = w_scale;
   p.bias = bias;
