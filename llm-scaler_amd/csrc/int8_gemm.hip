@@ -40,7 +40,7 @@ static int run_linear(Linear l, const void* w, const float* w_scale, const void*
   hipStream_t st = (hipStream_t)stream;
   Int8RowsArgs r{l.q.x, l.x_scale, l.q.residual, l.q.residual_out, l.q.norm_weight, (const int8_t*)w, w_scale, bias, out, M, N, K, 0, l.q.eps};
   // one launch; the new residual must not be what other workgroups still read
-  if (l.from != kFromCodes && N && int8_rows_quantise(M, K) && (l.from != kFromNorm || l.q.residual_out != l.q.residual))
+  if (l.from != kFromCodes && N && int8_rows_quantise(l.from, M, K) && (l.from != kFromNorm || l.q.residual_out != l.q.residual))
     return launch_int8_rows(l.from, r, act_dtype, st);
   Int8GemmArgs p{};
   if (l.from == kFromCodes) {
@@ -61,7 +61,7 @@ static int run_linear(Linear l, const void* w, const float* w_scale, const void*
     p.a_scale = l.q.scale;
   }
   if (!N) return MI_OK;
-  if (M <= kInt8Rows) {
+  if (int8_rows_codes(M, K)) {
     r.x = p.a;
     r.x_scale = p.a_scale;
     return launch_int8_rows(kFromCodes, r, act_dtype, st);

@@ -34,11 +34,6 @@ enum : int { kEpiOut = 0, kEpiF32 = 1, kEpiAct = 2 };
 
 constexpr int kInt8Step = 128;                        // bytes of a row per step
 
-template <int N>
-__device__ __forceinline__ void wait_loads() {         // all but the N newest
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
-}
-
 template <class Act, int BM, int BN, int WM, int WN, int STAGES, int EPI, bool GROUPED>
 __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_kernel(const Int8GemmArgs p) {
   using Elem = typename Act::elem;
@@ -115,7 +110,6 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_kernel(const Int8GemmA
   const __amdgpu_buffer_rsrc_t ra = make_rsrc(a0, (uint32_t)(a_bytes < 0x7FFFFFFFull ? a_bytes : 0x7FFFFFFFull));
   const __amdgpu_buffer_rsrc_t rb = make_rsrc(w + (size_t)n0 * K, (uint32_t)(w_bytes < 0x7FFFFFFFull ? w_bytes : 0x7FFFFFFFull));
 
-  using lds_ptr = __attribute__((address_space(3))) void*;
   const int steps = (K + kInt8Step - 1) / kInt8Step;
   auto request = [&](int s) __attribute__((always_inline)) {
     unsigned char* to = smem + (s % STAGES) * STAGE;
@@ -146,7 +140,6 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_kernel(const Int8GemmA
   for (int s = 0; s < STAGES - 1; ++s) request(s);
   for (int s = 0; s < steps; ++s) {
     wait_loads<(STAGES - 2) * (LA + LB)>();
-    asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     request(s + STAGES - 1);                           // into the buffer that every wavefront has left; past the end it fetches zeros

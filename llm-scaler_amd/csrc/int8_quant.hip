@@ -50,7 +50,7 @@ struct RowSource {
     for (int i = 0; i < 8; ++i) v[i] = v[i] * r * Act::to_f32(w[i]);
   }
   __device__ __forceinline__ void write(int k, const float* v, float inv) const {
-    int c[8];
+    uint32_t c[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[i] = code_of<FROM == kFromAct>(v[i], inv);
     *reinterpret_cast<u32x2*>(p.q + row * p.K + k) = u32x2{pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7])};

@@ -19,8 +19,8 @@ struct Int8RowsArgs {
   float eps;
 };
 
-constexpr int kInt8Rows = 64;                         // rows that the kernel takes as codes
-bool int8_rows_quantise(int M, int K);                // and as activations
+bool int8_rows_codes(int M, int K);                   // whether the kernel takes M rows of codes
+bool int8_rows_quantise(int from, int M, int K);      // and of activations
 int launch_int8_rows(int from, const Int8RowsArgs& p, int act_dtype, hipStream_t st);
 
 }  // namespace qlin
