@@ -5,21 +5,72 @@
 
 namespace qlin {
 
-template <class Act, int BM, int BN, int WM, int WN, int STAGES>
+template <class Act, int BM, int BN, int WM, int WN, int KG, int SA, int SB>
 static int launch_tiles(Int8GemmArgs p, hipStream_t st) {
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
   const long long tiles = (long long)p.tiles_m * p.tiles_n, grid = (tiles + 7) / 8 * 8;
   if (grid > 0x7FFFFFFFLL) return MI_ERR_SHAPE;
-  auto* kernel = int8_gemm_kernel<Act, BM, BN, WM, WN, STAGES, kEpiOut, false>;
-  constexpr size_t lds = (size_t)STAGES * (BM + BN) * kInt8Step;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * WM * WN), lds, st, p);
+  auto* kernel = int8_gemm_kernel<Act, BM, BN, WM, WN, KG, SA, SB, kEpiOut, false>;
+  constexpr size_t lds = int8_gemm_lds(BM, BN, WM * WN, KG, SA, SB);
+  if constexpr (lds > 64 * 1024) {
+    static std::atomic<unsigned long long> raised{0};
+    const int rc = int8_raise_lds(kernel, raised, lds);
+    if (rc != MI_OK) return rc;
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * WM * WN * KG), lds, st, p);
   return launch_status();
+}
+
+// The tiles, and what a round of the CUs costs with each: us = fixed + step x (steps of 128 KG of K), measured on 455 problems (M 17 .. 2048,
+// N 512 .. 14336, K 1024 .. 14336); the last has room for two workgroups on a CU, whose pair costs less than two rounds.  The tile with the
+// least sum of rounds is 0.3 % behind the best of 22 tiles in the mean, 8 % at most.  Some of them, us with the best / the second
+// best of another shape: 2048 x 4096 x 14336 256 x 256 112 / 256 x 192 123; 2048 x 14336 x 4096 256 x 128 101 / 128 x 128 118; 1000 x 4096 x 6144 128 x 192
+// 29.4 / 128 x 96 32.9; 128 x 4096 x 14336 128 x 64 16.1 / 128 x 128 19.2; 64 x 5120 x 5120 64 x 32 10.2 / 64 x 64 11.5; 32 x 14336 x 4096 32 x 16 13.6 /
+// 64 x 32 17.4.  A smaller tile reads more through the loads to LDS (68 GB/s per CU for whole lines, 54 for half lines of 64 bytes), a larger one
+// leaves CUs without work.
+struct Int8Tile {
+  int bm, bn, kg;
+  float fixed, step, pair_fixed, pair_step;            // the pair: 0 where a workgroup fills the CU
+};
+constexpr Int8Tile kTiles[] = {{256, 256, 1, 13.3f, 1.29f, 0, 0}, {256, 192, 1, 6.6f, 1.06f, 0, 0},  {256, 128, 1, 6.7f, 0.75f, 0, 0},
+                               {128, 192, 1, 7.3f, 0.62f, 0, 0},  {128, 128, 1, 3.7f, 0.48f, 0, 0},  {64, 96, 2, 4.3f, 0.47f, 0, 0},
+                               {64, 64, 2, 2.6f, 0.36f, 0, 0},    {64, 32, 4, 3.0f, 0.50f, 0, 0},    {32, 64, 4, 2.8f, 0.52f, 0, 0},
+                               {64, 16, 4, 2.4f, 0.39f, 0, 0},    {32, 16, 8, 2.6f, 0.49f, 0, 0},    {128, 64, 1, 1.4f, 0.37f, 2.7f, 0.58f}};
+
+static int pick_tile(long long M, long long N, long long K) {
+  const long long cus = int8_cu_count();
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
+    const Int8Tile& t = kTiles[i];
+    const long long tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn), rounds = (tiles + cus - 1) / cus;
+    const double steps = (double)((K + 128 * t.kg - 1) / (128 * t.kg)), one = t.fixed + t.step * steps;
+    const double cost = t.pair_step > 0 ? (rounds % 2) * one + (rounds / 2) * (t.pair_fixed + t.pair_step * steps) : rounds * one;
+    if (!i || cost < least) {
+      least = cost;
+      best = i;
+    }
+  }
+  return best;
 }
 
 template <class Act>
 static int launch_product(const Int8GemmArgs& p, hipStream_t st) {
-  return launch_tiles<Act, 128, 128, 2, 2, 2>(p, st);
+  switch (pick_tile(p.M, p.N, p.K)) {                  // rows, columns, wavefronts along both, KG, buffers of A and B
+    case 0: return launch_tiles<Act, 256, 256, 4, 2, 1, 3, 2>(p, st);
+    case 1: return launch_tiles<Act, 256, 192, 4, 2, 1, 3, 2>(p, st);
+    case 2: return launch_tiles<Act, 256, 128, 4, 2, 1, 3, 3>(p, st);
+    case 3: return launch_tiles<Act, 128, 192, 2, 4, 1, 3, 3>(p, st);
+    case 4: return launch_tiles<Act, 128, 128, 2, 4, 1, 3, 3>(p, st);
+    case 5: return launch_tiles<Act, 64, 96, 2, 2, 2, 3, 3>(p, st);
+    case 6: return launch_tiles<Act, 64, 64, 2, 2, 2, 4, 3>(p, st);
+    case 7: return launch_tiles<Act, 64, 32, 2, 1, 4, 3, 3>(p, st);
+    case 8: return launch_tiles<Act, 32, 64, 1, 2, 4, 3, 3>(p, st);
+    case 9: return launch_tiles<Act, 64, 16, 2, 1, 4, 3, 3>(p, st);
+    case 10: return launch_tiles<Act, 32, 16, 1, 1, 8, 3, 3>(p, st);
+    default: return launch_tiles<Act, 128, 64, 2, 2, 1, 3, 3>(p, st);
+  }
 }
 
 struct Linear {
@@ -70,7 +121,7 @@ static int run_linear(Linear l, const void* w, const float* w_scale, const void*
   p.w_scale = w_scale;
   p.bias = bias;
   p.out = out;
-  p.wide_out = N % 4 == 0 && ((uintptr_t)out & 7) == 0;
+  p.wide_out = N % 8 == 0 && aligned16(out);
   p.M = M;
   p.N = N;
   p.K = K;

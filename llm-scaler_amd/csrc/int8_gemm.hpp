@@ -1,12 +1,15 @@
 // Product of 8-bit codes on the matrix cores: out[m][n] = (sum_k a[m][k] w[n][k]) a_scale[m] w_scale[n].
 //
 // A workgroup owns a BM x BN tile.  Both operands go to LDS straight from memory (128-byte pieces of a row per step, no registers
-// and no vector instructions in between) into a ring of STAGES buffers; a wavefront multiplies (16 TM) x (16 TN) of the tile with
-// v_mfma_i32_16x16x64_i8.  16-byte chunk c of tile row r lies at place c ^ f(r) of its 128 bytes, so that the eight lanes that
+// and no vector instructions in between) into rings of SA and SB buffers; a wavefront multiplies (16 TM) x (16 TN) of the tile with
+// v_mfma_i32_16x16x64_i8; where a tile's K is long beside its rows and columns, KG groups of wavefronts take a 128-byte piece of every
+// step each, which keeps more loads under way, and their sums meet at the end.  16-byte chunk c of tile row r lies at place c ^ f(r) of its 128 bytes, so that the eight lanes that
 // read at a time find eight different places.  The weights are the first operand: a lane ends with consecutive output columns of
 // one row, 4 per MFMA tile, and the weight rows of GJ tiles are interleaved so that these are 4 GJ in a row.
 #pragma once
 #include "int8_common.hpp"
+
+#include <type_traits>
 
 namespace qlin {
 
@@ -18,7 +21,7 @@ struct Int8GemmArgs {
   const void* bias;           // [N] in the output's type, or null
   void* out;
   int M, N, K;                // M: rows of a
-  int wide_out;               // four outputs per store: N and out allow it
+  int wide_out;               // eight outputs per store: N and out allow it
   int tiles_m, tiles_n;
   // Grouped: tile i covers the rows [g_tile[4 i + 1], + g_tile[4 i + 2]) of the expert-sorted order and multiplies them with expert
   // g_tile[4 i]; row r of that order is row g_row[r] of a (null: r).  Expert E is the shared one.  g_tile[4 tiles_m]: tiles in use.
@@ -34,20 +37,30 @@ enum : int { kEpiOut = 0, kEpiF32 = 1, kEpiAct = 2 };
 
 constexpr int kInt8Step = 128;                        // bytes of a row per step
 
-template <class Act, int BM, int BN, int WM, int WN, int STAGES, int EPI, bool GROUPED>
-__global__ __launch_bounds__(64 * WM * WN) void int8_gemm_kernel(const Int8GemmArgs p) {
+// LDS of a tile: the rings and, where the tile's rows do not divide among the wavefronts, the place of the loads that are over.
+constexpr size_t int8_gemm_lds(int BM, int BN, int NW, int KG, int SA, int SB) {
+  return (size_t)KG * (SA * BM + SB * BN) * kInt8Step + (BM % (8 * NW) || BN % (8 * NW) ? 1024 : 0);
+}
+
+template <class Elem>
+using PairOf = Elem __attribute__((ext_vector_type(2)));
+
+template <class Act, int BM, int BN, int WM, int WN, int KG, int SA, int SB, int EPI, bool GROUPED>
+__global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8GemmArgs p) {
   using Elem = typename Act::elem;
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;   // 1 KiB loads of a wavefront per step
+  constexpr int LA = (BM / 8 + NW - 1) / NW, LB = (BN / 8 + NW - 1) / NW;       // 1 KiB loads of a wavefront per step
   constexpr int HN = EPI == kEpiAct ? TN / 2 : TN;    // MFMA tiles of gate (or all) columns
-  constexpr int GJ = HN < 4 ? HN : 4;
-  constexpr int STAGE = (BM + BN) * kInt8Step;
-  static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN && TM * 16 * WM == BM && TN * 16 * WN == BN, "tile");
+  constexpr int GJ = HN % 4 == 0 ? 4 : HN % 2 == 0 ? 2 : HN;
+  constexpr int A_PART = BM * kInt8Step, B_PART = BN * kInt8Step, B_RING = SA * KG * A_PART;   // the ring of A, that of B
+  constexpr int SPARE = B_RING + SB * KG * B_PART;    // and 1 KiB that a load lands in which a wavefront has over
+  static_assert(SB >= 2 && (SA == SB || SA == SB + 1), "rings");
+  static_assert(TM * 16 * WM == BM && TN * 16 * WN == BN, "tile");
   static_assert(HN * (EPI == kEpiAct ? 2 : 1) == TN && HN % GJ == 0, "columns");
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave % WM, wn = wave / WM;
+  const int wk = wave / NW, wg = wave % NW, wm = wg % WM, wn = wg / WM;        // part of the step, place in the tile
   const int K = p.K, N = p.N;
   constexpr int BNO = EPI == kEpiAct ? BN / 2 : BN;   // output columns of a tile
   const int NO = EPI == kEpiAct ? N / 2 : N;
@@ -83,8 +96,8 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_kernel(const Int8GemmA
   int chunk[LA + LB];
 #pragma unroll
   for (int i = 0; i < LA; ++i) {
-    const int r = (wave * LA + i) * 8 + (lane >> 3);
-    chunk[i] = ((lane & 7) ^ (r & 7)) * 16;
+    const int r = (wg * LA + i) * 8 + (lane >> 3);
+    chunk[i] = wk * kInt8Step + ((lane & 7) ^ (r & 7)) * 16;
     uint32_t row = (uint32_t)r;
     if constexpr (GROUPED) {
       const int at = m0 + (r < rows ? r : 0);
@@ -94,8 +107,8 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_kernel(const Int8GemmA
   }
 #pragma unroll
   for (int i = 0; i < LB; ++i) {
-    const int r = (wave * LB + i) * 8 + (lane >> 3);
-    chunk[LA + i] = ((lane & 7) ^ ((r & 3) | ((r / (4 * GJ)) & 1) << 2)) * 16;
+    const int r = (wg * LB + i) * 8 + (lane >> 3);
+    chunk[LA + i] = wk * kInt8Step + ((lane & 7) ^ ((r & 3) | ((r / (4 * GJ)) & 1) << 2)) * 16;
     int row = r;
     bool in = n0 + r < N;
     if constexpr (EPI == kEpiAct) {
@@ -103,25 +116,31 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_kernel(const Int8GemmA
       in = n0 + col < NO;
       row = q < TN * 8 ? col : NO + col;
     }
-    from[LA + i] = in ? (uint32_t)row * (uint32_t)K + chunk[LA + i] : kOOB;
+    from[LA + i] = in && r < BN ? (uint32_t)row * (uint32_t)K + chunk[LA + i] : kOOB;
   }
   const int8_t* a0 = GROUPED ? p.a : p.a + (size_t)m0 * K;
   const unsigned long long a_bytes = (unsigned long long)(GROUPED ? p.M : rows) * K, w_bytes = (unsigned long long)(N - n0) * K;
   const __amdgpu_buffer_rsrc_t ra = make_rsrc(a0, (uint32_t)(a_bytes < 0x7FFFFFFFull ? a_bytes : 0x7FFFFFFFull));
   const __amdgpu_buffer_rsrc_t rb = make_rsrc(w + (size_t)n0 * K, (uint32_t)(w_bytes < 0x7FFFFFFFull ? w_bytes : 0x7FFFFFFFull));
 
-  const int steps = (K + kInt8Step - 1) / kInt8Step;
-  auto request = [&](int s) __attribute__((always_inline)) {
-    unsigned char* to = smem + (s % STAGES) * STAGE;
-    const int k0 = s * kInt8Step;
-    const bool whole = k0 + kInt8Step <= K;
+  constexpr int STEP = KG * kInt8Step;
+  const int steps = (K + STEP - 1) / STEP;
+  auto request = [&](auto is_a, int s, int slot) __attribute__((always_inline)) {
+    constexpr bool A = decltype(is_a)::value;
+    constexpr int COUNT = A ? LA : LB, FIRST = A ? 0 : LA;
+    constexpr bool EVEN = A ? LA * NW * 8 == BM : LB * NW * 8 == BN;
+    const int to = A ? (slot * KG + wk) * A_PART + wg * LA * 1024 : B_RING + (slot * KG + wk) * B_PART + wg * LB * 1024;
+    const int k0 = s * STEP;
+    const bool whole = k0 + STEP <= K;
 #pragma unroll
-    for (int i = 0; i < LA + LB; ++i) {
-      const int at = i < LA ? wave * LA + i : BM / 8 + wave * LB + (i - LA);
-      const uint32_t f = whole || k0 + chunk[i] < K ? from[i] : kOOB;   // past the row's end: zeros
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(i < LA ? ra : rb, (lds_ptr)(to + at * 1024), 16, f, k0, 0, 0);
+    for (int i = 0; i < COUNT; ++i) {
+      const uint32_t f = whole || k0 + chunk[FIRST + i] < K ? from[FIRST + i] : kOOB;   // past the row's end: zeros
+      const int at = EVEN || (wg * COUNT + i) * 8 < (A ? BM : BN) ? to + i * 1024 : SPARE;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(A ? ra : rb, (lds_ptr)(smem + at), 16, f, k0, 0, 0);
     }
   };
+  constexpr std::true_type a_tag{};
+  constexpr std::false_type b_tag{};
 
   i32x4 acc[TN][TM];
 #pragma unroll
@@ -134,69 +153,172 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_gemm_kernel(const Int8GemmA
 #pragma unroll
   for (int h = 0; h < 2; ++h) place[h] = ((h * 4 + g) ^ (r16 & 7)) * 16;
   const int a_at = (wm * TM * 16 + r16) * kInt8Step;
-  const int b_at = (BM + wn * TN * 16 + (r16 >> 2) * 4 * GJ + (r16 & 3)) * kInt8Step;
+  const int b_at = (wn * TN * 16 + (r16 >> 2) * 4 * GJ + (r16 & 3)) * kInt8Step;
 
+  i32x4 fa[2][TM], fb[2][TN];
+  auto read = [&](int h, int slot_a, int slot_b) __attribute__((always_inline)) {
+    const unsigned char* a = smem + (slot_a * KG + wk) * A_PART + a_at + place[h];
+    const unsigned char* b = smem + B_RING + (slot_b * KG + wk) * B_PART + b_at + place[h];
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) request(s);
+    for (int j = 0; j < TN; ++j) fb[h][j] = *reinterpret_cast<const i32x4*>(b + (j / GJ * GJ * 16 + j % GJ * 4) * kInt8Step);
+#pragma unroll
+    for (int t = 0; t < TM; ++t) fa[h][t] = *reinterpret_cast<const i32x4*>(a + t * 16 * kInt8Step);
+  };
+  auto multiply = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int t = 0; t < TM; ++t) acc[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[h][j], fa[h][t], acc[j][t], 0, 0, 0);
+  };
+
+  // One barrier per step, in its middle: the operands of a half step are read while the half before it is multiplied.  Behind the barrier
+  // every wavefront has read all of step s, whose places take B of step s + SB and A of step s + SA, and step s + 1 has landed:
+  // what was requested behind B of step s + 1 may still be under way.  Past the end nothing but zeros is fetched, so that the loads can
+  // be counted.
+  constexpr int UNDER_WAY = (SB - 2) * (LA + LB) + (SA > SB ? LA : 0);
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int s = 0; s < SA; ++s) {
+    if (s >= SA - SB) request(b_tag, s - (SA - SB), s - (SA - SB));
+    request(a_tag, s, s);
+  }
+  wait_loads<UNDER_WAY + LA + LB>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  read(0, 0, 0);
+  int slot_a = 0, slot_b = 0;
   for (int s = 0; s < steps; ++s) {
-    wait_loads<(STAGES - 2) * (LA + LB)>();
+    read(1, slot_a, slot_b);
+    multiply(0);
+    wait_loads<UNDER_WAY>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    request(s + STAGES - 1);                           // into the buffer that every wavefront has left; past the end it fetches zeros
-    const unsigned char* from_lds = smem + (s % STAGES) * STAGE;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      i32x4 fa[TM], fb[TN];
-#pragma unroll
-      for (int t = 0; t < TM; ++t) fa[t] = *reinterpret_cast<const i32x4*>(from_lds + a_at + t * 16 * kInt8Step + place[h]);
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int row = j / GJ * GJ * 16 + j % GJ * 4;
-        fb[j] = *reinterpret_cast<const i32x4*>(from_lds + b_at + row * kInt8Step + place[h]);
-      }
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int t = 0; t < TM; ++t) acc[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[j], fa[t], acc[j][t], 0, 0, 0);
-    }
+    const int next_a = slot_a + 1 < SA ? slot_a + 1 : 0, next_b = slot_b + 1 < SB ? slot_b + 1 : 0;
+    read(0, next_a, next_b);
+    request(b_tag, s + SB, slot_b);
+    request(a_tag, s + SA, slot_a);
+    multiply(1);
+    slot_a = next_a;
+    slot_b = next_b;
   }
   wait_loads<0>();                                     // nothing is on its way to LDS when the workgroup ends
 
-  // lane: row m of the tile, columns [c, c + 4 GJ) per group of GJ tiles
+  if constexpr (KG > 1) {                              // the parts' sums meet in LDS
+    lds_barrier();
+    i32x4* sums = reinterpret_cast<i32x4*>(smem) + wg * (TN * TM) * 64 + lane;
+    constexpr int SUMS = NW * TN * TM * 64;
+    static_assert((KG - 1) * SUMS * 16 <= KG * (SA * A_PART + SB * B_PART), "the ring holds the sums");
+    if (wk > 0) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) sums[(wk - 1) * SUMS + (j * TM + t) * 64] = acc[j][t];
+    }
+    lds_barrier();
+    if (wk > 0) return;
+#pragma unroll
+    for (int q = 0; q < KG - 1; ++q)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) acc[j][t] += sums[q * SUMS + (j * TM + t) * 64];
+  }
+
+  // lane: row m of the tile, columns [c, c + 4 GJ) per group of GJ tiles.  The factors of all of its columns are requested together
+  // (indices held inside the row): one at a time, each is a round trip, and these came to 15 us at the end of a tile.
+  float cs[EPI == kEpiAct ? 2 : 1][HN][4], add[EPI == kEpiOut ? HN : 1][4];
+  auto column = [&](int q) __attribute__((always_inline)) { return n0 + wn * HN * 16 + q / GJ * GJ * 16 + g * 4 * GJ + q % GJ * 4; };
+#pragma unroll
+  for (int q = 0; q < HN; ++q)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = column(q) + i < NO ? column(q) + i : NO - 1;
+      cs[0][q][i] = ws[at];
+      if constexpr (EPI == kEpiAct) cs[1][q][i] = ws[NO + at];
+    }
+  if constexpr (EPI == kEpiOut) {
+#pragma unroll
+    for (int q = 0; q < HN; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) add[q][i] = 0.0f;
+    if (p.bias) {
+      Elem raw[HN][4];
+#pragma unroll
+      for (int q = 0; q < HN; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[q][i] = ((const Elem*)p.bias)[column(q) + i < NO ? column(q) + i : NO - 1];
+#pragma unroll
+      for (int q = 0; q < HN; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) add[q][i] = Act::to_f32(raw[q][i]);
+    }
+  }
+  constexpr int PITCH = HN * 16 + 2;
+  const int nb = n0 + wn * HN * 16;                    // the wavefront's first column
+  unsigned char* const turn = smem + (KG - 1) * BM * BN * 4 + wg * (16 * PITCH * 2);
+  static_assert((KG - 1) * BM * BN * 4 + NW * 16 * PITCH * 2 <= SPARE, "the rings hold the rows on their way out");
+  if constexpr (EPI == kEpiOut && KG == 1)
+    if (!p.wide_out) lds_barrier();                    // nothing is on its way to LDS any more, of no wavefront
+  float as[TM];
+#pragma unroll
+  for (int t = 0; t < TM; ++t) {
+    const int r = wm * TM * 16 + t * 16 + r16, at = m0 + (r < rows ? r : 0);
+    as[t] = p.a_scale[GROUPED && p.g_row ? p.g_row[at] : at];
+  }
+  constexpr int W = GJ % 2 == 0 ? 2 : 1;               // MFMA tiles per store
 #pragma unroll
   for (int t = 0; t < TM; ++t) {
     const int r = wm * TM * 16 + t * 16 + r16;
-    if (r >= rows) continue;
-    size_t row = (size_t)(m0 + r);
-    const float as = p.a_scale[GROUPED && p.g_row ? (size_t)p.g_row[m0 + r] : row];
+    const size_t row = (size_t)(m0 + r) * NO;
+    if (r < rows) {
 #pragma unroll
-    for (int jb = 0; jb < HN / GJ; ++jb) {
-      const int c = n0 + wn * HN * 16 + jb * GJ * 16 + g * 4 * GJ;
-#pragma unroll
-      for (int j = 0; j < GJ; ++j) {
-        const int n = c + j * 4;
+      for (int q = 0; q < HN; q += W) {
+        const int n = column(q);
         if (n >= NO) continue;
-        float v[4];
+        float v[W * 4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = n + i < NO ? n + i : NO - 1;
-          v[i] = (float)acc[jb * GJ + j][t][i] * (as * ws[at]);   // the sum times a large row scale may pass fp32
-          if constexpr (EPI == kEpiAct) v[i] = silu_mul(v[i], (float)acc[HN + jb * GJ + j][t][i] * (as * ws[NO + at]));
-          if constexpr (EPI == kEpiOut)
-            if (p.bias) v[i] += Act::to_f32(((const Elem*)p.bias)[at]);
+        for (int i = 0; i < W * 4; ++i) {              // the sum times a large row scale may pass fp32: the factors first
+          const int u = q + i / 4;
+          v[i] = (float)acc[u][t][i & 3] * (as[t] * cs[0][u][i & 3]);
+          if constexpr (EPI == kEpiAct) v[i] = silu_mul(v[i], (float)acc[HN + u][t][i & 3] * (as[t] * cs[1][u][i & 3]));
+          if constexpr (EPI == kEpiOut) v[i] += add[u][i & 3];
         }
         if constexpr (EPI == kEpiOut) {
-          Elem* o = (Elem*)p.out + row * NO + n;
-          if (p.wide_out) {
-            typedef __attribute__((ext_vector_type(4))) Elem v4;
-            *reinterpret_cast<v4*>(o) = v4{Act::from_f32(v[0]), Act::from_f32(v[1]), Act::from_f32(v[2]), Act::from_f32(v[3])};
-          } else {
+          typedef __attribute__((ext_vector_type(W * 4))) Elem VW;
+          Elem* o = (Elem*)p.out + row + n;
+          VW x;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (n + i < NO) o[i] = Act::from_f32(v[i]);
+          for (int i = 0; i < W * 4; ++i) x[i] = Act::from_f32(v[i]);
+          if (p.wide_out) {                            // N a multiple of 8, out on a 16-byte boundary
+            *reinterpret_cast<VW*>(o) = x;
+          } else {
+            PairOf<Elem>* to = reinterpret_cast<PairOf<Elem>*>(turn + (r16 * PITCH + n - nb) * 2);
+#pragma unroll
+            for (int i = 0; i < W * 2; ++i) to[i] = PairOf<Elem>{x[2 * i], x[2 * i + 1]};
           }
-        } else {
-          *reinterpret_cast<f32v4*>((float*)p.out + row * NO + n) = f32v4{v[0], v[1], v[2], v[3]};   // NO % 4 == 0
+        } else {                                       // NO a multiple of 16
+          f32v4* o = reinterpret_cast<f32v4*>((float*)p.out + row + n);
+#pragma unroll
+          for (int u = 0; u < W; ++u) o[u] = f32v4{v[u * 4], v[u * 4 + 1], v[u * 4 + 2], v[u * 4 + 3]};
+        }
+      }
+    }
+    if constexpr (EPI == kEpiOut) {
+      // Rows that start anywhere: through LDS, so that the lanes store a row's columns side by side, two to an aligned word.  Column by
+      // column from the registers, 1000 x 2048 x 12289 took 60 us, N = 12288 33.
+      if (!p.wide_out) {
+        constexpr int PER = HN * 8, RP = 64 / PER;     // lanes per row, rows at a time
+        const int valid = N - nb < HN * 16 ? N - nb : HN * 16, j = lane % PER;
+#pragma unroll
+        for (int r0 = 0; r0 < 16; r0 += RP) {
+          const int rr = r0 + lane / PER, at = wm * TM * 16 + t * 16 + rr;
+          if (lane / PER >= RP || rr >= 16 || at >= rows) continue;
+          Elem* o = (Elem*)p.out + (size_t)(m0 + at) * N + nb;
+          const Elem* s = reinterpret_cast<const Elem*>(turn) + rr * PITCH;
+          const int odd = (int)((uintptr_t)o >> 1 & 1), c = 2 * j + odd;
+          if (odd && j == 0 && valid > 0) o[0] = s[0];
+          if (c + 1 < valid) *reinterpret_cast<PairOf<Elem>*>(o + c) = PairOf<Elem>{s[c], s[c + 1]};
+          else if (c < valid) o[c] = s[c];
         }
       }
     }

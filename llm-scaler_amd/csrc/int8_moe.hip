@@ -114,8 +114,8 @@ static int launch_grouped(Int8GemmArgs p, long long tiles, hipStream_t st) {
   p.tiles_m = (int)tiles;
   p.tiles_n = EPI == kEpiAct ? (p.N / 2 + BN / 2 - 1) / (BN / 2) : (p.N + BN - 1) / BN;
   if (tiles * p.tiles_n > 0x7FFFFFFFLL) return MI_ERR_SHAPE;
-  auto* kernel = int8_gemm_kernel<Act, BM, BN, 2, 2, 2, EPI, true>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * p.tiles_n)), dim3(256), 2 * (BM + BN) * kInt8Step, st, p);
+  auto* kernel = int8_gemm_kernel<Act, BM, BN, 2, 2, 1, 2, 2, EPI, true>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * p.tiles_n)), dim3(256), int8_gemm_lds(BM, BN, 4, 1, 2, 2), st, p);
   return launch_status();
 }
 
