@@ -55,7 +55,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   constexpr int A_PART = BM * kInt8Step, B_PART = BN * kInt8Step, B_RING = SA * KG * A_PART;   // the ring of A, that of B
   constexpr int SPARE = B_RING + SB * KG * B_PART;    // and 1 KiB that a load lands in which a wavefront has over
   static_assert(SB >= 2 && (SA == SB || SA == SB + 1), "rings");
-  static_assert(TM * 16 * WM == BM && TN * 16 * WN == BN, "tile");
+  static_assert((!GROUPED || TM <= 5) && TM * 16 * WM == BM && TN * 16 * WN == BN, "tile");
   static_assert(HN * (EPI == kEpiAct ? 2 : 1) == TN && HN % GJ == 0, "columns");
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
 
@@ -68,20 +68,22 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   int tm, tn, m0, rows;
   const int8_t* w = p.w;
   const float* ws = p.w_scale;
+  // workgroups go to the 8 XCDs in turn: each takes a run of tiles
+  const int xcd = blockIdx.x & 7, nth = blockIdx.x >> 3;
   if constexpr (GROUPED) {
-    tm = blockIdx.x / p.tiles_n;
-    tn = blockIdx.x - tm * p.tiles_n;
-    if (tm >= p.g_tile[4 * p.tiles_m]) return;
+    const int total = p.g_tile[4 * p.tiles_m] * p.tiles_n, per = (total + 7) / 8, id = xcd * per + nth;
+    if (nth >= per || id >= total) return;
+    tm = id / p.tiles_n;                               // the tiles of a row tile share its rows
+    tn = id - tm * p.tiles_n;
     const int e = p.g_tile[4 * tm];
     m0 = p.g_tile[4 * tm + 1];
     rows = p.g_tile[4 * tm + 2];
     w = e == p.E ? p.shared_w : p.w + (size_t)e * N * K;
     ws = e == p.E ? p.shared_scale : p.w_scale + (size_t)e * N;
   } else {
-    // workgroups go to the 8 XCDs in turn: each takes a run of tiles, in bands of 8 row tiles that share the weights' tile
-    const int total = p.tiles_m * p.tiles_n, per = (total + 7) / 8;
-    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (id >= total || (int)(blockIdx.x >> 3) >= per) return;
+    // in bands of 8 row tiles that share the weights' tile
+    const int total = p.tiles_m * p.tiles_n, per = (total + 7) / 8, id = xcd * per + nth;
+    if (nth >= per || id >= total) return;
     const int band = id / (8 * p.tiles_n), in = id - band * 8 * p.tiles_n;
     const int high = p.tiles_m - band * 8 < 8 ? p.tiles_m - band * 8 : 8;
     tn = in / high;
@@ -152,23 +154,23 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   int place[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) place[h] = ((h * 4 + g) ^ (r16 & 7)) * 16;
-  const int a_at = (wm * TM * 16 + r16) * kInt8Step;
+  const int a_at = (wm * 16 + r16) * kInt8Step;       // row tile t of the wavefront: row tile t WM + wm of the workgroup
   const int b_at = (wn * TN * 16 + (r16 >> 2) * 4 * GJ + (r16 & 3)) * kInt8Step;
 
   i32x4 fa[2][TM], fb[2][TN];
-  auto read = [&](int h, int slot_a, int slot_b) __attribute__((always_inline)) {
+  auto read = [&](auto live, int h, int slot_a, int slot_b) __attribute__((always_inline)) {
     const unsigned char* a = smem + (slot_a * KG + wk) * A_PART + a_at + place[h];
     const unsigned char* b = smem + B_RING + (slot_b * KG + wk) * B_PART + b_at + place[h];
 #pragma unroll
     for (int j = 0; j < TN; ++j) fb[h][j] = *reinterpret_cast<const i32x4*>(b + (j / GJ * GJ * 16 + j % GJ * 4) * kInt8Step);
 #pragma unroll
-    for (int t = 0; t < TM; ++t) fa[h][t] = *reinterpret_cast<const i32x4*>(a + t * 16 * kInt8Step);
+    for (int t = 0; t < decltype(live)::value; ++t) fa[h][t] = *reinterpret_cast<const i32x4*>(a + t * WM * 16 * kInt8Step);
   };
-  auto multiply = [&](int h) __attribute__((always_inline)) {
+  auto multiply = [&](auto live, int h) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int t = 0; t < TM; ++t) acc[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[h][j], fa[h][t], acc[j][t], 0, 0, 0);
+      for (int t = 0; t < decltype(live)::value; ++t) acc[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[h][j], fa[h][t], acc[j][t], 0, 0, 0);
   };
 
   // One barrier per step, in its middle: the operands of a half step are read while the half before it is multiplied.  Behind the barrier
@@ -185,21 +187,33 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   wait_loads<UNDER_WAY + LA + LB>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  read(0, 0, 0);
-  int slot_a = 0, slot_b = 0;
-  for (int s = 0; s < steps; ++s) {
-    read(1, slot_a, slot_b);
-    multiply(0);
-    wait_loads<UNDER_WAY>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    const int next_a = slot_a + 1 < SA ? slot_a + 1 : 0, next_b = slot_b + 1 < SB ? slot_b + 1 : 0;
-    read(0, next_a, next_b);
-    request(b_tag, s + SB, slot_b);
-    request(a_tag, s + SA, slot_a);
-    multiply(1);
-    slot_a = next_a;
-    slot_b = next_b;
+  auto run = [&](auto live) __attribute__((always_inline)) {
+    read(live, 0, 0, 0);
+    int slot_a = 0, slot_b = 0;
+    for (int s = 0; s < steps; ++s) {
+      read(live, 1, slot_a, slot_b);
+      multiply(live, 0);
+      wait_loads<UNDER_WAY>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      const int next_a = slot_a + 1 < SA ? slot_a + 1 : 0, next_b = slot_b + 1 < SB ? slot_b + 1 : 0;
+      read(live, 0, next_a, next_b);
+      request(b_tag, s + SB, slot_b);
+      request(a_tag, s + SA, slot_a);
+      multiply(live, 1);
+      slot_a = next_a;
+      slot_b = next_b;
+    }
+  };
+  if constexpr (GROUPED && TM > 1) {                   // an expert's last tile is hardly ever full: only row tiles with rows are multiplied
+    const int live = ((rows + 15) / 16 - wm + WM - 1) / WM;
+    if (live >= TM) run(std::integral_constant<int, TM>{});
+    else if (TM > 4 && live == 4) run(std::integral_constant<int, (TM > 4 ? 4 : 1)>{});
+    else if (TM > 3 && live == 3) run(std::integral_constant<int, (TM > 3 ? 3 : 1)>{});
+    else if (TM > 2 && live == 2) run(std::integral_constant<int, (TM > 2 ? 2 : 1)>{});
+    else run(std::integral_constant<int, 1>{});
+  } else {
+    run(std::integral_constant<int, TM>{});
   }
   wait_loads<0>();                                     // nothing is on its way to LDS when the workgroup ends
 
@@ -262,13 +276,13 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   float as[TM];
 #pragma unroll
   for (int t = 0; t < TM; ++t) {
-    const int r = wm * TM * 16 + t * 16 + r16, at = m0 + (r < rows ? r : 0);
+    const int r = (t * WM + wm) * 16 + r16, at = m0 + (r < rows ? r : 0);
     as[t] = p.a_scale[GROUPED && p.g_row ? p.g_row[at] : at];
   }
   constexpr int W = GJ % 2 == 0 ? 2 : 1;               // MFMA tiles per store
 #pragma unroll
   for (int t = 0; t < TM; ++t) {
-    const int r = wm * TM * 16 + t * 16 + r16;
+    const int r = (t * WM + wm) * 16 + r16;
     const size_t row = (size_t)(m0 + r) * NO;
     if (r < rows) {
 #pragma unroll
@@ -311,7 +325,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
         const int valid = N - nb < HN * 16 ? N - nb : HN * 16, j = lane % PER;
 #pragma unroll
         for (int r0 = 0; r0 < 16; r0 += RP) {
-          const int rr = r0 + lane / PER, at = wm * TM * 16 + t * 16 + rr;
+          const int rr = r0 + lane / PER, at = (t * WM + wm) * 16 + rr;
           if (lane / PER >= RP || rr >= 16 || at >= rows) continue;
           Elem* o = (Elem*)p.out + (size_t)(m0 + at) * N + nb;
           const Elem* s = reinterpret_cast<const Elem*>(turn) + rr * PITCH;

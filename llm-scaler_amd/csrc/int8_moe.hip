@@ -8,6 +8,7 @@
 // Selection, codes of x, pairs sorted by expert, a tile table, the grouped product with SiLU(gate) x up, codes of h, the grouped down product
 // and the weighted sum.  The shared expert is one more expert, with a row for every token.
 #include "int8_gemm.hpp"
+#include "int8_moe.hpp"
 #include "../../include/mi355x_qlinear.h"
 
 namespace qlin {
@@ -108,15 +109,28 @@ static MoeLayout moe_layout(int T, int k, int E, int H, int I, int shared) {
   return l;
 }
 
-template <class Act, int EPI>
-static int launch_grouped(Int8GemmArgs p, long long tiles, hipStream_t st) {
-  constexpr int BM = kGroupRows, BN = 128;
+template <class Act, int EPI, int BM, int BN, int WM, int WN, int KG, int SA, int SB>
+static int launch_tiles(Int8GemmArgs p, long long tiles, hipStream_t st) {
+  constexpr int BNO = EPI == kEpiAct ? BN / 2 : BN;
+  const int NO = EPI == kEpiAct ? p.N / 2 : p.N;
   p.tiles_m = (int)tiles;
-  p.tiles_n = EPI == kEpiAct ? (p.N / 2 + BN / 2 - 1) / (BN / 2) : (p.N + BN - 1) / BN;
-  if (tiles * p.tiles_n > 0x7FFFFFFFLL) return MI_ERR_SHAPE;
-  auto* kernel = int8_gemm_kernel<Act, BM, BN, 2, 2, 1, 2, 2, EPI, true>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * p.tiles_n)), dim3(256), int8_gemm_lds(BM, BN, 4, 1, 2, 2), st, p);
+  p.tiles_n = (NO + BNO - 1) / BNO;
+  const long long grid = (tiles * p.tiles_n + 7) / 8 * 8;
+  if (grid > 0x7FFFFFFFLL) return MI_ERR_SHAPE;
+  auto* kernel = int8_gemm_kernel<Act, BM, BN, WM, WN, KG, SA, SB, EPI, true>;
+  constexpr size_t lds = int8_gemm_lds(BM, BN, WM * WN, KG, SA, SB);
+  if constexpr (lds > 64 * 1024) {
+    static std::atomic<unsigned long long> raised{0};
+    const int rc = int8_raise_lds(kernel, raised, lds);
+    if (rc != MI_OK) return rc;
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * WM * WN * KG), lds, st, p);
   return launch_status();
+}
+
+template <class Act, int EPI>
+static int launch_grouped(const Int8GemmArgs& p, long long tiles, hipStream_t st) {
+  return launch_tiles<Act, EPI, kGroupRows, 128, 2, 2, 1, 2, 2>(p, tiles, st);
 }
 
 static bool moe_sizes(int T, int k, int E, int H, int I) {
@@ -127,15 +141,15 @@ static bool moe_sizes(int T, int k, int E, int H, int I) {
 }
 
 template <class Act>
-static int run_moe(const void* x, const void* logits, void* out, const void* w13, const float* s13, const void* shared_w13,
-                   const float* shared_s13, const void* w2, const float* s2, const void* shared_w2, const float* shared_s2,
-                   const void* gate_weight, char* ws, int T, int k, int E, int H, int I, hipStream_t st) {
-  const bool shared = shared_w13 != nullptr;
+static int run_moe(const Int8MoeArgs& m, char* ws, hipStream_t st) {
+  const int T = m.T, k = m.k, E = m.E, H = m.H, I = m.I;
+  const void *x = m.x, *logits = m.logits;
+  const bool shared = m.shared_w13 != nullptr;
   const MoeLayout l = moe_layout(T, k, E, H, I, shared);
   int32_t *ids = (int32_t*)(ws + l.ids), *start = (int32_t*)(ws + l.start), *inv = (int32_t*)(ws + l.inv), *row = (int32_t*)(ws + l.row);
   int32_t* tile = (int32_t*)(ws + l.tile);
   float* gate = shared ? (float*)(ws + l.gate) : nullptr;
-  int rc = mi_moe_topk(logits, ws + l.top_w, ids, T, E, k, 1, nullptr, shared ? x : nullptr, gate_weight, gate, H, Act::dt, st);
+  int rc = mi_moe_topk(logits, ws + l.top_w, ids, T, E, k, 1, nullptr, shared ? x : nullptr, m.gate_weight, gate, H, Act::dt, st);
   if (rc != MI_OK) return rc;
   QuantArgs q{};
   q.x = x;
@@ -152,16 +166,16 @@ static int run_moe(const void* x, const void* logits, void* out, const void* w13
   Int8GemmArgs p{};
   p.a = q.q;
   p.a_scale = q.scale;
-  p.w = (const int8_t*)w13;
-  p.w_scale = s13;
+  p.w = m.w13;
+  p.w_scale = m.s13;
   p.out = ws + l.h;
   p.M = T;
   p.N = 2 * I;
   p.K = H;
   p.g_tile = tile;
   p.g_row = row;
-  p.shared_w = (const int8_t*)shared_w13;
-  p.shared_scale = shared_s13;
+  p.shared_w = m.shared_w13;
+  p.shared_scale = m.shared_s13;
   p.E = E;
   rc = launch_grouped<Act, kEpiAct>(p, l.tiles, st);
   if (rc != MI_OK) return rc;
@@ -174,19 +188,19 @@ static int run_moe(const void* x, const void* logits, void* out, const void* w13
   if (rc != MI_OK) return rc;
   p.a = q.q;
   p.a_scale = q.scale;
-  p.w = (const int8_t*)w2;
-  p.w_scale = s2;
+  p.w = m.w2;
+  p.w_scale = m.s2;
   p.out = ws + l.y;
   p.M = (int)l.rows;
   p.N = H;
   p.K = I;
   p.g_row = nullptr;
-  p.shared_w = (const int8_t*)shared_w2;
-  p.shared_scale = shared_s2;
+  p.shared_w = m.shared_w2;
+  p.shared_scale = m.shared_s2;
   rc = launch_grouped<Act, kEpiF32>(p, l.tiles, st);
   if (rc != MI_OK) return rc;
   hipLaunchKernelGGL(int8_combine_kernel<Act>, dim3((unsigned)(((long long)T * (H / 8) + 255) / 256)), dim3(256), 0, st,
-                     (const float*)(ws + l.y), inv, (const typename Act::elem*)(ws + l.top_w), gate, (typename Act::elem*)out, T, k, H);
+                     (const float*)(ws + l.y), inv, (const typename Act::elem*)(ws + l.top_w), gate, (typename Act::elem*)m.out, T, k, H);
   return launch_status();
 }
 
@@ -219,10 +233,13 @@ int mi_moe_forward_full_int8_ws(const void* x, const void* logits, void* out, co
     if (!aligned16(q)) return MI_ERR_ARG;
   if (!workspace || workspace_bytes < moe_layout(T, topk, num_experts, H, I, shared).bytes) return MI_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
-  return act_dtype == DT_F16 ? run_moe<ActF16>(x, logits, out, w13, w13_scale, shared_w13, shared_w13_scale, w2, w2_scale, shared_w2,
-                                               shared_w2_scale, gate_weight, (char*)workspace, T, topk, num_experts, H, I, st)
-                             : run_moe<ActBF16>(x, logits, out, w13, w13_scale, shared_w13, shared_w13_scale, w2, w2_scale, shared_w2,
-                                                shared_w2_scale, gate_weight, (char*)workspace, T, topk, num_experts, H, I, st);
+  const MoeLayout l = moe_layout(T, topk, num_experts, H, I, shared);
+  char* ws = (char*)workspace;
+  const Int8MoeArgs m{x, logits, out, (const int8_t*)w13, (const int8_t*)w2, w13_scale, w2_scale, (const int8_t*)shared_w13,
+                      (const int8_t*)shared_w2, shared_w13_scale, shared_w2_scale, gate_weight, ws + l.top_w, (int32_t*)(ws + l.ids),
+                      (float*)(ws + l.gate), (float*)(ws + l.h), T, topk, num_experts, H, I};
+  if (int8_moe_decode_pays(T, topk, H, I, shared)) return launch_int8_moe_decode(m, act_dtype, st);
+  return act_dtype == DT_F16 ? run_moe<ActF16>(m, ws, st) : run_moe<ActBF16>(m, ws, st);
 }
 
 }  // extern "C"
