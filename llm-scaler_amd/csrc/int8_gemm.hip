@@ -12,7 +12,7 @@ static int launch_tiles(Int8GemmArgs p, hipStream_t st) {
   const long long tiles = (long long)p.tiles_m * p.tiles_n, grid = (tiles + 7) / 8 * 8;
   if (grid > 0x7FFFFFFFLL) return MI_ERR_SHAPE;
   auto* kernel = int8_gemm_kernel<Act, BM, BN, WM, WN, KG, SA, SB, kEpiOut, false>;
-  constexpr size_t lds = int8_gemm_lds(BM, BN, WM * WN, KG, SA, SB);
+  constexpr size_t lds = int8_gemm_lds(BM, BN, WM * WN, KG, SA, SB, false);
   if constexpr (lds > 64 * 1024) {
     static std::atomic<unsigned long long> raised{0};
     const int rc = int8_raise_lds(kernel, raised, lds);

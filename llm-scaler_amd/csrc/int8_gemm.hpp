@@ -20,6 +20,7 @@ struct Int8GemmArgs {
   const float* w_scale;       // [N]; grouped [E, N]
   const void* bias;           // [N] in the output's type, or null
   void* out;
+  float* block_scale;
   int M, N, K;                // M: rows of a
   int wide_out;               // eight outputs per store: N and out allow it
   int tiles_m, tiles_n;
@@ -32,14 +33,17 @@ struct Int8GemmArgs {
   int E;
 };
 
-// What becomes of the sums: 16-bit outputs with a bias; fp32 rows; SiLU(gate) x up as fp32 rows, gate = weight rows [0, N / 2).
-enum : int { kEpiOut = 0, kEpiF32 = 1, kEpiAct = 2 };
+// What becomes of the sums: 16-bit outputs with a bias; rows of 16-bit integers with an fp32 scale for each wavefront's columns (out,
+// block_scale [rows, ceil(N / block)]: what another launch adds up, off by 2^-16 of the largest of 32 to 96 values, at half the
+// bytes of fp32); SiLU(gate) x up as fp32 rows, gate = weight rows [0, N / 2).
+enum : int { kEpiOut = 0, kEpiBlock = 1, kEpiAct = 2 };
 
 constexpr int kInt8Step = 128;                        // bytes of a row per step
 
-// LDS of a tile: the rings and, where the tile's rows do not divide among the wavefronts, the place of the loads that are over.
-constexpr size_t int8_gemm_lds(int BM, int BN, int NW, int KG, int SA, int SB) {
-  return (size_t)KG * (SA * BM + SB * BN) * kInt8Step + (BM % (8 * NW) || BN % (8 * NW) ? 1024 : 0);
+// LDS of a tile: the rings and, where the tile's rows do not divide among the wavefronts that load them, the place of the loads that are over.
+constexpr size_t int8_gemm_lds(int BM, int BN, int NW, int KG, int SA, int SB, bool grouped) {
+  const int loaders = grouped && NW % 2 == 0 ? NW / 2 : NW;
+  return (size_t)KG * (SA * BM + SB * BN) * kInt8Step + (BM % (8 * loaders) || BN % (8 * loaders) ? 1024 : 0);
 }
 
 template <class Elem>
@@ -49,12 +53,18 @@ template <class Act, int BM, int BN, int WM, int WN, int KG, int SA, int SB, int
 __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8GemmArgs p) {
   using Elem = typename Act::elem;
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr int LA = (BM / 8 + NW - 1) / NW, LB = (BN / 8 + NW - 1) / NW;       // 1 KiB loads of a wavefront per step
+  // 1 KiB loads of a wavefront per step.  Grouped: half of the wavefronts load A, half B.  Loads are waited for in the order of their requests,
+  // so a wavefront that loads both can have hardly more of one under way than of the other; an expert's weights come from HBM for few
+  // rows and take the deeper ring (128 experts, 4096 tokens, top 8, 2048 / 768: 193 + 166 us with both, 160 + 141 like this; dense
+  // products, whose operands are in L2 half of the time: 0 to 3 % slower).
+  constexpr bool ROLES = GROUPED && NW % 2 == 0;
+  constexpr int NL = ROLES ? NW / 2 : NW, LA = (BM / 8 + NL - 1) / NL, LB = (BN / 8 + NL - 1) / NL;
   constexpr int HN = EPI == kEpiAct ? TN / 2 : TN;    // MFMA tiles of gate (or all) columns
-  constexpr int GJ = HN % 4 == 0 ? 4 : HN % 2 == 0 ? 2 : HN;
+  // columns in a row per lane: a store instruction writes 64 bytes of 16 rows then (with 4 tiles in a row, half sectors: 85 us for 302 MB)
+  constexpr int GJ = EPI != kEpiAct && HN % 2 == 0 ? 2 : 1;
   constexpr int A_PART = BM * kInt8Step, B_PART = BN * kInt8Step, B_RING = SA * KG * A_PART;   // the ring of A, that of B
   constexpr int SPARE = B_RING + SB * KG * B_PART;    // and 1 KiB that a load lands in which a wavefront has over
-  static_assert(SB >= 2 && (SA == SB || SA == SB + 1), "rings");
+  static_assert(SA >= 2 && SB >= 2 && (ROLES || SA == SB || SA == SB + 1), "rings");
   static_assert((!GROUPED || TM <= 5) && TM * 16 * WM == BM && TN * 16 * WN == BN, "tile");
   static_assert(HN * (EPI == kEpiAct ? 2 : 1) == TN && HN % GJ == 0, "columns");
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -68,20 +78,19 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   int tm, tn, m0, rows;
   const int8_t* w = p.w;
   const float* ws = p.w_scale;
-  // workgroups go to the 8 XCDs in turn: each takes a run of tiles
+  // workgroups go to the 8 XCDs in turn
   const int xcd = blockIdx.x & 7, nth = blockIdx.x >> 3;
   if constexpr (GROUPED) {
-    const int total = p.g_tile[4 * p.tiles_m] * p.tiles_n, per = (total + 7) / 8, id = xcd * per + nth;
-    if (nth >= per || id >= total) return;
-    tm = id / p.tiles_n;                               // the tiles of a row tile share its rows
-    tn = id - tm * p.tiles_n;
+    tm = nth / p.tiles_n * 8 + xcd;                    // every 8th row tile to an XCD: its column tiles share its rows
+    tn = nth % p.tiles_n;
+    if (tm >= p.tiles_m || tm >= p.g_tile[4 * p.tiles_m]) return;
     const int e = p.g_tile[4 * tm];
     m0 = p.g_tile[4 * tm + 1];
     rows = p.g_tile[4 * tm + 2];
     w = e == p.E ? p.shared_w : p.w + (size_t)e * N * K;
     ws = e == p.E ? p.shared_scale : p.w_scale + (size_t)e * N;
   } else {
-    // in bands of 8 row tiles that share the weights' tile
+    // a run of tiles each, in bands of 8 row tiles that share the weights' tile
     const int total = p.tiles_m * p.tiles_n, per = (total + 7) / 8, id = xcd * per + nth;
     if (nth >= per || id >= total) return;
     const int band = id / (8 * p.tiles_n), in = id - band * 8 * p.tiles_n;
@@ -94,31 +103,38 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   const int n0 = tn * BNO;
 
   // where this lane's 16 bytes of each load come from
-  uint32_t from[LA + LB];
-  int chunk[LA + LB];
+  const int wl = wg % NL;
+  const bool loads_a = !ROLES || wg < NL, loads_b = !ROLES || wg >= NL;
+  constexpr int FIRST_B = ROLES ? 0 : LA, LOADS = ROLES ? (LA > LB ? LA : LB) : LA + LB;
+  uint32_t from[LOADS];
+  int chunk[LOADS];
+  if (loads_a) {
 #pragma unroll
-  for (int i = 0; i < LA; ++i) {
-    const int r = (wg * LA + i) * 8 + (lane >> 3);
-    chunk[i] = wk * kInt8Step + ((lane & 7) ^ (r & 7)) * 16;
-    uint32_t row = (uint32_t)r;
-    if constexpr (GROUPED) {
-      const int at = m0 + (r < rows ? r : 0);
-      row = (uint32_t)(p.g_row ? p.g_row[at] : at);
+    for (int i = 0; i < LA; ++i) {
+      const int r = (wl * LA + i) * 8 + (lane >> 3);
+      chunk[i] = wk * kInt8Step + ((lane & 7) ^ (r & 7)) * 16;
+      uint32_t row = (uint32_t)r;
+      if constexpr (GROUPED) {
+        const int at = m0 + (r < rows ? r : 0);
+        row = (uint32_t)(p.g_row ? p.g_row[at] : at);
+      }
+      from[i] = r < rows ? row * (uint32_t)K + chunk[i] : kOOB;
     }
-    from[i] = r < rows ? row * (uint32_t)K + chunk[i] : kOOB;
   }
+  if (loads_b) {
 #pragma unroll
-  for (int i = 0; i < LB; ++i) {
-    const int r = (wg * LB + i) * 8 + (lane >> 3);
-    chunk[LA + i] = wk * kInt8Step + ((lane & 7) ^ ((r & 3) | ((r / (4 * GJ)) & 1) << 2)) * 16;
-    int row = r;
-    bool in = n0 + r < N;
-    if constexpr (EPI == kEpiAct) {
-      const int q = r % (TN * 16), col = r / (TN * 16) * (TN * 8) + q % (TN * 8);
-      in = n0 + col < NO;
-      row = q < TN * 8 ? col : NO + col;
+    for (int i = 0; i < LB; ++i) {
+      const int r = (wl * LB + i) * 8 + (lane >> 3);
+      chunk[FIRST_B + i] = wk * kInt8Step + ((lane & 7) ^ ((r & 3) | ((r / (4 * GJ)) & 1) << 2)) * 16;
+      int row = r;
+      bool in = n0 + r < N;
+      if constexpr (EPI == kEpiAct) {
+        const int q = r % (TN * 16), col = r / (TN * 16) * (TN * 8) + q % (TN * 8);
+        in = n0 + col < NO;
+        row = q < TN * 8 ? col : NO + col;
+      }
+      from[FIRST_B + i] = in && r < BN ? (uint32_t)row * (uint32_t)K + chunk[FIRST_B + i] : kOOB;
     }
-    from[LA + i] = in && r < BN ? (uint32_t)row * (uint32_t)K + chunk[LA + i] : kOOB;
   }
   const int8_t* a0 = GROUPED ? p.a : p.a + (size_t)m0 * K;
   const unsigned long long a_bytes = (unsigned long long)(GROUPED ? p.M : rows) * K, w_bytes = (unsigned long long)(N - n0) * K;
@@ -129,15 +145,16 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   const int steps = (K + STEP - 1) / STEP;
   auto request = [&](auto is_a, int s, int slot) __attribute__((always_inline)) {
     constexpr bool A = decltype(is_a)::value;
-    constexpr int COUNT = A ? LA : LB, FIRST = A ? 0 : LA;
-    constexpr bool EVEN = A ? LA * NW * 8 == BM : LB * NW * 8 == BN;
-    const int to = A ? (slot * KG + wk) * A_PART + wg * LA * 1024 : B_RING + (slot * KG + wk) * B_PART + wg * LB * 1024;
+    constexpr int COUNT = A ? LA : LB, FIRST = A ? 0 : FIRST_B;
+    constexpr bool EVEN = COUNT * NL * 8 == (A ? BM : BN);
+    if (!(A ? loads_a : loads_b)) return;
+    const int to = A ? (slot * KG + wk) * A_PART + wl * LA * 1024 : B_RING + (slot * KG + wk) * B_PART + wl * LB * 1024;
     const int k0 = s * STEP;
     const bool whole = k0 + STEP <= K;
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
       const uint32_t f = whole || k0 + chunk[FIRST + i] < K ? from[FIRST + i] : kOOB;   // past the row's end: zeros
-      const int at = EVEN || (wg * COUNT + i) * 8 < (A ? BM : BN) ? to + i * 1024 : SPARE;
+      const int at = EVEN || (wl * COUNT + i) * 8 < (A ? BM : BN) ? to + i * 1024 : SPARE;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(A ? ra : rb, (lds_ptr)(smem + at), 16, f, k0, 0, 0);
     }
   };
@@ -174,17 +191,21 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   };
 
   // One barrier per step, in its middle: the operands of a half step are read while the half before it is multiplied.  Behind the barrier
-  // every wavefront has read all of step s, whose places take B of step s + SB and A of step s + SA, and step s + 1 has landed:
-  // what was requested behind B of step s + 1 may still be under way.  Past the end nothing but zeros is fetched, so that the loads can
-  // be counted.
-  constexpr int UNDER_WAY = (SB - 2) * (LA + LB) + (SA > SB ? LA : 0);
+  // every wavefront has read all of step s, whose places take B of step s + SB and A of step s + SA, and step s + 1 has landed.  Past
+  // the end nothing but zeros is fetched, so that the loads can be counted.
+  auto wait_step = [&](auto older) __attribute__((always_inline)) {            // steps behind the one that is needed: requested, not waited for
+    constexpr int O = decltype(older)::value;
+    if constexpr (!ROLES) wait_loads<(SB - 2 + O) * (LA + LB) + (SA > SB ? LA : 0)>();           // B's goes out before A's
+    else if (loads_a) wait_loads<(SA - 2 + O) * LA>();
+    else wait_loads<(SB - 2 + O) * LB>();
+  };
   asm volatile("" ::: "memory");
 #pragma unroll
-  for (int s = 0; s < SA; ++s) {
+  for (int s = SB > SA ? SA - SB : 0; s < SA; ++s) {
     if (s >= SA - SB) request(b_tag, s - (SA - SB), s - (SA - SB));
-    request(a_tag, s, s);
+    if (s >= 0) request(a_tag, s, s);
   }
-  wait_loads<UNDER_WAY + LA + LB>();
+  wait_step(std::integral_constant<int, 1>{});
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   auto run = [&](auto live) __attribute__((always_inline)) {
@@ -193,7 +214,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
     for (int s = 0; s < steps; ++s) {
       read(live, 1, slot_a, slot_b);
       multiply(live, 0);
-      wait_loads<UNDER_WAY>();
+      wait_step(std::integral_constant<int, 0>{});
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       const int next_a = slot_a + 1 < SA ? slot_a + 1 : 0, next_b = slot_b + 1 < SB ? slot_b + 1 : 0;
@@ -279,11 +300,25 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
     const int r = (t * WM + wm) * 16 + r16, at = m0 + (r < rows ? r : 0);
     as[t] = p.a_scale[GROUPED && p.g_row ? p.g_row[at] : at];
   }
-  constexpr int W = GJ % 2 == 0 ? 2 : 1;               // MFMA tiles per store
+  constexpr int W = GJ;                                // MFMA tiles per store
 #pragma unroll
   for (int t = 0; t < TM; ++t) {
     const int r = (t * WM + wm) * 16 + r16;
     const size_t row = (size_t)(m0 + r) * NO;
+    float to_code = 0.0f;
+    if constexpr (EPI == kEpiBlock) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int q = 0; q < HN; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = umax32(top, column(q) < NO ? abs_bits((float)acc[q][t][i] * (as[t] * cs[0][q][i])) : 0u);
+      top = umax32(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+      top = umax32(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+      const float m = __builtin_bit_cast(float, top);
+      const bool bad = top >= 0x7F800000u;             // a NaN, or past fp32
+      to_code = bad || m < 0x1p-100f ? 0.0f : 32767.0f / m;
+      if (g == 0 && r < rows && nb < NO) p.block_scale[(size_t)(m0 + r) * ((NO + HN * 16 - 1) / (HN * 16)) + nb / (HN * 16)] = bad ? __builtin_nanf("") : m / 32767.0f;
+    }
     if (r < rows) {
 #pragma unroll
       for (int q = 0; q < HN; q += W) {
@@ -310,10 +345,14 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
 #pragma unroll
             for (int i = 0; i < W * 2; ++i) to[i] = PairOf<Elem>{x[2 * i], x[2 * i + 1]};
           }
-        } else {                                       // NO a multiple of 16
-          f32v4* o = reinterpret_cast<f32v4*>((float*)p.out + row + n);
+        } else if constexpr (EPI == kEpiBlock) {       // NO a multiple of 16
+          typedef __attribute__((ext_vector_type(W * 4))) short SW;
+          SW x;
 #pragma unroll
-          for (int u = 0; u < W; ++u) o[u] = f32v4{v[u * 4], v[u * 4 + 1], v[u * 4 + 2], v[u * 4 + 3]};
+          for (int i = 0; i < W * 4; ++i) x[i] = (short)(int)__builtin_rintf(to_code == 0.0f ? 0.0f : v[i] * to_code);
+          *reinterpret_cast<SW*>((short*)p.out + row + n) = x;
+        } else {
+          *reinterpret_cast<f32v4*>((float*)p.out + row + n) = f32v4{v[0], v[1], v[2], v[3]};
         }
       }
     }

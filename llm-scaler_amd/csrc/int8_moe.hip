@@ -3,75 +3,155 @@
 //   out[t] = sum_j top_w[t][j] expert(ids[t][j], x[t]) + sigmoid(x[t] . gate_weight) shared(x[t]),
 //   expert(e, x) = W2[e] q(h),   h = SiLU(g) u,   (g, u) = W13[e] q(x)
 //
-// with q() the rows' quantisation of int8_common.hpp; g, u, h and the experts' results stay in fp32, the output is rounded once.
+// with q() the rows' quantisation of int8_common.hpp; g, u, h and the sums stay in fp32, the output is rounded once.
 //
 // Selection, codes of x, pairs sorted by expert, a tile table, the grouped product with SiLU(gate) x up, codes of h, the grouped down product
 // and the weighted sum.  The shared expert is one more expert, with a row for every token.
 #include "int8_gemm.hpp"
 #include "int8_moe.hpp"
+#include "int8_quant.hpp"
+#include "moe_topk.hpp"
 #include "../../include/mi355x_qlinear.h"
 
 namespace qlin {
 
-constexpr int kTileThreads = 1024;
+constexpr int kSortThreads = 1024;                    // E <= kSortThreads
+constexpr int kSortPairs = 8;                         // pairs per thread of int8_sort_kernel
 
-// Tiles of `bm` rows that cover each expert's rows (expert E: the T rows behind the P sorted pairs), and the row of x of every position.
-__global__ __launch_bounds__(kTileThreads) void int8_tiles_kernel(const int32_t* __restrict__ start, int32_t* __restrict__ tile,
-                                                                  int32_t* __restrict__ row, int E, int P, int T, int bm, int most) {
-  __shared__ int32_t total[kTileThreads / 64];
+// Tiles of at most `bm` rows that cover the `n` rows of every expert (thread = expert) from its first position on, and those of the
+// shared expert (E): the T rows behind the P sorted pairs.  Returns the expert's first position.  A workgroup of kSortThreads.
+__device__ __forceinline__ int write_tiles(int n, int32_t* __restrict__ tile, int32_t* __restrict__ row, int E, int P, int T, int bm, int most) {
+  __shared__ int32_t totals[2][kSortThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int first = tid < E ? start[tid] : 0, n = tid < E ? start[tid + 1] - first : 0;   // E <= kTileThreads
   const int mine = (n + bm - 1) / bm;
-  int sum = mine;
+  int tiles = mine, pairs = n;                        // inclusive sums
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(sum, off, 64);
-    if (lane >= off) sum += o;
+    const int a = __shfl_up(tiles, off, 64), b = __shfl_up(pairs, off, 64);
+    if (lane >= off) { tiles += a; pairs += b; }
   }
-  if (lane == 63) total[wave] = sum;
+  if (lane == 63) { totals[0][wave] = tiles; totals[1][wave] = pairs; }
   __syncthreads();
-  int before = 0, all = 0;
+  int all = 0;
 #pragma unroll
-  for (int w = 0; w < kTileThreads / 64; ++w) {
-    if (w < wave) before += total[w];
-    all += total[w];
+  for (int w = 0; w < kSortThreads / 64; ++w) {
+    if (w < wave) { tiles += totals[0][w]; pairs += totals[1][w]; }
+    all += totals[0][w];
   }
-  const int at = before + sum - mine;
+  const int first = pairs - n;
   for (int i = 0; i < mine; ++i) {
-    int32_t* t = tile + 4 * (at + i);
+    int32_t* t = tile + 4 * (tiles - mine + i);
     t[0] = tid;
     t[1] = first + i * bm;
     t[2] = n - i * bm < bm ? n - i * bm : bm;
   }
   const int shared = (T + bm - 1) / bm;               // T = 0: no shared expert
-  for (int i = tid; i < shared; i += kTileThreads) {
+  for (int i = tid; i < shared; i += kSortThreads) {
     int32_t* t = tile + 4 * (all + i);
     t[0] = E;
     t[1] = P + i * bm;
     t[2] = T - i * bm < bm ? T - i * bm : bm;
   }
-  for (int i = tid; i < T; i += kTileThreads) row[P + i] = i;
+  for (int i = tid; i < T; i += kSortThreads) row[P + i] = i;
   if (tid == 0) tile[4 * most] = all + shared;
+  return first;
 }
 
-// out[t] = sum_j w[t][j] y[inv[t k + j]] + gate[t] y[P + t], fp32, one rounding.  Eight columns per thread.
+// After mi_moe_sort: the tiles alone.
+__global__ __launch_bounds__(kSortThreads) void int8_tiles_kernel(const int32_t* __restrict__ start, int32_t* __restrict__ tile,
+                                                                  int32_t* __restrict__ row, int E, int P, int T, int bm, int most) {
+  const int e = threadIdx.x;
+  write_tiles(e < E ? start[e + 1] - start[e] : 0, tile, row, E, P, T, bm, most);
+}
+
+// Up to kSortPairs x kSortThreads pairs: sorted by expert and tiled by one workgroup.  inv: a pair's position, row: a position's token.  The order
+// inside an expert is that of the LDS atomics; every row's result is its own, so the outputs do not depend on it.
+__global__ __launch_bounds__(kSortThreads) void int8_sort_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ inv,
+                                                                 int32_t* __restrict__ row, int32_t* __restrict__ tile, int E, int k, int P, int T,
+                                                                 int bm, int most) {
+  __shared__ int32_t count[kSortThreads];
+  const int tid = threadIdx.x;
+  count[tid] = 0;
+  __syncthreads();
+  int id[kSortPairs], rank[kSortPairs];
+#pragma unroll
+  for (int i = 0; i < kSortPairs; ++i) {
+    if (i * kSortThreads >= P) break;
+    id[i] = ids[min(i * kSortThreads + tid, P - 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < kSortPairs; ++i) {
+    if (i * kSortThreads >= P) break;
+    if (i * kSortThreads + tid < P) rank[i] = atomicAdd(&count[id[i]], 1);
+  }
+  __syncthreads();
+  const int n = count[tid];
+  const int first = write_tiles(n, tile, row, E, P, T, bm, most);              // a barrier inside: every count is read
+  count[tid] = first;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kSortPairs; ++i) {
+    const int p = i * kSortThreads + tid;
+    if (i * kSortThreads >= P) break;
+    if (p < P) {
+      const int at = count[id[i]] + rank[i];
+      inv[p] = at;
+      row[at] = p / k;
+    }
+  }
+}
+
+// Selection of a token's experts (with the shared expert's gate) and codes of its row do not depend on each other: one launch, a
+// wavefront per token for the first, workgroups behind them for the second.
+template <class Act, int SLOTS, int NV>
+__global__ __launch_bounds__(256) void int8_route_kernel(const Int8MoeArgs p, int8_t* __restrict__ q, float* __restrict__ scale, int routing) {
+  using Elem = typename Act::elem;
+  using V8 = typename Act::v8;
+  if ((int)blockIdx.x < routing) {
+    moe_topk_body<Act, SLOTS>((const Elem*)p.logits, (Elem*)p.top_w, p.ids, p.T, p.E, p.k, 1, nullptr, (const V8*)p.x, (const V8*)p.gate_weight,
+                              p.shared_w13 ? p.gate : nullptr, p.H >> 3, blockIdx.x * 4 + (threadIdx.x >> 6));
+    return;
+  }
+  QuantArgs a{};
+  a.x = p.x;
+  a.q = q;
+  a.scale = scale;
+  a.rows = p.T;
+  a.K = p.H;
+  int8_quant_rows<Act, kFromAct, 256, NV>(a, (int)blockIdx.x - routing);
+}
+
+// out[t] = sum_j w[t][j] y[inv[t k + j]] + gate[t] y[P + t], fp32, one rounding; y as kEpiBlock leaves it.  Eight columns per thread.
 template <class Act>
-__global__ __launch_bounds__(256) void int8_combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ inv,
-                                                           const typename Act::elem* __restrict__ top_w, const float* __restrict__ gate,
-                                                           typename Act::elem* __restrict__ out, int T, int k, int H) {
+__global__ __launch_bounds__(256) void int8_combine_kernel(const short* __restrict__ y, const float* __restrict__ y_scale, int block,
+                                                           const int32_t* __restrict__ inv, const typename Act::elem* __restrict__ top_w,
+                                                           const float* __restrict__ gate, typename Act::elem* __restrict__ out, int T, int k, int H) {
+  typedef __attribute__((ext_vector_type(8))) short s16x8;
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int per = H / 8;
+  const int per = H / 8, blocks = (H + block - 1) / block;
   const long long t = i / per;
   if (t >= T) return;
-  const int c = (int)(i - t * per) * 8;
+  const int c = (int)(i - t * per) * 8, b = c / block;
   float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
   auto add = [&](size_t row, float w) __attribute__((always_inline)) {
-    const f32v4* src = reinterpret_cast<const f32v4*>(y + row * H + c);
-    const f32v4 a = src[0], b = src[1];
+    const s16x8 a = *reinterpret_cast<const s16x8*>(y + row * H + c);
+    const float f = w * y_scale[row * blocks + b];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { s[j] += w * a[j]; s[4 + j] += w * b[j]; }
+    for (int j = 0; j < 8; ++j) s[j] += f * (float)a[j];
   };
-  for (int j = 0; j < k; ++j) add((size_t)inv[t * k + j], Act::to_f32(top_w[t * k + j]));
+  for (int j0 = 0; j0 < k; j0 += 8) {                  // eight rows' positions, then eight rows
+    int at[8];
+    float w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const long long p = t * k + (j0 + j < k ? j0 + j : k - 1);
+      at[j] = inv[p];
+      w[j] = Act::to_f32(top_w[p]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j0 + j < k) add((size_t)at[j], w[j]);
+  }
   if (gate) add((size_t)T * k + t, gate[t]);
   typename Act::v8 o;
 #pragma unroll
@@ -79,18 +159,35 @@ __global__ __launch_bounds__(256) void int8_combine_kernel(const float* __restri
   *reinterpret_cast<typename Act::v8*>(out + t * H + c) = o;
 }
 
-constexpr int kGroupRows = 128;
+// Rows of a tile, by the rows that an expert has on average, and the columns that share a scale (kEpiBlock) with each.  The whole layer, us,
+// tile / next: 128 experts, top 8, 2048 / 768: 200 tokens 32 x 128 147 / 64 x 128 153; 512 tokens 64 x 128 166 / 32 x 128 179; 4096 tokens 320 x 192
+// 370 / 256 x 256 376; 64 experts, top 6, 2048 / 1408: 2048 tokens 256 x 256 269 / 128 x 128 304; 8 experts, top 2, 4096 / 1536: 1024 tokens 320 x 192
+// 136 / 128 x 128 153, 4096 tokens 256 x 256 347 / 320 x 192 364.
+enum : int { kRows32, kRows64, kRows128, kRows256, kRows320 };
+struct GroupTile {
+  int rows, block;
+};
+constexpr GroupTile kGroupTiles[] = {{32, 32}, {64, 32}, {128, 64}, {256, 128}, {320, 96}};
+static int group_tile(long long pairs, int E) {
+  if (pairs <= 24LL * E) return kRows32;
+  if (pairs <= 90LL * E) return kRows64;
+  if (pairs <= 120LL * E) return kRows128;
+  return pairs <= 230LL * E || pairs > 310LL * E ? kRows256 : kRows320;        // most experts in one row tile
+}
 
 struct MoeLayout {                                    // byte offsets into the workspace
-  long long top_w, ids, gate, pairs, start, inv, row, tile, xq, xs, h, hq, hs, y, bytes;
+  long long top_w, ids, gate, pairs, start, inv, row, tile, xq, xs, h, hq, hs, y, ys, bytes;
   long long P, rows, tiles;
+  int tile_kind, bm;
 };
 static MoeLayout moe_layout(int T, int k, int E, int H, int I, int shared) {
   MoeLayout l{};
   l.P = (long long)T * k;
   const long long S = shared ? T : 0;
   l.rows = l.P + S;
-  l.tiles = l.P / kGroupRows + (l.P < E ? l.P : E) + (S + kGroupRows - 1) / kGroupRows;
+  l.tile_kind = group_tile(l.P, E);
+  l.bm = kGroupTiles[l.tile_kind].rows;
+  l.tiles = l.P / l.bm + (l.P < E ? l.P : E) + (S + l.bm - 1) / l.bm;
   auto take = [&](long long n) { const long long at = l.bytes; l.bytes += (n + 255) / 256 * 256; return at; };
   l.top_w = take(2 * l.P);
   l.ids = take(4 * l.P);
@@ -105,7 +202,8 @@ static MoeLayout moe_layout(int T, int k, int E, int H, int I, int shared) {
   l.h = take(4 * l.rows * I);
   l.hq = take(l.rows * I);
   l.hs = take(4 * l.rows);
-  l.y = take(4 * l.rows * H);
+  l.y = take(2 * l.rows * H);
+  l.ys = take(4 * l.rows * ((H + 31) / 32));
   return l;
 }
 
@@ -115,10 +213,10 @@ static int launch_tiles(Int8GemmArgs p, long long tiles, hipStream_t st) {
   const int NO = EPI == kEpiAct ? p.N / 2 : p.N;
   p.tiles_m = (int)tiles;
   p.tiles_n = (NO + BNO - 1) / BNO;
-  const long long grid = (tiles * p.tiles_n + 7) / 8 * 8;
+  const long long grid = (tiles + 7) / 8 * 8 * p.tiles_n;
   if (grid > 0x7FFFFFFFLL) return MI_ERR_SHAPE;
   auto* kernel = int8_gemm_kernel<Act, BM, BN, WM, WN, KG, SA, SB, EPI, true>;
-  constexpr size_t lds = int8_gemm_lds(BM, BN, WM * WN, KG, SA, SB);
+  constexpr size_t lds = int8_gemm_lds(BM, BN, WM * WN, KG, SA, SB, true);
   if constexpr (lds > 64 * 1024) {
     static std::atomic<unsigned long long> raised{0};
     const int rc = int8_raise_lds(kernel, raised, lds);
@@ -129,8 +227,31 @@ static int launch_tiles(Int8GemmArgs p, long long tiles, hipStream_t st) {
 }
 
 template <class Act, int EPI>
-static int launch_grouped(const Int8GemmArgs& p, long long tiles, hipStream_t st) {
-  return launch_tiles<Act, EPI, kGroupRows, 128, 2, 2, 1, 2, 2>(p, tiles, st);
+static int launch_grouped(const Int8GemmArgs& p, const MoeLayout& l, hipStream_t st) {
+  switch (l.tile_kind) {
+    case kRows32: return launch_tiles<Act, EPI, 32, 128, 1, 4, 1, 3, 3>(p, l.tiles, st);
+    case kRows64: return launch_tiles<Act, EPI, 64, 128, 1, 4, 1, 3, 3>(p, l.tiles, st);
+    case kRows128: return launch_tiles<Act, EPI, 128, 128, 2, 2, 1, 2, 3>(p, l.tiles, st);
+    case kRows256: return launch_tiles<Act, EPI, 256, 256, 4, 2, 1, 2, 3>(p, l.tiles, st);
+    default: return launch_tiles<Act, EPI, 320, 192, 4, 2, 1, 2, 3>(p, l.tiles, st);
+  }
+}
+
+template <class Act, int SLOTS>
+static void launch_route2(const Int8MoeArgs& m, int8_t* q, float* scale, hipStream_t st) {
+  const int routing = (m.T + 3) / 4, pieces = m.H / 8;
+  const dim3 grid((unsigned)(routing + m.T)), block(256);
+  if (pieces <= 256) hipLaunchKernelGGL((int8_route_kernel<Act, SLOTS, 1>), grid, block, 0, st, m, q, scale, routing);
+  else if (pieces <= 512) hipLaunchKernelGGL((int8_route_kernel<Act, SLOTS, 2>), grid, block, 0, st, m, q, scale, routing);
+  else if (pieces <= 1024) hipLaunchKernelGGL((int8_route_kernel<Act, SLOTS, 4>), grid, block, 0, st, m, q, scale, routing);
+  else hipLaunchKernelGGL((int8_route_kernel<Act, SLOTS, 0>), grid, block, 0, st, m, q, scale, routing);
+}
+template <class Act>
+static int launch_route(const Int8MoeArgs& m, int8_t* q, float* scale, hipStream_t st) {
+  if (m.E <= 128) launch_route2<Act, 2>(m, q, scale, st);
+  else if (m.E <= 256) launch_route2<Act, 4>(m, q, scale, st);
+  else launch_route2<Act, 16>(m, q, scale, st);
+  return launch_status();
 }
 
 static bool moe_sizes(int T, int k, int E, int H, int I) {
@@ -143,26 +264,25 @@ static bool moe_sizes(int T, int k, int E, int H, int I) {
 template <class Act>
 static int run_moe(const Int8MoeArgs& m, char* ws, hipStream_t st) {
   const int T = m.T, k = m.k, E = m.E, H = m.H, I = m.I;
-  const void *x = m.x, *logits = m.logits;
   const bool shared = m.shared_w13 != nullptr;
   const MoeLayout l = moe_layout(T, k, E, H, I, shared);
-  int32_t *ids = (int32_t*)(ws + l.ids), *start = (int32_t*)(ws + l.start), *inv = (int32_t*)(ws + l.inv), *row = (int32_t*)(ws + l.row);
+  int32_t *start = (int32_t*)(ws + l.start), *inv = (int32_t*)(ws + l.inv), *row = (int32_t*)(ws + l.row);
   int32_t* tile = (int32_t*)(ws + l.tile);
-  float* gate = shared ? (float*)(ws + l.gate) : nullptr;
-  int rc = mi_moe_topk(logits, ws + l.top_w, ids, T, E, k, 1, nullptr, shared ? x : nullptr, m.gate_weight, gate, H, Act::dt, st);
-  if (rc != MI_OK) return rc;
   QuantArgs q{};
-  q.x = x;
   q.q = (int8_t*)(ws + l.xq);
   q.scale = (float*)(ws + l.xs);
-  q.rows = T;
-  q.K = H;
-  rc = launch_int8_quant(kFromAct, q, Act::dt, st);
+  int rc = launch_route<Act>(m, q.q, q.scale, st);
   if (rc != MI_OK) return rc;
-  rc = mi_moe_sort(ids, (int32_t*)(ws + l.pairs), start, inv, row, nullptr, T, k, E, st);
+  if (l.P <= (long long)kSortPairs * kSortThreads) {
+    hipLaunchKernelGGL(int8_sort_kernel, dim3(1), dim3(kSortThreads), 0, st, m.ids, inv, row, tile, E, k, (int)l.P, shared ? T : 0, l.bm,
+                       (int)l.tiles);
+  } else {
+    rc = mi_moe_sort(m.ids, (int32_t*)(ws + l.pairs), start, inv, row, nullptr, T, k, E, st);
+    if (rc != MI_OK) return rc;
+    hipLaunchKernelGGL(int8_tiles_kernel, dim3(1), dim3(kSortThreads), 0, st, start, tile, row, E, (int)l.P, shared ? T : 0, l.bm, (int)l.tiles);
+  }
+  rc = launch_status();
   if (rc != MI_OK) return rc;
-  hipLaunchKernelGGL(int8_tiles_kernel, dim3(1), dim3(kTileThreads), 0, st, start, tile, row, E, (int)l.P, shared ? T : 0, kGroupRows,
-                     (int)l.tiles);
   Int8GemmArgs p{};
   p.a = q.q;
   p.a_scale = q.scale;
@@ -177,7 +297,7 @@ static int run_moe(const Int8MoeArgs& m, char* ws, hipStream_t st) {
   p.shared_w = m.shared_w13;
   p.shared_scale = m.shared_s13;
   p.E = E;
-  rc = launch_grouped<Act, kEpiAct>(p, l.tiles, st);
+  rc = launch_grouped<Act, kEpiAct>(p, l, st);
   if (rc != MI_OK) return rc;
   q.x = ws + l.h;
   q.q = (int8_t*)(ws + l.hq);
@@ -191,16 +311,17 @@ static int run_moe(const Int8MoeArgs& m, char* ws, hipStream_t st) {
   p.w = m.w2;
   p.w_scale = m.s2;
   p.out = ws + l.y;
+  p.block_scale = (float*)(ws + l.ys);
   p.M = (int)l.rows;
   p.N = H;
   p.K = I;
   p.g_row = nullptr;
   p.shared_w = m.shared_w2;
   p.shared_scale = m.shared_s2;
-  rc = launch_grouped<Act, kEpiF32>(p, l.tiles, st);
+  rc = launch_grouped<Act, kEpiBlock>(p, l, st);
   if (rc != MI_OK) return rc;
   hipLaunchKernelGGL(int8_combine_kernel<Act>, dim3((unsigned)(((long long)T * (H / 8) + 255) / 256)), dim3(256), 0, st,
-                     (const float*)(ws + l.y), inv, (const typename Act::elem*)(ws + l.top_w), gate, (typename Act::elem*)m.out, T, k, H);
+                     (const short*)(ws + l.y), (const float*)(ws + l.ys), kGroupTiles[l.tile_kind].block, inv, (const typename Act::elem*)m.top_w, shared ? m.gate : nullptr, (typename Act::elem*)m.out, T, k, H);
   return launch_status();
 }
 

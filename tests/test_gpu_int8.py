@@ -310,7 +310,9 @@ def _moe_run(dev, c, k):
 
 
 def _moe_reference(dev, c, k):
-    """(out, slack, sum of the summands' sizes); routing weights and gates are those of the framework's own selection."""
+    """(out, slack, sum of the summands' sizes); routing weights and gates are those of the framework's own selection.  An expert's row
+    may pass from the down product to the weighted sum as 16-bit integers with a scale per 32 to 128 of its columns: off by half of
+    1 / 32767 of their largest value, which is at most the row's (and that of its own error)."""
     from mi355x_qlinear import ops
     T, H = c["x"].shape
     E, dt = c["w13"].shape[0], c["x"].dtype
@@ -324,7 +326,8 @@ def _moe_reference(dev, c, k):
 
     def expert(rows, w13, s13, w2, s2):
         gu, _ = R.product(q[rows], s[rows], near[rows], w13, s13)
-        return R.product(*R.quantise(R.silu_mul(gu), LOOSE), w2, s2)
+        y, sl = R.product(*R.quantise(R.silu_mul(gu), LOOSE), w2, s2)
+        return y, sl + (y.abs() + sl).amax(1, keepdim=True) * (0.5 / 32767 * (1 + 2.0 ** -10))
     out, slack, parts = (torch.zeros(T, H, dtype=torch.float64) for _ in range(3))
     for e in range(E):
         rows, j = (top == e).nonzero(as_tuple=True)
@@ -345,7 +348,8 @@ def _moe_reference(dev, c, k):
 # one token, few, a row or none per expert, every route the same expert's neighbours, tiles that end inside an expert, sizes off every power of two
 MOE = [(1, 1, 1, 16, 16), (1, 8, 2, 256, 128), (1, 32, 8, 2048, 768), (2, 5, 5, 272, 48), (3, 130, 8, 1040, 96), (4, 16, 4, 512, 256), (6, 64, 64, 128, 32),
        (8, 8, 8, 2048, 64), (12, 40, 8, 528, 208), (17, 300, 6, 640, 16), (33, 4, 2, 1024, 512), (64, 16, 8, 512, 112), (130, 3, 1, 400, 80),
-       (200, 32, 4, 256, 256), (515, 8, 2, 144, 144), (1100, 6, 3, 96, 64), (5, 1024, 10, 64, 16), (1, 4, 2, 8192, 256), (2, 4, 4, 256, 4096)]
+       (200, 32, 4, 256, 256), (515, 8, 2, 144, 144), (1100, 6, 3, 96, 64), (5, 1024, 10, 64, 16), (1, 4, 2, 8192, 256), (2, 4, 4, 256, 4096), (100, 2, 2, 336, 80), (750, 3, 1, 208, 112),
+       (4200, 8, 2, 64, 48)]
 
 
 @pytest.mark.parametrize("T,E,k,H,I", MOE)
