@@ -655,9 +655,14 @@ int mi_gemv_w16(const void* x, const void* w, void* out, int M, int N, int K, in
  * mi_resadd_norm_gemm_int8_ws: a = x + residual in fp32, residual_out = a rounded, v = a * rsqrt(mean(a^2) + eps) * norm_weight in
  *   fp32 are the rows.  residual_out may be residual; otherwise it overlaps neither x nor residual.
  * mi_silu_mul_gemm_int8_ws: gate_up [M, 2 K], v = silu(gate) * up in fp32 are the rows.
- * The workspace, mi_gemm_int8_workspace bytes, must stay untouched until the stream has passed the call; where x are codes and no
- * slices of K are summed it is not needed and may be NULL. */
-int mi_gemm_int8_workspace(int M, int N, int K, long long* bytes);
+ * The workspace, mi_gemm_int8_workspace bytes for what the rows are made of (MI_INT8_*), must stay untouched until the stream has
+ * passed the call; 0 bytes: the call takes none (NULL). */
+#define MI_INT8_CODES 0
+#define MI_INT8_ACT 1
+#define MI_INT8_RESADD_NORM 2
+#define MI_INT8_RESADD_NORM_IN_PLACE 3
+#define MI_INT8_SILU_MUL 4
+int mi_gemm_int8_workspace(int rows_from, int M, int N, int K, long long* bytes);
 int mi_gemm_int8_ws(const void* x, const float* x_scale, const void* w, const float* w_scale, const void* bias, void* out,
                     void* workspace, long long workspace_bytes, int M, int N, int K, int act_dtype, void* stream);
 int mi_resadd_norm_gemm_int8_ws(const void* x, const void* residual, void* residual_out, const void* norm_weight, float eps,

@@ -80,6 +80,12 @@ struct Linear {
 };
 
 static long long round256(long long v) { return (v + 255) / 256 * 256; }
+static long long codes_workspace(int M, int K) { return round256((long long)M * K) + round256(4LL * M); }
+
+// Whether the rows are quantised by the launch that multiplies them.  The new residual must not be what other workgroups still read.
+static bool one_launch(int from, bool in_place, int M, int N, int K) {
+  return from != kFromCodes && N && int8_rows_quantise(from, M, K) && !in_place;
+}
 
 static int run_linear(Linear l, const void* w, const float* w_scale, const void* bias, void* out, void* workspace,
                       long long workspace_bytes, int M, int N, int K, int act_dtype, void* stream) {
@@ -90,24 +96,18 @@ static int run_linear(Linear l, const void* w, const float* w_scale, const void*
   if (!aligned16(l.q.x) || !aligned16(w)) return MI_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
   Int8RowsArgs r{l.q.x, l.x_scale, l.q.residual, l.q.residual_out, l.q.norm_weight, (const int8_t*)w, w_scale, bias, out, M, N, K, 0, l.q.eps};
-  // one launch; the new residual must not be what other workgroups still read
-  if (l.from != kFromCodes && N && int8_rows_quantise(l.from, M, K) && (l.from != kFromNorm || l.q.residual_out != l.q.residual))
-    return launch_int8_rows(l.from, r, act_dtype, st);
+  if (one_launch(l.from, l.from == kFromNorm && l.q.residual_out == l.q.residual, M, N, K)) return launch_int8_rows(l.from, r, act_dtype, st);
   Int8GemmArgs p{};
-  if (l.from == kFromCodes) {
-    p.a = (const int8_t*)l.q.x;
-    p.a_scale = l.x_scale;
-  } else {
-    long long need = 0;
-    const int rc = mi_gemm_int8_workspace(M, N, K, &need);
-    if (rc != MI_OK) return rc;
-    if (!workspace || !aligned16(workspace) || workspace_bytes < need) return MI_ERR_ARG;
+  p.a = (const int8_t*)l.q.x;
+  p.a_scale = l.x_scale;
+  if (l.from != kFromCodes) {
+    if (!workspace || !aligned16(workspace) || workspace_bytes < codes_workspace(M, K)) return MI_ERR_ARG;
     l.q.q = (int8_t*)workspace;
     l.q.scale = (float*)((char*)workspace + round256((long long)M * K));
     l.q.rows = M;
     l.q.K = K;
-    const int qc = launch_int8_quant(l.from, l.q, act_dtype, st);
-    if (qc != MI_OK) return qc;
+    const int rc = launch_int8_quant(l.from, l.q, act_dtype, st);
+    if (rc != MI_OK) return rc;
     p.a = l.q.q;
     p.a_scale = l.q.scale;
   }
@@ -134,10 +134,11 @@ using namespace qlin;
 
 extern "C" {
 
-int mi_gemm_int8_workspace(int M, int N, int K, long long* bytes) {
-  if (!bytes) return MI_ERR_ARG;
+int mi_gemm_int8_workspace(int rows_from, int M, int N, int K, long long* bytes) {
+  if (!bytes || rows_from < MI_INT8_CODES || rows_from > MI_INT8_SILU_MUL) return MI_ERR_ARG;
   if (!int8_sizes(M, N, K)) return MI_ERR_SHAPE;
-  *bytes = round256((long long)M * K) + round256(4LL * M);
+  const int from = rows_from == MI_INT8_CODES ? kFromCodes : rows_from == MI_INT8_ACT ? kFromAct : rows_from == MI_INT8_SILU_MUL ? kFromSilu : kFromNorm;
+  *bytes = from == kFromCodes || one_launch(from, rows_from == MI_INT8_RESADD_NORM_IN_PLACE, M, N, K) ? 0 : codes_workspace(M, K);
   return MI_OK;
 }
 

@@ -359,7 +359,7 @@ int mi_moe_forward_full_int8_ws(const void* x, const void* logits, void* out, co
   const Int8MoeArgs m{x, logits, out, (const int8_t*)w13, (const int8_t*)w2, w13_scale, w2_scale, (const int8_t*)shared_w13,
                       (const int8_t*)shared_w2, shared_w13_scale, shared_w2_scale, gate_weight, ws + l.top_w, (int32_t*)(ws + l.ids),
                       (float*)(ws + l.gate), (float*)(ws + l.h), T, topk, num_experts, H, I};
-  if (int8_moe_decode_pays(T, topk, H, I, shared)) return launch_int8_moe_decode(m, act_dtype, st);
+  if (int8_moe_decode_pays(T, topk, num_experts, H, I, shared)) return launch_int8_moe_decode(m, act_dtype, st);
   return act_dtype == DT_F16 ? run_moe<ActF16>(m, ws, st) : run_moe<ActBF16>(m, ws, st);
 }
 

@@ -21,7 +21,7 @@ struct Int8MoeArgs {
   int T, k, E, H, I;
 };
 
-bool int8_moe_decode_pays(int T, int k, int H, int I, bool shared);
+bool int8_moe_decode_pays(int T, int k, int E, int H, int I, bool shared);
 int launch_int8_moe_decode(const Int8MoeArgs& p, int act_dtype, hipStream_t st);
 
 }  // namespace qlin

@@ -457,10 +457,12 @@ Int8Linear int8_linear(const char* who, const Tensor& x, int64_t per_row, const 
 }
 const void* data_or_null(const c10::optional<Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 
-Tensor int8_workspace(const Tensor& x, const Int8Linear& l, long long& bytes) {
-  CALL(mi_gemm_int8_workspace, l.M, l.N, l.K, &bytes);
-  return buffer(x, bytes);
+// undefined where the call takes none
+Tensor int8_workspace(int rows_from, const Tensor& x, const Int8Linear& l, long long& bytes) {
+  CALL(mi_gemm_int8_workspace, rows_from, l.M, l.N, l.K, &bytes);
+  return bytes ? buffer(x, bytes) : Tensor();
 }
+void* int8_buffer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 Tensor gemm_int8(const Tensor& x, const c10::optional<Tensor>& x_scale, const Tensor& w, const Tensor& ws,
                  const c10::optional<Tensor>& bias, const Tensor& out) {
@@ -480,9 +482,9 @@ Tensor gemm_int8(const Tensor& x, const c10::optional<Tensor>& x_scale, const Te
   if (!l.M) return out;
   const On on(x);
   long long bytes = 0;
-  const Tensor buf = int8_workspace(x, l, bytes);
+  const Tensor buf = int8_workspace(x_scale.has_value() ? MI_INT8_CODES : MI_INT8_ACT, x, l, bytes);
   CALL(mi_gemm_int8_ws, x.data_ptr(), (const float*)data_or_null(x_scale), w.data_ptr(), ws.data_ptr<float>(), data_or_null(bias),
-       out.data_ptr(), buf.data_ptr(), bytes, l.M, l.N, l.K, l.adt, on.stream);
+       out.data_ptr(), int8_buffer(buf), bytes, l.M, l.N, l.K, l.adt, on.stream);
   return out;
 }
 
@@ -509,9 +511,9 @@ Tensor resadd_norm_gemm_int8(const Tensor& x, const Tensor& res, const Tensor& r
   if (!l.M) return out;
   const On on(x);
   long long bytes = 0;
-  const Tensor buf = int8_workspace(x, l, bytes);
+  const Tensor buf = int8_workspace(res_out.data_ptr() == res.data_ptr() ? MI_INT8_RESADD_NORM_IN_PLACE : MI_INT8_RESADD_NORM, x, l, bytes);
   CALL(mi_resadd_norm_gemm_int8_ws, x.data_ptr(), res.data_ptr(), res_out.data_ptr(), nw.data_ptr(), (float)eps, w.data_ptr(),
-       ws.data_ptr<float>(), data_or_null(bias), out.data_ptr(), buf.data_ptr(), bytes, l.M, l.N, l.K, l.adt, on.stream);
+       ws.data_ptr<float>(), data_or_null(bias), out.data_ptr(), int8_buffer(buf), bytes, l.M, l.N, l.K, l.adt, on.stream);
   return out;
 }
 
@@ -523,8 +525,8 @@ Tensor silu_mul_gemm_int8(const Tensor& gate_up, const Tensor& w, const Tensor& 
   if (!l.M) return out;
   const On on(gate_up);
   long long bytes = 0;
-  const Tensor buf = int8_workspace(gate_up, l, bytes);
-  CALL(mi_silu_mul_gemm_int8_ws, gate_up.data_ptr(), w.data_ptr(), ws.data_ptr<float>(), data_or_null(bias), out.data_ptr(), buf.data_ptr(),
+  const Tensor buf = int8_workspace(MI_INT8_SILU_MUL, gate_up, l, bytes);
+  CALL(mi_silu_mul_gemm_int8_ws, gate_up.data_ptr(), w.data_ptr(), ws.data_ptr<float>(), data_or_null(bias), out.data_ptr(), int8_buffer(buf),
        bytes, l.M, l.N, l.K, l.adt, on.stream);
   return out;
 }

@@ -369,19 +369,23 @@ moe_forward_tiny_cutlass_nmajor_int4_full_fp16_shared_from_logits = _NotProvided
     "moe_forward_tiny_cutlass_nmajor_int4_full_fp16_shared_from_logits", "DISABLE_ESIMD_INT4=1 (sym_int4 MoE models)")
 
 
+_gemm_int8, _resadd_norm_gemm_int8 = _ops.gemm_int8.default, _ops.resadd_norm_gemm_int8.default
+_silu_mul_gemm_int8 = _ops.silu_mul_gemm_int8.default
+
+
 def gemm_int8(x, x_scale, weight, weight_scale, bias, output):
     """W8A8: output = (codes @ weight^T) * row scale * weight_scale + bias.  x int8 [M, K] with x_scale fp32 [M], or fp16 / bf16
     with x_scale None (quantised per row: scale max|x| / 127); weight int8 [N, K], weight_scale fp32 [N], bias [N] or None in
     output's type; K a multiple of 16."""
-    return _ops.gemm_int8(x, x_scale, weight, weight_scale, bias, output)
+    return _gemm_int8(x, x_scale, weight, weight_scale, bias, output)
 
 
 def resadd_norm_gemm_int8(hidden_states, residual, residual_out, norm_weight, weight, weight_scale, bias, output, eps):
     """residual_out = hidden_states + residual, then gemm_int8 on its RMS norm.  residual_out may be residual itself (in place)
     or a buffer that overlaps neither input; the second is one launch less for few rows."""
-    return _ops.resadd_norm_gemm_int8(hidden_states, residual, residual_out, norm_weight, weight, weight_scale, bias, output, eps)
+    return _resadd_norm_gemm_int8(hidden_states, residual, residual_out, norm_weight, weight, weight_scale, bias, output, eps)
 
 
 def silu_mul_gemm_int8(gate_up, weight, weight_scale, bias, output):
     """gate_up [M, 2K], gate columns first: gemm_int8 on silu(gate) * up."""
-    return _ops.silu_mul_gemm_int8(gate_up, weight, weight_scale, bias, output)
+    return _silu_mul_gemm_int8(gate_up, weight, weight_scale, bias, output)

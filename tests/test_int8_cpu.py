@@ -15,19 +15,24 @@ def _ws(*a):
 
 
 def test_workspace_of_the_linears():
-    rc, n = _ws(100, 64, 4096)
-    assert rc == 0 and n >= 100 * 4096 + 400
-    assert _ws(0, 64, 4096)[0] == 0
+    codes, act, norm, in_place, silu = range(5)
+    for rows in (act, norm, in_place, silu):
+        rc, n = _ws(rows, 100, 64, 4096)
+        assert rc == 0 and n >= 100 * 4096 + 400
+    assert _ws(codes, 100, 64, 4096) == (0, 0) and _ws(act, 0, 64, 4096)[0] == 0
+    # one launch: none, unless the new residual is written over the old one
+    assert _ws(act, 1, 64, 4096) == _ws(norm, 1, 64, 4096) == _ws(silu, 1, 64, 4096) == (0, 0) and _ws(in_place, 1, 64, 4096)[1] > 0
+    assert _ws(act, 16, 64, 4096)[1] > 0 and _ws(act, 17, 64, 64)[1] > 0 and _ws(norm, 1, 0, 4096)[1] > 0
     for bad in ((-1, 64, 4096), (1, -1, 64), (1, 1, 0), (1, 1, 24), (1, 1, 131072)):
-        assert _ws(*bad)[0] == -2
-    assert capi.lib().mi_gemm_int8_workspace(1, 1, 16, None) == -1
+        assert _ws(act, *bad)[0] == -2
+    assert _ws(5, 1, 1, 16)[0] == _ws(-1, 1, 1, 16)[0] == capi.lib().mi_gemm_int8_workspace(act, 1, 1, 16, None) == -1
 
 
 def test_linears_answer_bad_arguments_before_a_launch():
     lib = capi.lib()
     f = ctypes.c_float(1e-6)
 
-    def plain(x=OK, xs=None, w=OK, ws=OK, out=OK, buf=OK, n=1 << 40, M=2, N=8, K=32, dt=0):
+    def plain(x=OK, xs=None, w=OK, ws=OK, out=OK, buf=OK, n=1 << 40, M=20, N=8, K=32, dt=0):
         return lib.mi_gemm_int8_ws(x, xs, w, ws, None, out, buf, ctypes.c_longlong(n), M, N, K, dt, None)
     assert plain(M=0) == 0 and plain(M=0, x=None) == 0
     assert plain(dt=2) == -1 and plain(x=None) == -1 and plain(w=None) == -1 and plain(ws=None) == -1 and plain(out=None) == -1
@@ -35,7 +40,7 @@ def test_linears_answer_bad_arguments_before_a_launch():
     assert plain(x=ctypes.c_void_p(264)) == -1 and plain(w=ctypes.c_void_p(257)) == -1 and plain(buf=ctypes.c_void_p(264)) == -1
     assert plain(K=24) == -2 and plain(K=131072) == -2 and plain(M=-1) == -2 and plain(N=-1) == -2 and plain(K=0) == -2
 
-    def norm(x=OK, res=OK, ro=OK, nw=OK, M=2):
+    def norm(x=OK, res=OK, ro=OK, nw=OK, M=20):
         return lib.mi_resadd_norm_gemm_int8_ws(x, res, ro, nw, f, OK, OK, None, OK, None, ctypes.c_longlong(0), M, 8, 32, 0, None)
     assert norm(M=0) == 0 and norm(res=None) == -1 and norm(ro=None) == -1 and norm(nw=None) == -1 and norm(x=None) == -1
     assert norm(res=ctypes.c_void_p(264)) == -1
