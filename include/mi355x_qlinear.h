@@ -648,8 +648,8 @@ int mi_gemv_w16(const void* x, const void* w, void* out, int M, int N, int K, in
  * out[M, N] = (sum_k q[m, k] w[n, k]) s[m] w_scale[n] + bias[n]: weights w [N, K] int8 with one fp32 scale per output channel,
  * activations as int8 codes with one fp32 scale per row.  A row v becomes q = rint(127 v / max) (ties to even), s = max / 127 with
  * max = max(max|v|, 2^-40); a row with an infinity or a NaN gives NaN outputs.  Integer sums are exact; the result is
- * scaled, biased and rounded once.  bias [N] (may be NULL) and out in the activation type.  K % 16 == 0, K < 131072; any M
- * and N.  x, w, residual, residual_out, norm_weight and the workspace 16-byte aligned; out overlaps no operand.  No counterpart in the
+ * scaled, biased and rounded once.  bias [N] (may be NULL) and out in the activation type.  K % 16 == 0, K < 131072; M and
+ * N below 2^24 and outputs up to 2^31 at the least.  x, w, residual, residual_out, norm_weight and the workspace 16-byte aligned; out overlaps no operand.  No counterpart in the
  * reference's kernels (w8a16, V/csrc/xpu/esimd_kernels/fp8_GEMV_v2.h:46-162).
  * mi_gemm_int8_ws: x_scale given: x [M, K] are codes and x_scale [M] their scales; NULL: x is fp16 / bf16.
  * mi_resadd_norm_gemm_int8_ws: a = x + residual in fp32, residual_out = a rounded, v = a * rsqrt(mean(a^2) + eps) * norm_weight in
@@ -674,9 +674,11 @@ int mi_silu_mul_gemm_int8_ws(const void* gate_up, const void* w, const float* w_
 /* A whole mixture-of-experts layer on the same quantisation: softmax top-k of logits [T, E] (renormalised, lowest index first among
  * equals, weights in the activation type as mi_moe_topk gives them), then per token
  *   out = sum_j top_w[j] W2[e_j] q(h_j) + sigmoid(x . gate_weight) shared(x),   h = silu(g) u,   (g, u) = W13[e] q(x),
- * g, u, h and the experts' results in fp32, one rounding at the end.  w13 [E, 2 I, H] (gate rows first), w2 [E, H, I], shared_w13
+ * g, u, h and the sum over the experts in fp32, one rounding at the end; with many tokens an expert's result passes to that sum as 16-bit
+ * integers with one fp32 scale per 32 to 128 columns (off by 2^-16 of the largest of them; an infinity or a NaN among them, of a w2 scale
+ * or past fp32, makes them all NaN).  w13 [E, 2 I, H] (gate rows first), w2 [E, H, I], shared_w13
  * [2 I, H], shared_w2 [H, I] int8 with one fp32 scale per row of weights; the shared expert's four operands and gate_weight [H] are all
- * given or all NULL.  H and I as K above, E <= 1024, topk <= 64; T H, T (topk + 1) I and 2 I H below 2^31.  x, out, the weights,
+ * given or all NULL.  H and I as K above, E <= 1024, topk <= 64; T (topk + 1) below 2^24; T H, T (topk + 1) I and 2 I H below 2^31.  x, out, the weights,
  * gate_weight and the workspace (mi_moe_forward_full_int8_workspace bytes) 16-byte aligned; out overlaps no operand.  The 8-bit form
  * of moe_forward_full_fp8_block (V/csrc/moe_batch/moe.sycl:1707-1853), which has no integer counterpart there. */
 int mi_moe_forward_full_int8_workspace(int T, int topk, int num_experts, int H, int I, int shared, long long* bytes);

@@ -93,19 +93,19 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 // Where a row comes from.
 enum : int { kFromAct = 0, kFromNorm = 1, kFromSilu = 2, kFromF32 = 3, kFromCodes = 4 };
 
-// K a multiple of 16 that the integer sums hold; the sizes of one call in 64 bits.
+// K a multiple of 16 that the integer sums hold; M and N such that a workgroup of 256 per row is a grid of less than 2^32 threads.
+constexpr int kInt8MaxRows = (1 << 24) - 1;
 static inline bool int8_sizes(int M, int N, int K) {
-  return M >= 0 && N >= 0 && K > 0 && K % 16 == 0 && K <= kInt8MaxK;
+  return M >= 0 && N >= 0 && M <= kInt8MaxRows && N <= kInt8MaxRows && K > 0 && K % 16 == 0 && K <= kInt8MaxK;
 }
 static inline int int8_cu_count() {
-  static int cus = 0;
-  if (!cus) {
+  static const int count = [] {
     int dev = 0;
     hipDeviceProp_t prop;
-    if (hipGetDevice(&dev) == hipSuccess && hipGetDeviceProperties(&prop, dev) == hipSuccess) cus = prop.multiProcessorCount;
-    if (cus <= 0) cus = 256;
-  }
-  return cus;
+    const bool known = hipGetDevice(&dev) == hipSuccess && hipGetDeviceProperties(&prop, dev) == hipSuccess && prop.multiProcessorCount > 0;
+    return known ? prop.multiProcessorCount : 256;
+  }();
+  return count;
 }
 // A kernel that asks for more LDS than a launch gets unasked: once per device.
 template <class Kernel>

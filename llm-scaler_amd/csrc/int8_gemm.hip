@@ -9,8 +9,7 @@ template <class Act, int BM, int BN, int WM, int WN, int KG, int SA, int SB>
 static int launch_tiles(Int8GemmArgs p, hipStream_t st) {
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
-  const long long tiles = (long long)p.tiles_m * p.tiles_n, grid = (tiles + 7) / 8 * 8;
-  if (grid > 0x7FFFFFFFLL) return MI_ERR_SHAPE;
+  const long long tiles = (long long)p.tiles_m * p.tiles_n, grid = (tiles + 7) / 8 * 8;          // linear_sizes: below 2^23
   auto* kernel = int8_gemm_kernel<Act, BM, BN, WM, WN, KG, SA, SB, kEpiOut, false>;
   constexpr size_t lds = int8_gemm_lds(BM, BN, WM * WN, KG, SA, SB, false);
   if constexpr (lds > 64 * 1024) {
@@ -54,6 +53,13 @@ static int pick_tile(long long M, long long N, long long K) {
   }
   return best;
 }
+// Sizes that every launch of a call holds: a grid has less than 2^32 threads.
+static bool linear_sizes(int M, int N, int K) {
+  if (!int8_sizes(M, N, K)) return false;
+  if ((long long)M * N < (1LL << 31)) return true;     // M N / 512 + M / 32 + N / 16 + 1 tiles of 512 threads at most
+  const Int8Tile& t = kTiles[pick_tile(M, N, K)];
+  return (((long long)M + t.bm - 1) / t.bm) * (((long long)N + t.bn - 1) / t.bn) < (1LL << 23) - 8;
+}
 
 template <class Act>
 static int launch_product(const Int8GemmArgs& p, hipStream_t st) {
@@ -90,7 +96,7 @@ static bool one_launch(int from, bool in_place, int M, int N, int K) {
 static int run_linear(Linear l, const void* w, const float* w_scale, const void* bias, void* out, void* workspace,
                       long long workspace_bytes, int M, int N, int K, int act_dtype, void* stream) {
   if (act_dtype != DT_F16 && act_dtype != DT_BF16) return MI_ERR_ARG;
-  if (!int8_sizes(M, N, K)) return MI_ERR_SHAPE;
+  if (!linear_sizes(M, N, K)) return MI_ERR_SHAPE;
   if (!M) return MI_OK;
   if (!l.q.x || (N && (!w || !w_scale || !out))) return MI_ERR_ARG;
   if (!aligned16(l.q.x) || !aligned16(w)) return MI_ERR_ARG;
@@ -136,7 +142,7 @@ extern "C" {
 
 int mi_gemm_int8_workspace(int rows_from, int M, int N, int K, long long* bytes) {
   if (!bytes || rows_from < MI_INT8_CODES || rows_from > MI_INT8_SILU_MUL) return MI_ERR_ARG;
-  if (!int8_sizes(M, N, K)) return MI_ERR_SHAPE;
+  if (!linear_sizes(M, N, K)) return MI_ERR_SHAPE;
   const int from = rows_from == MI_INT8_CODES ? kFromCodes : rows_from == MI_INT8_ACT ? kFromAct : rows_from == MI_INT8_SILU_MUL ? kFromSilu : kFromNorm;
   *bytes = from == kFromCodes || one_launch(from, rows_from == MI_INT8_RESADD_NORM_IN_PLACE, M, N, K) ? 0 : codes_workspace(M, K);
   return MI_OK;

@@ -5,8 +5,9 @@
 //
 // with q() the rows' quantisation of int8_common.hpp; g, u, h and the sums stay in fp32, the output is rounded once.
 //
-// Selection, codes of x, pairs sorted by expert, a tile table, the grouped product with SiLU(gate) x up, codes of h, the grouped down product
-// and the weighted sum.  The shared expert is one more expert, with a row for every token.
+// Few tokens: int8_moe_decode.hip.  Otherwise six launches: selection beside the codes of x, pairs sorted by expert with a tile table, the grouped
+// product with SiLU(gate) x up, codes of h, the grouped down product, the weighted sum.  The shared expert is one more expert, with a
+// row for every token.
 #include "int8_gemm.hpp"
 #include "int8_moe.hpp"
 #include "int8_quant.hpp"
@@ -258,7 +259,7 @@ static bool moe_sizes(int T, int k, int E, int H, int I) {
   if (T < 0 || E < 1 || E > 1024 || k < 1 || k > 64 || k > E) return false;
   if (!int8_sizes(T, 2, H) || !int8_sizes(T, 2, I)) return false;
   const long long pairs = (long long)T * (k + 1);
-  return 2LL * I * H < (1LL << 31) && (long long)T * H < (1LL << 31) && pairs * I < (1LL << 31) && pairs < (1LL << 31) - 1024;
+  return 2LL * I * H < (1LL << 31) && (long long)T * H < (1LL << 31) && pairs * I < (1LL << 31) && pairs <= kInt8MaxRows;
 }
 
 template <class Act>

@@ -439,7 +439,7 @@ Int8Linear int8_linear(const char* who, const Tensor& x, int64_t per_row, const 
   REFUSE_UNLESS(K > 0 && K % 16 == 0 && K < 131072, "K=", K, " must be a multiple of 16 below 131072");
   REFUSE_UNLESS(x.dim() >= 1 && x.size(-1) == per_row * K, "the input's rows must have ", per_row * K, " elements, got ", x.sizes());
   const int64_t M = x.numel() / (per_row * K);
-  REFUSE_UNLESS(M <= INT_MAX && N <= INT_MAX, "more than 2^31 - 1 rows");
+  REFUSE_UNLESS(M < (1 << 24) && N < (1 << 24), "M=", M, " and N=", N, " must be below 2^24");
   REFUSE_UNLESS(ws.scalar_type() == at::kFloat && ws.numel() == N, "weight_scale must be fp32 with N=", N, " entries");
   REFUSE_UNLESS(is16(out), "output must be fp16 or bf16, got ", out.scalar_type());
   REFUSE_UNLESS(out.numel() == M * N, "output has ", out.numel(), " elements, expected M*N=", M * N);
@@ -587,7 +587,7 @@ Tensor moe_forward_full_int8(const Tensor& x, const Tensor& logits, const Tensor
   int8_aligned(who, out, "output");
   int8_apart(who, out, "output", x, "x");
   int8_apart(who, out, "output", logits, "logits");
-  REFUSE_UNLESS(T <= INT_MAX, "more than 2^31 - 1 tokens");
+  REFUSE_UNLESS(T < (1 << 24), "T=", T, " must be below 2^24");
   if (!T) return out;
   const On on(x);
   long long bytes = 0;

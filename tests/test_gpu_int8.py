@@ -385,6 +385,104 @@ def test_expert_layer_graph(dev, T):
                                                                       c["sw2"], c["ss2"], c["gw"], 4, 1, 24), [out])
 
 
+@pytest.mark.parametrize("T", [1, 20, 40, 300, 5000])
+def test_expert_layer_on_two_streams(dev, T):
+    """Two captured calls of their own inputs replayed side by side, with an eager call of another size between."""
+    import custom_esimd_kernels_vllm  # noqa: F401
+    streams, sets = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    names = ("w13", "s13", "sw13", "ss13", "w2", "s2", "sw2", "ss2", "gw")
+
+    def call(c, out):
+        torch.ops.moe_ops.moe_forward_full_int8(c["x"], c["logits"], out, *[c[n] for n in names], 4, 1, 24)
+    other = {n: t.to(dev) for n, t in _moe(33, 24, 4, 256, 128, torch.bfloat16, 40, True).items()}
+    other_want, other_out = torch.empty_like(other["x"]), torch.empty_like(other["x"])
+    call(other, other_want)
+    for i in range(2):
+        c = {n: t.to(dev) for n, t in _moe(T, 24, 4, 256, 128, torch.bfloat16, 30 + i, True).items()}
+        want, out = torch.empty_like(c["x"]), torch.empty_like(c["x"])
+        call(c, want)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(c, out)
+        sets.append((c, want, out, graph))
+    for _ in range(5):
+        for st, (c, want, out, graph) in zip(streams, sets):
+            out.fill_(float("nan"))
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                graph.replay()
+        other_out.fill_(float("nan"))
+        call(other, other_out)
+        torch.cuda.synchronize()
+        assert torch.equal(other_out, other_want)
+        for _, want, out, _ in sets:
+            assert torch.equal(out, want)
+
+
+def test_expert_layer_masked_and_bad_logits(dev):
+    """Experts at -inf are taken last and weigh nothing; the token of a NaN logit is NaN, the others are as they were."""
+    import custom_esimd_kernels_vllm  # noqa: F401
+    for T in (1, 7, 150):
+        c = _moe(T, 16, 4, 256, 64, torch.float16, 8, False)
+        c["logits"][:, ::2] = float("-inf")
+        c["logits"][0, 5:] = float("-inf")                # two experts left for four places
+        out, slack, parts = _moe_reference(dev, c, 4)
+        want = _moe_run(dev, c, 4)
+        ok, worst = R.within(want, out, slack, torch.float16, SILU, parts)
+        assert ok, f"{worst:.2f} of the tolerance"
+        if T > 1:
+            c["logits"][1, 3] = float("nan")
+            got = _moe_run(dev, c, 4)
+            others = torch.arange(T) != 1
+            assert bool(got[1].isnan().all()) and torch.equal(got[others], want[others])
+
+
+@pytest.mark.parametrize("T", [3, 90, 900, 10000])
+def test_expert_layer_all_to_one_expert(dev, T):
+    """Every token takes the same two of many experts: one expert fills tile after tile, the others have no row."""
+    import custom_esimd_kernels_vllm  # noqa: F401
+    c = _moe(T, 200, 2, 64, 48, torch.bfloat16, 9, True)
+    c["logits"][:, 199] += 20
+    c["logits"][:, 70] += 20
+    out, slack, parts = _moe_reference(dev, c, 2)
+    ok, worst = R.within(_moe_run(dev, c, 2), out, slack, torch.bfloat16, SILU, parts)
+    assert ok, f"{worst:.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("T", [1, 40, 700])
+def test_expert_weights_past_32_bit_offsets(dev, T):
+    """72 experts of 67 + 34 MB; the four that are taken lie at both ends and past 2^31 and 2^32 bytes."""
+    import custom_esimd_kernels_vllm  # noqa: F401
+    E, k, H, I, taken = 72, 2, 4096, 8192, [0, 33, 70, 71]
+    c = _moe(T, 4, k, H, I, torch.bfloat16, 10, False)
+    ops_in = {n: torch.zeros(E, *c[n].shape[1:], dtype=c[n].dtype, device=dev) for n in ("w13", "s13", "w2", "s2")}
+    for n, t in ops_in.items():
+        t[taken] = c[n].to(dev)
+    logits = torch.full((T, E), float("-inf"), dtype=torch.bfloat16)
+    logits[:, taken] = c["logits"]
+    x = c["x"].to(dev)
+    out = torch.full_like(x, float("nan"))
+    torch.ops.moe_ops.moe_forward_full_int8(x, logits.to(dev), out, ops_in["w13"], ops_in["s13"], None, None, ops_in["w2"], ops_in["s2"], None, None,
+                                            None, k, 0, E)
+    few = torch.arange(T)[:: max(1, T // 8)]
+    ref, slack, parts = _moe_reference(dev, {**c, "x": c["x"][few], "logits": c["logits"][few]}, k)
+    ok, worst = R.within(out.cpu()[few], ref, slack, torch.bfloat16, SILU, parts)
+    assert ok and bool(torch.isfinite(out).all()), f"{worst:.2f} of the tolerance"
+
+
+def test_expert_results_past_32_bit_offsets(dev):
+    """560000 routes of 4096 columns: more than 2^31 results between the down product and the sum."""
+    import custom_esimd_kernels_vllm  # noqa: F401
+    T, E, k, H, I = 70000, 8, 8, 4096, 16
+    c = _moe(T, E, k, H, I, torch.bfloat16, 11, False)
+    got = _moe_run(dev, c, k)
+    few = torch.tensor([0, 1, 32767, 32768, 65535, 65536, 69998, 69999])
+    ref, slack, parts = _moe_reference(dev, {**c, "x": c["x"][few], "logits": c["logits"][few]}, k)
+    ok, worst = R.within(got[few], ref, slack, torch.bfloat16, SILU, parts)
+    assert ok and bool(torch.isfinite(got).all()), f"{worst:.2f} of the tolerance"
+
+
 def test_expert_layer_refusals(dev):
     import custom_esimd_kernels_vllm  # noqa: F401
     c = {n: t.to(dev) for n, t in _moe(2, 4, 2, 64, 32, torch.float16, 7, True).items()}

@@ -28,6 +28,17 @@ def test_workspace_of_the_linears():
     assert _ws(5, 1, 1, 16)[0] == _ws(-1, 1, 1, 16)[0] == capi.lib().mi_gemm_int8_workspace(act, 1, 1, 16, None) == -1
 
 
+def test_sizes_past_a_grid_are_refused():
+    # a grid holds less than 2^32 threads, and an answer comes before the first launch (the residual is not written yet)
+    for rows_from in range(5):
+        assert _ws(rows_from, (1 << 24) - 1, 16, 16)[0] == _ws(rows_from, 1, (1 << 24) - 1, 16)[0] == _ws(rows_from, 1 << 20, 4096, 4096)[0] == 0
+        for bad in ((1 << 24, 16, 16), (1, 1 << 24, 16), ((1 << 24) - 1, (1 << 24) - 1, 16), (2**31 - 1, 2**31 - 1, 16)):
+            assert _ws(rows_from, *bad)[0] == -2, bad
+    n = ctypes.c_longlong()
+    size = capi.lib().mi_moe_forward_full_int8_workspace
+    assert size(1 << 22, 2, 8, 256, 64, 1, ctypes.byref(n)) == 0 and size(1 << 23, 1, 8, 16, 16, 1, ctypes.byref(n)) == -2
+
+
 def test_linears_answer_bad_arguments_before_a_launch():
     lib = capi.lib()
     f = ctypes.c_float(1e-6)
