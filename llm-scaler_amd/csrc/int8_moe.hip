@@ -160,20 +160,24 @@ __global__ __launch_bounds__(256) void int8_combine_kernel(const short* __restri
   *reinterpret_cast<typename Act::v8*>(out + t * H + c) = o;
 }
 
-// Rows of a tile, by the rows that an expert has on average, and the columns that share a scale (kEpiBlock) with each.  The whole layer, us,
-// tile / next: 128 experts, top 8, 2048 / 768: 200 tokens 32 x 128 147 / 64 x 128 153; 512 tokens 64 x 128 166 / 32 x 128 179; 4096 tokens 320 x 192
-// 370 / 256 x 256 376; 64 experts, top 6, 2048 / 1408: 2048 tokens 256 x 256 269 / 128 x 128 304; 8 experts, top 2, 4096 / 1536: 1024 tokens 320 x 192
-// 136 / 128 x 128 153, 4096 tokens 256 x 256 347 / 320 x 192 364.
-enum : int { kRows32, kRows64, kRows128, kRows256, kRows320 };
+// Rows of a tile, by the rows that an expert has on average: most experts in one row tile, up to 320.  The columns that share a scale
+// (kEpiBlock) are a wavefront's.  Up to 192 rows there is room for two workgroups on a CU, of eight wavefronts each: one begins and ends its tile
+// while the other multiplies (four wavefronts per workgroup: 3 % slower).  The whole layer, us, tile / next: 128 experts, top 8, 2048 / 768: 200
+// tokens 32 x 128 148 / 64 x 128 150; 600 tokens 64 x 128 166 / 128 x 128 186; 1500 tokens 128 x 128 224 / 192 x 128 236; 2300 tokens 192 x 128 268 /
+// 256 x 256 291; 3500 tokens 256 x 256 341 / 320 x 192 363; 4096 tokens 320 x 192 382 / 256 x 256 394; 64 experts, top 6, 2048 / 1408: 1000 tokens 128 x
+// 128 197 / 192 x 128 212, 1700 tokens 192 x 128 244 / 256 x 256 263; 8 experts, top 2, 4096 / 1536: 1200 tokens 320 x 192 143 / 192 x 128 156, 4096
+// tokens 256 x 256 364 / 192 x 128 372.
+enum : int { kRows32, kRows64, kRows128, kRows192, kRows256, kRows320 };
 struct GroupTile {
   int rows, block;
 };
-constexpr GroupTile kGroupTiles[] = {{32, 32}, {64, 32}, {128, 64}, {256, 128}, {320, 96}};
+constexpr GroupTile kGroupTiles[] = {{32, 32}, {64, 32}, {128, 32}, {192, 64}, {256, 128}, {320, 96}};
 static int group_tile(long long pairs, int E) {
   if (pairs <= 24LL * E) return kRows32;
-  if (pairs <= 90LL * E) return kRows64;
-  if (pairs <= 120LL * E) return kRows128;
-  return pairs <= 230LL * E || pairs > 310LL * E ? kRows256 : kRows320;        // most experts in one row tile
+  if (pairs <= 66LL * E) return kRows64;
+  if (pairs <= 125LL * E) return kRows128;
+  if (pairs <= 187LL * E) return kRows192;
+  return pairs <= 230LL * E || pairs > 310LL * E ? kRows256 : kRows320;
 }
 
 struct MoeLayout {                                    // byte offsets into the workspace
@@ -230,9 +234,10 @@ static int launch_tiles(Int8GemmArgs p, long long tiles, hipStream_t st) {
 template <class Act, int EPI>
 static int launch_grouped(const Int8GemmArgs& p, const MoeLayout& l, hipStream_t st) {
   switch (l.tile_kind) {
-    case kRows32: return launch_tiles<Act, EPI, 32, 128, 1, 4, 1, 3, 3>(p, l.tiles, st);
-    case kRows64: return launch_tiles<Act, EPI, 64, 128, 1, 4, 1, 3, 3>(p, l.tiles, st);
-    case kRows128: return launch_tiles<Act, EPI, 128, 128, 2, 2, 1, 2, 3>(p, l.tiles, st);
+    case kRows32: return launch_tiles<Act, EPI, 32, 128, 2, 4, 1, 3, 3>(p, l.tiles, st);
+    case kRows64: return launch_tiles<Act, EPI, 64, 128, 2, 4, 1, 3, 3>(p, l.tiles, st);
+    case kRows128: return launch_tiles<Act, EPI, 128, 128, 2, 4, 1, 2, 3>(p, l.tiles, st);
+    case kRows192: return launch_tiles<Act, EPI, 192, 128, 4, 2, 1, 2, 2>(p, l.tiles, st);
     case kRows256: return launch_tiles<Act, EPI, 256, 256, 4, 2, 1, 2, 3>(p, l.tiles, st);
     default: return launch_tiles<Act, EPI, 320, 192, 4, 2, 1, 2, 3>(p, l.tiles, st);
   }
