@@ -21,21 +21,22 @@ static int launch_tiles(Int8GemmArgs p, hipStream_t st) {
   return launch_status();
 }
 
-// The tiles, and what a round of the CUs costs with each: us = fixed + step x (steps of 128 KG of K), measured on 455 problems (M 17 .. 2048,
-// N 512 .. 14336, K 1024 .. 14336); the last has room for two workgroups on a CU, whose pair costs less than two rounds.  The tile with the
-// least sum of rounds is 0.3 % behind the best of 22 tiles in the mean, 8 % at most.  Some of them, us with the best / the second
-// best of another shape: 2048 x 4096 x 14336 256 x 256 112 / 256 x 192 123; 2048 x 14336 x 4096 256 x 128 101 / 128 x 128 118; 1000 x 4096 x 6144 128 x 192
-// 29.4 / 128 x 96 32.9; 128 x 4096 x 14336 128 x 64 16.1 / 128 x 128 19.2; 64 x 5120 x 5120 64 x 32 10.2 / 64 x 64 11.5; 32 x 14336 x 4096 32 x 16 13.6 /
-// 64 x 32 17.4.  A smaller tile reads more through the loads to LDS (68 GB/s per CU for whole lines, 54 for half lines of 64 bytes), a larger one
-// leaves CUs without work.
+// The tiles, and what a round of the CUs costs with each: us = fixed + step x (steps of 128 KG of K), fitted to 675 problems (M 17 .. 2048,
+// N 512 .. 14336, K 1024 .. 14336); the last three have room for two workgroups on a CU, whose pair costs less than two rounds.  The
+// tile with the least sum of rounds is 0.3 % behind the best one in the mean.  Some of them, us with the best / the second best of another shape:
+// 2048 x 4096 x 14336 256 x 256 112 / 256 x 192 123; 2048 x 14336 x 4096 256 x 128 101 / 128 x 128 118; 1000 x 4096 x 6144 128 x 192 29.4 / 128 x 96 32.9;
+// 201 x 2048 x 5120 128 x 64 9.1 / 64 x 96 9.9; 64 x 5120 x 5120 64 x 32 10.6 / 64 x 64 11.5; 32 x 14336 x 4096 32 x 16 13.6 / 64 x 32 17.4.  A smaller
+// tile reads more through the loads to LDS (68 GB/s per CU for whole lines, 54 for half lines of 64 bytes), a larger one leaves CUs without
+// work.  Eight wavefronts in every tile: 128 x 64 with four is 3 % slower in the median, 11 % at most.
 struct Int8Tile {
   int bm, bn, kg;
   float fixed, step, pair_fixed, pair_step;            // the pair: 0 where a workgroup fills the CU
 };
-constexpr Int8Tile kTiles[] = {{256, 256, 1, 13.3f, 1.29f, 0, 0}, {256, 192, 1, 6.6f, 1.06f, 0, 0},  {256, 128, 1, 6.7f, 0.75f, 0, 0},
-                               {128, 192, 1, 7.3f, 0.62f, 0, 0},  {128, 128, 1, 3.7f, 0.48f, 0, 0},  {64, 96, 2, 4.3f, 0.47f, 0, 0},
-                               {64, 64, 2, 2.6f, 0.36f, 0, 0},    {64, 32, 4, 3.0f, 0.50f, 0, 0},    {32, 64, 4, 2.8f, 0.52f, 0, 0},
-                               {64, 16, 4, 2.4f, 0.39f, 0, 0},    {32, 16, 8, 2.6f, 0.49f, 0, 0},    {128, 64, 1, 1.4f, 0.37f, 2.7f, 0.58f}};
+constexpr Int8Tile kTiles[] = {{256, 256, 1, 9.77f, 1.34f, 0, 0},        {256, 192, 1, 7.54f, 1.11f, 0, 0}, {256, 128, 1, 6.45f, 0.82f, 0, 0},
+                               {128, 192, 1, 6.76f, 0.64f, 0, 0},        {128, 128, 1, 4.21f, 0.52f, 0, 0}, {64, 96, 2, 4.89f, 0.52f, 0, 0},
+                               {64, 64, 2, 3.92f, 0.37f, 0, 0},          {64, 32, 4, 4.22f, 0.52f, 0, 0},   {64, 16, 4, 4.06f, 0.38f, 0, 0},
+                               {32, 16, 8, 3.92f, 0.49f, 0, 0},          {64, 64, 1, 3.49f, 0.24f, 3.39f, 0.40f},
+                               {64, 32, 2, 3.70f, 0.28f, 4.10f, 0.53f},  {128, 64, 1, 3.52f, 0.34f, 3.92f, 0.62f}};
 
 static int pick_tile(long long M, long long N, long long K) {
   const long long cus = int8_cu_count();
@@ -72,10 +73,11 @@ static int launch_product(const Int8GemmArgs& p, hipStream_t st) {
     case 5: return launch_tiles<Act, 64, 96, 2, 2, 2, 3, 3>(p, st);
     case 6: return launch_tiles<Act, 64, 64, 2, 2, 2, 4, 3>(p, st);
     case 7: return launch_tiles<Act, 64, 32, 2, 1, 4, 3, 3>(p, st);
-    case 8: return launch_tiles<Act, 32, 64, 1, 2, 4, 3, 3>(p, st);
-    case 9: return launch_tiles<Act, 64, 16, 2, 1, 4, 3, 3>(p, st);
-    case 10: return launch_tiles<Act, 32, 16, 1, 1, 8, 3, 3>(p, st);
-    default: return launch_tiles<Act, 128, 64, 2, 2, 1, 3, 3>(p, st);
+    case 8: return launch_tiles<Act, 64, 16, 2, 1, 4, 3, 3>(p, st);
+    case 9: return launch_tiles<Act, 32, 16, 1, 1, 8, 3, 3>(p, st);
+    case 10: return launch_tiles<Act, 64, 64, 4, 2, 1, 4, 4>(p, st);
+    case 11: return launch_tiles<Act, 64, 32, 2, 2, 2, 3, 3>(p, st);
+    default: return launch_tiles<Act, 128, 64, 4, 2, 1, 3, 3>(p, st);
   }
 }
 

@@ -65,6 +65,18 @@ def test_product(v, dev, M, K, N, dt):
     _check(out, codes.double(), cs.double(), torch.zeros_like(codes, dtype=torch.bool), w, ws, b, dt, PLAIN)
 
 
+# large and small tiles by what a round of the CUs costs with them, rows of outputs that start on 16 bytes and anywhere
+TILES = [(1500, 656, 8200), (1030, 656, 12289), (517, 656, 14336), (517, 672, 12289), (400, 656, 14336), (400, 672, 12289), (400, 656, 8200),
+         (260, 656, 12289), (201, 656, 8200), (129, 656, 12289), (77, 4112, 8200), (77, 4112, 9001), (30, 2064, 8200), (30, 2064, 9001),
+         (49, 2064, 4008), (49, 2064, 2049), (30, 272, 4008), (30, 656, 6008), (49, 656, 2049), (77, 656, 8200), (77, 656, 9001), (17, 14352, 6144),
+         (31, 14352, 6007)]
+
+
+@pytest.mark.parametrize("M,K,N", TILES)
+def test_product_of_tiles(v, dev, M, K, N):
+    test_product(v, dev, M, K, N, torch.bfloat16 if K % 32 else torch.float16)
+
+
 @pytest.mark.parametrize("M,K,N", SIZES)
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 def test_silu_and_norm_in_front(v, dev, M, K, N, dt):
