@@ -129,7 +129,6 @@ static int run_linear(Linear l, const void* w, const float* w_scale, const void*
   p.w_scale = w_scale;
   p.bias = bias;
   p.out = out;
-  p.wide_out = N % 8 == 0 && aligned16(out);
   p.M = M;
   p.N = N;
   p.K = K;

@@ -22,7 +22,6 @@ struct Int8GemmArgs {
   void* out;
   float* block_scale;
   int M, N, K;                // M: rows of a
-  int wide_out;               // eight outputs per store: N and out allow it
   int tiles_m, tiles_n;
   // Grouped: tile i covers the rows [g_tile[4 i + 1], + g_tile[4 i + 2]) of the expert-sorted order and multiplies them with expert
   // g_tile[4 i]; row r of that order is row g_row[r] of a (null: r).  Expert E is the shared one.  g_tile[4 tiles_m]: tiles in use.
@@ -45,9 +44,6 @@ constexpr size_t int8_gemm_lds(int BM, int BN, int NW, int KG, int SA, int SB, b
   const int loaders = grouped && NW % 2 == 0 ? NW / 2 : NW;
   return (size_t)KG * (SA * BM + SB * BN) * kInt8Step + (BM % (8 * loaders) || BN % (8 * loaders) ? 1024 : 0);
 }
-
-template <class Elem>
-using PairOf = Elem __attribute__((ext_vector_type(2)));
 
 template <class Act, int BM, int BN, int WM, int WN, int KG, int SA, int SB, int EPI, bool GROUPED>
 __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8GemmArgs p) {
@@ -288,18 +284,13 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
         for (int i = 0; i < 4; ++i) add[q][i] = Act::to_f32(raw[q][i]);
     }
   }
-  constexpr int PITCH = HN * 16 + 2;
-  const int nb = n0 + wn * HN * 16;                    // the wavefront's first column
-  unsigned char* const turn = smem + (KG - 1) * BM * BN * 4 + wg * (16 * PITCH * 2);
-  static_assert((KG - 1) * BM * BN * 4 + NW * 16 * PITCH * 2 <= SPARE, "the rings hold the rows on their way out");
-  if constexpr (EPI == kEpiOut && KG == 1)
-    if (!p.wide_out) lds_barrier();                    // nothing is on its way to LDS any more, of no wavefront
   float as[TM];
 #pragma unroll
   for (int t = 0; t < TM; ++t) {
     const int r = (t * WM + wm) * 16 + r16, at = m0 + (r < rows ? r : 0);
     as[t] = p.a_scale[GROUPED && p.g_row ? p.g_row[at] : at];
   }
+  const int nb = n0 + wn * HN * 16;                    // the wavefront's first column
   constexpr int W = GJ;                                // MFMA tiles per store
 #pragma unroll
   for (int t = 0; t < TM; ++t) {
@@ -333,17 +324,18 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
           if constexpr (EPI == kEpiOut) v[i] += add[u][i & 3];
         }
         if constexpr (EPI == kEpiOut) {
-          typedef __attribute__((ext_vector_type(W * 4))) Elem VW;
+          // one store wherever a row starts: global memory takes any address (201 x 2048 x 12290 through LDS to words 14.5 us, like this 12.1)
+          typedef __attribute__((ext_vector_type(W * 4), aligned(sizeof(Elem)))) Elem VW;
           Elem* o = (Elem*)p.out + row + n;
           VW x;
 #pragma unroll
           for (int i = 0; i < W * 4; ++i) x[i] = Act::from_f32(v[i]);
-          if (p.wide_out) {                            // N a multiple of 8, out on a 16-byte boundary
+          if (n + W * 4 <= N) {
             *reinterpret_cast<VW*>(o) = x;
           } else {
-            PairOf<Elem>* to = reinterpret_cast<PairOf<Elem>*>(turn + (r16 * PITCH + n - nb) * 2);
 #pragma unroll
-            for (int i = 0; i < W * 2; ++i) to[i] = PairOf<Elem>{x[2 * i], x[2 * i + 1]};
+            for (int i = 0; i < W * 4; ++i)
+              if (n + i < N) o[i] = x[i];
           }
         } else if constexpr (EPI == kEpiBlock) {       // NO a multiple of 16
           typedef __attribute__((ext_vector_type(W * 4))) short SW;
@@ -353,25 +345,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
           *reinterpret_cast<SW*>((short*)p.out + row + n) = x;
         } else {
           *reinterpret_cast<f32v4*>((float*)p.out + row + n) = f32v4{v[0], v[1], v[2], v[3]};
-        }
-      }
-    }
-    if constexpr (EPI == kEpiOut) {
-      // Rows that start anywhere: through LDS, so that the lanes store a row's columns side by side, two to an aligned word.  Column by
-      // column from the registers, 1000 x 2048 x 12289 took 60 us, N = 12288 33.
-      if (!p.wide_out) {
-        constexpr int PER = HN * 8, RP = 64 / PER;     // lanes per row, rows at a time
-        const int valid = N - nb < HN * 16 ? N - nb : HN * 16, j = lane % PER;
-#pragma unroll
-        for (int r0 = 0; r0 < 16; r0 += RP) {
-          const int rr = r0 + lane / PER, at = (t * WM + wm) * 16 + rr;
-          if (lane / PER >= RP || rr >= 16 || at >= rows) continue;
-          Elem* o = (Elem*)p.out + (size_t)(m0 + at) * N + nb;
-          const Elem* s = reinterpret_cast<const Elem*>(turn) + rr * PITCH;
-          const int odd = (int)((uintptr_t)o >> 1 & 1), c = 2 * j + odd;
-          if (odd && j == 0 && valid > 0) o[0] = s[0];
-          if (c + 1 < valid) *reinterpret_cast<PairOf<Elem>*>(o + c) = PairOf<Elem>{s[c], s[c + 1]};
-          else if (c < valid) o[c] = s[c];
         }
       }
     }
