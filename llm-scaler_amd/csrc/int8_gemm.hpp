@@ -3,9 +3,13 @@
 // A workgroup owns a BM x BN tile.  Both operands go to LDS straight from memory (128-byte pieces of a row per step, no registers
 // and no vector instructions in between) into rings of SA and SB buffers; a wavefront multiplies (16 TM) x (16 TN) of the tile with
 // v_mfma_i32_16x16x64_i8; where a tile's K is long beside its rows and columns, KG groups of wavefronts take a 128-byte piece of every
-// step each, which keeps more loads under way, and their sums meet at the end.  16-byte chunk c of tile row r lies at place c ^ f(r) of its 128 bytes, so that the eight lanes that
-// read at a time find eight different places.  The weights are the first operand: a lane ends with consecutive output columns of
-// one row, 4 per MFMA tile, and the weight rows of GJ tiles are interleaved so that these are 4 GJ in a row.
+// step each, which keeps more loads under way, and their sums meet at the end.  16-byte chunk c of tile row r lies at
+// place c ^ f(r) of its 128 bytes, so that the eight lanes that read at a time find eight different places.  The weights are the first
+// operand: a lane ends with consecutive output columns of one row, 4 per MFMA tile, and the weight rows of GJ tiles are interleaved so that
+// these are 4 GJ in a row.
+//
+// Bound: the matrix cores and the loads that feed them for many rows (2048 x 4096 x 14336 118 us, 2.0 POP/s; 8192^3 2.4), the weights' way from
+// HBM through LDS for few (64 x 5120 x 5120 9.8 us, 2.8 TB/s).
 #pragma once
 #include "int8_common.hpp"
 
@@ -33,7 +37,7 @@ struct Int8GemmArgs {
 };
 
 // What becomes of the sums: 16-bit outputs with a bias; rows of 16-bit integers with an fp32 scale for each wavefront's columns (out,
-// block_scale [rows, ceil(N / block)]: what another launch adds up, off by 2^-16 of the largest of 32 to 96 values, at half the
+// block_scale [rows, ceil(N / block)]: what another launch adds up, off by 2^-16 of the largest of 32 to 128 values, at half the
 // bytes of fp32); SiLU(gate) x up as fp32 rows, gate = weight rows [0, N / 2).
 enum : int { kEpiOut = 0, kEpiBlock = 1, kEpiAct = 2 };
 
@@ -51,7 +55,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   // 1 KiB loads of a wavefront per step.  Grouped: half of the wavefronts load A, half B.  Loads are waited for in the order of their requests,
   // so a wavefront that loads both can have hardly more of one under way than of the other; an expert's weights come from HBM for few
-  // rows and take the deeper ring (128 experts, 4096 tokens, top 8, 2048 / 768: 193 + 166 us with both, 160 + 141 like this; dense
+  // rows and take the deeper ring (128 experts, 4096 tokens, top 8, 2048 / 768: 193 + 166 us with both, 160 + 141 with these roles; dense
   // products, whose operands are in L2 half of the time: 0 to 3 % slower).
   constexpr bool ROLES = GROUPED && NW % 2 == 0;
   constexpr int NL = ROLES ? NW / 2 : NW, LA = (BM / 8 + NL - 1) / NL, LB = (BN / 8 + NL - 1) / NL;
@@ -255,29 +259,57 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
         for (int t = 0; t < TM; ++t) acc[j][t] += sums[q * SUMS + (j * TM + t) * 64];
   }
 
-  // lane: row m of the tile, columns [c, c + 4 GJ) per group of GJ tiles.  The factors of all of its columns are requested together
-  // (indices held inside the row): one at a time, each is a round trip, and these came to 15 us at the end of a tile.
-  float cs[EPI == kEpiAct ? 2 : 1][HN][4], add[EPI == kEpiOut ? HN : 1][4];
+  // lane: row m of the tile, columns [c, c + 4 GJ) per group of GJ tiles.  The factors of all of its columns are requested together, four at
+  // a time (in the tile at N's end one by one, indices held inside the row).
+  typedef __attribute__((ext_vector_type(4), aligned(4))) float Floats;
+  typedef __attribute__((ext_vector_type(4), aligned(2))) Elem Elems;
+  f32v4 cs[EPI == kEpiAct ? 2 : 1][HN];
+  float add[EPI == kEpiOut ? HN : 1][4];
   auto column = [&](int q) __attribute__((always_inline)) { return n0 + wn * HN * 16 + q / GJ * GJ * 16 + g * 4 * GJ + q % GJ * 4; };
+  if (n0 + BNO <= NO) {
 #pragma unroll
-  for (int q = 0; q < HN; ++q)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = column(q) + i < NO ? column(q) + i : NO - 1;
-      cs[0][q][i] = ws[at];
-      if constexpr (EPI == kEpiAct) cs[1][q][i] = ws[NO + at];
+    for (int q = 0; q < HN; ++q) {
+      cs[0][q] = *reinterpret_cast<const Floats*>(ws + column(q));
+      if constexpr (EPI == kEpiAct) cs[1][q] = *reinterpret_cast<const Floats*>(ws + NO + column(q));
     }
+  } else {
+#pragma unroll
+    for (int q = 0; q < HN; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = column(q) + i < NO ? column(q) + i : NO - 1;
+        cs[0][q][i] = ws[at];
+        if constexpr (EPI == kEpiAct) cs[1][q][i] = ws[NO + at];
+      }
+  }
+  bool bad_scale = false;
+  if constexpr (EPI == kEpiBlock) {                    // of the wavefront's columns; those past the last count as zeros
+#pragma unroll
+    for (int q = 0; q < HN; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (column(q) + i >= NO) cs[0][q][i] = 0.0f;
+        bad_scale |= abs_bits(cs[0][q][i]) >= 0x7F800000u;
+      }
+    bad_scale = __any(bad_scale);
+  }
   if constexpr (EPI == kEpiOut) {
 #pragma unroll
     for (int q = 0; q < HN; ++q)
 #pragma unroll
       for (int i = 0; i < 4; ++i) add[q][i] = 0.0f;
     if (p.bias) {
-      Elem raw[HN][4];
+      const Elem* bias = (const Elem*)p.bias;
+      Elems raw[HN];
+      if (n0 + BNO <= NO) {
 #pragma unroll
-      for (int q = 0; q < HN; ++q)
+        for (int q = 0; q < HN; ++q) raw[q] = *reinterpret_cast<const Elems*>(bias + column(q));
+      } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) raw[q][i] = ((const Elem*)p.bias)[column(q) + i < NO ? column(q) + i : NO - 1];
+        for (int q = 0; q < HN; ++q)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) raw[q][i] = bias[column(q) + i < NO ? column(q) + i : NO - 1];
+      }
 #pragma unroll
       for (int q = 0; q < HN; ++q)
 #pragma unroll
@@ -296,25 +328,42 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   for (int t = 0; t < TM; ++t) {
     const int r = (t * WM + wm) * 16 + r16;
     const size_t row = (size_t)(m0 + r) * NO;
-    float to_code = 0.0f;
+    // 16-bit integers: the row's scale goes into theirs alone, the largest value is found in the same pass as the values, and the code is the
+    // low half of a sum whose last place is 1.  The vector ALU bounds this: with eleven instructions per value instead of five, the down
+    // product of 4096 tokens (128 experts, top 8, 2048 / 768) took 146 us, like this 130; without any epilogue 86.
+    float to_code = 0.0f, part[EPI == kEpiBlock ? HN : 1][4];
     if constexpr (EPI == kEpiBlock) {
-      uint32_t top = 0;
+      float m = 0.0f;
 #pragma unroll
       for (int q = 0; q < HN; ++q)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = umax32(top, column(q) < NO ? abs_bits((float)acc[q][t][i] * (as[t] * cs[0][q][i])) : 0u);
-      top = umax32(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-      top = umax32(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-      const float m = __builtin_bit_cast(float, top);
-      const bool bad = top >= 0x7F800000u;             // a NaN, or past fp32
+        for (int i = 0; i < 4; ++i) {
+          part[q][i] = (float)acc[q][t][i] * cs[0][q][i];
+          m = fmaxf(m, __builtin_fabsf(part[q][i]));
+        }
+      m = fmaxf(m, __shfl_xor(m, 16, 64));
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      const bool bad = bad_scale || !(m < INFINITY);
       to_code = bad || m < 0x1p-100f ? 0.0f : 32767.0f / m;
-      if (g == 0 && r < rows && nb < NO) p.block_scale[(size_t)(m0 + r) * ((NO + HN * 16 - 1) / (HN * 16)) + nb / (HN * 16)] = bad ? __builtin_nanf("") : m / 32767.0f;
+      if (g == 0 && r < rows && nb < NO)
+        p.block_scale[(size_t)(m0 + r) * ((NO + HN * 16 - 1) / (HN * 16)) + nb / (HN * 16)] = bad ? __builtin_nanf("") : m / 32767.0f * as[t];
     }
     if (r < rows) {
 #pragma unroll
       for (int q = 0; q < HN; q += W) {
         const int n = column(q);
         if (n >= NO) continue;
+        if constexpr (EPI == kEpiBlock) {              // NO a multiple of 16
+          typedef __attribute__((ext_vector_type(W * 2))) uint32_t CodesW;
+          CodesW x;
+#pragma unroll
+          for (int i = 0; i < W * 2; ++i) {
+            const float lo = __builtin_fmaf(part[q + i / 2][i % 2 * 2], to_code, 0x1.8p23f), hi = __builtin_fmaf(part[q + i / 2][i % 2 * 2 + 1], to_code, 0x1.8p23f);
+            x[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x05040100u);
+          }
+          *reinterpret_cast<CodesW*>((short*)p.out + row + n) = x;
+          continue;
+        }
         float v[W * 4];
 #pragma unroll
         for (int i = 0; i < W * 4; ++i) {              // the sum times a large row scale may pass fp32: the factors first
@@ -337,12 +386,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
             for (int i = 0; i < W * 4; ++i)
               if (n + i < N) o[i] = x[i];
           }
-        } else if constexpr (EPI == kEpiBlock) {       // NO a multiple of 16
-          typedef __attribute__((ext_vector_type(W * 4))) short SW;
-          SW x;
-#pragma unroll
-          for (int i = 0; i < W * 4; ++i) x[i] = (short)(int)__builtin_rintf(to_code == 0.0f ? 0.0f : v[i] * to_code);
-          *reinterpret_cast<SW*>((short*)p.out + row + n) = x;
         } else {
           *reinterpret_cast<f32v4*>((float*)p.out + row + n) = f32v4{v[0], v[1], v[2], v[3]};
         }

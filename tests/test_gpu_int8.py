@@ -450,6 +450,19 @@ def test_expert_layer_masked_and_bad_logits(dev):
             assert bool(got[1].isnan().all()) and torch.equal(got[others], want[others])
 
 
+def test_expert_layer_nan_weight_scale(dev):
+    """A NaN among the down product's scales reaches its own column and at most the 128 that share its tile, of the expert's tokens alone."""
+    import custom_esimd_kernels_vllm  # noqa: F401
+    for T in (1, 60, 300, 900):
+        c = _moe(T, 4, 1, 512, 64, torch.bfloat16, 12, False)
+        want = _moe_run(dev, c, 1)
+        c["s2"][2, 200] = float("nan")
+        got = _moe_run(dev, c, 1)
+        hit = c["logits"].double().argmax(1) == 2
+        assert bool(got[hit, 200].isnan().all()) and torch.equal(got[~hit], want[~hit])
+        assert torch.equal(got[hit][:, :72], want[hit][:, :72]) and torch.equal(got[hit][:, 328:], want[hit][:, 328:])
+
+
 @pytest.mark.parametrize("T", [3, 90, 900, 10000])
 def test_expert_layer_all_to_one_expert(dev, T):
     """Every token takes the same two of many experts: one expert fills tile after tile, the others have no row."""
