@@ -84,8 +84,8 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
 }
 
 // SiLU(g) u, off by a few units in the last place: the exponential and the reciprocal are the hardware's (1 unit each), the rounding of
-// -g log2(e) adds |g| / 2 units where g is negative.  With expf and a division the vector ALU bounds the rows of a decode step: two rows of
-// 14336 in every workgroup 21 us, like this 13.
+// -g log2(e) adds |g| / 2 units where g is negative.  With expf and a division the vector ALU bounds the rows that every workgroup of a
+// decode step makes for itself: the call took 1.6 times as long.
 __device__ __forceinline__ float silu_mul(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -0x1.715476p0f)) * u;
 }

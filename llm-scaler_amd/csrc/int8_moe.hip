@@ -126,6 +126,7 @@ __global__ __launch_bounds__(256) void int8_route_kernel(const Int8MoeArgs p, in
 }
 
 // out[t] = sum_j w[t][j] y[inv[t k + j]] + gate[t] y[P + t], fp32, one rounding; y as kEpiBlock leaves it.  Eight columns per thread.
+// Bound: HBM (4096 tokens of 9 rows of 2048: 29 us, 5.8 TB/s).
 template <class Act>
 __global__ __launch_bounds__(256) void int8_combine_kernel(const short* __restrict__ y, const float* __restrict__ y_scale, int block,
                                                            const int32_t* __restrict__ inv, const typename Act::elem* __restrict__ top_w,
@@ -167,9 +168,9 @@ __global__ __launch_bounds__(256) void int8_combine_kernel(const short* __restri
 // (kEpiBlock) are a wavefront's.  Up to 192 rows there is room for two workgroups on a CU, of eight wavefronts each: one begins and ends its tile
 // while the other multiplies (four wavefronts per workgroup: 3 % slower).  The whole layer, us, tile / next: 128 experts, top 8, 2048 / 768: 200
 // tokens 32 x 128 148 / 64 x 128 150; 600 tokens 64 x 128 166 / 128 x 128 186; 1500 tokens 128 x 128 224 / 192 x 128 236; 2300 tokens 192 x 128 268 /
-// 256 x 256 291; 3500 tokens 256 x 256 341 / 320 x 192 363; 4096 tokens 320 x 192 382 / 256 x 256 394; 64 experts, top 6, 2048 / 1408: 1000 tokens 128 x
-// 128 197 / 192 x 128 212, 1700 tokens 192 x 128 244 / 256 x 256 263; 8 experts, top 2, 4096 / 1536: 1200 tokens 320 x 192 143 / 192 x 128 156, 4096
-// tokens 256 x 256 364 / 192 x 128 372.
+// 256 x 256 281; 3500 tokens 256 x 256 326 / 320 x 192 345; 4096 tokens 320 x 192 367 / 256 x 256 375; 64 experts, top 6, 2048 / 1408: 1000 tokens 128 x
+// 128 197 / 192 x 128 212, 1700 tokens 192 x 128 244 / 256 x 256 263; 8 experts, top 2, 4096 / 1536: 1200 tokens 320 x 192 138 / 192 x 128 152, 4096
+// tokens 256 x 256 357 / 192 x 128 359.
 enum : int { kRows32, kRows64, kRows128, kRows192, kRows256, kRows320 };
 struct GroupTile {
   int rows, block;

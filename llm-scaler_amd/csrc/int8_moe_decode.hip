@@ -1,5 +1,5 @@
 // The expert layer of int8_moe.hip for a few tokens, in two launches.  Bound: the weights of the selected experts, once per token, behind
-// two round trips each.
+// two round trips each: one token of 128 experts, top 8, 2048 / 768 with a shared expert (43 MB) takes 14.6 us, a copy of its bytes 8.3.
 //
 // int8_gate_up_kernel: a wavefront picks the experts of its own columns (as many rounds of the selection as they are down the list),
 // quantises the token's row in its registers and multiplies it with gate and up rows of those columns, all of them in flight; SiLU(gate) x up
@@ -289,8 +289,8 @@ static int launch_decode(const Int8MoeArgs& p, hipStream_t st) {
 
 // Every token reads the experts of its routes and the shared expert for itself; sorted by expert they are read once, by four launches more.
 // The two launches are ahead while what is expected to be read again stays below 120 MB (two launches / six, us; E, top, H, I): 128, 8, 2048,
-// 768: 1 token 16.9 / 30.3, 8 tokens 61 / 75, 12 tokens 86 / 87, 16 tokens 113 / 103; 8, 2, 4096, 1536: 2 tokens 28.5 / 40, 4 tokens 46 / 44,
-// 6 tokens 64 / 42; 64, 6, 2048, 1408: 6 tokens 72 / 73, 10 tokens 110 / 98.
+// 768: 1 token 16.6 / 30, 8 tokens 61 / 75, 12 tokens 87 / 88, 16 tokens 113 / 103; 8, 2, 4096, 1536: 2 tokens 27 / 37, 4 tokens 46 / 45,
+// 6 tokens 64 / 48; 64, 6, 2048, 1408: 6 tokens 69 / 72, 10 tokens 108 / 90.
 bool int8_moe_decode_pays(int T, int k, int E, int H, int I, bool shared) {
   const int routes = k + (shared ? 1 : 0);
   if (H > 4096 || (I / 8 + 63) / 64 * routes > kDownHeld * kDownWaves || routes * I > 60 * 1024) return false;
