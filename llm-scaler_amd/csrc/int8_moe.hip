@@ -164,11 +164,12 @@ __global__ __launch_bounds__(256) void int8_combine_kernel(const short* __restri
   *reinterpret_cast<typename Act::v8*>(out + t * H + c) = o;
 }
 
-// Rows of a tile, by the rows that an expert has on average: most experts in one row tile, up to 320.  The columns that share a scale
+// Rows of a tile, by the rows that an expert has on average: most experts in one row tile, up to 318, then in two.  The columns that share a scale
 // (kEpiBlock) are a wavefront's.  Up to 192 rows there is room for two workgroups on a CU, of eight wavefronts each: one begins and ends its tile
 // while the other multiplies (four wavefronts per workgroup: 3 % slower).  The whole layer, us, tile / next: 128 experts, top 8, 2048 / 768: 200
 // tokens 32 x 128 148 / 64 x 128 150; 600 tokens 64 x 128 166 / 128 x 128 186; 1500 tokens 128 x 128 224 / 192 x 128 236; 2300 tokens 192 x 128 268 /
-// 256 x 256 281; 3500 tokens 256 x 256 326 / 320 x 192 345; 4096 tokens 320 x 192 367 / 256 x 256 375; 64 experts, top 6, 2048 / 1408: 1000 tokens 128 x
+// 256 x 256 281; 3500 tokens 256 x 256 326 / 320 x 192 345; 4096 tokens 320 x 192 367 / 256 x 256 375; 5600
+// tokens 192 x 128 490 / 256 x 256 525, 6500 tokens 256 x 256 568 / 192 x 128 597; 64 experts, top 6, 2048 / 1408: 1000 tokens 128 x
 // 128 197 / 192 x 128 212, 1700 tokens 192 x 128 244 / 256 x 256 263; 8 experts, top 2, 4096 / 1536: 1200 tokens 320 x 192 138 / 192 x 128 152, 4096
 // tokens 256 x 256 357 / 192 x 128 359.
 enum : int { kRows32, kRows64, kRows128, kRows192, kRows256, kRows320 };
@@ -180,8 +181,10 @@ static int group_tile(long long pairs, int E) {
   if (pairs <= 24LL * E) return kRows32;
   if (pairs <= 66LL * E) return kRows64;
   if (pairs <= 125LL * E) return kRows128;
-  if (pairs <= 187LL * E) return kRows192;
-  return pairs <= 230LL * E || pairs > 310LL * E ? kRows256 : kRows320;
+  if (pairs <= 182LL * E) return kRows192;
+  if (pairs <= 245LL * E) return kRows256;
+  if (pairs <= 318LL * E) return kRows320;
+  return pairs <= 385LL * E ? kRows192 : kRows256;     // two of 192, two and more of 256
 }
 
 struct MoeLayout {                                    // byte offsets into the workspace

@@ -361,7 +361,7 @@ def _moe_reference(dev, c, k):
 MOE = [(1, 1, 1, 16, 16), (1, 8, 2, 256, 128), (1, 32, 8, 2048, 768), (2, 5, 5, 272, 48), (3, 130, 8, 1040, 96), (4, 16, 4, 512, 256), (6, 64, 64, 128, 32),
        (8, 8, 8, 2048, 64), (12, 40, 8, 528, 208), (17, 300, 6, 640, 16), (33, 4, 2, 1024, 512), (64, 16, 8, 512, 112), (130, 3, 1, 400, 80),
        (200, 32, 4, 256, 256), (515, 8, 2, 144, 144), (1100, 6, 3, 96, 64), (5, 1024, 10, 64, 16), (1, 4, 2, 8192, 256), (2, 4, 4, 256, 4096), (100, 2, 2, 336, 80), (750, 3, 1, 208, 112),
-       (4200, 8, 2, 64, 48)]
+       (4200, 8, 2, 64, 48), (480, 3, 1, 144, 160), (640, 3, 1, 160, 144), (1050, 3, 1, 208, 112)]
 
 
 @pytest.mark.parametrize("T,E,k,H,I", MOE)
