@@ -175,6 +175,23 @@ def test_nothing_outside_the_output_is_written(v, dev, M):
             assert bool((buf[:lead] == 7).all()) and bool((buf[lead + M * N:] == 7).all())
 
 
+@pytest.mark.parametrize("M", [1, 16, 40, 300])
+def test_operands_on_odd_addresses(v, dev, M):
+    """Scales, bias and row scales start on their element's boundary alone; the results are those of aligned ones."""
+    K, N = 512, 203
+    g, x, w, ws, b = _case(M, K, N, torch.float16, 22, bias=True)
+    xd, wd, wsd, bd = _to(dev, x, w, ws, b)
+    cs = (0.01 + 0.05 * torch.rand(M, generator=g)).to(dev)
+    codes = R.codes_like_weights(g, M, K).to(dev)
+    late = lambda t: torch.cat([t.new_zeros(1), t])[1:]
+    new = lambda: torch.full((M, N), float("nan"), dtype=torch.float16, device=dev)
+    want, got = [new(), new()], [new(), late(new().view(-1)).view(M, N)]
+    for (a, s, r), out in zip(((wsd, bd, cs), (late(wsd), late(bd), late(cs))), (want, got)):
+        v.gemm_int8(xd, None, wd, a, s, out[0])
+        v.gemm_int8(codes, r, wd, a, s, out[1])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and bool(torch.isfinite(got[0]).all())
+
+
 @pytest.mark.parametrize("M", [1, 4, 40, 130])
 def test_weights_past_32_bit_offsets(v, dev, M):
     N, K = 36000, 65536                                   # 2.4 GB
@@ -430,6 +447,17 @@ def test_expert_layer_on_two_streams(dev, T):
         assert torch.equal(other_out, other_want)
         for _, want, out, _ in sets:
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("T", [1, 40, 700])
+def test_expert_layer_on_odd_addresses(dev, T):
+    import custom_esimd_kernels_vllm  # noqa: F401
+    c = {n: t.to(dev) for n, t in _moe(T, 6, 2, 256, 80, torch.bfloat16, 13, True).items()}
+    want = _moe_run(dev, c, 2)
+    for n in ("logits", "s13", "s2", "ss13", "ss2"):
+        c[n] = torch.cat([c[n].new_zeros(1), c[n].reshape(-1)])[1:].view(c[n].shape)
+        assert c[n].data_ptr() % 16
+    assert torch.equal(_moe_run(dev, c, 2), want)
 
 
 def test_expert_layer_masked_and_bad_logits(dev):
