@@ -1,9 +1,9 @@
 // The expert layer of int8_moe.hip for a few tokens, in two launches.  Bound: the weights of the selected experts, once per token, behind
 // two round trips each: one token of 128 experts, top 8, 2048 / 768 with a shared expert (43 MB) takes 14.6 us, a copy of its bytes 8.3.
 //
-// int8_gate_up_kernel: a wavefront picks the experts of its own columns (as many rounds of the selection as they are down the list),
-// quantises the token's row in its registers and multiplies it with gate and up rows of those columns, all of them in flight; SiLU(gate) x up
-// goes out in fp32.  One more workgroup per token writes the selection for the second launch.
+// int8_gate_up_kernel: the first wavefront of a workgroup picks the experts of its columns (as many rounds of the selection as they are down
+// the list); gate and up rows of a wavefront's columns are requested, all of them, and the workgroup quantises the token's row in the
+// meantime, eight values a thread; SiLU(gate) x up goes out in fp32.  One more workgroup per token writes the selection for the second launch.
 //
 // int8_down_kernel: a workgroup quantises the h of a token's routes and of the shared expert into LDS; the k + 1 weight rows that make
 // up an output are one sequence of 16-byte pieces over a wavefront's lanes, every lane scales its partial sums itself (route's weight, h's
@@ -13,7 +13,7 @@
 
 namespace qlin {
 
-constexpr int kGateWaves = 8, kDownWaves = 8;
+constexpr int kGateWaves = 8, kDownWaves = 8, kGateMaxH = 4096;
 constexpr int kDownPieces = 8;                        // weight pieces in flight per lane and row
 constexpr int kDownHeld = 6;                          // pieces of 8 values of h per thread
 
@@ -39,6 +39,10 @@ template <class Act, int SLOTS, int NI, int RP>
 __global__ __launch_bounds__(64 * kGateWaves) void int8_gate_up_kernel(const Int8MoeArgs p) {
   using Elem = typename Act::elem;
   using V8 = typename Act::v8;
+  static_assert(64 * kGateWaves * 8 >= kGateMaxH && NI * 1024 <= kGateMaxH && kGateWaves * RP <= 16, "a piece of x per thread; two routes");
+  __shared__ __attribute__((aligned(16))) unsigned char codes[kGateMaxH];
+  __shared__ uint32_t tops[kGateWaves];
+  __shared__ int chosen[2];                           // the expert of the first and of the last column
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t = blockIdx.y, k = p.k, E = p.E, H = p.H, I = p.I;
   const bool shared = p.shared_w13 != nullptr;
@@ -48,78 +52,87 @@ __global__ __launch_bounds__(64 * kGateWaves) void int8_gate_up_kernel(const Int
                                 shared ? p.gate : nullptr, H >> 3, t);
     return;
   }
-  const int columns = (k + (shared ? 1 : 0)) * I, q0 = (blockIdx.x * kGateWaves + wave) * RP;
-  if (q0 >= columns) return;
+  // the workgroup's columns are of one route or two (kGateWaves RP <= 16 <= I); a wavefront past the last has none
+  const int columns = (k + (shared ? 1 : 0)) * I, c0 = blockIdx.x * kGateWaves * RP, q0 = c0 + wave * RP;
+  const int ra = c0 / I, rb = (min(c0 + kGateWaves * RP, columns) - 1) / I;
   const int pieces = H >> 4;                          // 16-byte pieces of a weight row
-  Elem raws[SLOTS];
+  const int mine_at = threadIdx.x * 8;                // this thread's eight values of x
+  const V8 xv = *reinterpret_cast<const V8*>((const Elem*)p.x + (size_t)t * H + (mine_at < H ? mine_at : 0));
+  if (wave == 0 && ra < k) {
+    Elem raws[SLOTS];
 #pragma unroll
-  for (int s = 0; s < SLOTS; ++s) raws[s] = ((const Elem*)p.logits)[(size_t)t * E + min(s * 64 + lane, E - 1)];
-  V8 xv[NI][2];
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int c = i * 64 + lane < pieces ? i * 64 + lane : pieces - 1;
-    const V8* src = reinterpret_cast<const V8*>((const Elem*)p.x + (size_t)t * H) + 2 * c;
-    xv[i][0] = src[0];
-    xv[i][1] = src[1];
-  }
-  // the experts of this wavefront's first and last column
-  const int r0 = q0 / I, q1 = min(q0 + RP, columns) - 1, r1 = q1 / I;
-  int e0 = 0, e1 = 0;
-  if (r0 < k) {
+    for (int s = 0; s < SLOTS; ++s) raws[s] = ((const Elem*)p.logits)[(size_t)t * E + min(s * 64 + lane, E - 1)];
     uint32_t key[SLOTS];
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       const int e = s * 64 + lane;
       key[s] = e < E ? (f16_order((uint32_t)__builtin_bit_cast(uint16_t, raws[s])) << 16) | (0xFFFFu - (uint32_t)e) : 0u;
     }
-    for (int r = 0; r <= min(r1, k - 1); ++r) {
+    int first = 0, last = 0;
+    for (int r = 0; r <= min(rb, k - 1); ++r) {
       uint32_t best = 0;
 #pragma unroll
       for (int s = 0; s < SLOTS; ++s) best = key[s] > best ? key[s] : best;
       best = wave_max_u32(best);
-      const int cand = __builtin_amdgcn_readfirstlane((int)(0xFFFFu - (best & 0xFFFFu)));
+      last = (int)(0xFFFFu - (best & 0xFFFFu));
 #pragma unroll
       for (int s = 0; s < SLOTS; ++s)
-        if (s * 64 + lane == cand) key[s] = 0u;
-      if (r == r0) e0 = cand;
-      e1 = cand;
+        if (s * 64 + lane == last) key[s] = 0u;
+      if (r == ra) first = last;
     }
-  }
-  i32x4 wv[RP][2][NI];
-  float ws[RP][2];
-#pragma unroll
-  for (int j = 0; j < RP; ++j) {
-    const int q = min(q0 + j, q1), r = q >= r1 * I ? r1 : r0, n = q - r * I;
-    const size_t e = (size_t)(r == r1 ? e1 : e0);
-    const int8_t* w = r >= k ? p.shared_w13 : p.w13 + e * 2 * (size_t)I * H;
-    const float* sc = r >= k ? p.shared_s13 : p.s13 + e * 2 * (size_t)I;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const size_t row = (size_t)(n + u * I);
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int c = i * 64 + lane < pieces ? i * 64 + lane : pieces - 1;
-        wv[j][u][i] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(w + row * H) + c);
-      }
-      ws[j][u] = sc[row];
+    if (lane == 0) {
+      chosen[0] = first;
+      chosen[1] = last;
     }
   }
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
+  for (int j = 0; j < 8; ++j) top = umax32(top, abs_bits(Act::to_f32(xv[j])));         // past the row's end: its first piece again
+  top = wave_umax(top);
+  if (lane == 0) tops[wave] = top;
+  lds_barrier();
+  const int e0 = __builtin_amdgcn_readfirstlane(chosen[0]), e1 = __builtin_amdgcn_readfirstlane(chosen[1]);
+  const int q1 = min(q0 + RP, columns) - 1;
+  i32x4 wv[RP][2][NI];
+  float ws[RP][2];
+  if (q0 < columns) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) top = umax32(top, abs_bits(Act::to_f32(xv[i][j >> 3][j & 7])));   // past the row's end: its last piece again
-  const RowScale s = row_scale(wave_umax(top));
+    for (int j = 0; j < RP; ++j) {
+      const int q = min(q0 + j, q1), r = q >= rb * I ? rb : ra, n = q - r * I;
+      const size_t e = (size_t)(r == ra ? e0 : e1);
+      const int8_t* w = r >= k ? p.shared_w13 : p.w13 + e * 2 * (size_t)I * H;
+      const float* sc = r >= k ? p.shared_s13 : p.s13 + e * 2 * (size_t)I;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const size_t row = (size_t)(n + u * I);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int c = i * 64 + lane < pieces ? i * 64 + lane : pieces - 1;
+          wv[j][u][i] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(w + row * H) + c);
+        }
+        ws[j][u] = sc[row];
+      }
+    }
+  }
+  top = 0;
+#pragma unroll
+  for (int w = 0; w < kGateWaves; ++w) top = umax32(top, tops[w]);
+  const RowScale s = row_scale(top);
+  if (mine_at < H) {
+    uint32_t c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = code_of<true>(Act::to_f32(xv[j]), s.inv);
+    *reinterpret_cast<u32x2*>(codes + mine_at) = u32x2{pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7])};
+  }
+  lds_barrier();
+  if (q0 >= columns) return;
   i32x4 xq[NI];
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t c[4];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) c[b] = code_of<true>(Act::to_f32(xv[i][j >> 1][(j & 1) * 4 + b]), s.inv);
-      xq[i][j] = i * 64 + lane < pieces ? (int)pack4(c[0], c[1], c[2], c[3]) : 0;
-    }
+  for (int i = 0; i < NI; ++i) {
+    const bool in = i * 64 + lane < pieces;
+    xq[i] = *reinterpret_cast<const i32x4*>(codes + (in ? i * 64 + lane : 0) * 16);
+    if (!in) xq[i] = i32x4{0, 0, 0, 0};
+  }
   float mine = 0.0f;                                  // lane j: column q0 + j
 #pragma unroll
   for (int j = 0; j < RP; ++j) {
@@ -293,7 +306,7 @@ static int launch_decode(const Int8MoeArgs& p, hipStream_t st) {
 // 6 tokens 64 / 48; 64, 6, 2048, 1408: 6 tokens 69 / 72, 10 tokens 108 / 90.
 bool int8_moe_decode_pays(int T, int k, int E, int H, int I, bool shared) {
   const int routes = k + (shared ? 1 : 0);
-  if (H > 4096 || (I / 8 + 63) / 64 * routes > kDownHeld * kDownWaves || routes * I > 60 * 1024) return false;
+  if (H > kGateMaxH || (I / 8 + 63) / 64 * routes > kDownHeld * kDownWaves || routes * I > 60 * 1024) return false;
   if ((long long)T * k > 96) return false;
   double missed = 1.0;                                // the share of the experts that no token takes
   for (int t = 0; t < T; ++t) missed *= 1.0 - (double)k / E;
