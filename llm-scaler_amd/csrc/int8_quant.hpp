@@ -58,11 +58,13 @@ struct RowSource {
   }
 };
 
-// TPR threads per row (64 or 256), NV pieces of 8 values per thread in registers; NV = 0: the row is read again for every step.
+// TPR threads per row, NV pieces of 8 values per thread in registers; NV = 0: the row is read again for every step.  TPR = 64: four rows in a
+// workgroup of 256; otherwise a workgroup per row.
 template <class Act, int FROM, int TPR, int NV>
 __device__ __forceinline__ void int8_quant_rows(const QuantArgs& p, int block) {
-  __shared__ float sums[4];
-  __shared__ uint32_t tops[4];
+  constexpr int WAVES = TPR == 64 ? 4 : TPR / 64;
+  __shared__ float sums[WAVES];
+  __shared__ uint32_t tops[WAVES];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, at = TPR == 64 ? lane : threadIdx.x;
   const long long row = TPR == 64 ? (long long)block * 4 + wave : (long long)block;
   if (TPR == 64 && row >= p.rows) return;
@@ -99,7 +101,9 @@ __device__ __forceinline__ void int8_quant_rows(const QuantArgs& p, int block) {
     if constexpr (TPR > 64) {
       if (lane == 0) sums[wave] = ss;
       __syncthreads();
-      ss = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      ss = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; w += 4) ss += (sums[w] + sums[w + 1]) + (sums[w + 2] + sums[w + 3]);
     }
     r = rsqrtf(ss / (float)K + p.eps);
     if constexpr (NV > 0) {
@@ -131,7 +135,8 @@ __device__ __forceinline__ void int8_quant_rows(const QuantArgs& p, int block) {
   if constexpr (TPR > 64) {
     if (lane == 0) tops[wave] = top;
     __syncthreads();
-    top = umax32(umax32(tops[0], tops[1]), umax32(tops[2], tops[3]));
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = umax32(top, tops[w]);
   }
   const RowScale s = row_scale(top);
   if (at == 0) p.scale[row] = s.scale;
