@@ -1,5 +1,5 @@
 // Rows of activations as 8-bit codes and a scale (int8_quant.hip; the expert layer's first launch too).  Bound: HBM (2 bytes in and 1 out per
-// value; 6 and 1 with the residual): SiLU rows of 2048 x 14336 30 us, 4.9 TB/s; 36864 rows of 768 in fp32 22 us, 6.4 TB/s.
+// value; 6 and 1 with the residual): SiLU rows of 2048 x 14336 26 us, 5.6 TB/s; 36864 rows of 768 in fp32 22 us, 6.4 TB/s.
 //
 // A row belongs to a wavefront (short rows) or a workgroup, and its values stay in registers from the one read to the codes: the norm's sum and
 // the row's maximum are reductions in between.  Rows longer than the registers hold are read again for each of these steps.

@@ -220,9 +220,9 @@ __global__ __launch_bounds__(kThreads) void int8_rows_kernel(const Int8RowsArgs 
 
 static long long codes_bytes(int M, int K) { return (long long)M * ((K + 127) / 128) * 128; }
 
-// Every workgroup repeats the work on the rows, a launch in front does it once.  This / a launch of its own, us, bf16: 1 x 4096 x 14336 11.5 / 13.0,
-// 4 x 4096 x 4096 6.9 / 7.5, 8 x 4096 x 4096 9.1 / 8.1, 16 x 2048 x 14336 11.4 / 9.7; SiLU 1 x 14336 x 4096 13.5 / 15.5, 4 x 8192 x 4096 12.3 / 11.1;
-// norm 1 x 4096 x 14336 12.6 / 13.6, 4 x 4096 x 14336 15.0 / 14.0.
+// Every workgroup repeats the work on the rows, a launch in front does it once.  This / a launch of its own, us, bf16: 1 x 4096 x 4096 5.7 / 7.2,
+// 4 x 4096 x 4096 7.0 / 7.9, 8 x 4096 x 4096 9.1 / 8.1, 16 x 2048 x 14336 11.4 / 9.7; SiLU 1 x 14336 x 4096 13.6 / 13.8, 4 x 8192 x 4096 12.3 / 10.9;
+// norm 1 x 4096 x 14336 13.3 / 14.0, 4 x 4096 x 14336 15.0 / 14.0.
 bool int8_rows_quantise(int from, int M, int K) {
   return M <= 16 && (long long)M * ((K / 8 + 63) / 64) <= (from == kFromNorm ? 1 : kPieces) * kWaves;
 }
