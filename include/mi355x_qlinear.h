@@ -674,9 +674,8 @@ int mi_silu_mul_gemm_int8_ws(const void* gate_up, const void* w, const float* w_
 /* A whole mixture-of-experts layer on the same quantisation: softmax top-k of logits [T, E] (renormalised, lowest index first among
  * equals, weights in the activation type as mi_moe_topk gives them), then per token
  *   out = sum_j top_w[j] W2[e_j] q(h_j) + sigmoid(x . gate_weight) shared(x),   h = silu(g) u,   (g, u) = W13[e] q(x),
- * g, u, h and the sum over the experts in fp32, one rounding at the end; with many tokens an expert's result passes to that sum as 16-bit
- * integers with one fp32 scale per 32 to 128 columns (off by 2^-16 of the largest of them; an infinity or a NaN among them, of a w2 scale
- * or past fp32, makes them all NaN).  w13 [E, 2 I, H] (gate rows first), w2 [E, H, I], shared_w13
+ * g, u, h and the sum over the experts in fp32, one rounding at the end; with many tokens an expert's result passes to that sum as a float of
+ * 24 bits (each value off by 2^-16 of itself).  w13 [E, 2 I, H] (gate rows first), w2 [E, H, I], shared_w13
  * [2 I, H], shared_w2 [H, I] int8 with one fp32 scale per row of weights; the shared expert's four operands and gate_weight [H] are all
  * given or all NULL.  H and I as K above, E <= 1024, topk <= 64; T (topk + 1) below 2^24; T H, T (topk + 1) I and 2 I H below 2^31.  x, out, the weights,
  * gate_weight and the workspace (mi_moe_forward_full_int8_workspace bytes) 16-byte aligned; out overlaps no operand.  The 8-bit form

@@ -24,7 +24,7 @@ struct Int8GemmArgs {
   const float* w_scale;       // [N]; grouped [E, N]
   const void* bias;           // [N] in the output's type, or null
   void* out;
-  float* block_scale;
+  unsigned char* low;         // kEpiFloat24
   int M, N, K;                // M: rows of a
   int tiles_m, tiles_n;
   // Grouped: tile i covers the rows [g_tile[4 i + 1], + g_tile[4 i + 2]) of the expert-sorted order and multiplies them with expert
@@ -36,10 +36,14 @@ struct Int8GemmArgs {
   int E;
 };
 
-// What becomes of the sums: 16-bit outputs with a bias; rows of 16-bit integers with an fp32 scale for each wavefront's columns (out,
-// block_scale [rows, ceil(N / block)]: what another launch adds up, off by 2^-16 of the largest of 32 to 128 values, at half the
-// bytes of fp32); SiLU(gate) x up as fp32 rows, gate = weight rows [0, N / 2).
-enum : int { kEpiOut = 0, kEpiBlock = 1, kEpiAct = 2 };
+// What becomes of the sums: 16-bit outputs with a bias; floats of 24 bits, which another launch adds up; SiLU(gate) x up as fp32 rows,
+// gate = weight rows [0, N / 2).
+//
+// kEpiFloat24: an fp32 number's upper 16 bits in out [rows, N], the next 8 in low [rows, N].  Every value is off by 2^-16 of itself, a 32nd of
+// an fp16 output's rounding, whatever the channels beside it are scaled by, for three quarters of the bytes that both launches wait for.
+// (The whole layer of 4096 tokens, 128 experts, top 8, 2048 / 768, us: 383; fp32 numbers 400; 16-bit integers with one scale for a row's 32 to 128
+// columns 346, but beside a channel of 1000 times their scale the others had six bits left.)
+enum : int { kEpiOut = 0, kEpiFloat24 = 1, kEpiAct = 2 };
 
 constexpr int kInt8Step = 128;                        // bytes of a row per step
 
@@ -282,16 +286,11 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
         if constexpr (EPI == kEpiAct) cs[1][q][i] = ws[NO + at];
       }
   }
-  bool bad_scale = false;
-  if constexpr (EPI == kEpiBlock) {                    // of the wavefront's columns; those past the last count as zeros
+  if constexpr (EPI == kEpiFloat24) {                  // a NaN of all ones would be rounded to a number
 #pragma unroll
     for (int q = 0; q < HN; ++q)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (column(q) + i >= NO) cs[0][q][i] = 0.0f;
-        bad_scale |= abs_bits(cs[0][q][i]) >= 0x7F800000u;
-      }
-    bad_scale = __any(bad_scale);
+      for (int i = 0; i < 4; ++i) cs[0][q][i] = cs[0][q][i] == cs[0][q][i] ? cs[0][q][i] : __builtin_nanf("");
   }
   if constexpr (EPI == kEpiOut) {
 #pragma unroll
@@ -322,48 +321,16 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
     const int r = (t * WM + wm) * 16 + r16, at = m0 + (r < rows ? r : 0);
     as[t] = p.a_scale[GROUPED && p.g_row ? p.g_row[at] : at];
   }
-  const int nb = n0 + wn * HN * 16;                    // the wavefront's first column
   constexpr int W = GJ;                                // MFMA tiles per store
 #pragma unroll
   for (int t = 0; t < TM; ++t) {
     const int r = (t * WM + wm) * 16 + r16;
     const size_t row = (size_t)(m0 + r) * NO;
-    // 16-bit integers: the row's scale goes into theirs alone, the largest value is found in the same pass as the values, and the code is the
-    // low half of a sum whose last place is 1.  The vector ALU bounds this: with eleven instructions per value instead of five, the down
-    // product of 4096 tokens (128 experts, top 8, 2048 / 768) took 146 us, like this 130; without any epilogue 86.
-    float to_code = 0.0f, part[EPI == kEpiBlock ? HN : 1][4];
-    if constexpr (EPI == kEpiBlock) {
-      float m = 0.0f;
-#pragma unroll
-      for (int q = 0; q < HN; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          part[q][i] = (float)acc[q][t][i] * cs[0][q][i];
-          m = fmaxf(m, __builtin_fabsf(part[q][i]));
-        }
-      m = fmaxf(m, __shfl_xor(m, 16, 64));
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      const bool bad = bad_scale || !(m < INFINITY);
-      to_code = bad || m < 0x1p-100f ? 0.0f : 32767.0f / m;
-      if (g == 0 && r < rows && nb < NO)
-        p.block_scale[(size_t)(m0 + r) * ((NO + HN * 16 - 1) / (HN * 16)) + nb / (HN * 16)] = bad ? __builtin_nanf("") : m / 32767.0f * as[t];
-    }
     if (r < rows) {
 #pragma unroll
       for (int q = 0; q < HN; q += W) {
         const int n = column(q);
         if (n >= NO) continue;
-        if constexpr (EPI == kEpiBlock) {              // NO a multiple of 16
-          typedef __attribute__((ext_vector_type(W * 2))) uint32_t CodesW;
-          CodesW x;
-#pragma unroll
-          for (int i = 0; i < W * 2; ++i) {
-            const float lo = __builtin_fmaf(part[q + i / 2][i % 2 * 2], to_code, 0x1.8p23f), hi = __builtin_fmaf(part[q + i / 2][i % 2 * 2 + 1], to_code, 0x1.8p23f);
-            x[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x05040100u);
-          }
-          *reinterpret_cast<CodesW*>((short*)p.out + row + n) = x;
-          continue;
-        }
         float v[W * 4];
 #pragma unroll
         for (int i = 0; i < W * 4; ++i) {              // the sum times a large row scale may pass fp32: the factors first
@@ -386,6 +353,21 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
             for (int i = 0; i < W * 4; ++i)
               if (n + i < N) o[i] = x[i];
           }
+        } else if constexpr (EPI == kEpiFloat24) {     // N a multiple of 16
+          typedef __attribute__((ext_vector_type(W * 2))) uint32_t High;
+          typedef __attribute__((ext_vector_type(W))) uint32_t Low;
+          uint32_t b[W * 4];
+#pragma unroll
+          for (int i = 0; i < W * 4; ++i) b[i] = __builtin_bit_cast(uint32_t, v[i]) + 0x80u;
+          High x;
+          Low y;
+#pragma unroll
+          for (int i = 0; i < W * 2; ++i) x[i] = __builtin_amdgcn_perm(b[i * 2 + 1], b[i * 2], 0x07060302u);
+#pragma unroll
+          for (int i = 0; i < W; ++i)                  // the second bytes of four
+            y[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[i * 4 + 3], b[i * 4 + 2], 0x0C0C0501u), __builtin_amdgcn_perm(b[i * 4 + 1], b[i * 4], 0x0C0C0501u), 0x05040100u);
+          *reinterpret_cast<High*>((uint16_t*)p.out + row + n) = x;
+          *reinterpret_cast<Low*>(p.low + row + n) = y;
         } else {
           *reinterpret_cast<f32v4*>((float*)p.out + row + n) = f32v4{v[0], v[1], v[2], v[3]};
         }

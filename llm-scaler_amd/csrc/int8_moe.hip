@@ -17,8 +17,8 @@
 namespace qlin {
 
 constexpr int kSortThreads = 1024;                    // E <= kSortThreads
-// The shared expert's row tiles come last and have fewer rows, so that the last round of workgroups is a short one.  The whole layer, us, with /
-// without: 128 experts, top 8, 2048 / 768, 4096 tokens 349 / 358; 8 experts, top 2, 4096 / 1536, 4096 tokens 327 / 341; of 128 rows 346 and 359.
+// The shared expert's row tiles come last and have fewer rows, so that the last round of workgroups is a short one.  The whole layer, us (with results
+// of 16 bits), with / without: 128 experts, top 8, 2048 / 768, 4096 tokens 349 / 358; 8 experts, top 2, 4096 / 1536, 4096 tokens 327 / 341; of 128 rows 346 and 359.
 __host__ __device__ static inline int shared_rows(int bm) { return bm < 192 ? bm : 192; }
 constexpr int kSortPairs = 8;                         // pairs per thread of int8_sort_kernel
 
@@ -125,24 +125,26 @@ __global__ __launch_bounds__(256) void int8_route_kernel(const Int8MoeArgs p, in
   int8_quant_rows<Act, kFromAct, 256, NV>(a, (int)blockIdx.x - routing);
 }
 
-// out[t] = sum_j w[t][j] y[inv[t k + j]] + gate[t] y[P + t], fp32, one rounding; y as kEpiBlock leaves it.  Eight columns per thread.
-// Bound: HBM (4096 tokens of 9 rows of 2048: 29 us, 5.8 TB/s).
+// out[t] = sum_j w[t][j] y[inv[t k + j]] + gate[t] y[P + t], fp32, one rounding; y as kEpiFloat24 leaves it.  Eight columns per thread.
+// Bound: HBM (4096 tokens of 9 rows of 2048: 40 us, 6.1 TB/s).
 template <class Act>
-__global__ __launch_bounds__(256) void int8_combine_kernel(const short* __restrict__ y, const float* __restrict__ y_scale, int block,
+__global__ __launch_bounds__(256) void int8_combine_kernel(const uint16_t* __restrict__ y, const unsigned char* __restrict__ y_low,
                                                            const int32_t* __restrict__ inv, const typename Act::elem* __restrict__ top_w,
                                                            const float* __restrict__ gate, typename Act::elem* __restrict__ out, int T, int k, int H) {
-  typedef __attribute__((ext_vector_type(8))) short s16x8;
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int per = H / 8, blocks = (H + block - 1) / block;
+  const int per = H / 8;
   const long long t = i / per;
   if (t >= T) return;
-  const int c = (int)(i - t * per) * 8, b = c / block;
+  const int c = (int)(i - t * per) * 8;
   float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
   auto add = [&](size_t row, float w) __attribute__((always_inline)) {
-    const s16x8 a = *reinterpret_cast<const s16x8*>(y + row * H + c);
-    const float f = w * y_scale[row * blocks + b];
+    const u32x4 high = *reinterpret_cast<const u32x4*>(y + row * H + c);
+    const u32x2 low = *reinterpret_cast<const u32x2*>(y_low + row * H + c);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] += f * (float)a[j];
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t bytes = (j & 1 ? 0x07060000u : 0x05040000u) | (uint32_t)(j & 3) << 8 | 0x0Cu;
+      s[j] += w * __builtin_bit_cast(float, __builtin_amdgcn_perm(high[j >> 1], low[j >> 2], bytes));
+    }
   };
   for (int j0 = 0; j0 < k; j0 += 8) {                  // eight rows' positions, then eight rows
     int at[8];
@@ -164,19 +166,15 @@ __global__ __launch_bounds__(256) void int8_combine_kernel(const short* __restri
   *reinterpret_cast<typename Act::v8*>(out + t * H + c) = o;
 }
 
-// Rows of a tile, by the rows that an expert has on average: most experts in one row tile, up to 318, then in two.  The columns that share a scale
-// (kEpiBlock) are a wavefront's.  Up to 192 rows there is room for two workgroups on a CU, of eight wavefronts each: one begins and ends its tile
-// while the other multiplies (four wavefronts per workgroup: 3 % slower).  The whole layer, us, tile / next: 128 experts, top 8, 2048 / 768: 200
-// tokens 32 x 128 148 / 64 x 128 150; 600 tokens 64 x 128 166 / 128 x 128 186; 1500 tokens 128 x 128 224 / 192 x 128 236; 2300 tokens 192 x 128 268 /
-// 256 x 256 281; 3500 tokens 256 x 256 326 / 320 x 192 345; 4096 tokens 320 x 192 367 / 256 x 256 375; 5600
-// tokens 192 x 128 490 / 256 x 256 525, 6500 tokens 256 x 256 568 / 192 x 128 597; 64 experts, top 6, 2048 / 1408: 1000 tokens 128 x
-// 128 197 / 192 x 128 212, 1700 tokens 192 x 128 244 / 256 x 256 263; 8 experts, top 2, 4096 / 1536: 1200 tokens 320 x 192 138 / 192 x 128 152, 4096
-// tokens 256 x 256 357 / 192 x 128 359.
+// Rows of a tile, by the rows that an expert has on average: most experts in one row tile, up to 318, then in two.  Up to 192 rows there is
+// room for two workgroups on a CU, of eight wavefronts each: one begins and ends its tile while the other multiplies (four wavefronts per workgroup:
+// 3 % slower).  The whole layer, us, tile / next: 128 experts, top 8, 2048 / 768: 200 tokens 32 x 128 144 / 64 x 128 146; 600 tokens 64 x 128 168 /
+// 128 x 128 189; 1500 tokens 128 x 128 232 / 192 x 128 245; 2300 tokens 192 x 128 280 / 256 x 256 290; 3500 tokens 256 x 256 344 / 320 x 192 355; 4096 tokens
+// 320 x 192 386 / 256 x 256 405; 5600 tokens 192 x 128 529 / 256 x 256 566, 7000 tokens 256 x 256 638 / 192 x 128 676; 64 experts, top 6, 2048 / 1408:
+// 900 tokens 128 x 128 197 / 192 x 128 212, 1700 tokens 192 x 128 250 / 256 x 256 255; 8 experts, top 2, 4096 / 1536: 1200 tokens 320 x 192 140 /
+// 192 x 128 151, 4096 tokens 256 x 256 347 / 192 x 128 373.
 enum : int { kRows32, kRows64, kRows128, kRows192, kRows256, kRows320 };
-struct GroupTile {
-  int rows, block;
-};
-constexpr GroupTile kGroupTiles[] = {{32, 32}, {64, 32}, {128, 32}, {192, 64}, {256, 128}, {320, 96}};
+constexpr int kGroupRows[] = {32, 64, 128, 192, 256, 320};
 static int group_tile(long long pairs, int E) {
   if (pairs <= 24LL * E) return kRows32;
   if (pairs <= 66LL * E) return kRows64;
@@ -188,7 +186,7 @@ static int group_tile(long long pairs, int E) {
 }
 
 struct MoeLayout {                                    // byte offsets into the workspace
-  long long top_w, ids, gate, pairs, start, inv, row, tile, xq, xs, h, hq, hs, y, ys, bytes;
+  long long top_w, ids, gate, pairs, start, inv, row, tile, xq, xs, h, hq, hs, y, yl, bytes;
   long long P, rows, tiles;
   int tile_kind, bm;
 };
@@ -198,7 +196,7 @@ static MoeLayout moe_layout(int T, int k, int E, int H, int I, int shared) {
   const long long S = shared ? T : 0;
   l.rows = l.P + S;
   l.tile_kind = group_tile(l.P, E);
-  l.bm = kGroupTiles[l.tile_kind].rows;
+  l.bm = kGroupRows[l.tile_kind];
   l.tiles = l.P / l.bm + (l.P < E ? l.P : E) + (S + shared_rows(l.bm) - 1) / shared_rows(l.bm);
   auto take = [&](long long n) { const long long at = l.bytes; l.bytes += (n + 255) / 256 * 256; return at; };
   l.top_w = take(2 * l.P);
@@ -215,7 +213,7 @@ static MoeLayout moe_layout(int T, int k, int E, int H, int I, int shared) {
   l.hq = take(l.rows * I);
   l.hs = take(4 * l.rows);
   l.y = take(2 * l.rows * H);
-  l.ys = take(4 * l.rows * ((H + 31) / 32));
+  l.yl = take(l.rows * H);
   return l;
 }
 
@@ -324,17 +322,18 @@ static int run_moe(const Int8MoeArgs& m, char* ws, hipStream_t st) {
   p.w = m.w2;
   p.w_scale = m.s2;
   p.out = ws + l.y;
-  p.block_scale = (float*)(ws + l.ys);
+  p.low = (unsigned char*)(ws + l.yl);
   p.M = (int)l.rows;
   p.N = H;
   p.K = I;
   p.g_row = nullptr;
   p.shared_w = m.shared_w2;
   p.shared_scale = m.shared_s2;
-  rc = launch_grouped<Act, kEpiBlock>(p, l, st);
+  rc = launch_grouped<Act, kEpiFloat24>(p, l, st);
   if (rc != MI_OK) return rc;
   hipLaunchKernelGGL(int8_combine_kernel<Act>, dim3((unsigned)(((long long)T * (H / 8) + 255) / 256)), dim3(256), 0, st,
-                     (const short*)(ws + l.y), (const float*)(ws + l.ys), kGroupTiles[l.tile_kind].block, inv, (const typename Act::elem*)m.top_w, shared ? m.gate : nullptr, (typename Act::elem*)m.out, T, k, H);
+                     (const uint16_t*)(ws + l.y), p.low, inv, (const typename Act::elem*)m.top_w, shared ? m.gate : nullptr,
+                     (typename Act::elem*)m.out, T, k, H);
   return launch_status();
 }
 
