@@ -93,7 +93,8 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 // Where a row comes from.
 enum : int { kFromAct = 0, kFromNorm = 1, kFromSilu = 2, kFromF32 = 3, kFromCodes = 4 };
 
-// K a multiple of 16 that the integer sums hold; M and N such that a workgroup of 256 per row is a grid of less than 2^32 threads.
+// K a multiple of 16 that the integer sums hold; M and N such that a workgroup of 256 per row is a grid of less than 2^32 threads (a larger one
+// is not refused by the runtime: it starts fewer workgroups).
 constexpr int kInt8MaxRows = (1 << 24) - 1;
 static inline bool int8_sizes(int M, int N, int K) {
   return M >= 0 && N >= 0 && M <= kInt8MaxRows && N <= kInt8MaxRows && K > 0 && K % 16 == 0 && K <= kInt8MaxK;

@@ -25,10 +25,13 @@ static void launch_quant(const QuantArgs& p, hipStream_t st) {
     constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
     hipLaunchKernelGGL((int8_quant_kernel<Act, FROM, TPR, NV>), dim3((unsigned)(TPR == 64 ? (p.rows + 3) / 4 : p.rows)), dim3(TPR == 64 ? 256 : TPR), 0, st, p);
   };
+  // a grid has less than 2^32 threads: past it rows take 256 threads, and are read again where those do not hold them (rows < 2^24: int8_sizes)
+  const auto grid_holds = [&](long long threads) { return p.rows * threads < 1LL << 32; };
   if (pieces <= 64) go(Int<64>{}, Int<1>{});
   else if (pieces <= 128) go(Int<64>{}, Int<2>{});
   else if (pieces <= 256) go(Int<256>{}, Int<1>{});
   else if (pieces <= 512 && FROM != kFromSilu) go(Int<256>{}, Int<2>{});
+  else if (!grid_holds(pieces <= 1024 ? 512 : 1024)) go(Int<256>{}, Int<0>{});
   else if (pieces <= 512) go(Int<512>{}, Int<1>{});
   else if (pieces <= 1024) go(Int<512>{}, Int<2>{});
   else if (pieces <= 2048) go(Int<1024>{}, Int<2>{});
@@ -37,7 +40,7 @@ static void launch_quant(const QuantArgs& p, hipStream_t st) {
 
 int launch_int8_quant(int from, const QuantArgs& p, int act_dtype, hipStream_t st) {
   if (!p.rows) return MI_OK;
-  if (p.rows > 0x7FFFFFFFLL) return MI_ERR_SHAPE;
+  if (p.rows > kInt8MaxRows) return MI_ERR_SHAPE;
   const bool f16 = act_dtype == DT_F16;
   switch (from) {
     case kFromAct: f16 ? launch_quant<ActF16, kFromAct>(p, st) : launch_quant<ActBF16, kFromAct>(p, st); break;

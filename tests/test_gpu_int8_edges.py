@@ -1,4 +1,5 @@
-"""Edges of the 8-bit integer operators: what an expert's result keeps on its way to the weighted sum.  References in 64 bits, as in test_gpu_int8.py."""
+"""Edges of the 8-bit integer operators: what an expert's result keeps on its way to the weighted sum, row counts near the end
+of a grid.  References in 64 bits, as in test_gpu_int8.py."""
 import pytest
 import torch
 
@@ -77,3 +78,45 @@ def test_an_expert_scale_of_nan_stays_in_its_column(v, dev, T):  # noqa: F811
     assert len(hit)
     bad[hit, torch.tensor([40, 41, 43])] = True
     assert bool(got[bad].isnan().all()) and torch.equal(got[~bad], want[~bad])
+
+
+# ------------------------------------------------------------------------------------------------ many rows
+@pytest.mark.parametrize("what,M,K", [("act", (1 << 23) + 5, 4112), ("act", (1 << 22) + 5, 8208), ("norm", (1 << 23) + 5, 4112), ("silu", (1 << 23) + 5, 2064)])
+def test_rows_up_to_the_stated_limit(v, dev, what, M, K):  # noqa: F811
+    """2^32 threads at 512 or 1024 per row are no launch: such a call takes fewer threads per row.  Few rows are filled and looked at."""
+    dt, N = torch.bfloat16, 3
+    row_bytes = {"act": 3 * K, "norm": 5 * K, "silu": 5 * K}[what] + 64
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < M * row_bytes * 1.05:
+        pytest.skip("not enough free memory")
+    g = torch.Generator().manual_seed(K)
+    few = torch.tensor([0, 1, 2, (1 << 22) - 1, 1 << 22, M - 2, M - 1], device=dev)
+    cols = 2 * K if what == "silu" else K
+    rows = torch.randn(len(few), cols, generator=g).to(dt)
+    w, ws = R.codes_like_weights(g, N, K), R.scales(g, N)
+    nw = torch.ones(K, dtype=dt, device=dev)
+    try:
+        x = torch.zeros(M, cols, dtype=dt, device=dev)
+        x[few] = rows.to(dev)
+        out = torch.full((M, N), float("nan"), dtype=dt, device=dev)
+        if what == "act":
+            v.gemm_int8(x, None, w.to(dev), ws.to(dev), None, out)
+            q, rel = R.quantise(rows.double()), 2.0 ** -21
+        elif what == "norm":
+            x_out = torch.empty_like(x)
+            v.resadd_norm_gemm_int8(x, x, x_out, nw, w.to(dev), ws.to(dev), None, out, 1e-6)
+            assert torch.equal(x_out[few], x[few] * 2)
+            del x_out
+            q, rel = R.quantise(R.norm(rows, rows, nw.cpu(), 1e-6)[1], LOOSE), 2.0 ** -15
+        else:
+            v.silu_mul_gemm_int8(x, w.to(dev), ws.to(dev), None, out)
+            q, rel = R.quantise(R.silu_mul(rows.double()), LOOSE), SILU
+        ref, slack = R.product(*q, w, ws)
+        ok, worst = R.within(out[few].cpu(), ref, slack, dt, rel)
+        assert ok, f"{worst:.2f} of the tolerance"
+        rest = torch.ones(M, dtype=torch.bool, device=dev)
+        rest[few] = False
+        assert bool((out[rest] == 0).all())
+    finally:
+        x = x_out = out = rest = None
+        torch.cuda.empty_cache()
