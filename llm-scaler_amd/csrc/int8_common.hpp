@@ -90,6 +90,16 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -0x1.715476p0f)) * u;
 }
 
+// The sum of squares of a wavefront's consecutive values, eight per lane.  A row's sum is that of these parts in their order, in every kernel, and
+// the multiplications and additions are told apart here: a row has the same bits wherever it is quantised.
+constexpr int kNormPart = 512;
+__device__ __forceinline__ float norm_part(const float* v) {
+  float s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s = __builtin_fmaf(v[j], v[j], s);
+  return wave_sum(s);
+}
+
 // Where a row comes from.
 enum : int { kFromAct = 0, kFromNorm = 1, kFromSilu = 2, kFromF32 = 3, kFromCodes = 4 };
 

@@ -63,7 +63,7 @@ struct RowSource {
 template <class Act, int FROM, int TPR, int NV>
 __device__ __forceinline__ void int8_quant_rows(const QuantArgs& p, int block) {
   constexpr int WAVES = TPR == 64 ? 4 : TPR / 64;
-  __shared__ float sums[WAVES];
+  __shared__ float sums[FROM != kFromNorm || TPR == 64 ? 1 : NV ? WAVES * NV : (kInt8MaxK + kNormPart - 1) / kNormPart];
   __shared__ uint32_t tops[WAVES];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, at = TPR == 64 ? lane : threadIdx.x;
   const long long row = TPR == 64 ? (long long)block * 4 + wave : (long long)block;
@@ -85,25 +85,30 @@ __device__ __forceinline__ void int8_quant_rows(const QuantArgs& p, int block) {
   }
   if constexpr (FROM == kFromNorm) {
     float ss = 0.0f;
-    if constexpr (NV > 0) {
+    if constexpr (TPR == 64) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+      for (int i = 0; i < NV; ++i) ss += norm_part(v[i]);
     } else {
-      for (int k = at * 8; k < K; k += TPR * 8) {
-        src.load(k, v[0]);
+      if constexpr (NV > 0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss += v[0][j] * v[0][j];
+        for (int i = 0; i < NV; ++i) {
+          const float part = norm_part(v[i]);
+          if (lane == 0) sums[i * WAVES + wave] = part;
+        }
+      } else {
+        for (int k0 = wave * kNormPart; k0 < K; k0 += TPR * 8) {
+          const int k = k0 + lane * 8;
+          if (k < K) src.load(k, v[0]);
+          else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[0][j] = 0.0f;
+          }
+          const float part = norm_part(v[0]);
+          if (lane == 0) sums[k0 / kNormPart] = part;
+        }
       }
-    }
-    ss = wave_sum(ss);
-    if constexpr (TPR > 64) {
-      if (lane == 0) sums[wave] = ss;
       __syncthreads();
-      ss = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WAVES; w += 4) ss += (sums[w] + sums[w + 1]) + (sums[w + 2] + sums[w + 3]);
+      for (int q = 0; q < (K + kNormPart - 1) / kNormPart; ++q) ss += sums[q];
     }
     r = rsqrtf(ss / (float)K + p.eps);
     if constexpr (NV > 0) {

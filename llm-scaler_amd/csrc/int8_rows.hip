@@ -42,6 +42,7 @@ __global__ __launch_bounds__(kThreads) void int8_rows_kernel(const Int8RowsArgs 
   unsigned char* const codes = smem + kWaves * UNITS * kUnit;                  // [block of 64][row][64]
 
   // rows to be quantised: pieces of 8 values, whole wavefronts per row
+  static_assert(kNormPart == 64 * 8, "a part of the norm's sum is a piece");
   const int waves_per_row = (K / 8 + 63) / 64, pieces = waves_per_row * 64 * M;
   auto row_of = [&](int i) __attribute__((always_inline)) { return (i * kWaves + wave) / waves_per_row; };
   auto k_of = [&](int i, int row) __attribute__((always_inline)) { return ((i * kWaves + wave - row * waves_per_row) * 64 + lane) * 8; };
@@ -110,10 +111,7 @@ __global__ __launch_bounds__(kThreads) void int8_rows_kernel(const Int8RowsArgs 
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         if (i * kThreads >= pieces) break;
-        float ss = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
-        ss = wave_sum(ss);
+        const float ss = norm_part(v[i]);
         if (lane == 0) part_sum[i * kWaves + wave] = ss;
       }
       lds_barrier();

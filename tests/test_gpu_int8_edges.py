@@ -1,5 +1,5 @@
-"""Edges of the 8-bit integer operators: what an expert's result keeps on its way to the weighted sum, row counts near the end
-of a grid.  References in 64 bits, as in test_gpu_int8.py."""
+"""Edges of the 8-bit integer operators: what an expert's result keeps on its way to the weighted sum, a norm's row over batch
+sizes, row counts near the end of a grid.  References in 64 bits, as in test_gpu_int8.py."""
 import pytest
 import torch
 
@@ -78,6 +78,36 @@ def test_an_expert_scale_of_nan_stays_in_its_column(v, dev, T):  # noqa: F811
     assert len(hit)
     bad[hit, torch.tensor([40, 41, 43])] = True
     assert bool(got[bad].isnan().all()) and torch.equal(got[~bad], want[~bad])
+
+
+# ------------------------------------------------------------------------------------------------ rows over batch sizes
+@pytest.mark.parametrize("K", [272, 512, 1024, 1040, 2048, 2064, 4096, 4112, 8192, 16384, 16400, 40000])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_a_row_behind_norm_or_silu_depends_on_itself_alone(v, dev, K, dt):  # noqa: F811
+    """A row's bits are the same whichever launch quantises it: alone, among few or many, residual in place or not."""
+    M, N = 400, 1000
+    g = torch.Generator().manual_seed(K)
+    x, res = (torch.randn(M, K, generator=g).to(dt).to(dev) for _ in range(2))
+    nw = (1 + 0.1 * torch.randn(K, generator=g)).to(dt).to(dev)
+    w, ws, b = R.codes_like_weights(g, N, K).to(dev), R.scales(g, N).to(dev), torch.randn(N, generator=g).to(dt).to(dev)
+    gate_up = torch.cat([x, res], 1)
+
+    def norm(lo, hi, in_place=False):
+        out, r = x.new_empty(hi - lo, N), res[lo:hi].clone()
+        r_out = r if in_place else torch.empty_like(r)
+        v.resadd_norm_gemm_int8(x[lo:hi], r, r_out, nw, w, ws, b, out, 1e-6)
+        return out
+
+    def silu(lo, hi):
+        out = x.new_empty(hi - lo, N)
+        v.silu_mul_gemm_int8(gate_up[lo:hi], w, ws, b, out)
+        return out
+    whole, whole_silu = norm(0, M), silu(0, M)
+    assert torch.equal(norm(0, M, True), whole)
+    cuts = list(range(48)) + [50, 54, 62, 78, 110, 210, M]
+    for lo, hi in zip(cuts, cuts[1:]):
+        assert torch.equal(norm(lo, hi), whole[lo:hi]) and torch.equal(norm(lo, hi, True), whole[lo:hi])
+        assert torch.equal(silu(lo, hi), whole_silu[lo:hi])
 
 
 # ------------------------------------------------------------------------------------------------ many rows
