@@ -11,7 +11,7 @@ static int launch_tiles(Int8GemmArgs p, hipStream_t st) {
   p.tiles_n = (p.N + BN - 1) / BN;
   const long long tiles = (long long)p.tiles_m * p.tiles_n, grid = (tiles + 7) / 8 * 8;          // linear_sizes: below 2^23
   auto* kernel = int8_gemm_kernel<Act, BM, BN, WM, WN, KG, SA, SB, kEpiOut, false>;
-  constexpr size_t lds = int8_gemm_lds(BM, BN, WM * WN, KG, SA, SB, false);
+  constexpr size_t lds = int8_gemm_lds(BM, BN, KG, SA, SB);
   if constexpr (lds > 64 * 1024) {
     static std::atomic<unsigned long long> raised{0};
     const int rc = int8_raise_lds(kernel, raised, lds);

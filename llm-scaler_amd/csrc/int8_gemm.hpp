@@ -47,11 +47,8 @@ enum : int { kEpiOut = 0, kEpiFloat24 = 1, kEpiAct = 2 };
 
 constexpr int kInt8Step = 128;                        // bytes of a row per step
 
-// LDS of a tile: the rings and, where the tile's rows do not divide among the wavefronts that load them, the place of the loads that are over.
-constexpr size_t int8_gemm_lds(int BM, int BN, int NW, int KG, int SA, int SB, bool grouped) {
-  const int loaders = grouped && NW % 2 == 0 ? NW / 2 : NW;
-  return (size_t)KG * (SA * BM + SB * BN) * kInt8Step + (BM % (8 * loaders) || BN % (8 * loaders) ? 1024 : 0);
-}
+// LDS of a tile: the rings
+constexpr size_t int8_gemm_lds(int BM, int BN, int KG, int SA, int SB) { return (size_t)KG * (SA * BM + SB * BN) * kInt8Step; }
 
 template <class Act, int BM, int BN, int WM, int WN, int KG, int SA, int SB, int EPI, bool GROUPED>
 __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8GemmArgs p) {
@@ -62,14 +59,13 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   // rows and take the deeper ring (128 experts, 4096 tokens, top 8, 2048 / 768: 193 + 166 us with both, 160 + 141 with these roles; dense
   // products, whose operands are in L2 half of the time: 0 to 3 % slower).
   constexpr bool ROLES = GROUPED && NW % 2 == 0;
-  constexpr int NL = ROLES ? NW / 2 : NW, LA = (BM / 8 + NL - 1) / NL, LB = (BN / 8 + NL - 1) / NL;
+  constexpr int NL = ROLES ? NW / 2 : NW, LA = BM / (8 * NL), LB = BN / (8 * NL);
   constexpr int HN = EPI == kEpiAct ? TN / 2 : TN;    // MFMA tiles of gate (or all) columns
   // columns in a row per lane: a store instruction writes 64 bytes of 16 rows then (with 4 tiles in a row, half sectors: 85 us for 302 MB)
   constexpr int GJ = EPI != kEpiAct && HN % 2 == 0 ? 2 : 1;
   constexpr int A_PART = BM * kInt8Step, B_PART = BN * kInt8Step, B_RING = SA * KG * A_PART;   // the ring of A, that of B
-  constexpr int SPARE = B_RING + SB * KG * B_PART;    // and 1 KiB that a load lands in which a wavefront has over
   static_assert(SA >= 2 && SB >= 2 && (ROLES || SA == SB || SA == SB + 1), "rings");
-  static_assert((!GROUPED || TM <= 5) && TM * 16 * WM == BM && TN * 16 * WN == BN, "tile");
+  static_assert((!GROUPED || TM <= 5) && TM * 16 * WM == BM && TN * 16 * WN == BN && LA * 8 * NL == BM && LB * 8 * NL == BN, "tile");
   static_assert(HN * (EPI == kEpiAct ? 2 : 1) == TN && HN % GJ == 0, "columns");
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
 
@@ -137,7 +133,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
         in = n0 + col < NO;
         row = q < TN * 8 ? col : NO + col;
       }
-      from[FIRST_B + i] = in && r < BN ? (uint32_t)row * (uint32_t)K + chunk[FIRST_B + i] : kOOB;
+      from[FIRST_B + i] = in ? (uint32_t)row * (uint32_t)K + chunk[FIRST_B + i] : kOOB;
     }
   }
   const int8_t* a0 = GROUPED ? p.a : p.a + (size_t)m0 * K;
@@ -150,7 +146,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
   auto request = [&](auto is_a, int s, int slot) __attribute__((always_inline)) {
     constexpr bool A = decltype(is_a)::value;
     constexpr int COUNT = A ? LA : LB, FIRST = A ? 0 : FIRST_B;
-    constexpr bool EVEN = COUNT * NL * 8 == (A ? BM : BN);
     if (!(A ? loads_a : loads_b)) return;
     const int to = A ? (slot * KG + wk) * A_PART + wl * LA * 1024 : B_RING + (slot * KG + wk) * B_PART + wl * LB * 1024;
     const int k0 = s * STEP;
@@ -158,8 +153,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void int8_gemm_kernel(const Int8
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
       const uint32_t f = whole || k0 + chunk[FIRST + i] < K ? from[FIRST + i] : kOOB;   // past the row's end: zeros
-      const int at = EVEN || (wl * COUNT + i) * 8 < (A ? BM : BN) ? to + i * 1024 : SPARE;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(A ? ra : rb, (lds_ptr)(smem + at), 16, f, k0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(A ? ra : rb, (lds_ptr)(smem + to + i * 1024), 16, f, k0, 0, 0);
     }
   };
   constexpr std::true_type a_tag{};

@@ -226,7 +226,7 @@ static int launch_tiles(Int8GemmArgs p, long long tiles, hipStream_t st) {
   const long long grid = (tiles + 7) / 8 * 8 * p.tiles_n;
   if (grid > 0x7FFFFFFFLL) return MI_ERR_SHAPE;
   auto* kernel = int8_gemm_kernel<Act, BM, BN, WM, WN, KG, SA, SB, EPI, true>;
-  constexpr size_t lds = int8_gemm_lds(BM, BN, WM * WN, KG, SA, SB, true);
+  constexpr size_t lds = int8_gemm_lds(BM, BN, KG, SA, SB);
   if constexpr (lds > 64 * 1024) {
     static std::atomic<unsigned long long> raised{0};
     const int rc = int8_raise_lds(kernel, raised, lds);
