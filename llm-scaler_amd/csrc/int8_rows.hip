@@ -2,7 +2,7 @@
 //
 // A workgroup of 16 wavefronts owns 16 columns per slot; the KS = 16 / slots wavefronts of a slot each take a part of K, so that all of a
 // CU's loads are in flight at once however few columns there are.  Weights go to LDS straight from memory, 128 bytes of 16 rows
-// (2 KiB) at a time into a ring of UNITS that is the wavefront's own: whole lines for the loads, and the operands of
+// (2 KiB) at a time into a ring of kUnits that is the wavefront's own: whole lines for the loads, and the operands of
 // v_mfma_i32_16x16x64_i8 read back without a barrier.  16-byte chunk c of row r lies at place c ^ (r & 7) of its 128 bytes.  The
 // codes lie in LDS in operand order.  The parts of K meet in LDS as integers.
 //
@@ -19,9 +19,9 @@ namespace qlin {
 constexpr int kWaves = 16, kThreads = 64 * kWaves;
 constexpr int kPieces = 2;                            // pieces of 8 values per thread that a workgroup quantises
 constexpr int kChunks = 4;                            // chunks of 16 codes per thread that it takes as they are
-constexpr int kUnit = 2048;                           // bytes of a ring's unit: 16 rows x 128
+constexpr int kUnit = 2048, kUnits = 2;               // bytes of a ring's unit: 16 rows x 128; units of a ring
 
-template <class Act, int FROM, int UNITS>
+template <class Act, int FROM>
 __global__ __launch_bounds__(kThreads) void int8_rows_kernel(const Int8RowsArgs p) {
   using Elem = typename Act::elem;
   using V8 = typename Act::v8;
@@ -38,8 +38,8 @@ __global__ __launch_bounds__(kThreads) void int8_rows_kernel(const Int8RowsArgs 
   const int b0 = part * per, b1 = b0 + per < blocks ? b0 + per : blocks;
   const int n0 = (blockIdx.x * slots + slot) * 16, cols = n0 < N ? (N - n0 < 16 ? N - n0 : 16) : 0;
   const __amdgpu_buffer_rsrc_t rw = make_rsrc(cols ? p.w + (size_t)n0 * K : p.w, (uint32_t)cols * (uint32_t)K);
-  unsigned char* const ring = smem + wave * (UNITS * kUnit);
-  unsigned char* const codes = smem + kWaves * UNITS * kUnit;                  // [block of 64][row][64]
+  unsigned char* const ring = smem + wave * (kUnits * kUnit);
+  unsigned char* const codes = smem + kWaves * kUnits * kUnit;                  // [block of 64][row][64]
 
   // rows to be quantised: pieces of 8 values, whole wavefronts per row
   static_assert(kNormPart == 64 * 8, "a part of the norm's sum is a piece");
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kThreads) void int8_rows_kernel(const Int8RowsArgs 
   };
   asm volatile("" ::: "memory");
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) request(u, b0 + u);
+  for (int u = 0; u < kUnits; ++u) request(u, b0 + u);
 
   if constexpr (!kCodes) {
     float v[kPieces][8];
@@ -172,11 +172,11 @@ __global__ __launch_bounds__(kThreads) void int8_rows_kernel(const Int8RowsArgs 
   int w_at[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) w_at[h] = r16 * 128 + (((h * 4 + g) ^ (r16 & 7)) * 16);
-  for (int b = b0; b < b1; b += UNITS) {
+  for (int b = b0; b < b1; b += kUnits) {
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
+    for (int u = 0; u < kUnits; ++u) {
       const int at = b + u < blocks ? b + u : blocks - 1;        // the weights beyond are zeros
-      wait_loads<2 * (UNITS - 1)>();
+      wait_loads<2 * (kUnits - 1)>();
       i32x4 w[2], x[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(kThreads) void int8_rows_kernel(const Int8RowsArgs 
         x[h] = *reinterpret_cast<const i32x4*>(x_at + (at * 2 + h) * M * 64);
       }
       wait_loads<63>();                                // read before the unit is asked for again
-      request(u, b + UNITS + u);
+      request(u, b + kUnits + u);
 #pragma unroll
       for (int h = 0; h < 2; ++h) acc[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[h], x[h], acc[h], 0, 0, 0);
     }
@@ -226,15 +226,15 @@ bool int8_rows_quantise(int from, int M, int K) {
 }
 bool int8_rows_codes(int M, int K) { return M <= 16 && codes_bytes(M, K) <= kChunks * kThreads * 16; }
 
-template <class Act, int FROM, int UNITS>
+template <class Act, int FROM>
 static int go(const Int8RowsArgs& p, hipStream_t st) {
   const int width = (kWaves >> p.ks_log2) * 16;
-  auto* kernel = int8_rows_kernel<Act, FROM, UNITS>;
+  auto* kernel = int8_rows_kernel<Act, FROM>;
   static std::atomic<unsigned long long> raised{0};
-  const int rc = int8_raise_lds(kernel, raised, kWaves * UNITS * kUnit + (FROM == kFromCodes ? 64 : 16) * 1024);
+  const int rc = int8_raise_lds(kernel, raised, kWaves * kUnits * kUnit + (FROM == kFromCodes ? 64 : 16) * 1024);
   if (rc != MI_OK) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)((p.N + width - 1) / width)), dim3(kThreads),
-                     kWaves * UNITS * kUnit + (size_t)codes_bytes(p.M, p.K), st, p);
+                     kWaves * kUnits * kUnit + (size_t)codes_bytes(p.M, p.K), st, p);
   return launch_status();
 }
 
@@ -244,11 +244,11 @@ static int launch(int from, Int8RowsArgs p, hipStream_t st) {
   p.ks_log2 = 4;                                       // as many parts of K as leave the columns in one round of the CUs
   while (p.ks_log2 > 0 && tiles > cus * (kWaves >> p.ks_log2)) --p.ks_log2;
   switch (from) {
-    case kFromAct: return go<Act, kFromAct, 2>(p, st);
-    case kFromNorm: return go<Act, kFromNorm, 2>(p, st);
-    case kFromSilu: return go<Act, kFromSilu, 2>(p, st);
+    case kFromAct: return go<Act, kFromAct>(p, st);
+    case kFromNorm: return go<Act, kFromNorm>(p, st);
+    case kFromSilu: return go<Act, kFromSilu>(p, st);
   }
-  return go<Act, kFromCodes, 2>(p, st);
+  return go<Act, kFromCodes>(p, st);
 }
 
 int launch_int8_rows(int from, const Int8RowsArgs& p, int act_dtype, hipStream_t st) {
