@@ -22,21 +22,6 @@ __device__ __forceinline__ uint32_t umax32(uint32_t a, uint32_t b) { return a > 
 // |v| as an ordered integer: NaN above infinity above every number
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
 
-template <int CTRL>
-__device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
-  return umax32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true));
-}
-__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-  v = dpp_umax<0xB1>(v);
-  v = dpp_umax<0x4E>(v);
-  v = dpp_umax<0x141>(v);
-  v = dpp_umax<0x140>(v);
-  uint32_t r = (uint32_t)__builtin_amdgcn_readlane((int)v, 0);
-  r = umax32(r, (uint32_t)__builtin_amdgcn_readlane((int)v, 16));
-  r = umax32(r, (uint32_t)__builtin_amdgcn_readlane((int)v, 32));
-  return umax32(r, (uint32_t)__builtin_amdgcn_readlane((int)v, 48));
-}
-
 // LDS that is written straight from memory (no registers in between): the compiler does not see when such a load lands, so every kernel
 // here waits for itself.  N: loads that may still be under way, the newest ones; LDS reads and writes of the wavefront are done too.
 template <int N>

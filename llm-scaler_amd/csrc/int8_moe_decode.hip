@@ -89,7 +89,7 @@ __global__ __launch_bounds__(64 * kGateWaves) void int8_gate_up_kernel(const Int
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) top = umax32(top, abs_bits(Act::to_f32(xv[j])));         // past the row's end: its first piece again
-  top = wave_umax(top);
+  top = wave_max_u32(top);
   if (lane == 0) tops[wave] = top;
   lds_barrier();
   const int e0 = __builtin_amdgcn_readfirstlane(chosen[0]), e1 = __builtin_amdgcn_readfirstlane(chosen[1]);
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(64 * kDownWaves) void int8_down_kernel(const Int8Mo
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = umax32(top, abs_bits(hv[i][j >> 2][j & 3]));
     }
-    top = wave_umax(top);
+    top = wave_max_u32(top);
     if (lane == 0) tops[i * kDownWaves + wave] = top;
   }
   lds_barrier();

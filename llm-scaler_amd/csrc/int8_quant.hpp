@@ -136,7 +136,7 @@ __device__ __forceinline__ void int8_quant_rows(const QuantArgs& p, int block) {
       for (int j = 0; j < 8; ++j) top = umax32(top, abs_bits(v[0][j]));
     }
   }
-  top = wave_umax(top);
+  top = wave_max_u32(top);
   if constexpr (TPR > 64) {
     if (lane == 0) tops[wave] = top;
     __syncthreads();

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(kThreads) void int8_rows_kernel(const Int8RowsArgs 
       uint32_t top = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = umax32(top, abs_bits(v[i][j]));
-      top = wave_umax(top);
+      top = wave_max_u32(top);
       if (lane == 0) part_top[i * kWaves + wave] = top;
     }
     lds_barrier();

@@ -14,24 +14,6 @@ namespace qlin {
 // the winner's logit is recovered from the key itself.
 constexpr int kTopkSlots = 16;                       // up to 1024 experts
 
-template <int CTRL>
-__device__ __forceinline__ uint32_t dpp_max_u32(uint32_t v) {
-  const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
-  return o > v ? o : v;
-}
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-  v = dpp_max_u32<0xB1>(v);
-  v = dpp_max_u32<0x4E>(v);
-  v = dpp_max_u32<0x141>(v);
-  v = dpp_max_u32<0x140>(v);
-  uint32_t r = 0;
-#pragma unroll
-  for (int row = 0; row < 4; ++row) {
-    const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)v, row * 16);
-    r = o > r ? o : r;
-  }
-  return r;
-}
 // 16-bit float pattern (fp16 or bf16) -> unsigned, monotone, and back; the smallest key, 0, is kept for
 // "no value" (it would be the pattern of the negative NaN with every bit set)
 // -0 is ordered as +0: a float compare calls them equal, and then the lowest index wins the tie

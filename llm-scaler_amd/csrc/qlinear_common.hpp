@@ -243,6 +243,26 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// Maximum of unsigned integers over the 64 lanes, as wave_sum goes.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max_u32(uint32_t v) {
+  const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+  return o > v ? o : v;
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  v = dpp_max_u32<0xB1>(v);
+  v = dpp_max_u32<0x4E>(v);
+  v = dpp_max_u32<0x141>(v);
+  v = dpp_max_u32<0x140>(v);
+  uint32_t r = 0;
+#pragma unroll
+  for (int row = 0; row < 4; ++row) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)v, row * 16);
+    r = o > r ? o : r;
+  }
+  return r;
+}
+
 static inline int launch_status() {
   return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }
