@@ -304,9 +304,10 @@ static int launch_decode(const Int8MoeArgs& p, hipStream_t st) {
 }
 
 // Every token reads the experts of its routes and the shared expert for itself; sorted by expert they are read once, by four launches more.
-// The two launches are ahead while what is expected to be read again stays below 120 MB (two launches / six, us; E, top, H, I): 128, 8, 2048,
-// 768: 1 token 16.6 / 30, 8 tokens 61 / 75, 12 tokens 87 / 88, 16 tokens 113 / 103; 8, 2, 4096, 1536: 2 tokens 27 / 37, 4 tokens 46 / 45,
-// 6 tokens 64 / 48; 64, 6, 2048, 1408: 6 tokens 69 / 72, 10 tokens 108 / 90.
+// The two launches are ahead while what is expected to be read again stays below 100 MB (two launches / six, us, with a shared expert; E, top, H, I):
+// 128, 8, 2048, 768: 1 token 14.8 / 29.6, 8 tokens (91 MB) 60 / 74, 10 tokens (133) 76 / 78, 14 tokens 102 / 92; 8, 2, 4096, 1536: 2 tokens 26 / 37,
+// 3 tokens (64) 39 / 41, 4 tokens (104) 44 / 41, 6 tokens 63 / 47; 64, 6, 2048, 1408: 4 tokens (53) 47 / 62, 6 tokens (108) 71 / 72, 8 tokens 82 / 80; 16, 2,
+// 2048, 1024: 6 tokens (51) 30 / 31, 8 tokens (79) 34 / 33, 12 tokens (140) 47 / 34; 32, 4, 1024, 512: 8 tokens (28) 19 / 27, 16 tokens (80) 30 / 28.
 bool int8_moe_decode_pays(int T, int k, int E, int H, int I, bool shared) {
   const int routes = k + (shared ? 1 : 0);
   if (H > kGateMaxH || (I / 8 + 63) / 64 * routes > kDownHeld * kDownWaves || routes * I > 60 * 1024) return false;
@@ -314,7 +315,7 @@ bool int8_moe_decode_pays(int T, int k, int E, int H, int I, bool shared) {
   double missed = 1.0;                                // the share of the experts that no token takes
   for (int t = 0; t < T; ++t) missed *= 1.0 - (double)k / E;
   const double again = (double)T * routes - E * (1.0 - missed) - (shared ? 1 : 0);
-  return again * 3.0 * H * I <= 120e6;
+  return again * 3.0 * H * I <= 100e6;
 }
 int launch_int8_moe_decode(const Int8MoeArgs& p, int act_dtype, hipStream_t st) {
   return act_dtype == DT_F16 ? launch_decode<ActF16>(p, st) : launch_decode<ActBF16>(p, st);
