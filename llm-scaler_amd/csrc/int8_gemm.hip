@@ -23,9 +23,10 @@ static int launch_tiles(Int8GemmArgs p, hipStream_t st) {
 
 // The tiles, and what a round of the CUs costs with each: us = fixed + step x (steps of 128 KG of K), fitted to 675 problems (M 17 .. 2048,
 // N 512 .. 14336, K 1024 .. 14336); the last three have room for two workgroups on a CU, whose pair costs less than two rounds.  The
-// tile with the least sum of rounds is 0.3 % behind the best one in the mean.  Some of them, us with the best / the second best of another shape:
-// 2048 x 4096 x 14336 256 x 256 112 / 256 x 192 123; 2048 x 14336 x 4096 256 x 128 101 / 128 x 128 118; 1000 x 4096 x 6144 128 x 192 29.4 / 128 x 96 32.9;
-// 201 x 2048 x 5120 128 x 64 9.1 / 64 x 96 9.9; 64 x 5120 x 5120 64 x 32 10.6 / 64 x 64 11.5; 32 x 14336 x 4096 32 x 16 13.6 / 64 x 32 17.4.  A smaller
+// tile with the least sum of rounds is 0.3 % behind the best one in the mean.  Some of them, us with the best / the second best of another shape,
+// all tiles one after the other (the clocks of the large ones are lower then than in a call alone): 2048 x 4096 x 14336 256 x 256 135 / 256 x 192 147;
+// 2048 x 14336 x 4096 256 x 128 116 / 128 x 128 135; 1000 x 4096 x 6144 128 x 192 29.6 / 256 x 128 32.5; 201 x 2048 x 5120 128 x 64 9.3 / 64 x 64 9.7;
+// 64 x 5120 x 5120 64 x 32 10.3 / 64 x 64 12.3; 32 x 14336 x 4096 32 x 16 13.4 / 64 x 16 14.8.  A smaller
 // tile reads more through the loads to LDS (68 GB/s per CU for whole lines, 54 for half lines of 64 bytes), a larger one leaves CUs without
 // work.  Eight wavefronts in every tile: 128 x 64 with four is 3 % slower in the median, 11 % at most.
 struct Int8Tile {

@@ -8,8 +8,8 @@
 // operand: a lane ends with consecutive output columns of one row, 4 per MFMA tile, and the weight rows of GJ tiles are interleaved so that
 // these are 4 GJ in a row.
 //
-// Bound: the matrix cores and the loads that feed them for many rows (2048 x 4096 x 14336 118 us, 2.0 POP/s; 8192^3 2.4), the weights' way from
-// HBM through LDS for few (64 x 5120 x 5120 9.8 us, 2.8 TB/s).
+// Bound: the matrix cores and the loads that feed them for many rows (2048 x 4096 x 14336 116 us, 2.1 POP/s; 8192^3 454 us, 2.4), the weights' way
+// from HBM through LDS for few (64 x 5120 x 5120 10.0 us, 2.9 TB/s).
 #pragma once
 #include "int8_common.hpp"
 

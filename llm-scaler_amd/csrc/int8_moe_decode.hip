@@ -1,5 +1,5 @@
 // The expert layer of int8_moe.hip for a few tokens, in two launches.  Bound: the weights of the selected experts, once per token, behind
-// two round trips each: one token of 128 experts, top 8, 2048 / 768 with a shared expert (43 MB) takes 13.2 us (7.2 + 6.0), a copy of its bytes 8.3.
+// two round trips each: one token of 128 experts, top 8, 2048 / 768 with a shared expert (43 MB) takes 13.3 us (7.3 + 6.0), a copy of its bytes 8.3.
 // With a selection and a quantised row in every wavefront 14.6.
 //
 // int8_gate_up_kernel: the first wavefront of a workgroup picks the experts of its columns (as many rounds of the selection as they are down
