@@ -203,8 +203,10 @@ def _run_own(s):
                        s["interleaved"])
         return {"q": s["q"], "key_cache": s["kc"], "value_cache": s["vc"]}
     if s["family"] == "tree":
-        return v.tree_attention(s["q"], s["kc"], s["vc"], s["table"], s["seq"], s["cu"], s["mask"], s["out"], s["scale"], s["most"])
-    return v.paged_attention(s["q"], s["kc"], s["vc"], s["table"], s["seq"], s["cu"], s["out"], s["scale"], s["window"], s["sinks"], s["most"])
+        return v.tree_attention(s["q"], s["kc"], s["vc"], s["table"], s["seq"], s["cu"], s["mask"], s["out"], s["scale"], max(s["news"]),
+                                s["most"])
+    return v.paged_attention(s["q"], s["kc"], s["vc"], s["table"], s["seq"], s["cu"], s["out"], s["scale"], s["window"], s["sinks"],
+                             max(s["news"]), s["most"])
 
 
 def _head_norm(x, w):
