@@ -686,6 +686,59 @@ int mi_moe_forward_full_int8_ws(const void* x, const void* logits, void* out, co
                                 const void* shared_w2, const float* shared_w2_scale, const void* gate_weight, void* workspace,
                                 long long workspace_bytes, int T, int topk, int num_experts, int H, int I, int act_dtype, void* stream);
 
+/* ---- attention over a paged cache -----------------------------------------------------
+ * A cache of `pages` pages of `page_size` places each; place o of page g holds num_kv_heads heads of head_dim elements (fp16 or bf16, as the
+ * activations), keys and values in arrays of the same strides.  Strides in elements, multiples of 8; the array ends below 64 GiB - 16 behind its
+ * start; 16-byte aligned.  A slot is page x page_size + place. */
+typedef struct {
+  void* key;
+  void* value;
+  long long page_stride, token_stride, head_stride;
+  int pages, page_size;
+} MiPagedCache;
+
+/* What lies between a fused q, k, v projection and attention: qkv [T, (num_heads + 2 num_kv_heads) head_dim] (row stride qkv_stride), query heads
+ * first, then keys, then values.  Each query and key head: v = x rsqrt(mean(x^2) + eps) w, where a weight [head_dim] is given (NULL: v = x);
+ * then the first rot elements are rotated by the token's row of cos_sin [places, rot] (rot / 2 cosines, rot / 2 sines; fp32 if table_f32, else the
+ * activations' type): (a, b) -> (a cos - b sin, b cos + a sin) for the pairs (i, i + rot / 2), or (2 i, 2 i + 1) if interleaved; fp32, one
+ * rounding.  Queries go to q_out, keys to k_out (NULL: nowhere), keys and the untouched values to slot slots[t] of the cache (NULL: nowhere).
+ * A slot outside the cache is not written; a position outside the table gives NaN.  q_out may be qkv's own query columns and k_out its key
+ * columns; otherwise nothing overlaps.  Slots of a call differ.  head_dim 64, 128 or 256; rot a multiple of 16.  One launch.
+ * In place of esimd_qkv_split_norm_rope (V/csrc/xpu/torch_extension.cc), with a paged cache behind it. */
+int mi_qk_norm_rope(const void* qkv, long long qkv_stride, const void* q_weight, const void* k_weight, const void* cos_sin, int table_f32,
+                    const int64_t* positions, void* q_out, long long q_token_stride, long long q_head_stride, void* k_out,
+                    long long k_token_stride, long long k_head_stride, const MiPagedCache* cache, const int64_t* slots, int T, int num_heads,
+                    int num_kv_heads, int head_dim, int rot, int places, float eps, int interleaved, int act_dtype, void* stream);
+
+/* Attention of T tokens, those of sequence b in rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] (from 0; rows behind the last are not written), over
+ * the cache: sequence b has seq_lens[b] keys, the last ones its tokens' own; key j lies at place j % page_size of page
+ * block_table[b][j / page_size] (table [B, table_width]).  Token i stands at place p = seq_lens[b] - n + i and sees key j if j <= p and
+ * (window = -1, or p - j < window, or j < sinks); query head h reads kv head h / (num_heads / num_kv_heads):
+ *   out = sum_j softmax_j(scale q . k_j) v_j.
+ * A token that sees nothing gets zeros.  Keys behind the table's end or on a page outside the cache are not seen.  Scores, softmax and sums in
+ * fp32; the weights are rounded to the activations' type in front of their product with the values; one rounding at the end.  What lies in
+ * places that a token does not see does not reach it, infinities and NaN included.
+ * query [T, num_heads, head_dim] with strides (multiples of 8), out contiguous; head_dim 64, 128 or 256; T num_heads below 2^28;
+ * table_width x page_size below 2^30; scale > 0.  max_query_len and max_seq_len, the largest n and seq_lens, choose kernels and splits only:
+ * results are right for any values, up to the order of sums.  The workspace (mi_paged_attention_workspace bytes for the same arguments; 16-byte
+ * aligned) must stay untouched until the stream has passed the call; 0 bytes: none.
+ * In place of eagle_ops::page_attn_decode and of the sdp kernels of prompts (V/csrc/eagle, V/csrc/xpu). */
+int mi_paged_attention_workspace(int T, int B, int num_heads, int num_kv_heads, int head_dim, int max_query_len, int max_seq_len,
+                                 long long* bytes);
+int mi_paged_attention_ws(const void* query, long long token_stride, long long head_stride, const MiPagedCache* cache,
+                          const int32_t* block_table, int table_width, const int32_t* seq_lens, const int32_t* cu_seqlens_q, void* out,
+                          void* workspace, long long workspace_bytes, int T, int B, int num_heads, int num_kv_heads, int head_dim,
+                          float scale, int window, int sinks, int max_query_len, int max_seq_len, int act_dtype, void* stream);
+
+/* The same for drafted tokens: the last n places of a sequence hold a tree of n drafted tokens.  Token i sees all keys in front of them
+ * (j < seq_lens[b] - n) and drafted token u if bit u % 64 of tree_mask[row of i][u / 64] is set (tree_mask [T, mask_words]); bits from n on are
+ * ignored.  Workspace as above. */
+int mi_tree_attention_ws(const void* query, long long token_stride, long long head_stride, const MiPagedCache* cache,
+                         const int32_t* block_table, int table_width, const int32_t* seq_lens, const int32_t* cu_seqlens_q,
+                         const int64_t* tree_mask, int mask_words, void* out, void* workspace, long long workspace_bytes, int T, int B,
+                         int num_heads, int num_kv_heads, int head_dim, float scale, int max_query_len, int max_seq_len, int act_dtype,
+                         void* stream);
+
 /* ---- measurement yardstick -------------------------------------------------------------
  * No counterpart in the reference.  mi_stream_read fetches `bytes` (a multiple of 16, src 16-byte
  * aligned) from HBM with non-temporal 16-byte loads and keeps nothing: the time a kernel that

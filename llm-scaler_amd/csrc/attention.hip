@@ -1,0 +1,184 @@
+// C entries of the attention over a paged cache: checks, the choice of kernel, the workspace.
+#include "attention.hpp"
+
+#include "../../include/mi355x_qlinear.h"
+
+namespace qlin {
+
+// Which kernels a call runs.  Up to 32 rows (tokens x heads of a group) per sequence go to the rows kernel, more to the tiles kernel; where
+// sequences of both kinds can be in a call both are launched, and each takes its own.
+struct AttnPlan {
+  bool rows, tiles;
+  int rows_from, groups, slots, splits;
+  long long rows_bytes, tiles_bytes;
+};
+
+static int cus() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0) {
+      (void)hipGetLastError();
+      return 256;                                      // without a device only sizes are asked for
+    }
+    return v;
+  }();
+  return n;
+}
+
+static long long round256(long long v) { return (v + 255) / 256 * 256; }
+
+static int attn_plan(int T, int B, int Hq, int Hkv, int D, int max_query_len, int max_seq_len, AttnPlan& a) {
+  if (D != 64 && D != 128 && D != 256) return MI_ERR_SHAPE;
+  if (T < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || max_query_len < 0 || max_seq_len < 0) return MI_ERR_SHAPE;
+  if ((long long)T * Hq >= 1 << 28 || B >= 1 << 24 || Hq > 1 << 16) return MI_ERR_SHAPE;
+  const int G = Hq / Hkv, most = max_query_len < T ? max_query_len : T;
+  a = AttnPlan{};
+  if (!T || !B) return MI_OK;
+  a.rows = a.tiles = true;
+  a.rows_from = 33;
+  if ((long long)most * G <= 32) {
+    a.tiles = false;
+    a.rows_from = INT32_MAX;
+  } else if (B == 1 || (long long)B * most == T) {     // all sequences are as long as the longest
+    a.rows = false;
+    a.rows_from = 0;
+  }
+  const long long blocks = ((long long)(max_seq_len < 1 ? 1 : max_seq_len) + kBlock - 1) / kBlock;
+  if (a.rows) {
+    const long long full = (long long)cus() * (D == 64 ? 2 : 1);                 // workgroups that the device holds
+    const long long some = ((long long)T * G / 32 + B) * Hkv * blocks;
+    a.groups = (int)(some < full ? some : full);
+    a.rows_bytes = round256(attn_rows_bytes(a.groups, D));
+  }
+  if (a.tiles) {
+    const int R = attn_tile_rows(D);
+    const long long slots = (long long)T * G / R + B;
+    if (slots * Hkv >= 1 << 30) return MI_ERR_SHAPE;
+    a.slots = (int)slots;
+    // about three workgroups per CU, of 512 keys at least
+    const long long tiles = (((long long)T * G + R - 1) / R) * Hkv;
+    long long s = 3LL * cus() / tiles, most_s = blocks / 8;
+    if (s > most_s) s = most_s;
+    if (s > 64) s = 64;
+    a.splits = s < 2 ? 1 : (int)s;
+    if (slots * Hkv * a.splits >= 1LL << 30) a.splits = 1;
+    if (a.splits > 1) a.tiles_bytes = round256((long long)a.splits * T * Hq * (D + 2) * 4);
+  }
+  return MI_OK;
+}
+
+// key / d for keys below 2^30: (umulhi(key, mul) + key) >> shift
+static void divide_by(uint32_t d, uint32_t& mul, uint32_t& shift) {
+  shift = 0;
+  while ((1ull << shift) < d) ++shift;
+  mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+}
+
+static int run(const AttnArgs& base, const MiPagedCache* cache, int D, float scale, int max_query_len, int max_seq_len, void* workspace,
+               long long workspace_bytes, int act_dtype, hipStream_t st) {
+  AttnArgs p = base;
+  if (act_dtype != DT_F16 && act_dtype != DT_BF16) return MI_ERR_ARG;
+  AttnPlan a;
+  const int rc = attn_plan(p.T, p.B, p.Hq, p.Hkv, D, max_query_len, max_seq_len, a);
+  if (rc != MI_OK) return rc;
+  if (!a.rows && !a.tiles) return MI_OK;
+  if (!cache || !p.q || !p.out || !p.seq_lens || !p.cu || !cache->key || !cache->value || !(scale > 0.f) || scale > 3e38f) return MI_ERR_ARG;
+  if (!aligned16(p.q) || !aligned16(p.out) || !aligned16(cache->key) || !aligned16(cache->value) || !aligned16(workspace)) return MI_ERR_ARG;
+  if (p.q_token % 8 || p.q_head % 8 || cache->page_stride % 8 || cache->token_stride % 8 || cache->head_stride % 8) return MI_ERR_SHAPE;
+  if (cache->pages <= 0 || cache->page_size <= 0 || p.width < 0 || (p.width && !p.table)) return MI_ERR_ARG;
+  if ((long long)p.width * cache->page_size >= 1 << 30) return MI_ERR_SHAPE;
+  if (cache->page_stride < 0 || cache->token_stride < 0 || cache->head_stride < 0) return MI_ERR_SHAPE;
+  const long long end = (cache->pages - 1LL) * (cache->page_stride / 8) + (cache->page_size - 1LL) * (cache->token_stride / 8) +
+                        (p.Hkv - 1LL) * (cache->head_stride / 8) + D / 8;
+  if (end >= (long long)kNoRow) return MI_ERR_SHAPE;
+  if (a.rows_bytes + a.tiles_bytes > 0 && (!workspace || workspace_bytes < a.rows_bytes + a.tiles_bytes)) return MI_ERR_ARG;
+  p.k = cache->key;
+  p.v = cache->value;
+  p.page16 = (uint32_t)(cache->page_stride / 8);
+  p.row16 = (uint32_t)(cache->token_stride / 8);
+  p.head16 = (uint32_t)(cache->head_stride / 8);
+  p.page = cache->page_size;
+  p.pages = cache->pages;
+  divide_by((uint32_t)p.page, p.page_mul, p.page_shift);
+  p.G = p.Hq / p.Hkv;
+  p.c = scale * 1.4426950408889634f;
+  p.rows_from = a.rows_from;
+  p.groups = a.groups;
+  p.slots = a.slots;
+  p.splits = a.splits;
+  if (a.tiles) {
+    p.part = (float*)((char*)workspace + a.rows_bytes);
+    const int r = launch_attn_tiles(p, D, act_dtype, st);
+    if (r != MI_OK) return r;
+  }
+  if (a.rows) {
+    p.part = (float*)workspace;
+    return launch_attn_rows(p, D, act_dtype, st);
+  }
+  return MI_OK;
+}
+
+}  // namespace qlin
+
+using namespace qlin;
+
+extern "C" {
+
+int mi_paged_attention_workspace(int T, int B, int num_heads, int num_kv_heads, int head_dim, int max_query_len, int max_seq_len,
+                                 long long* bytes) {
+  if (!bytes) return MI_ERR_ARG;
+  AttnPlan a;
+  const int rc = attn_plan(T, B, num_heads, num_kv_heads, head_dim, max_query_len, max_seq_len, a);
+  if (rc == MI_OK) *bytes = a.rows_bytes + a.tiles_bytes;
+  return rc;
+}
+
+int mi_paged_attention_ws(const void* query, long long token_stride, long long head_stride, const MiPagedCache* cache,
+                          const int32_t* block_table, int table_width, const int32_t* seq_lens, const int32_t* cu_seqlens_q, void* out,
+                          void* workspace, long long workspace_bytes, int T, int B, int num_heads, int num_kv_heads, int head_dim,
+                          float scale, int window, int sinks, int max_query_len, int max_seq_len, int act_dtype, void* stream) {
+  if ((window < 1 && window != -1) || sinks < 0) return MI_ERR_SHAPE;
+  AttnArgs p{};
+  p.q = query;
+  p.q_token = token_stride;
+  p.q_head = head_stride;
+  p.table = block_table;
+  p.width = table_width;
+  p.seq_lens = seq_lens;
+  p.cu = cu_seqlens_q;
+  p.out = out;
+  p.T = T;
+  p.B = B;
+  p.Hq = num_heads;
+  p.Hkv = num_kv_heads;
+  p.window = window < 0 || window >= 1 << 30 ? 0 : window;       // no place is that far from another
+  p.sinks = sinks;
+  return run(p, cache, head_dim, scale, max_query_len, max_seq_len, workspace, workspace_bytes, act_dtype, (hipStream_t)stream);
+}
+
+int mi_tree_attention_ws(const void* query, long long token_stride, long long head_stride, const MiPagedCache* cache,
+                         const int32_t* block_table, int table_width, const int32_t* seq_lens, const int32_t* cu_seqlens_q,
+                         const int64_t* tree_mask, int mask_words, void* out, void* workspace, long long workspace_bytes, int T, int B,
+                         int num_heads, int num_kv_heads, int head_dim, float scale, int max_query_len, int max_seq_len, int act_dtype,
+                         void* stream) {
+  if (T > 0 && B > 0 && !tree_mask) return MI_ERR_ARG;
+  if (mask_words < 1 || mask_words > 1 << 20) return MI_ERR_SHAPE;
+  AttnArgs p{};
+  p.q = query;
+  p.q_token = token_stride;
+  p.q_head = head_stride;
+  p.table = block_table;
+  p.width = table_width;
+  p.seq_lens = seq_lens;
+  p.cu = cu_seqlens_q;
+  p.tree = tree_mask;
+  p.tree_words = mask_words;
+  p.out = out;
+  p.T = T;
+  p.B = B;
+  p.Hq = num_heads;
+  p.Hkv = num_kv_heads;
+  return run(p, cache, head_dim, scale, max_query_len, max_seq_len, workspace, workspace_bytes, act_dtype, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,306 @@
+// Attention over a paged cache: what its two kernels share.
+//
+//   o_i = sum_j p_ij v_j,   p_ij = 2^(c s_ij - m_i) / l_i,   s_ij = q_i . k_j,   c = scale log2(e)
+//
+// in one pass over the keys: m is the running maximum of c times a row's scores, l the running sum, and both o and l are multiplied by
+// 2^(m_old - m_new) where a row's maximum grows.  s, m, l and o are fp32; p is rounded to the type of the values in front of its product with
+// them (off by half a step of a 16-bit number, below the output's rounding, as v_j is already such a number), and l sums the rounded p.
+//
+// The rows of a kv head are (token, head of the group) pairs of a sequence, token first: row r is head r % G of token r / G.  A wavefront holds 32
+// rows as columns of v_mfma_f32_32x32x16: S^T = K Q^T has a row's scores in the registers of two lanes (16 of 32 keys each), so that maximum and sum
+// take one exchange, and those 16 values, rounded, are what the second product O^T = V^T P^T takes as its operand: the keys of V^T come in the order
+// that they have in the registers (ds_read_b64_tr_b16 gathers four keys of a column).
+//
+// Keys and values come to LDS straight from memory, 16 bytes a lane.  A lane looks up the page of one key; a key that no row of the tile sees
+// (behind the end, outside the window, on a page outside the cache) reads zeros, so what lies there, NaN included, reaches nothing.
+#pragma once
+#include "int8_common.hpp"
+
+namespace qlin {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short i16x4;
+typedef __attribute__((ext_vector_type(8))) short i16x8;
+typedef const __attribute__((address_space(1))) void* global_ptr;
+typedef __attribute__((address_space(3))) void* lds_void;
+
+struct AttnArgs {
+  const void *q, *k, *v;
+  void* out;                   // [T, Hq, D]
+  const int32_t *table, *seq_lens, *cu;
+  const int64_t* tree;         // [T, tree_words]: tree_attention; null: causal
+  float* part;                 // partial results
+  long long q_token, q_head;   // strides of q in elements
+  uint32_t page16, row16, head16;        // strides of the cache in 16 bytes
+  uint32_t page_mul, page_shift;         // key / page
+  int T, B, Hq, Hkv, G, page, width, pages;
+  int window, sinks, tree_words;         // window 0: none
+  float c;
+  int groups;                  // rows kernel: workgroups
+  int slots, splits;           // tiles kernel
+  int rows_from;               // sequences with that many rows (tokens x G) or more belong to the tiles kernel
+};
+
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;
+constexpr int kBlock = 64;                            // keys of a block of work
+
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+// v of lanes l % 32 and 32 + l % 32
+struct Halves { float low, high; };
+__device__ __forceinline__ Halves both_halves(float v) {
+  const uint32_t a = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  const uint32_t low = r[0], high = r[1];              // a bit cast of r[1] itself would be one of r[0]
+  return {__builtin_bit_cast(float, low), __builtin_bit_cast(float, high)};
+}
+
+// ---- a sequence of the call -------------------------------------------------------------------
+struct AttnSeq {
+  int q0, n;                   // its tokens
+  int first;                   // place of its first token: length - n
+  int cap;                     // keys that can be there: min(length, places of the table)
+};
+__device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& p, int b) {
+  AttnSeq s;
+  s.q0 = min(max(p.cu[b], 0), p.T);
+  s.n = min(max(p.cu[b + 1], s.q0), p.T) - s.q0;
+  const int len = max(p.seq_lens[b], 0);
+  s.first = len - s.n;
+  s.cap = min(len, p.width * p.page);
+  return s;
+}
+
+// The blocks of BLOCK keys that tokens t0 .. t1 of a sequence see some of: first the `head` blocks with visible first tokens, then all from `from` on.
+struct AttnRange { int lo, hi, head, from, blocks; };
+template <int BLOCK>
+__device__ __forceinline__ AttnRange attn_range(const AttnArgs& p, const AttnSeq& s, int t0, int t1) {
+  AttnRange r;
+  r.lo = 0;
+  r.hi = s.cap;
+  if (!p.tree) {
+    r.hi = min(s.cap, max(s.first + t1 + 1, 0));
+    if (p.window) r.lo = min(max(s.first + t0 - p.window + 1, 0), r.hi);
+  }
+  r.from = r.lo / BLOCK * BLOCK;
+  r.head = min(r.from, (min(p.sinks, r.hi) + BLOCK - 1) / BLOCK * BLOCK) / BLOCK;
+  r.blocks = r.head + (r.hi - r.from + BLOCK - 1) / BLOCK;
+  return r;
+}
+template <int BLOCK>
+__device__ __forceinline__ int attn_key(const AttnRange& r, int block) {
+  return block < r.head ? block * BLOCK : r.from + (block - r.head) * BLOCK;
+}
+
+// Where key `key` of a table row lies, in 16 bytes from the cache's start; kNoRow: nowhere, or no token of the range sees it.
+__device__ __forceinline__ int attn_page_of(const AttnArgs& p, int key) {
+  return (int)((__umulhi((uint32_t)key, p.page_mul) + (uint32_t)key) >> p.page_shift);
+}
+__device__ __forceinline__ int attn_lookup(const AttnArgs& p, const int32_t* row, const AttnRange& r, int key) {
+  const bool seen = key < r.hi && (key >= r.lo || key < p.sinks);
+  return seen ? row[attn_page_of(p, key)] : -1;
+}
+__device__ __forceinline__ uint32_t attn_place(const AttnArgs& p, int page, int key, int head) {
+  if ((uint32_t)page >= (uint32_t)p.pages) return kNoRow;
+  return (uint32_t)page * p.page16 + (uint32_t)(key - attn_page_of(p, key) * p.page) * p.row16 + (uint32_t)head * p.head16;
+}
+
+// Bit i: a token sees key kb + i.  The token stands at place s.first + t (negative: before the cache's start), its tree bits in `tree`.
+__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
+__device__ __forceinline__ uint64_t attn_sees(const AttnArgs& p, int first, int t, const int64_t* tree, int kb) {
+  if (p.tree) {
+    const int at = kb - first;                         // the drafted token of key kb
+    if (at <= -64) return ~0ull;
+    auto word = [&](int w) { return w >= 0 && w < p.tree_words ? (uint64_t)tree[w] : 0ull; };
+    if (at < 0) return low_bits(-at) | word(0) << -at;
+    const int w = at >> 6, by = at & 63;
+    return word(w) >> by | (by ? word(w + 1) << (64 - by) : 0ull);
+  }
+  const int place = first + t;
+  uint64_t m = low_bits(place - kb + 1);
+  if (p.window) m &= ~low_bits(place - p.window + 1 - kb) | low_bits(p.sinks - kb);
+  return m;
+}
+// Whether every token from t0 to t1 sees all of the N keys from kb on
+template <int N>
+__device__ __forceinline__ bool attn_all_seen(const AttnArgs& p, int first, int t0, int t1, int kb) {
+  if (p.tree) return kb + N <= first;
+  return kb + N - 1 <= first + t0 && (!p.window || kb > first + t1 - p.window || kb + N <= p.sinks);
+}
+
+// ---- loads ------------------------------------------------------------------------------------
+__device__ const u32x4 kZeroRow[64] = {};             // what a key that nothing sees is read from
+
+// 16-byte chunk c of key row r lies at place c ^ swizzle of its row: eight lanes that read a column of K rows at a time, and the four rows of 64
+// bytes that a transposing read of V takes, find different banks.
+template <int D> __device__ __forceinline__ int k_swizzle(int r) { return r & (D / 8 < 16 ? D / 8 - 1 : 15); }
+template <int D> __device__ __forceinline__ int v_swizzle(int r) { return D == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2; }
+
+// Rows [first, first + ROWS) of a block of keys to LDS by one wavefront: lane i holds the place of row i of the block.
+template <int D, int ROWS>
+__device__ __forceinline__ void attn_load(const void* k, const void* v, uint32_t place, int first, unsigned char* to_k, unsigned char* to_v) {
+  constexpr int CH = D / 8, RPI = 64 / CH, N = ROWS / RPI;     // chunks of a row, rows per load
+  static_assert(RPI * N == ROWS && (64 % CH) == 0, "rows per load");
+  const int lane = threadIdx.x & 63, c = lane % CH;
+  const unsigned char* src[N];
+  bool there[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const uint32_t at = __shfl(place, first + j * RPI + lane / CH, 64);
+    there[j] = at != kNoRow;
+    src[j] = (const unsigned char*)((uint64_t)at * 16);
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int r = first + j * RPI + lane / CH, ck = (c ^ k_swizzle<D>(r)) * 16;
+    const unsigned char* a = (there[j] ? (const unsigned char*)k + (uint64_t)src[j] : (const unsigned char*)kZeroRow) + ck;
+    __builtin_amdgcn_global_load_lds((global_ptr)a, (lds_void)(to_k + j * 1024), 16, 0, 0);
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int r = first + j * RPI + lane / CH, cv = (c ^ v_swizzle<D>(r)) * 16;
+    const unsigned char* a = (there[j] ? (const unsigned char*)v + (uint64_t)src[j] : (const unsigned char*)kZeroRow) + cv;
+    __builtin_amdgcn_global_load_lds((global_ptr)a, (lds_void)(to_v + j * 1024), 16, 0, 0);
+  }
+}
+
+// ---- 32 rows of a wavefront -------------------------------------------------------------------
+template <class Act, int D>
+struct AttnRows {
+  using v8 = typename Act::v8;
+  typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
+  static constexpr int DT = D / 32;
+  static constexpr unsigned short EXPONENT = Act::dt == DT_F16 ? 0x7C00 : 0x7F80;
+  v8 q[D / 16];
+  f32x16 o[DT];                // o[t][i]: column 32 t + 8 (i / 4) + 4 (lane / 32) + i % 4 of row lane % 32
+  float m, l;                  // m: c times the row's largest score; l: of this lane's keys
+  int ka, va;                  // where this lane reads K and V of a block
+
+  __device__ __forceinline__ void start() {
+    const int lane = threadIdx.x & 63, h = lane >> 5, i = lane & 15;
+    m = -__builtin_inff();
+    l = 0.f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = f32x16{};
+    ka = (lane & 31) * 2 * D + ((h ^ k_swizzle<D>(lane & 31)) * 16);
+    // keys 4 h + i / 4, columns 16 (lane / 16 % 2) + 4 (i % 4)
+    va = (4 * h + (i >> 2)) * 2 * D + (((2 * (lane >> 4 & 1) + (i >> 1 & 1)) ^ v_swizzle<D>(i >> 2)) * 16) + (i & 1) * 8;
+  }
+  __device__ __forceinline__ void load_q(const void* row) {      // null: zeros
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      u32x4 x = {};
+      if (row) x = *(const u32x4*)((const unsigned char*)row + s * 32 + h * 16);
+      q[s] = as_v8<v8>(x);
+    }
+  }
+  // V^T of 16 keys (from 16 t of the block) and columns 32 d ..: element e is key 4 (lane / 32) + e % 4 + 8 (e / 4)
+  __device__ __forceinline__ v8 v_operand(const unsigned char* v, int t, int d) const {
+    const unsigned char* at = v + ((va ^ ((d & 3) * 64)) + (d >> 2) * 256 + t * 32 * D);
+    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)at);
+    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(at + 16 * D));
+    return __builtin_bit_cast(v8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  // A block of N keys.  mask: bit i of this lane's row: it sees key i; null bits everywhere a key is not there.  full: all bits of all lanes are set.
+  template <int N>
+  __device__ __forceinline__ void block(const unsigned char* k, const unsigned char* v, bool full, uint64_t mask, float c) {
+    constexpr int KT = N / 32;
+    const int h = (threadIdx.x & 63) >> 5;
+    f32x16 s[KT];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) s[t] = f32x16{};
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const u32x4 x = *(const u32x4*)(k + ((ka ^ (ks % 8 * 32)) + ks / 8 * 256 + t * 64 * D));
+        s[t] = mfma32(as_v8<v8>(x), q[ks], s[t]);
+      }
+    if (!full) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const uint32_t bits = (uint32_t)(mask >> (32 * t)) >> (4 * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i] = bits >> (8 * (i / 4) + i % 4) & 1 ? s[t][i] : -__builtin_inff();
+      }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+    const Halves x = both_halves(mx);
+    mx = fmaxf(m, fmaxf(x.low, x.high) * c);
+    const float top = mx == -__builtin_inff() ? 0.f : mx;        // a row that has seen nothing yet
+    if (__builtin_amdgcn_ballot_w64(mx != m)) {
+      const float a = __builtin_amdgcn_exp2f(m - top);
+      l *= a;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= a;
+      m = mx;
+    }
+    v8 p[2 * KT];
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2 * KT; ++t)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[t][e] = Act::from_f32(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][8 * (t % 2) + e], c, -top)));
+        sum += Act::to_f32(p[t][e]);
+      }
+    l += sum;
+    if (full) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int t = 0; t < 2 * KT; ++t) o[d] = mfma32(v_operand(v, t, d), p[t], o[d]);
+      return;
+    }
+    // 0 times an infinity or a NaN that a row does not see would not be 0: such values go to the rows that see them by themselves.
+    u16x8 one = 1;                                     // 0 where a value was not finite
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < 2 * KT; ++t) {
+        const u16x8 x = __builtin_bit_cast(u16x8, v_operand(v, t, d));
+        const u16x8 finite = __builtin_elementwise_min(EXPONENT - (x & EXPONENT), (u16x8)1);
+        one &= finite;
+        o[d] = mfma32(__builtin_bit_cast(v8, x & (0 - finite)), p[t], o[d]);
+      }
+    }
+    const u32x4 all = __builtin_bit_cast(u32x4, one);
+    if (__builtin_amdgcn_ballot_w64((all[0] & all[1] & all[2] & all[3]) != 0x00010001u)) add_not_finite<N>(v, mask);
+  }
+  template <int N>
+  __device__ __forceinline__ void add_not_finite(const unsigned char* v, uint64_t mask) {
+    const int h = (threadIdx.x & 63) >> 5;
+    typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
+    typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
+#pragma unroll 1
+    for (int j = 0; j < N; ++j) {
+      const bool sees = mask >> j & 1;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                  // columns 32 d + 8 i + 4 h ..
+          const u16x4 x = *(const u16x4*)(v + j * 2 * D + ((4 * d + i) ^ v_swizzle<D>(j)) * 16 + h * 8);
+          const e4 y = __builtin_bit_cast(e4, x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[d][4 * i + e] += sees && (x[e] & EXPONENT) == EXPONENT ? Act::to_f32(y[e]) : 0.f;
+        }
+      }
+    }
+  }
+};
+
+int launch_attn_rows(const AttnArgs& p, int D, int act_dtype, hipStream_t st);       // and what joins the parts
+int launch_attn_tiles(const AttnArgs& p, int D, int act_dtype, hipStream_t st);
+long long attn_rows_bytes(int groups, int D);
+constexpr int attn_tile_rows(int D) { return D == 256 ? 128 : 256; }
+
+}  // namespace qlin

@@ -8,8 +8,8 @@
 // operator (registered as mi355x_checked::<name>), which runs it or raises, so that accepted calls, results and
 // error messages are those of that implementation.  Only the checks decide that, before anything is enqueued: once an
 // entry of the C ABI has been called, a status other than 0 is raised.  Running the call again would hide a launch that
-// failed and would add to an in-place operand twice (the residual of the norm operators).  The operators on 8-bit integers have no
-// other implementation: their checks, all of them, are here.
+// failed and would add to an in-place operand twice (the residual of the norm operators).  The operators on 8-bit integers and the
+// attention over a paged cache have no other implementation: their checks, all of them, are here.
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/stack.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -18,7 +18,9 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <array>
 #include <climits>
+#include <cstdlib>
 #include <initializer_list>
 
 #include "../../include/mi355x_qlinear.h"
@@ -599,6 +601,241 @@ Tensor moe_forward_full_int8(const Tensor& x, const Tensor& logits, const Tensor
   return out;
 }
 
+// ---------------------------------------------------------------------------------------- attention over a paged cache
+// As above, every check is made here.
+struct Span { const char *from, *to; };
+Span span(const Tensor& t) {                           // from the first byte to behind the last, whatever the strides
+  if (!t.numel()) return {nullptr, nullptr};
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  const char* p = (const char*)t.data_ptr();
+  return {p, p + (last + 1) * t.element_size()};
+}
+void attn_apart(const char* who, const Tensor& out, const char* out_name, const Tensor& t, const char* name) {
+  const Span a = span(out), b = span(t);
+  REFUSE_UNLESS(!a.from || !b.from || a.from >= b.to || b.from >= a.to, out_name, " must not overlap ", name);
+}
+void attn_device(const char* who, const Tensor& x, const Tensor& t, const char* name) {
+  REFUSE_UNLESS(t.is_cuda() && t.device() == x.device(), name, " must be on the same ROCm device as the input, got ", t.device());
+}
+// dim heads last two: [.., heads, D] with elements of a head side by side, strides of whole 16 bytes
+void attn_heads(const char* who, const Tensor& t, const char* name) {
+  REFUSE_UNLESS(t.size(-1) == 64 || t.size(-1) == 128 || t.size(-1) == 256, name, " must have heads of 64, 128 or 256 elements, got ", t.sizes());
+  if (!t.numel()) return;
+  REFUSE_UNLESS(t.stride(-1) == 1, name, " must have the elements of a head side by side");
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    REFUSE_UNLESS(t.size(d) == 1 || t.stride(d) % 8 == 0, name, " must have strides of multiples of 8 elements, got ", t.strides());
+  int8_aligned(who, t, name);
+}
+// Written tensors: no element in two places.
+void attn_apart_inside(const char* who, const Tensor& t, const char* name) {
+  if (!t.numel()) return;
+  std::array<std::pair<int64_t, int64_t>, 3> dims;     // stride and size, by growing stride
+  size_t n = 0;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    if (t.size(d) > 1) dims.at(n++) = {t.stride(d), t.size(d)};
+  std::sort(dims.begin(), dims.begin() + n);
+  int64_t extent = t.size(-1);
+  for (size_t i = 0; i < n; ++i) {
+    REFUSE_UNLESS(dims[i].first >= extent, name, " must not hold an element more than once, got strides ", t.strides());
+    extent += (dims[i].second - 1) * dims[i].first;
+  }
+}
+// A dimension of one element has a stride that means nothing.
+long long stride_of(const Tensor& t, int64_t d) { return t.size(d) == 1 ? 0 : t.stride(d); }
+
+MiPagedCache paged_cache(const char* who, const Tensor& x, const Tensor& kc, const Tensor& vc, int64_t Hkv, int64_t D) {
+  attn_device(who, x, kc, "key_cache");
+  attn_device(who, x, vc, "value_cache");
+  REFUSE_UNLESS(kc.dim() == 4 && kc.size(3) == D, "key_cache must be [pages, page_size, kv heads, ", D, "], got ", kc.sizes());
+  REFUSE_UNLESS(Hkv == 0 || kc.size(2) == Hkv, "key_cache must have ", Hkv, " kv heads, got ", kc.sizes());
+  REFUSE_UNLESS(kc.scalar_type() == x.scalar_type() && vc.scalar_type() == x.scalar_type(), "the cache must have the input's type, got ",
+                kc.scalar_type(), " and ", vc.scalar_type());
+  REFUSE_UNLESS(kc.size(0) > 0 && kc.size(1) > 0 && kc.size(2) > 0 && kc.size(0) < (1LL << 31) && kc.size(1) < (1LL << 30),
+                "key_cache must have pages, places and heads, got ", kc.sizes());
+  attn_heads(who, kc, "key_cache");
+  attn_heads(who, vc, "value_cache");
+  REFUSE_UNLESS(kc.sizes() == vc.sizes() && stride_of(kc, 0) == stride_of(vc, 0) && stride_of(kc, 1) == stride_of(vc, 1) &&
+                    stride_of(kc, 2) == stride_of(vc, 2),
+                "value_cache must have the sizes and strides of key_cache, got ", vc.sizes(), " ", vc.strides());
+  // one array may hold both, side by side at any level: between the places of one lie those of the other
+  const int64_t apart = std::abs((const char*)vc.data_ptr() - (const char*)kc.data_ptr()) / 2;
+  int64_t inner = D, next = INT64_MAX;
+  for (int64_t d = 0; d < 3; ++d) {
+    if (kc.size(d) > 1 && kc.stride(d) <= apart) inner += (kc.size(d) - 1) * kc.stride(d);
+    if (kc.size(d) > 1 && kc.stride(d) > apart) next = std::min(next, kc.stride(d));
+  }
+  REFUSE_UNLESS(inner <= apart && (next == INT64_MAX || inner <= next - apart), "value_cache must not overlap key_cache");
+  const Span s = span(kc);
+  REFUSE_UNLESS(s.to - s.from < (1LL << 36) - 16, "a cache must end below 64 GiB, got ", s.to - s.from, " bytes");
+  return {kc.data_ptr(), vc.data_ptr(), stride_of(kc, 0), stride_of(kc, 1), stride_of(kc, 2), (int)kc.size(0), (int)kc.size(1)};
+}
+
+Tensor qk_norm_rope(const Tensor& qkv, const c10::optional<Tensor>& qw, const c10::optional<Tensor>& kw, const Tensor& table,
+                    const Tensor& positions, const Tensor& q, const c10::optional<Tensor>& k, const c10::optional<Tensor>& kc,
+                    const c10::optional<Tensor>& vc, const c10::optional<Tensor>& slots, double eps, bool interleaved) {
+  const char* who = "qk_norm_rope";
+  REFUSE_UNLESS(qkv.is_cuda(), "qkv must be on a ROCm device, got ", qkv.device());
+  REFUSE_UNLESS(is16(qkv) && qkv.dim() == 2, "qkv must be fp16 or bf16 [T, (Hq + 2 Hkv) D], got ", qkv.scalar_type(), " ", qkv.sizes());
+  attn_device(who, qkv, q, "q_out");
+  REFUSE_UNLESS(q.dim() == 3 && q.size(0) == qkv.size(0) && q.scalar_type() == qkv.scalar_type(), "q_out must be [T, Hq, D] in qkv's type, got ",
+                q.scalar_type(), " ", q.sizes());
+  attn_heads(who, q, "q_out");
+  const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2), W = qkv.size(1);
+  REFUSE_UNLESS(Hq > 0 && W % D == 0 && W / D > Hq && (W / D - Hq) % 2 == 0, "qkv must have (Hq + 2 Hkv) D columns, got ", W, " for Hq=", Hq,
+                ", D=", D);
+  const int64_t Hkv = (W / D - Hq) / 2;
+  REFUSE_UNLESS(Hq <= 65536 && Hkv <= 65536 && T <= INT_MAX && T * (W / D) * (D / 16) < (1LL << 31), "too many heads or tokens: ", qkv.sizes());
+  REFUSE_UNLESS(!qkv.numel() || (qkv.stride(1) == 1 && (T == 1 || (qkv.stride(0) % 8 == 0 && qkv.stride(0) >= W))),
+                "qkv must have rows of consecutive elements that start on 16 bytes, got strides ", qkv.strides());
+  int8_aligned(who, qkv, "qkv");
+  for (const auto& w : {std::make_pair(&qw, "q_weight"), std::make_pair(&kw, "k_weight")})
+    if (w.first->has_value()) {
+      int8_device(who, qkv, **w.first, w.second);
+      REFUSE_UNLESS((*w.first)->scalar_type() == qkv.scalar_type() && (*w.first)->numel() == D, w.second, " must have D=", D,
+                    " entries in qkv's type");
+      int8_aligned(who, **w.first, w.second);
+    }
+  int8_device(who, qkv, table, "cos_sin");
+  REFUSE_UNLESS(table.dim() == 2 && (table.scalar_type() == at::kFloat || table.scalar_type() == qkv.scalar_type()),
+                "cos_sin must be [places, rot] in fp32 or qkv's type, got ", table.scalar_type(), " ", table.sizes());
+  const int64_t rot = table.size(1);
+  REFUSE_UNLESS(rot % 16 == 0 && rot <= D && table.size(0) < (1LL << 31), "cos_sin must have a multiple of 16 columns up to D=", D, ", got ",
+                table.sizes());
+  REFUSE_UNLESS(!T || !rot || table.size(0) > 0, "cos_sin has no rows");
+  int8_aligned(who, table, "cos_sin");
+  int8_device(who, qkv, positions, "positions");
+  REFUSE_UNLESS(positions.scalar_type() == at::kLong && positions.numel() == T, "positions must be int64 with T=", T, " entries");
+  if (k.has_value()) {
+    attn_device(who, qkv, *k, "k_out");
+    REFUSE_UNLESS(k->dim() == 3 && k->size(0) == T && k->size(1) == Hkv && k->size(2) == D && k->scalar_type() == qkv.scalar_type(),
+                  "k_out must be [T, Hkv, D] in qkv's type, got ", k->scalar_type(), " ", k->sizes());
+    attn_heads(who, *k, "k_out");
+  }
+  REFUSE_UNLESS(kc.has_value() == vc.has_value() && kc.has_value() == slots.has_value(),
+                "key_cache, value_cache and slot_mapping are given together or not at all");
+  REFUSE_UNLESS(k.has_value() || kc.has_value(), "keys have nowhere to go: give k_out or a cache");
+  // in place: exactly the columns that are read
+  auto own = [&](const Tensor& t, int64_t column) {
+    return t.data_ptr() == (const char*)qkv.data_ptr() + column * 2 && (T == 1 || t.stride(0) == qkv.stride(0)) &&
+           (t.size(1) == 1 || t.stride(1) == D);
+  };
+  const bool q_own = own(q, 0), k_own = k.has_value() && own(*k, Hq * D);
+  const Tensor* outs[4] = {&q, k.has_value() ? &*k : nullptr, kc.has_value() ? &*kc : nullptr, vc.has_value() ? &*vc : nullptr};
+  const char* names[4] = {"q_out", "k_out", "key_cache", "value_cache"};
+  MiPagedCache cache{};
+  if (kc.has_value()) {
+    cache = paged_cache(who, qkv, *kc, *vc, Hkv, D);
+    int8_device(who, qkv, *slots, "slot_mapping");
+    REFUSE_UNLESS(slots->scalar_type() == at::kLong && slots->numel() == T, "slot_mapping must be int64 with T=", T, " entries");
+  }
+  for (int i = 0; i < 4; ++i) {
+    if (!outs[i]) continue;
+    attn_apart_inside(who, *outs[i], names[i]);
+    if (!(i == 0 && q_own) && !(i == 1 && k_own)) attn_apart(who, *outs[i], names[i], qkv, "qkv");
+    if (qw.has_value()) attn_apart(who, *outs[i], names[i], *qw, "q_weight");
+    if (kw.has_value()) attn_apart(who, *outs[i], names[i], *kw, "k_weight");
+    attn_apart(who, *outs[i], names[i], table, "cos_sin");
+    attn_apart(who, *outs[i], names[i], positions, "positions");
+    if (slots.has_value()) attn_apart(who, *outs[i], names[i], *slots, "slot_mapping");
+    for (int j = 0; j < i; ++j)                        // keys and values against each other: in paged_cache
+      if (outs[j] && !(i == 1 && j == 0 && q_own && k_own) && !(i == 3 && j == 2)) attn_apart(who, *outs[i], names[i], *outs[j], names[j]);
+  }
+  if (!T) return q;
+  const On on(qkv);
+  CALL(mi_qk_norm_rope, qkv.data_ptr(), stride_of(qkv, 0), data_or_null(qw), data_or_null(kw), table.data_ptr(), table.scalar_type() == at::kFloat,
+       positions.data_ptr<int64_t>(), q.data_ptr(), stride_of(q, 0), stride_of(q, 1), k.has_value() ? k->data_ptr() : nullptr,
+       k.has_value() ? stride_of(*k, 0) : 0, k.has_value() ? stride_of(*k, 1) : 0, kc.has_value() ? &cache : nullptr,
+       slots.has_value() ? slots->data_ptr<int64_t>() : nullptr, (int)T, (int)Hq, (int)Hkv, (int)D, (int)rot, (int)table.size(0), (float)eps,
+       interleaved, act(qkv), on.stream);
+  return q;
+}
+
+// What the two attentions have in common
+struct AttnCall { int T, B, Hq, Hkv, D, width, longest, keys; MiPagedCache cache; };
+AttnCall attn_call(const char* who, const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& seq, const Tensor& cu,
+                   const Tensor& out, double scale, int64_t max_query_len, int64_t max_seq_len) {
+  REFUSE_UNLESS(q.is_cuda(), "query must be on a ROCm device, got ", q.device());
+  REFUSE_UNLESS(is16(q) && q.dim() == 3, "query must be fp16 or bf16 [T, heads, D], got ", q.scalar_type(), " ", q.sizes());
+  attn_heads(who, q, "query");
+  AttnCall a{};
+  const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2);
+  a.cache = paged_cache(who, q, kc, vc, 0, D);
+  const int64_t Hkv = kc.size(2);
+  REFUSE_UNLESS(Hq > 0 && Hq <= 65536 && Hq % Hkv == 0, "the query's heads must be a multiple of the cache's, got ", Hq, " and ", Hkv);
+  REFUSE_UNLESS(T * Hq < (1LL << 28), "T x heads must be below 2^28, got ", q.sizes());
+  int8_device(who, q, table, "block_table");
+  int8_device(who, q, seq, "seq_lens");
+  int8_device(who, q, cu, "cu_seqlens_q");
+  int8_device(who, q, out, "output");
+  REFUSE_UNLESS(table.scalar_type() == at::kInt && table.dim() == 2, "block_table must be int32 [B, width], got ", table.scalar_type(), " ",
+                table.sizes());
+  const int64_t B = table.size(0), width = table.size(1);
+  REFUSE_UNLESS(B < (1 << 24) && width < (1LL << 30) && width * kc.size(1) < (1LL << 30), "block_table ", table.sizes(), " of pages of ",
+                kc.size(1), " is too large");
+  REFUSE_UNLESS(seq.scalar_type() == at::kInt && seq.numel() == B, "seq_lens must be int32 with B=", B, " entries");
+  REFUSE_UNLESS(cu.scalar_type() == at::kInt && cu.numel() == B + 1, "cu_seqlens_q must be int32 with B + 1 = ", B + 1, " entries");
+  REFUSE_UNLESS(out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes(), "output must have the query's type and sizes, got ",
+                out.scalar_type(), " ", out.sizes());
+  int8_aligned(who, out, "output");
+  REFUSE_UNLESS(scale > 0 && scale < 1e30, "scale must be positive, got ", scale);
+  REFUSE_UNLESS(max_query_len >= 0 && max_seq_len >= 0, "max_query_len and max_seq_len must not be negative");
+  attn_apart(who, out, "output", q, "query");
+  attn_apart(who, out, "output", kc, "key_cache");
+  attn_apart(who, out, "output", vc, "value_cache");
+  attn_apart(who, out, "output", table, "block_table");
+  attn_apart(who, out, "output", seq, "seq_lens");
+  attn_apart(who, out, "output", cu, "cu_seqlens_q");
+  a.T = (int)T;
+  a.B = (int)B;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.D = (int)D;
+  a.width = (int)width;
+  a.longest = (int)std::min<int64_t>(max_query_len, INT_MAX);
+  a.keys = (int)std::min<int64_t>(max_seq_len, INT_MAX);
+  return a;
+}
+Tensor attn_workspace(const Tensor& q, const AttnCall& a, long long& bytes) {
+  CALL(mi_paged_attention_workspace, a.T, a.B, a.Hq, a.Hkv, a.D, a.longest, a.keys, &bytes);
+  return bytes ? buffer(q, bytes) : Tensor();
+}
+
+Tensor paged_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& seq, const Tensor& cu,
+                       const Tensor& out, double scale, int64_t window, int64_t sinks, int64_t max_query_len, int64_t max_seq_len) {
+  const char* who = "paged_attention";
+  const AttnCall a = attn_call(who, q, kc, vc, table, seq, cu, out, scale, max_query_len, max_seq_len);
+  REFUSE_UNLESS(window == -1 || window >= 1, "window must be -1 (none) or at least 1, got ", window);
+  REFUSE_UNLESS(sinks >= 0, "sinks must not be negative, got ", sinks);
+  if (!a.T || !a.B) return out;
+  const On on(q);
+  long long bytes = 0;
+  const Tensor ws = attn_workspace(q, a, bytes);
+  CALL(mi_paged_attention_ws, q.data_ptr(), stride_of(q, 0), stride_of(q, 1), &a.cache, table.data_ptr<int>(), a.width, seq.data_ptr<int>(),
+       cu.data_ptr<int>(), out.data_ptr(), int8_buffer(ws), bytes, a.T, a.B, a.Hq, a.Hkv, a.D, (float)scale,
+       (int)std::min<int64_t>(window, INT_MAX), (int)std::min<int64_t>(sinks, INT_MAX), a.longest, a.keys, act(q), on.stream);
+  return out;
+}
+
+Tensor tree_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& seq, const Tensor& cu,
+                      const Tensor& mask, const Tensor& out, double scale, int64_t max_query_len, int64_t max_seq_len) {
+  const char* who = "tree_attention";
+  const AttnCall a = attn_call(who, q, kc, vc, table, seq, cu, out, scale, max_query_len, max_seq_len);
+  int8_device(who, q, mask, "tree_mask");
+  REFUSE_UNLESS(mask.scalar_type() == at::kLong && mask.dim() == 2 && mask.size(0) == a.T && mask.size(1) >= 1 && mask.size(1) <= 1 << 20,
+                "tree_mask must be int64 [T, words], got ", mask.scalar_type(), " ", mask.sizes());
+  REFUSE_UNLESS(max_query_len <= 64 * mask.size(1), "tree_mask has ", mask.size(1), " words for up to ", max_query_len, " drafted tokens");
+  attn_apart(who, out, "output", mask, "tree_mask");
+  if (!a.T || !a.B) return out;
+  const On on(q);
+  long long bytes = 0;
+  const Tensor ws = attn_workspace(q, a, bytes);
+  CALL(mi_tree_attention_ws, q.data_ptr(), stride_of(q, 0), stride_of(q, 1), &a.cache, table.data_ptr<int>(), a.width, seq.data_ptr<int>(),
+       cu.data_ptr<int>(), mask.data_ptr<int64_t>(), (int)mask.size(1), out.data_ptr(), int8_buffer(ws), bytes, a.T, a.B, a.Hq, a.Hkv, a.D,
+       (float)scale, a.longest, a.keys, act(q), on.stream);
+  return out;
+}
+
 }  // namespace
 
 #define IMPL(name) m.impl(#name, &name)
@@ -614,6 +851,7 @@ Tensor moe_forward_full_int8(const Tensor& x, const Tensor& logits, const Tensor
 TORCH_LIBRARY_IMPL(custom_esimd_kernels_vllm, CUDA, m) {
   DECODE_OPS(); GEMM_OPS();
   IMPL(gemm_int8); IMPL(resadd_norm_gemm_int8); IMPL(silu_mul_gemm_int8);
+  IMPL(qk_norm_rope); IMPL(paged_attention); IMPL(tree_attention);
 }
 TORCH_LIBRARY_IMPL(custom_esimd_kernels, CUDA, m) { GEMM_OPS(); }
 TORCH_LIBRARY_IMPL(custom_esimd_kernels_sglang, CUDA, m) {

@@ -389,3 +389,30 @@ def resadd_norm_gemm_int8(hidden_states, residual, residual_out, norm_weight, we
 def silu_mul_gemm_int8(gate_up, weight, weight_scale, bias, output):
     """gate_up [M, 2K], gate columns first: gemm_int8 on silu(gate) * up."""
     return _silu_mul_gemm_int8(gate_up, weight, weight_scale, bias, output)
+
+
+_qk_norm_rope, _paged_attention, _tree_attention = _ops.qk_norm_rope.default, _ops.paged_attention.default, _ops.tree_attention.default
+
+
+def qk_norm_rope(qkv, q_weight, k_weight, cos_sin, positions, q_out, k_out, key_cache, value_cache, slot_mapping, eps, interleaved=False):
+    """qkv [T, (Hq + 2 Hkv) D]: an RMS norm of every query and key head (weights [D] or None), the rotation by cos_sin[positions]
+    ([places, rot], cosines first; fp32 or qkv's type) on the first rot elements of a head (halves, or neighbours if interleaved), queries to
+    q_out [T, Hq, D], keys to k_out [T, Hkv, D] (or None), keys and values to slot_mapping [T] of the cache [pages, page, Hkv, D] (all three
+    or None; slots outside the cache are left out).  q_out and k_out may be qkv's own columns."""
+    return _qk_norm_rope(qkv, q_weight, k_weight, cos_sin, positions, q_out, k_out, key_cache, value_cache, slot_mapping, eps, interleaved)
+
+
+def paged_attention(query, key_cache, value_cache, block_table, seq_lens, cu_seqlens_q, output, scale, window, sinks, max_query_len,
+                    max_seq_len):
+    """query [T, Hq, D], rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] the last tokens of sequence b with seq_lens[b] keys in the cache
+    [pages, page, Hkv, D] through block_table [B, width]; int32 each.  Causal; window -1, or a token sees that many keys back from itself and
+    the first `sinks` of the sequence.  max_query_len and max_seq_len: the longest ones, for the choice of kernels alone."""
+    return _paged_attention(query, key_cache, value_cache, block_table, seq_lens, cu_seqlens_q, output, scale, window, sinks, max_query_len,
+                            max_seq_len)
+
+
+def tree_attention(query, key_cache, value_cache, block_table, seq_lens, cu_seqlens_q, tree_mask, output, scale, max_query_len, max_seq_len):
+    """paged_attention for drafted tokens, the last ones of each sequence: each sees the whole context and the drafted tokens whose bits
+    tree_mask [T, words] (int64) has in its row."""
+    return _tree_attention(query, key_cache, value_cache, block_table, seq_lens, cu_seqlens_q, tree_mask, output, scale, max_query_len,
+                           max_seq_len)

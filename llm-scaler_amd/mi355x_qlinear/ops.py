@@ -2459,6 +2459,16 @@ def register():
                        "Tensor? shared_gate_up_weight, Tensor? shared_gate_up_scale, Tensor down_weight, Tensor down_scale, "
                        "Tensor? shared_down_weight, Tensor? shared_down_scale, Tensor? shared_expert_gate_weight, int top_k, "
                        "int num_shared_experts, int n_routed_experts) -> Tensor(a!)", None, _ret(2))
+    # attention over a paged cache: no operators of these schemas in the reference
+    _define(_V, "qk_norm_rope(Tensor qkv, Tensor? q_weight, Tensor? k_weight, Tensor cos_sin, Tensor positions, Tensor(a!) q_out, "
+                "Tensor(b!)? k_out, Tensor(c!)? key_cache, Tensor(d!)? value_cache, Tensor? slot_mapping, float eps, "
+                "bool interleaved) -> Tensor(a!)", None, _ret(5))
+    _define(_V, "paged_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor seq_lens, "
+                "Tensor cu_seqlens_q, Tensor(a!) output, float scale, int window, int sinks, int max_query_len, int max_seq_len) "
+                "-> Tensor(a!)", None, _ret(6))
+    _define(_V, "tree_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor seq_lens, "
+                "Tensor cu_seqlens_q, Tensor tree_mask, Tensor(a!) output, float scale, int max_query_len, int max_seq_len) "
+                "-> Tensor(a!)", None, _ret(7))
 
 
 register()
