@@ -45,8 +45,8 @@ static int attn_plan(int T, int B, int Hq, int Hkv, int D, int max_query_len, in
   }
   const long long blocks = ((long long)(max_seq_len < 1 ? 1 : max_seq_len) + kBlock - 1) / kBlock;
   if (a.rows) {
-    const long long full = (long long)cus() * (D == 64 ? 2 : 1);                 // workgroups that the device holds
-    const long long some = ((long long)T * G / 32 + B) * Hkv * blocks;
+    const long long full = (long long)cus() * (D == 64 ? 8 : D == 128 ? 4 : 2);  // workgroups that the device holds
+    const long long some = ((long long)T * G / 32 + B) * Hkv * 2 * blocks;
     a.groups = (int)(some < full ? some : full);
     a.rows_bytes = round256(attn_rows_bytes(a.groups, D));
   }

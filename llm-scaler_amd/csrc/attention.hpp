@@ -2,8 +2,8 @@
 //
 //   o_i = sum_j p_ij v_j,   p_ij = 2^(c s_ij - m_i) / l_i,   s_ij = q_i . k_j,   c = scale log2(e)
 //
-// in one pass over the keys: m is the running maximum of c times a row's scores, l the running sum, and both o and l are multiplied by
-// 2^(m_old - m_new) where a row's maximum grows.  s, m, l and o are fp32; p is rounded to the type of the values in front of its product with
+// in one pass over the keys: m follows the largest c s of a row, l is the running sum, and both o and l are multiplied by
+// 2^(m_old - m_new) where m moves.  s, m, l and o are fp32; p is rounded to the type of the values in front of its product with
 // them (off by half a step of a 16-bit number, below the output's rounding, as v_j is already such a number), and l sums the rounded p.
 //
 // The rows of a kv head are (token, head of the group) pairs of a sequence, token first: row r is head r % G of token r / G.  A wavefront holds 32
@@ -21,8 +21,6 @@ namespace qlin {
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) short i16x4;
 typedef __attribute__((ext_vector_type(8))) short i16x8;
-typedef const __attribute__((address_space(1))) void* global_ptr;
-typedef __attribute__((address_space(3))) void* lds_void;
 
 struct AttnArgs {
   const void *q, *k, *v;
@@ -96,10 +94,7 @@ __device__ __forceinline__ int attn_key(const AttnRange& r, int block) {
 __device__ __forceinline__ int attn_page_of(const AttnArgs& p, int key) {
   return (int)((__umulhi((uint32_t)key, p.page_mul) + (uint32_t)key) >> p.page_shift);
 }
-__device__ __forceinline__ int attn_lookup(const AttnArgs& p, const int32_t* row, const AttnRange& r, int key) {
-  const bool seen = key < r.hi && (key >= r.lo || key < p.sinks);
-  return seen ? row[attn_page_of(p, key)] : -1;
-}
+__device__ __forceinline__ bool attn_in(const AttnArgs& p, const AttnRange& r, int key) { return key < r.hi && (key >= r.lo || key < p.sinks); }
 __device__ __forceinline__ uint32_t attn_place(const AttnArgs& p, int page, int key, int head) {
   if ((uint32_t)page >= (uint32_t)p.pages) return kNoRow;
   return (uint32_t)page * p.page16 + (uint32_t)(key - attn_page_of(p, key) * p.page) * p.row16 + (uint32_t)head * p.head16;
@@ -136,64 +131,87 @@ __device__ const u32x4 kZeroRow[64] = {};             // what a key that nothing
 template <int D> __device__ __forceinline__ int k_swizzle(int r) { return r & (D / 8 < 16 ? D / 8 - 1 : 15); }
 template <int D> __device__ __forceinline__ int v_swizzle(int r) { return D == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2; }
 
-// Rows [first, first + ROWS) of a block of keys to LDS by one wavefront: lane i holds the place of row i of the block.
-template <int D, int ROWS>
-__device__ __forceinline__ void attn_load(const void* k, const void* v, uint32_t place, int first, unsigned char* to_k, unsigned char* to_v) {
-  constexpr int CH = D / 8, RPI = 64 / CH, N = ROWS / RPI;     // chunks of a row, rows per load
-  static_assert(RPI * N == ROWS && (64 % CH) == 0, "rows per load");
-  const int lane = threadIdx.x & 63, c = lane % CH;
-  const unsigned char* src[N];
-  bool there[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const uint32_t at = __shfl(place, first + j * RPI + lane / CH, 64);
-    there[j] = at != kNoRow;
-    src[j] = (const unsigned char*)((uint64_t)at * 16);
-  }
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int r = first + j * RPI + lane / CH, ck = (c ^ k_swizzle<D>(r)) * 16;
-    const unsigned char* a = (there[j] ? (const unsigned char*)k + (uint64_t)src[j] : (const unsigned char*)kZeroRow) + ck;
-    __builtin_amdgcn_global_load_lds((global_ptr)a, (lds_void)(to_k + j * 1024), 16, 0, 0);
-  }
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int r = first + j * RPI + lane / CH, cv = (c ^ v_swizzle<D>(r)) * 16;
-    const unsigned char* a = (there[j] ? (const unsigned char*)v + (uint64_t)src[j] : (const unsigned char*)kZeroRow) + cv;
-    __builtin_amdgcn_global_load_lds((global_ptr)a, (lds_void)(to_v + j * 1024), 16, 0, 0);
-  }
+__device__ const int32_t kNoPage[1] = {-1};
+
+// 16 (4) bytes per lane from memory to LDS, side by side.  As a builtin the compiler waits for all of them in front of every transposing read of
+// LDS, loads for the next block included; here the kernels wait for themselves (wait_loads) and the compiler counts none of them.
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
+}
+__device__ __forceinline__ void to_lds16(const void* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
+}
+__device__ __forceinline__ void to_lds4(const void* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(to) : "memory", "m0");
 }
 
-// ---- 32 rows of a wavefront -------------------------------------------------------------------
-template <class Act, int D>
+// Rows [first, first + ROWS) of a block of keys to LDS by one wavefront: lane i holds the place of row i of the block, from which every lane takes
+// those of the rows that it loads a part of.
+template <int D, int ROWS>
+struct RowPlaces {
+  static constexpr int CH = D / 8, RPI = 64 / CH, N = ROWS / RPI;          // chunks of a row, rows per load
+  static_assert(RPI * N == ROWS && (64 % CH) == 0, "rows per load");
+  uint32_t of[N];
+  __device__ __forceinline__ void take(uint32_t place, int first) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) of[j] = __shfl(place, first + j * RPI + (int)(threadIdx.x & 63) / CH, 64);
+  }
+  template <bool IS_K>
+  __device__ __forceinline__ void load(const void* from, int first, const unsigned char* to) const {
+    const int lane = threadIdx.x & 63;
+    const uint32_t lds = lds_address(to);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int r = first + j * RPI + lane / CH, chunk = (lane % CH) ^ (IS_K ? k_swizzle<D>(r) : v_swizzle<D>(r));
+      const unsigned char* a = of[j] != kNoRow ? (const unsigned char*)from + (uint64_t)of[j] * 16 : (const unsigned char*)kZeroRow;
+      to_lds16(a + chunk * 16, lds + j * 1024);
+    }
+  }
+};
+
+// ---- the rows of a wavefront ------------------------------------------------------------------
+// 32 NQ rows over blocks of N keys, a step at a time: scores (K Q^T), their maximum, weights (exp), and the product with V.
+template <class Act, int D, int N, int NQ>
 struct AttnRows {
   using v8 = typename Act::v8;
   typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
-  static constexpr int DT = D / 32;
+  static constexpr int DT = D / 32, KT = N / 32;
+  static constexpr float kRaise = 7.f;
   static constexpr unsigned short EXPONENT = Act::dt == DT_F16 ? 0x7C00 : 0x7F80;
-  v8 q[D / 16];
-  f32x16 o[DT];                // o[t][i]: column 32 t + 8 (i / 4) + 4 (lane / 32) + i % 4 of row lane % 32
-  float m, l;                  // m: c times the row's largest score; l: of this lane's keys
+  struct Scores { f32x16 s[NQ][KT]; };                 // s[n][t][i]: key 32 t + 8 (i / 4) + 4 (lane / 32) + i % 4, row 32 n + lane % 32
+  struct Weights { v8 p[NQ][2 * KT]; };                // p[n][t][e]: key 16 t + 8 (e / 4) + 4 (lane / 32) + e % 4
+  struct Mask { uint64_t of[NQ]; };                    // bit i: row 32 n + lane % 32 sees key i; null where a key is not there
+
+  v8 q[NQ][D / 16];
+  f32x16 o[NQ][DT];            // o[n][t][i]: column 32 t + 8 (i / 4) + 4 (lane / 32) + i % 4
+  float m[NQ], l[NQ];          // m: what a row's exponents are taken from, at most 8 below the largest; l: of this lane's keys
   int ka, va;                  // where this lane reads K and V of a block
 
   __device__ __forceinline__ void start() {
     const int lane = threadIdx.x & 63, h = lane >> 5, i = lane & 15;
-    m = -__builtin_inff();
-    l = 0.f;
 #pragma unroll
-    for (int t = 0; t < DT; ++t) o[t] = f32x16{};
+    for (int n = 0; n < NQ; ++n) {
+      m[n] = -__builtin_inff();
+      l[n] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) o[n][t] = f32x16{};
+    }
     ka = (lane & 31) * 2 * D + ((h ^ k_swizzle<D>(lane & 31)) * 16);
     // keys 4 h + i / 4, columns 16 (lane / 16 % 2) + 4 (i % 4)
     va = (4 * h + (i >> 2)) * 2 * D + (((2 * (lane >> 4 & 1) + (i >> 1 & 1)) ^ v_swizzle<D>(i >> 2)) * 16) + (i & 1) * 8;
   }
-  __device__ __forceinline__ void load_q(const void* row) {      // null: zeros
+  __device__ __forceinline__ void load_q(int n, const void* row) {         // null: zeros
     const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
       u32x4 x = {};
       if (row) x = *(const u32x4*)((const unsigned char*)row + s * 32 + h * 16);
-      q[s] = as_v8<v8>(x);
+      q[n][s] = as_v8<v8>(x);
     }
+  }
+  // K of 32 keys (from 32 t of the block) and columns 16 ks ..
+  __device__ __forceinline__ v8 k_operand(const unsigned char* k, int t, int ks) const {
+    return as_v8<v8>(*(const u32x4*)(k + ((ka ^ (ks % 8 * 32)) + ks / 8 * 256 + t * 64 * D)));
   }
   // V^T of 16 keys (from 16 t of the block) and columns 32 d ..: element e is key 4 (lane / 32) + e % 4 + 8 (e / 4)
   __device__ __forceinline__ v8 v_operand(const unsigned char* v, int t, int d) const {
@@ -202,64 +220,131 @@ struct AttnRows {
     const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(at + 16 * D));
     return __builtin_bit_cast(v8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   }
-  // A block of N keys.  mask: bit i of this lane's row: it sees key i; null bits everywhere a key is not there.  full: all bits of all lanes are set.
-  template <int N>
-  __device__ __forceinline__ void block(const unsigned char* k, const unsigned char* v, bool full, uint64_t mask, float c) {
-    constexpr int KT = N / 32;
-    const int h = (threadIdx.x & 63) >> 5;
-    f32x16 s[KT];
+
+  __device__ __forceinline__ void scores(const unsigned char* k, Scores& x) const {
 #pragma unroll
-    for (int t = 0; t < KT; ++t) s[t] = f32x16{};
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int t = 0; t < KT; ++t) x.s[n][t] = f32x16{};
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
-        const u32x4 x = *(const u32x4*)(k + ((ka ^ (ks % 8 * 32)) + ks / 8 * 256 + t * 64 * D));
-        s[t] = mfma32(as_v8<v8>(x), q[ks], s[t]);
+        const v8 a = k_operand(k, t, ks);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) x.s[n][t] = mfma32(a, q[n][ks], x.s[n][t]);
       }
-    if (!full) {
+  }
+  // A step of the tiles kernel in pieces whose reads of LDS go out long before their products: keys a step ahead, values while the scores are made.
+  // Reads stay on their side of a `pin`; everything else may move.
+  struct Keys { v8 k[D / 16]; };
+  struct Values { v8 v[DT]; };
+  static __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0x40E); }
+  __device__ __forceinline__ void read_keys(const unsigned char* k, Keys& f) const {
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) f.k[ks] = k_operand(k, 0, ks);
+  }
+  __device__ __forceinline__ void read_values(const unsigned char* v, int t, Values& f) const {
+#pragma unroll
+    for (int d = 0; d < DT; ++d) f.v[d] = v_operand(v, t, d);
+  }
+  // Weights of this step's scores x, the product with its values, the next step's scores y and their maximum; f: the next step's keys, then those at k2
+  __device__ __forceinline__ void step(const Scores& x, const unsigned char* v, Keys& f, const unsigned char* k2, float c, Scores& y, float (&top)[NQ]) {
+    static_assert(NQ == 1 && KT == 1, "a step of 32 keys");
+    Values va, vb;
+    Weights w;
+    read_values(v, 0, va);
+    pin();
+    y.s[0][0] = f32x16{};
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) y.s[0][0] = mfma32(f.k[ks], q[0][ks], y.s[0][0]);
+    read_values(v, 1, vb);
+    pin();
+    weigh(x, c, w);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[0][d] = mfma32(va.v[d], w.p[0][0], o[0][d]);
+    read_keys(k2, f);
+    pin();
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[0][d] = mfma32(vb.v[d], w.p[0][1], o[0][d]);
+    largest(y, c, top);
+    follow(top);
+  }
+  __device__ __forceinline__ void hide(Scores& x, const Mask& mask) const {
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
-        const uint32_t bits = (uint32_t)(mask >> (32 * t)) >> (4 * h);
+        const uint32_t bits = (uint32_t)(mask.of[n] >> (32 * t)) >> (4 * h);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[t][i] = bits >> (8 * (i / 4) + i % 4) & 1 ? s[t][i] : -__builtin_inff();
+        for (int i = 0; i < 16; ++i) x.s[n][t][i] = bits >> (8 * (i / 4) + i % 4) & 1 ? x.s[n][t][i] : -__builtin_inff();
       }
+  }
+  // c times the largest score of a row
+  __device__ __forceinline__ void largest(const Scores& x, float c, float (&top)[NQ]) const {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float mx = x.s[n][0][0];
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x.s[n][t][i]);
+      const Halves y = both_halves(mx);
+      top[n] = fmaxf(y.low, y.high) * c;
     }
-    float mx = s[0][0];
+  }
+  // Sums move to a new m only where an exponent would pass it by 8.  Weights are 2^kRaise times as large, up to 2^15, so that in fp16 those of a
+  // long tail keep their bits (half of the smallest number is 2^-32 of the largest weight).
+  __device__ __forceinline__ void follow(const float (&top)[NQ]) {
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
-    const Halves x = both_halves(mx);
-    mx = fmaxf(m, fmaxf(x.low, x.high) * c);
-    const float top = mx == -__builtin_inff() ? 0.f : mx;        // a row that has seen nothing yet
-    if (__builtin_amdgcn_ballot_w64(mx != m)) {
-      const float a = __builtin_amdgcn_exp2f(m - top);
-      l *= a;
+    for (int n = 0; n < NQ; ++n) {
+      const bool moves = top[n] > m[n] + 8.f;          // row by row: a row's bits depend on no other row
+      if (!__builtin_amdgcn_ballot_w64(moves)) continue;
+      const float to = moves ? top[n] : m[n], a = moves ? __builtin_amdgcn_exp2f(m[n] - to) : 1.f;
+      l[n] *= a;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] *= a;
-      m = mx;
+        for (int i = 0; i < 16; ++i) o[n][d][i] *= a;
+      m[n] = to;
     }
-    v8 p[2 * KT];
-    float sum = 0.f;
+  }
+  __device__ __forceinline__ void weigh(const Scores& x, float c, Weights& w) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const float top = m[n] == -__builtin_inff() ? 0.f : m[n] - kRaise;   // first: a row that has seen nothing yet
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2 * KT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          w.p[n][t][e] = Act::from_f32(__builtin_amdgcn_exp2f(__builtin_fmaf(x.s[n][t / 2][8 * (t % 2) + e], c, -top)));
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) sum = add_two(w.p[n][t], e, sum);
+      }
+      l[n] += sum;
+    }
+  }
+  static __device__ __forceinline__ float add_two(v8 p, int e, float sum) {
+    typedef __attribute__((ext_vector_type(2))) typename Act::elem e2;
+    const e2 two = {p[e], p[e + 1]}, one = {(typename Act::elem)1.f, (typename Act::elem)1.f};
+    if constexpr (Act::dt == DT_F16) return __builtin_amdgcn_fdot2(two, one, sum, false);
+    else return __builtin_amdgcn_fdot2_f32_bf16(two, one, sum, false);
+  }
+  __device__ __forceinline__ void add(const unsigned char* v, const Weights& w) {
 #pragma unroll
     for (int t = 0; t < 2 * KT; ++t)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[t][e] = Act::from_f32(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][8 * (t % 2) + e], c, -top)));
-        sum += Act::to_f32(p[t][e]);
+      for (int d = 0; d < DT; ++d) {
+        const v8 a = v_operand(v, t, d);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) o[n][d] = mfma32(a, w.p[n][t], o[n][d]);
       }
-    l += sum;
-    if (full) {
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int t = 0; t < 2 * KT; ++t) o[d] = mfma32(v_operand(v, t, d), p[t], o[d]);
-      return;
-    }
-    // 0 times an infinity or a NaN that a row does not see would not be 0: such values go to the rows that see them by themselves.
+  }
+  // The same where some row does not see some key: 0 times an infinity or a NaN there would not be 0, so such values go to the rows that see
+  // them by themselves.
+  __device__ __forceinline__ void add_hidden(const unsigned char* v, const Weights& w, const Mask& mask) {
     u16x8 one = 1;                                     // 0 where a value was not finite
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -269,20 +354,20 @@ struct AttnRows {
         const u16x8 x = __builtin_bit_cast(u16x8, v_operand(v, t, d));
         const u16x8 finite = __builtin_elementwise_min(EXPONENT - (x & EXPONENT), (u16x8)1);
         one &= finite;
-        o[d] = mfma32(__builtin_bit_cast(v8, x & (0 - finite)), p[t], o[d]);
+        const v8 a = __builtin_bit_cast(v8, x & (0 - finite));
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) o[n][d] = mfma32(a, w.p[n][t], o[n][d]);
       }
     }
     const u32x4 all = __builtin_bit_cast(u32x4, one);
-    if (__builtin_amdgcn_ballot_w64((all[0] & all[1] & all[2] & all[3]) != 0x00010001u)) add_not_finite<N>(v, mask);
+    if (__builtin_amdgcn_ballot_w64((all[0] & all[1] & all[2] & all[3]) != 0x00010001u)) add_not_finite(v, mask);
   }
-  template <int N>
-  __device__ __forceinline__ void add_not_finite(const unsigned char* v, uint64_t mask) {
+  __device__ __forceinline__ void add_not_finite(const unsigned char* v, const Mask& mask) {
     const int h = (threadIdx.x & 63) >> 5;
     typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
     typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
 #pragma unroll 1
     for (int j = 0; j < N; ++j) {
-      const bool sees = mask >> j & 1;
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         __builtin_amdgcn_sched_barrier(0);
@@ -291,7 +376,10 @@ struct AttnRows {
           const u16x4 x = *(const u16x4*)(v + j * 2 * D + ((4 * d + i) ^ v_swizzle<D>(j)) * 16 + h * 8);
           const e4 y = __builtin_bit_cast(e4, x);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[d][4 * i + e] += sees && (x[e] & EXPONENT) == EXPONENT ? Act::to_f32(y[e]) : 0.f;
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              o[n][d][4 * i + e] += (mask.of[n] >> j & 1) && (x[e] & EXPONENT) == EXPONENT ? Act::to_f32(y[e]) : 0.f;
         }
       }
     }

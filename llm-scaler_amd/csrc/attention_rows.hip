@@ -1,10 +1,10 @@
-// Attention of few rows per sequence (single tokens, small trees): 32 rows at most are in a tile, and the wavefronts of a workgroup take 32 keys
-// each, with their loads two steps ahead and no barrier between them; their results meet in LDS.
+// Attention of few rows per sequence (single tokens, small trees): up to 32 rows are in a tile, a wavefront by itself takes a part of the keys of one
+// tile after another, 32 at a time, with its loads two steps ahead.
 //
-// The work is cut evenly whatever the sequences' lengths are: all blocks of 64 keys of all (sequence, tile, kv head) in a row, and
-// workgroup w takes [w, w + 1) total / groups of them.  A tile whose blocks all lie in one workgroup is finished there; of the others each
-// workgroup has at most one that it continues and one that it begins, kept as unscaled fp32 sums with their m and l, and a second
-// launch joins them.
+// The work is cut evenly whatever the sequences' lengths are: the blocks of 32 keys of all (sequence, tile, kv head) in a row, each of these with
+// kItem blocks more for what beginning it costs, and workgroup w takes [w, w + 1) total / groups of them.  A tile whose blocks all lie in one
+// workgroup is finished there; of the others each workgroup has at most one that it continues and one that it begins, kept as unscaled fp32 sums
+// with their m and l, and a second launch joins them.
 //
 // Bound: HBM.
 #include "attention.hpp"
@@ -12,26 +12,25 @@
 namespace qlin {
 
 template <int D> struct RowsCfg {
-  static constexpr int NW = D == 256 ? 2 : 4;          // wavefronts
-  static constexpr int STAGES = 2;
-  static constexpr int HALF = 32 * D * 2;              // K or V of a step
-  static constexpr int LDS = NW * STAGES * 2 * HALF;
-  static constexpr int PITCH = D + 4;                  // of the floats in LDS
+  static constexpr int KEYS = 32, STAGES = 2;
+  static constexpr int HALF = KEYS * D * 2;            // K or V of a step
+  static constexpr int LDS = STAGES * 2 * HALF + 512;  // behind the ring: pages of 64 keys, twice
   static constexpr int PART = 32 * (D + 2);            // floats of a part: sums, m, l
 };
+constexpr int kItem = 3;
 
 // How many tiles a sequence has here, and how many blocks each of them
 struct RowsSeq { AttnSeq s; AttnRange r; int tiles; };
 __device__ __forceinline__ RowsSeq rows_seq(const AttnArgs& p, int b) {
   RowsSeq x;
   x.s = attn_seq(p, b);
-  x.r = attn_range<kBlock>(p, x.s, 0, x.s.n - 1);
+  x.r = attn_range<32>(p, x.s, 0, x.s.n - 1);
   x.r.blocks = max(x.r.blocks, 1);                     // a row that sees nothing is written too
   const int rows = x.s.n * p.G;
   x.tiles = rows >= p.rows_from ? 0 : (rows + 31) / 32;
   return x;
 }
-__device__ __forceinline__ long long rows_work(const AttnArgs& p, const RowsSeq& x) { return (long long)x.tiles * p.Hkv * x.r.blocks; }
+__device__ __forceinline__ long long rows_work(const AttnArgs& p, const RowsSeq& x) { return (long long)x.tiles * p.Hkv * (x.r.blocks + kItem); }
 
 __device__ __forceinline__ long long shfl64(long long v, int lane) {
   return (long long)(uint32_t)__shfl((int)v, lane, 64) | (long long)__shfl((int)(v >> 32), lane, 64) << 32;
@@ -72,14 +71,31 @@ __device__ __forceinline__ void rows_find(const AttnArgs& p, const RowsPlan& a, 
   in = rest;
 }
 
+// A tile's place in the work: its sequence's `in`-th unit
+struct RowsItem { int tile, head, rows, unit; };      // unit: of the tile; its first kItem are none of its blocks
+__device__ __forceinline__ RowsItem rows_item(const AttnArgs& p, const RowsSeq& x, long long in) {
+  const int per = x.r.blocks + kItem;
+  const int item = __builtin_amdgcn_readfirstlane((int)(in / per));
+  RowsItem y;
+  y.unit = __builtin_amdgcn_readfirstlane((int)(in - (long long)item * per));
+  y.tile = item / p.Hkv;
+  y.head = item - y.tile * p.Hkv;
+  y.rows = min(32, x.s.n * p.G - y.tile * 32);
+  return y;
+}
+// Row `row` of a tile in q and out
+__device__ __forceinline__ long long rows_row(const AttnArgs& p, const RowsSeq& x, const RowsItem& y, int row) {
+  const int r = y.tile * 32 + row, t = r / p.G;
+  return (long long)(x.s.q0 + t) * p.Hq + y.head * p.G + r - t * p.G;
+}
+
 template <class Act, int D>
-__global__ __launch_bounds__(64 * RowsCfg<D>::NW) void attn_rows_kernel(const AttnArgs p) {
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2))) void attn_rows_kernel(const AttnArgs p) {
   using C = RowsCfg<D>;
-  constexpr int NW = C::NW, LOADS = 2 * C::HALF / 1024;
+  using Rows = AttnRows<Act, D, 32, 1>;
+  constexpr int LOADS = 2 * C::HALF / 1024;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  __shared__ float ml[2][NW][32];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  unsigned char* ring = smem + wave * (C::STAGES * 2 * C::HALF);
+  const int lane = threadIdx.x;
 
   const RowsPlan plan = rows_plan(p);
   long long at = plan.share * blockIdx.x;
@@ -92,107 +108,107 @@ __global__ __launch_bounds__(64 * RowsCfg<D>::NW) void attn_rows_kernel(const At
 
   while (at < end) {
     const RowsSeq x = rows_seq(p, b);
-    const int item = __builtin_amdgcn_readfirstlane((int)(in / x.r.blocks));
-    const int block0 = __builtin_amdgcn_readfirstlane((int)(in - (long long)item * x.r.blocks));
-    const int block1 = __builtin_amdgcn_readfirstlane((int)min((long long)x.r.blocks, block0 + (end - at)));
-    const int tile = item / p.Hkv, head = item - tile * p.Hkv, rows = min(32, x.s.n * p.G - tile * 32);
-    const int32_t* table = p.table + (size_t)b * p.width;
+    const RowsItem y = rows_item(p, x, in);
+    const int take = __builtin_amdgcn_readfirstlane((int)min((long long)(x.r.blocks + kItem - y.unit), end - at));
+    const int first = max(y.unit - kItem, 0), last = y.unit + take - kItem;      // blocks
+    at += take;
+    in += take;
+    if (last > first) {
+      const int32_t* table = p.table + (size_t)b * p.width;
+      const int r = y.tile * 32 + (lane & 31), t = r / p.G;                      // this lane's row
+      const bool has = (lane & 31) < y.rows;
+      const int64_t* tree = p.tree ? p.tree + (size_t)(x.s.q0 + (has ? t : 0)) * p.tree_words : nullptr;
+      const int t0 = y.tile * 32 / p.G, t1 = (y.tile * 32 + y.rows - 1) / p.G;
+      Rows a;
+      a.start();
+      a.load_q(0, has ? (const typename Act::elem*)p.q + (x.s.q0 + t) * p.q_token + (y.head * p.G + r - t * p.G) * p.q_head : nullptr);
 
-    // this lane's row
-    const int r = tile * 32 + (lane & 31), t = r / p.G;
-    const bool has = (lane & 31) < rows;
-    const int64_t* tree = p.tree ? p.tree + (size_t)(x.s.q0 + (has ? t : 0)) * p.tree_words : nullptr;
-    const int t0 = tile * 32 / p.G, t1 = (tile * 32 + rows - 1) / p.G;
-    AttnRows<Act, D> a;
-    a.start();
-    a.load_q(has ? (const typename Act::elem*)p.q + (x.s.q0 + t) * p.q_token + (head * p.G + r - t * p.G) * p.q_head : nullptr);
-
-    // steps of 32 keys: first + NW i is this wavefront's i-th
-    const int first = 2 * block0 + wave, last = 2 * block1;
-    auto key_of = [&](int step) { return attn_key<kBlock>(x.r, step >> 1) + (step & 1) * 32; };
-    auto lookup = [&](int step) { return step < last ? attn_lookup(p, table, x.r, key_of(step) + (lane & 31)) : -1; };
-    auto place = [&](int page, int step) { return step < last ? attn_place(p, page, key_of(step) + (lane & 31), head) : kNoRow; };
-    uint64_t there[2];
-    int step = first;
-    int page = lookup(step);
+      // block i's keys and values lie in half (i - first) % 2 of the ring, the pages of its keys likewise behind it
+      const unsigned char* pages = smem + C::STAGES * 2 * C::HALF;
+      auto lookup = [&](int i, int u) {
+        const int key = attn_key<32>(x.r, i) + (lane & 31);
+        to_lds4(i < last && attn_in(p, x.r, key) ? table + attn_page_of(p, key) : kNoPage, lds_address(pages + u * 256));
+      };
+      auto place = [&](int i, int u) {
+        const int page = *(const int*)(pages + u * 256 + lane * 4);
+        return i < last ? attn_place(p, page, attn_key<32>(x.r, i) + (lane & 31), y.head) : kNoRow;
+      };
+      auto request = [&](uint32_t at16, int u) {
+        RowPlaces<D, 32> rows;
+        rows.take(at16, 0);
+        rows.template load<true>(p.k, 0, smem + u * 2 * C::HALF);
+        rows.template load<false>(p.v, 0, smem + u * 2 * C::HALF + C::HALF);
+        return (uint32_t)__builtin_amdgcn_ballot_w64(at16 != kNoRow);
+      };
+      uint32_t there[2];
+      lookup(first, 0);
+      lookup(first + 1, 1);
+      wait_loads<0>();
+      const uint32_t at0 = place(first, 0), at1 = place(first + 1, 1);
+      there[0] = request(at0, 0);
+      lookup(first + 2, 0);
+      there[1] = request(at1, 1);
+      for (int i = first; i < last;) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint32_t at16 = place(page, step + u * NW);
-      page = lookup(step + (u + 1) * NW);
-      there[u] = __builtin_amdgcn_ballot_w64(at16 != kNoRow) & 0xFFFFFFFFull;
-      attn_load<D, 32>(p.k, p.v, at16, 0, ring + u * 2 * C::HALF, ring + u * 2 * C::HALF + C::HALF);
-    }
-    while (step < last) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (step >= last) break;
-        wait_loads<LOADS>();
-        __builtin_amdgcn_sched_barrier(0);
-        const int kb = key_of(step);
-        const bool full = there[u] == 0xFFFFFFFFull && attn_all_seen<32>(p, x.s.first, t0, t1, kb);
-        uint64_t mask = there[u];
-        if (!full) mask &= attn_sees(p, x.s.first, t, tree, kb);
-        a.template block<32>(ring + u * 2 * C::HALF, ring + u * 2 * C::HALF + C::HALF, full, mask, p.c);
-        __builtin_amdgcn_sched_barrier(0);
-        const uint32_t at16 = place(page, step + 2 * NW);
-        page = lookup(step + 3 * NW);
-        there[u] = __builtin_amdgcn_ballot_w64(at16 != kNoRow) & 0xFFFFFFFFull;
-        attn_load<D, 32>(p.k, p.v, at16, 0, ring + u * 2 * C::HALF, ring + u * 2 * C::HALF + C::HALF);
-        step += NW;
+        for (int u = 0; u < 2; ++u) {
+          if (i >= last) break;
+          wait_loads<LOADS>();                         // block i is there, and the pages of block i + 2
+          __builtin_amdgcn_sched_barrier(0);
+          const unsigned char *k = smem + u * 2 * C::HALF, *v = k + C::HALF;
+          const int kb = attn_key<32>(x.r, i);
+          const bool full = there[u] == 0xFFFFFFFFu && attn_all_seen<32>(p, x.s.first, t0, t1, kb);
+          typename Rows::Scores s;
+          typename Rows::Weights w;
+          typename Rows::Mask mask;
+          float top[1];
+          a.scores(k, s);
+          if (!full) {
+            mask.of[0] = there[u] & attn_sees(p, x.s.first, t, tree, kb);
+            a.hide(s, mask);
+          }
+          a.largest(s, p.c, top);
+          a.follow(top);
+          a.weigh(s, p.c, w);
+          if (full) a.add(v, w);
+          else a.add_hidden(v, w, mask);
+          __builtin_amdgcn_sched_barrier(0);
+          const uint32_t at16 = place(i + 2, u);
+          lookup(i + 3, u ^ 1);
+          there[u] = request(at16, u);
+          ++i;
+        }
       }
-    }
-    wait_loads<0>();
-    __syncthreads();                                   // all rings are free
+      wait_loads<0>();                                 // the ring is filled anew for the next tile
 
-    float* sums = (float*)smem;
-    const Halves ls = both_halves(a.l);
-    const float l = ls.low + ls.high;
-    if (lane < 32) {
-      ml[0][wave][lane] = a.m;
-      ml[1][wave][lane] = l;
-    }
+      const Halves ls = both_halves(a.l[0]);
+      const float l = ls.low + ls.high;
+      if (has) {
+        const int h = lane >> 5;
+        if (first == 0 && last == x.r.blocks) {
+          const float f = l == 0.f ? 0.f : 1.f / l;
+          typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
+          typename Act::elem* to = (typename Act::elem*)p.out + rows_row(p, x, y, lane & 31) * D + h * 4;
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+          for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *(f32x4*)(sums + (wave * 32 + (lane & 31)) * C::PITCH + d * 32 + i * 2 + (lane >> 5) * 4) =
-            f32x4{a.o[d][i], a.o[d][i + 1], a.o[d][i + 2], a.o[d][i + 3]};
-    __syncthreads();
-    const bool whole = block0 == 0 && block1 == x.r.blocks;
-    float* part = p.part + ((size_t)blockIdx.x * 2 + (block0 == 0)) * C::PART;
-    for (int idx = threadIdx.x; idx < rows * (D / 4); idx += 64 * NW) {
-      const int row = idx / (D / 4), col = idx % (D / 4) * 4;
-      float m = ml[0][0][row], sum = 0.f;
+            for (int j = 0; j < 16; j += 4) {
+              e4 z;
 #pragma unroll
-      for (int w = 1; w < NW; ++w) m = fmaxf(m, ml[0][w][row]);
-      const float top = m == -__builtin_inff() ? 0.f : m;
-      f32x4 o = {};
+              for (int e = 0; e < 4; ++e) z[e] = Act::from_f32(a.o[0][d][j + e] * f);
+              *(e4*)(to + d * 32 + j * 2) = z;
+            }
+        } else {
+          float* part = p.part + ((size_t)blockIdx.x * 2 + (first == 0)) * C::PART;
+          if (h == 0) *(f32x2*)(part + 32 * D + 2 * lane) = f32x2{a.m[0], l};
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float f = __builtin_amdgcn_exp2f(ml[0][w][row] - top);
-        sum += f * ml[1][w][row];
-        o += f * *(const f32x4*)(sums + (w * 32 + row) * C::PITCH + col);
-      }
-      if (whole) {
-        const float f = sum == 0.f ? 0.f : 1.f / sum;
-        const int rr = tile * 32 + row, tt = rr / p.G;
-        typename Act::elem* to = (typename Act::elem*)p.out + ((size_t)(x.s.q0 + tt) * p.Hq + head * p.G + rr - tt * p.G) * D + col;
-        typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
-        e4 y;
+          for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = Act::from_f32(o[i] * f);
-        *(e4*)to = y;
-      } else {
-        *(f32x4*)(part + row * D + col) = o;
-        if (col == 0) {
-          part[32 * D + row] = m;
-          part[32 * D + 32 + row] = sum;
+            for (int j = 0; j < 16; j += 4)
+              *(f32x4*)(part + (lane & 31) * D + h * 4 + d * 32 + j * 2) =
+                  f32x4{a.o[0][d][j], a.o[0][d][j + 1], a.o[0][d][j + 2], a.o[0][d][j + 3]};
         }
       }
     }
-    __syncthreads();                                   // before the rings are filled again
-    at += block1 - block0;
-    in += block1 - block0;
     if (in >= rows_work(p, x)) {
       in = 0;
       do ++b;
@@ -201,7 +217,7 @@ __global__ __launch_bounds__(64 * RowsCfg<D>::NW) void attn_rows_kernel(const At
   }
 }
 
-// Workgroup w joins the tile that the boundary in front of share w cuts, if no earlier boundary cuts it too.
+// Workgroup w joins the tile whose blocks the boundary in front of share w + 1 cuts, if no earlier boundary cuts them too.
 template <class Act, int D>
 __global__ __launch_bounds__(256) void attn_rows_join_kernel(const AttnArgs p) {
   using C = RowsCfg<D>;
@@ -212,32 +228,29 @@ __global__ __launch_bounds__(256) void attn_rows_join_kernel(const AttnArgs p) {
   long long in;
   rows_find(p, plan, at, b, in);
   const RowsSeq x = rows_seq(p, b);
-  const int item = (int)(in / x.r.blocks), block0 = (int)(in - (long long)item * x.r.blocks);
-  const long long begin = at - block0;
-  if (block0 == 0 || (w - 1) * plan.share > begin) return;
+  const RowsItem y = rows_item(p, x, in);
+  const long long begin = at - y.unit + kItem;         // of its blocks
+  if (at <= begin || (w - 1) * plan.share > begin) return;
   const int parts = 1 + (int)((begin + x.r.blocks - 1) / plan.share - (w - 1));
-  const int tile = item / p.Hkv, head = item - tile * p.Hkv, rows = min(32, x.s.n * p.G - tile * 32);
-  for (int idx = threadIdx.x; idx < rows * (D / 4); idx += 256) {
+  for (int idx = threadIdx.x; idx < y.rows * (D / 4); idx += 256) {
     const int row = idx / (D / 4), col = idx % (D / 4) * 4;
     float m = -__builtin_inff(), sum = 0.f;
     auto part = [&](int i) { return p.part + ((size_t)(w - 1 + i) * 2 + (i == 0)) * C::PART; };
-    for (int i = 0; i < parts; ++i) m = fmaxf(m, part(i)[32 * D + row]);
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, part(i)[32 * D + 2 * row]);
     const float top = m == -__builtin_inff() ? 0.f : m;
     f32x4 o = {};
     for (int i = 0; i < parts; ++i) {
-      const float* from = part(i);
-      const float f = __builtin_amdgcn_exp2f(from[32 * D + row] - top);
-      sum += f * from[32 * D + 32 + row];
-      o += f * *(const f32x4*)(from + row * D + col);
+      const f32x2 ml = *(const f32x2*)(part(i) + 32 * D + 2 * row);
+      const float f = __builtin_amdgcn_exp2f(ml[0] - top);
+      sum += f * ml[1];
+      o += f * *(const f32x4*)(part(i) + row * D + col);
     }
     const float f = sum == 0.f ? 0.f : 1.f / sum;
-    const int rr = tile * 32 + row, tt = rr / p.G;
-    typename Act::elem* to = (typename Act::elem*)p.out + ((size_t)(x.s.q0 + tt) * p.Hq + head * p.G + rr - tt * p.G) * D + col;
     typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
-    e4 y;
+    e4 z;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = Act::from_f32(o[i] * f);
-    *(e4*)to = y;
+    for (int e = 0; e < 4; ++e) z[e] = Act::from_f32(o[e] * f);
+    *(e4*)((typename Act::elem*)p.out + rows_row(p, x, y, row) * D + col) = z;
   }
 }
 
@@ -248,7 +261,7 @@ static int launch(const AttnArgs& p, hipStream_t st) {
   static std::atomic<unsigned long long> raised{0};
   const int rc = int8_raise_lds(attn_rows_kernel<Act, D>, raised, RowsCfg<D>::LDS);
   if (rc != MI_OK) return rc;
-  attn_rows_kernel<Act, D><<<p.groups, 64 * RowsCfg<D>::NW, RowsCfg<D>::LDS, st>>>(p);
+  attn_rows_kernel<Act, D><<<p.groups, 64, RowsCfg<D>::LDS, st>>>(p);
   if (p.groups > 1) attn_rows_join_kernel<Act, D><<<p.groups - 1, 256, 0, st>>>(p);
   return launch_status();
 }

@@ -1,8 +1,8 @@
 """Attention over a paged cache in 64 bits, with how far a right result may be off.
 
 A kernel's score is an fp32 sum of D products (each addition at most half a step of 2^-24 of the sum of magnitudes), scaled by a 32-bit factor; a
-weight exp(s - m) carries the errors of its score and of the maximum, each rounded weight one half step u of the 16-bit type (fp16: or 2^-25, half
-of its smallest number), and the sum of the weights is of the rounded ones.  Normalised weights are then off by 2 (u + e) relative at most, e
+weight exp(s - m) carries the errors of its score and of the maximum, each rounded weight one half step u of the 16-bit type (fp16: or 2^-32 of
+the row's largest, as they are raised by 2^7), and the sum of the weights is of the rounded ones.  Normalised weights are then off by 2 (u + e) relative at most, e
 the error of the scores with a few steps of the exponential, the sums and the rescalings; the output is rounded once (u)."""
 import torch
 
@@ -64,7 +64,7 @@ def attention(q, kc, vc, table, lens, news, scale, window=-1, sinks=0, masks=Non
                 w = torch.where(total > 0, w / total.clamp_min(1e-300), 0.0)
                 o = w @ vh
                 parts = w @ vh.abs()
-                small = 2.0 ** -25 * (see.double() @ vh.abs()) if q.dtype == torch.float16 else 0.0
+                small = 2.0 ** -32 * (see.double() @ vh.abs()) if q.dtype == torch.float16 else 0.0
                 out[at:at + n, h] = o
                 tol[at:at + n, h] = u * o.abs() + 2 * (u + 2 * e) * parts + 2 * small + (2.0 ** -24 if q.dtype == torch.float16 else 1e-38)
         at += n

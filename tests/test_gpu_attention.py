@@ -315,3 +315,23 @@ def test_refusals(v, dev):
                     (dict(masks=masks, mq=65), "words for up to")):
         with pytest.raises(RuntimeError, match=why):
             call(**kw)
+
+
+@pytest.mark.parametrize("dt", DTS)
+def test_long_tails_keep_their_weight(v, dev, dt):
+    """One key far above 100000 others whose weights are subnormal in 16 bits: together they count for more than the output's rounding."""
+    L, D = 100000, 64
+    for n in (1, 40):
+        case = R.make(dev, 1, [L], [n], 1, 1, D, 64, dt)
+        q, kc, vc, table = case[:4]
+        q.zero_()
+        q[..., 0] = 8.0
+        flat = kc[table[0].long()]
+        flat.view(-1, D)[:L] = 0
+        flat.view(-1, D)[5, 0] = 11.0                   # a score of 11: the others have 2^-15.9 of its weight
+        kc[table[0].long()] = flat
+        vals = vc[table[0].long()]
+        vals.view(-1, D)[:L] = 1.0
+        vals.view(-1, D)[5] = -1.0
+        vc[table[0].long()] = vals
+        _check(_run(v, case, [L], [n], D), *R.attention(*case[:4], [L], [n], D ** -0.5))
