@@ -386,6 +386,86 @@ struct AttnRows {
   }
 };
 
+// ---- joining parts ------------------------------------------------------------------------------
+// A workgroup of kJoin threads makes `rows` (up to 32) rows of out from `parts` parts of each: sums(i, row) points to the D sums of part i, ml(i, row)
+// to its m and l (m = -inf: the part has no sums), to(row) to the row of out.  A thread has four columns of a row; where threads are left over they
+// share a row's parts, and what they have meets in LDS.  All loads of four parts are under way together.
+constexpr int kJoin = 1024;
+template <class Act, int D, class Sums, class Ml, class To>
+__device__ __forceinline__ void attn_join(int rows, int parts, Sums sums, Ml ml, To to) {
+  constexpr int Q = D / 4, PLACES = kJoin / Q;         // threads of a row; rows, or shares of rows, at a time
+  __shared__ f32x4 part_o[kJoin];
+  __shared__ f32x2 part_ml[PLACES];
+  const int col = threadIdx.x % Q * 4, place = threadIdx.x / Q;
+  int share = 1;
+  while (2 * share * rows <= PLACES && 2 * share <= parts) share *= 2;
+  for (int row0 = 0; row0 < rows; row0 += PLACES / share) {
+    const int row = row0 + place / share, who = place % share;
+    float m = -__builtin_inff(), sum = 0.f;
+    f32x4 o = {};
+    if (row < rows)
+      for (int i = who; i < parts; i += 4 * share) {
+        f32x2 a[4];
+        f32x4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = i + j * share < parts ? i + j * share : i;
+          a[j] = *(const f32x2*)ml(at, row);
+          x[j] = *(const f32x4*)(sums(at, row) + col);
+        }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (i + j * share >= parts) a[j] = f32x2{-__builtin_inff(), 0.f};
+          top = fmaxf(top, a[j][0]);
+        }
+        if (top == -__builtin_inff()) {                // nothing but rows that see nothing, or see NaN alone
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum += a[j][1];
+          continue;
+        }
+        const float f = __builtin_amdgcn_exp2f(m - top);
+        sum *= f;
+        o *= f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float g = __builtin_amdgcn_exp2f(a[j][0] - top);
+          sum += g * a[j][1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] += a[j][0] == -__builtin_inff() ? 0.f : g * x[j][e];
+        }
+        m = top;
+      }
+    if (share > 1) {
+      __syncthreads();
+      part_o[threadIdx.x] = o;
+      if (col == 0) part_ml[place] = f32x2{m, sum};
+      __syncthreads();
+      if (who == 0 && row < rows) {
+        float top = m;
+        for (int j = 1; j < share; ++j) top = fmaxf(top, part_ml[place + j][0]);
+        float f = top == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - top);
+        sum *= f;
+        o *= f;
+        for (int j = 1; j < share; ++j) {
+          const f32x2 b = part_ml[place + j];
+          f = top == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(b[0] - top);
+          sum += f * b[1];
+          o += f * part_o[threadIdx.x + j * Q];
+        }
+      }
+    }
+    if (who == 0 && row < rows) {
+      const float f = sum == 0.f ? 0.f : 1.f / sum;
+      typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
+      e4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = Act::from_f32(sum != sum ? sum : o[e] * f);
+      *(e4*)((typename Act::elem*)to(row) + col) = y;
+    }
+  }
+}
+
 int launch_attn_rows(const AttnArgs& p, int D, int act_dtype, hipStream_t st);       // and what joins the parts
 int launch_attn_tiles(const AttnArgs& p, int D, int act_dtype, hipStream_t st);
 long long attn_rows_bytes(int groups, int D);

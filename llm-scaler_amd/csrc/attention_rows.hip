@@ -83,11 +83,14 @@ __device__ __forceinline__ RowsItem rows_item(const AttnArgs& p, const RowsSeq& 
   y.rows = min(32, x.s.n * p.G - y.tile * 32);
   return y;
 }
-// Row `row` of a tile in q and out
-__device__ __forceinline__ long long rows_row(const AttnArgs& p, const RowsSeq& x, const RowsItem& y, int row) {
-  const int r = y.tile * 32 + row, t = r / p.G;
-  return (long long)(x.s.q0 + t) * p.Hq + y.head * p.G + r - t * p.G;
+// Row `row` of a tile in out
+__device__ __forceinline__ long long rows_row(const AttnArgs& p, int q0, int tile, int head, int row) {
+  const int r = tile * 32 + row, t = r / p.G;
+  return (long long)(q0 + t) * p.Hq + head * p.G + r - t * p.G;
 }
+// Behind the parts: for the cut in front of each share how many parts are to be joined there (0: none), and the tile
+template <int D>
+__device__ __forceinline__ i32x4* rows_cuts(const AttnArgs& p) { return (i32x4*)(p.part + (size_t)p.groups * 2 * RowsCfg<D>::PART); }
 
 template <class Act, int D>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2))) void attn_rows_kernel(const AttnArgs p) {
@@ -100,15 +103,23 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
   const RowsPlan plan = rows_plan(p);
   long long at = plan.share * blockIdx.x;
   const long long end = min(at + plan.share, plan.total);
-  if (at >= end) return;
+  if (at >= end) {
+    if (lane == 0) rows_cuts<D>(p)[blockIdx.x] = i32x4{};
+    return;
+  }
   int b;
   long long in;
   rows_find(p, plan, at, b, in);
   b = __builtin_amdgcn_readfirstlane(b);
 
-  while (at < end) {
+  for (bool starts = true; at < end; starts = false) {
     const RowsSeq x = rows_seq(p, b);
     const RowsItem y = rows_item(p, x, in);
+    if (starts) {                                      // the cut in front of this share is one to join at if it goes through blocks, as the tile's first
+      const long long begin = at - y.unit + kItem, w = blockIdx.x;
+      const int parts = at <= begin || (w - 1) * plan.share > begin ? 0 : 1 + (int)((begin + x.r.blocks - 1) / plan.share - (w - 1));
+      if (lane == 0) rows_cuts<D>(p)[w] = i32x4{parts, x.s.q0, y.tile, y.head * 64 + y.rows};
+    }
     const int take = __builtin_amdgcn_readfirstlane((int)min((long long)(x.r.blocks + kItem - y.unit), end - at));
     const int first = max(y.unit - kItem, 0), last = y.unit + take - kItem;      // blocks
     at += take;
@@ -187,7 +198,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
         if (first == 0 && last == x.r.blocks) {
           const float f = l == 0.f ? 0.f : 1.f / l;
           typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
-          typename Act::elem* to = (typename Act::elem*)p.out + rows_row(p, x, y, lane & 31) * D + h * 4;
+          typename Act::elem* to = (typename Act::elem*)p.out + rows_row(p, x.s.q0, y.tile, y.head, lane & 31) * D + h * 4;
 #pragma unroll
           for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -217,44 +228,20 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
   }
 }
 
-// Workgroup w joins the tile whose blocks the boundary in front of share w + 1 cuts, if no earlier boundary cuts them too.
+// Workgroup w joins the tile that the cut in front of share w + 1 goes through.
 template <class Act, int D>
-__global__ __launch_bounds__(256) void attn_rows_join_kernel(const AttnArgs p) {
-  using C = RowsCfg<D>;
-  const RowsPlan plan = rows_plan(p);
-  const long long w = blockIdx.x + 1, at = w * plan.share;
-  if (at >= plan.total) return;
-  int b;
-  long long in;
-  rows_find(p, plan, at, b, in);
-  const RowsSeq x = rows_seq(p, b);
-  const RowsItem y = rows_item(p, x, in);
-  const long long begin = at - y.unit + kItem;         // of its blocks
-  if (at <= begin || (w - 1) * plan.share > begin) return;
-  const int parts = 1 + (int)((begin + x.r.blocks - 1) / plan.share - (w - 1));
-  for (int idx = threadIdx.x; idx < y.rows * (D / 4); idx += 256) {
-    const int row = idx / (D / 4), col = idx % (D / 4) * 4;
-    float m = -__builtin_inff(), sum = 0.f;
-    auto part = [&](int i) { return p.part + ((size_t)(w - 1 + i) * 2 + (i == 0)) * C::PART; };
-    for (int i = 0; i < parts; ++i) m = fmaxf(m, part(i)[32 * D + 2 * row]);
-    const float top = m == -__builtin_inff() ? 0.f : m;
-    f32x4 o = {};
-    for (int i = 0; i < parts; ++i) {
-      const f32x2 ml = *(const f32x2*)(part(i) + 32 * D + 2 * row);
-      const float f = __builtin_amdgcn_exp2f(ml[0] - top);
-      sum += f * ml[1];
-      o += f * *(const f32x4*)(part(i) + row * D + col);
-    }
-    const float f = sum == 0.f ? 0.f : 1.f / sum;
-    typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
-    e4 z;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) z[e] = Act::from_f32(o[e] * f);
-    *(e4*)((typename Act::elem*)p.out + rows_row(p, x, y, row) * D + col) = z;
-  }
+__global__ __launch_bounds__(kJoin) void attn_rows_join_kernel(const AttnArgs p) {
+  constexpr int PART = RowsCfg<D>::PART;
+  const int w = blockIdx.x + 1;
+  const i32x4 cut = rows_cuts<D>(p)[w];
+  if (!cut[0]) return;
+  // the first part is the one that share w - 1 began, the others those that a share continued
+  auto part = [&](int i) { return p.part + ((size_t)(w - 1 + i) * 2 + (i == 0)) * PART; };
+  attn_join<Act, D>(cut[3] % 64, cut[0], [&](int i, int row) { return part(i) + row * D; }, [&](int i, int row) { return part(i) + 32 * D + 2 * row; },
+                    [&](int row) { return (typename Act::elem*)p.out + rows_row(p, cut[1], cut[2], cut[3] / 64, row) * D; });
 }
 
-long long attn_rows_bytes(int groups, int D) { return (long long)groups * 2 * 32 * (D + 2) * 4; }
+long long attn_rows_bytes(int groups, int D) { return (long long)groups * (2 * 32 * (D + 2) * 4 + 16); }
 
 template <class Act, int D>
 static int launch(const AttnArgs& p, hipStream_t st) {
@@ -262,7 +249,7 @@ static int launch(const AttnArgs& p, hipStream_t st) {
   const int rc = int8_raise_lds(attn_rows_kernel<Act, D>, raised, RowsCfg<D>::LDS);
   if (rc != MI_OK) return rc;
   attn_rows_kernel<Act, D><<<p.groups, 64, RowsCfg<D>::LDS, st>>>(p);
-  if (p.groups > 1) attn_rows_join_kernel<Act, D><<<p.groups - 1, 256, 0, st>>>(p);
+  if (p.groups > 1) attn_rows_join_kernel<Act, D><<<p.groups - 1, kJoin, 0, st>>>(p);
   return launch_status();
 }
 

@@ -250,7 +250,7 @@ __global__ __launch_bounds__(64 * TilesCfg<D>::NW) __attribute__((amdgpu_waves_p
     return;
   }
   if (lane < 32) *(f32x2*)part_ml(p, D, split, row) = f32x2{a.m[0], l};
-  if (first == last) return;                           // the sums of an empty part are not read
+  if (first == last) return;                           // m = -inf: the sums are not read
   float* to = part_sums(p, D, split, row) + (lane >> 5) * 4;
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
@@ -259,33 +259,20 @@ __global__ __launch_bounds__(64 * TilesCfg<D>::NW) __attribute__((amdgpu_waves_p
       *(f32x4*)(to + d * 32 + i * 2) = f32x4{a.o[0][d][i], a.o[0][d][i + 1], a.o[0][d][i + 2], a.o[0][d][i + 3]};
 }
 
-// A workgroup per slot and kv head.
+// A workgroup per 32 rows of a slot and kv head.
 template <class Act, int D>
-__global__ __launch_bounds__(256) void attn_tiles_join_kernel(const AttnArgs p) {
-  const int head = blockIdx.x % p.Hkv, slot = blockIdx.x / p.Hkv;
+__global__ __launch_bounds__(kJoin) void attn_tiles_join_kernel(const AttnArgs p) {
+  using C = TilesCfg<D>;
+  const int piece = blockIdx.x % C::NW, rest = blockIdx.x / C::NW, head = rest % p.Hkv, slot = rest / p.Hkv;
   Tile x;
-  if (!tile_at<TilesCfg<D>::ROWS, TilesCfg<D>::KEYS>(p, slot, x)) return;
-  for (int idx = threadIdx.x; idx < x.rows * (D / 4); idx += 256) {
-    const int r = x.row0 + idx / (D / 4), col = idx % (D / 4) * 4, t = r / p.G;
-    const long long row = (long long)(x.s.q0 + t) * p.Hq + head * p.G + r - t * p.G;
-    float m = -__builtin_inff(), sum = 0.f;
-    for (int i = 0; i < p.splits; ++i) m = fmaxf(m, part_ml(p, D, i, row)[0]);
-    const float top = m == -__builtin_inff() ? 0.f : m;
-    f32x4 o = {};
-    for (int i = 0; i < p.splits; ++i) {
-      if ((long long)x.r.blocks * i / p.splits == (long long)x.r.blocks * (i + 1) / p.splits) continue;
-      const f32x2 ml = *(const f32x2*)part_ml(p, D, i, row);
-      const float f = __builtin_amdgcn_exp2f(ml[0] - top);
-      sum += f * ml[1];
-      o += f * *(const f32x4*)(part_sums(p, D, i, row) + col);
-    }
-    const float f = sum == 0.f ? 0.f : 1.f / sum;
-    typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
-    e4 y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = Act::from_f32(o[e] * f);
-    *(e4*)((typename Act::elem*)p.out + row * D + col) = y;
-  }
+  if (!tile_at<C::ROWS, C::KEYS>(p, slot, x) || piece * 32 >= x.rows) return;
+  auto row_of = [&](int row) {
+    const int r = x.row0 + piece * 32 + row, t = r / p.G;
+    return (long long)(x.s.q0 + t) * p.Hq + head * p.G + r - t * p.G;
+  };
+  attn_join<Act, D>(min(32, x.rows - piece * 32), p.splits, [&](int i, int row) { return part_sums(p, D, i, row_of(row)); },
+                    [&](int i, int row) { return part_ml(p, D, i, row_of(row)); },
+                    [&](int row) { return (typename Act::elem*)p.out + row_of(row) * D; });
 }
 
 template <class Act, int D>
@@ -294,7 +281,7 @@ static int launch(const AttnArgs& p, hipStream_t st) {
   const int rc = int8_raise_lds(attn_tiles_kernel<Act, D>, raised, TilesCfg<D>::LDS);
   if (rc != MI_OK) return rc;
   attn_tiles_kernel<Act, D><<<(unsigned)(p.slots * p.splits * p.Hkv), 64 * TilesCfg<D>::NW, TilesCfg<D>::LDS, st>>>(p);
-  if (p.splits > 1) attn_tiles_join_kernel<Act, D><<<(unsigned)(p.slots * p.Hkv), 256, 0, st>>>(p);
+  if (p.splits > 1) attn_tiles_join_kernel<Act, D><<<(unsigned)(p.slots * p.Hkv * TilesCfg<D>::NW), kJoin, 0, st>>>(p);
   return launch_status();
 }
 
