@@ -141,6 +141,10 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 __device__ __forceinline__ void to_lds16(const void* from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
 }
+// from a scalar address and a distance per lane
+__device__ __forceinline__ void to_lds16_from(const void* base, uint32_t by, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(by), "s"(base), "s"(to) : "memory", "m0");
+}
 __device__ __forceinline__ void to_lds4(const void* from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(to) : "memory", "m0");
 }
@@ -235,8 +239,8 @@ struct AttnRows {
         for (int n = 0; n < NQ; ++n) x.s[n][t] = mfma32(a, q[n][ks], x.s[n][t]);
       }
   }
-  // A step of the tiles kernel in pieces whose reads of LDS go out long before their products: keys a step ahead, values while the scores are made.
-  // Reads stay on their side of a `pin`; everything else may move.
+  // A step of the tiles kernel: weights of the scores x, the product with their values, and the next step's scores y.  Reads of LDS go out long before
+  // their products, keys a step ahead (f: the next step's, then those at k2), values while the scores are made: they stay on their side of a `pin`.
   struct Keys { v8 k[D / 16]; };
   struct Values { v8 v[DT]; };
   static __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0x40E); }
@@ -248,16 +252,18 @@ struct AttnRows {
 #pragma unroll
     for (int d = 0; d < DT; ++d) f.v[d] = v_operand(v, t, d);
   }
-  // Weights of this step's scores x, the product with its values, the next step's scores y and their maximum; f: the next step's keys, then those at k2
-  __device__ __forceinline__ void step(const Scores& x, const unsigned char* v, Keys& f, const unsigned char* k2, float c, Scores& y, float (&top)[NQ]) {
+  __device__ __forceinline__ void scores_of(const Keys& f, Scores& y) const {
+    y.s[0][0] = f32x16{};
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) y.s[0][0] = mfma32(f.k[ks], q[0][ks], y.s[0][0]);
+  }
+  __device__ __forceinline__ void step(const Scores& x, const unsigned char* v, Keys& f, const unsigned char* k2, float c, Scores& y) {
     static_assert(NQ == 1 && KT == 1, "a step of 32 keys");
     Values va, vb;
     Weights w;
     read_values(v, 0, va);
     pin();
-    y.s[0][0] = f32x16{};
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) y.s[0][0] = mfma32(f.k[ks], q[0][ks], y.s[0][0]);
+    scores_of(f, y);
     read_values(v, 1, vb);
     pin();
     weigh(x, c, w);
@@ -267,8 +273,6 @@ struct AttnRows {
     pin();
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[0][d] = mfma32(vb.v[d], w.p[0][1], o[0][d]);
-    largest(y, c, top);
-    follow(top);
   }
   __device__ __forceinline__ void hide(Scores& x, const Mask& mask) const {
     const int h = (threadIdx.x & 63) >> 5;
@@ -278,7 +282,11 @@ struct AttnRows {
       for (int t = 0; t < KT; ++t) {
         const uint32_t bits = (uint32_t)(mask.of[n] >> (32 * t)) >> (4 * h);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x.s[n][t][i] = bits >> (8 * (i / 4) + i % 4) & 1 ? x.s[n][t][i] : -__builtin_inff();
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t sees = (uint32_t)((int32_t)(bits << (31 - 8 * (i / 4) - i % 4)) >> 31);
+          const float s = x.s[n][t][i];                // its own variable: a bit cast of an element is one of element 0
+          x.s[n][t][i] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, s) & sees) | (0xFF800000u & ~sees));
+        }
       }
   }
   // c times the largest score of a row
@@ -340,6 +348,37 @@ struct AttnRows {
         const v8 a = v_operand(v, t, d);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) o[n][d] = mfma32(a, w.p[n][t], o[n][d]);
+      }
+  }
+  // Zeros in place of infinities and NaN in 8 rows of values in LDS; whether there were any in the rows whose bits `there` has
+  template <int PIECES>
+  static __device__ __forceinline__ bool clean(unsigned char* v, uint32_t there) {
+    bool spoilt = false;
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      u16x8* at = (u16x8*)(v + j * 1024 + (threadIdx.x & 63) * 16);
+      const u16x8 x = *at, finite = __builtin_elementwise_min(EXPONENT - (x & EXPONENT), (u16x8)1);
+      const u32x4 all = __builtin_bit_cast(u32x4, finite);
+      const bool found = (all[0] & all[1] & all[2] & all[3]) != 0x00010001u;
+      if (!__builtin_amdgcn_ballot_w64(found)) continue;
+      *at = x & (0 - finite);
+      spoilt |= found && there >> (j * (512 / D) + (threadIdx.x & 63) / (D / 8)) & 1;
+    }
+    return __builtin_amdgcn_ballot_w64(spoilt) != 0;
+  }
+  // The infinities and NaN of a row of values in memory, where this lane's row sees it
+  __device__ __forceinline__ void add_not_finite(const unsigned char* v, bool sees) {
+    const int h = (threadIdx.x & 63) >> 5;
+    typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
+    typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {                    // columns 32 d + 8 i + 4 h ..
+        const u16x4 x = *(const u16x4*)(v + (32 * d + 8 * i + 4 * h) * 2);
+        const e4 y = __builtin_bit_cast(e4, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][d][4 * i + e] += sees && (x[e] & EXPONENT) == EXPONENT ? Act::to_f32(y[e]) : 0.f;
       }
   }
   // The same where some row does not see some key: 0 times an infinity or a NaN there would not be 0, so such values go to the rows that see

@@ -1,8 +1,10 @@
 // Attention of many rows per sequence (prompts, chunks, large trees): a workgroup of eight wavefronts has 256 rows of a kv head (four and 128 with heads
 // of 256), 32 a wavefront, which all use the same keys and values.
 //
-// A block of 64 keys is two steps.  While the scores of the next step's keys are on the matrix cores, the vector units make weights of this
-// step's; then the product with the values goes along with the maximum of the next step's scores.  Keys come to LDS two blocks ahead, values one.
+// A step is 32 keys: while the scores of the next step's keys are on the matrix cores, the vector units make weights of this step's; then the product with
+// the values goes along with the maximum of the next step's scores.  A block, what comes to LDS together, is two steps (one with heads of
+// 256); keys come two blocks ahead (three), values one.  Where pages hold whole groups of 8 places (GROUPS), the keys that a wavefront loads
+// lie on one page: their address is a scalar.
 //
 // Where there are few tiles, their keys are cut into `splits` parts; a second launch joins them.  Tiles of the last tokens, which see
 // the most keys, go first; the kv heads go round the XCDs, so that the tiles of a head share its keys in L2.
@@ -10,15 +12,19 @@
 // Bound: the matrix cores; for a few hundred rows HBM.
 #include "attention.hpp"
 
+#include <type_traits>
+
 namespace qlin {
 
 template <int D> struct TilesCfg {
   static constexpr int ROWS = attn_tile_rows(D), NW = ROWS / 32;
   static constexpr int KEYS = D == 256 ? 32 : 64;      // of a block: a step or two
   static constexpr int HALF = KEYS * D * 2;            // K or V of a block
+  static constexpr int WAVES = D == 64 ? 4 : D == 128 ? 2 : 1;   // per SIMD
   static constexpr int AHEAD = KEYS == 64 ? 2 : 3;     // how many blocks ahead keys are asked for: two steps are there when a block begins
-  static constexpr int PAGES = (AHEAD + 1 + 2) * HALF; // behind the rings of keys and values
-  static constexpr int LDS = PAGES + NW * 2 * 4 * KEYS;          // two blocks' pages per wavefront
+  static constexpr int FLAGS = (AHEAD + 1 + 2) * HALF; // behind the rings of keys and values: 8 x 8 and 8 words
+  static constexpr int PAGES = FLAGS + 512;            // two blocks' pages per wavefront
+  static constexpr int LDS = PAGES + NW * 2 * 4 * KEYS;
 };
 
 // Slot i of the grid is tile i - start(b) of the sequence b with start(b) <= i < start(b + 1), start(b) = floor(cu[b] G / rows) + b: at least as many
@@ -67,10 +73,12 @@ __device__ __forceinline__ float* part_ml(const AttnArgs& p, int D, int split, l
   return p.part + (long long)p.splits * p.T * p.Hq * D + ((long long)split * p.T * p.Hq + row) * 2;
 }
 
-template <class Act, int D>
-__global__ __launch_bounds__(64 * TilesCfg<D>::NW) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2))) void attn_tiles_kernel(const AttnArgs p) {
+template <class Act, int D, bool GROUPS>
+__global__ __launch_bounds__(64 * TilesCfg<D>::NW) __attribute__((amdgpu_waves_per_eu(TilesCfg<D>::WAVES, TilesCfg<D>::WAVES)))
+void attn_tiles_kernel(const AttnArgs p) {
   using C = TilesCfg<D>;
-  constexpr int KEYS = C::KEYS, NW = C::NW, OWN = KEYS / NW, AHEAD = C::AHEAD;     // OWN: rows of a block that a wavefront loads
+  constexpr int KEYS = C::KEYS, NW = C::NW, OWN = KEYS / NW, AHEAD = C::AHEAD;   // OWN: rows of a block that a wavefront loads
+  static_assert(OWN == 8 && NW <= 8, "a group of 8 places per wavefront");
   using Rows = AttnRows<Act, D, 32, 1>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -83,39 +91,95 @@ __global__ __launch_bounds__(64 * TilesCfg<D>::NW) __attribute__((amdgpu_waves_p
   // the wavefront's rows wr0 .. wr1 of the sequence, tokens t0 .. t1
   const int wr0 = x.row0 + wave * 32, wr1 = min(wr0 + 32, x.row0 + x.rows) - 1;
   const int t0 = wr0 / p.G, t1 = max(wr1, wr0) / p.G;
+  const bool live = wr0 <= wr1;
   const int r = wr0 + (lane & 31), t = r / p.G;
   const bool has = r <= wr1;
   Rows a;
   a.start();
   a.load_q(0, has ? (const typename Act::elem*)p.q + (x.s.q0 + t) * p.q_token + (head * p.G + r - t * p.G) * p.q_head : nullptr);
 
-  // pages of the keys of block i: by direct loads to LDS like the keys, a block ahead of what is asked for with them
-  const unsigned char* pages = smem + C::PAGES + wave * (2 * 4 * KEYS);
   auto key_of = [&](int i) { return attn_key<KEYS>(x.r, i); };
-  auto lookup = [&](int i, int u) {
-    const int key = key_of(i) + lane % KEYS;
-    if (KEYS == 64 || lane < KEYS) to_lds4(i < last && attn_in(p, x.r, key) ? table + attn_page_of(p, key) : kNoPage, lds_address(pages + u * 4 * KEYS));
-  };
-  using Places = RowPlaces<D, OWN>;
-  auto place = [&](int i, int u, Places& to) {         // and which keys of the block are there
-    const int page = *(const int*)(pages + u * 4 * KEYS + lane % KEYS * 4);
-    const uint32_t at = i < last ? attn_place(p, page, key_of(i) + lane % KEYS, head) : kNoRow;
-    to.take(at, wave * OWN);
-    return __builtin_amdgcn_ballot_w64(at != kNoRow);
-  };
+  constexpr uint64_t ALL = KEYS == 64 ? ~0ull : (1ull << (KEYS % 64)) - 1;
   constexpr int OFFSET = OWN * D * 2;
 
-  // Whether the wavefront has something to do with block i, and whether all of its rows see all of it
-  auto some_of = [&](int i) {
-    if (i >= last || wr0 > wr1) return false;
-    const int kb = key_of(i);
-    return p.tree || (kb <= x.s.first + t1 && (!p.window || kb + KEYS - 1 > x.s.first + t0 - p.window || kb < p.sinks));
+  // Where the wavefront's rows of a block lie: GROUPS: one place for all of them; otherwise a place per row, of pages that come by direct loads to LDS
+  // like the keys, a block ahead of what is asked for with them
+  using Places = std::conditional_t<GROUPS, uint32_t, RowPlaces<D, OWN>>;
+  using Row = RowPlaces<D, OWN>;
+  const unsigned char* pages = smem + C::PAGES + wave * (2 * 4 * KEYS);
+  uint32_t* bad = (uint32_t*)(smem + C::FLAGS);        // [block % 8][wave]: its page is outside the cache
+  uint32_t* dirty = bad + 64;                          // [wave]: it put zeros in place of values that some row sees
+  uint32_t from_k[Row::N], from_v[Row::N];             // bytes from a group's first place
+  if constexpr (GROUPS)
+#pragma unroll
+    for (int j = 0; j < Row::N; ++j) {
+      const int g = j * Row::RPI + lane / Row::CH, row = wave * OWN + g;
+      from_k[j] = g * p.row16 * 16 + ((lane % Row::CH) ^ k_swizzle<D>(row)) * 16;
+      from_v[j] = g * p.row16 * 16 + ((lane % Row::CH) ^ v_swizzle<D>(row)) * 16;
+    }
+  int page = -1;                                       // GROUPS: of the block whose places come next
+  auto lookup = [&](int i, int u) {
+    if constexpr (GROUPS) {
+      const int key = key_of(i) + wave * OWN;
+      const bool seen = i < last && key < x.r.hi && (key + OWN > x.r.lo || key < p.sinks);
+      page = 0;
+      if (seen) page = __builtin_amdgcn_readfirstlane(table[attn_page_of(p, key)]);          // a group that nothing sees: some place of the cache
+    } else {
+      const int key = key_of(i) + lane % KEYS;
+      if (KEYS == 64 || lane < KEYS)
+        to_lds4(i < last && attn_in(p, x.r, key) ? table + attn_page_of(p, key) : kNoPage, lds_address(pages + u * 4 * KEYS));
+    }
   };
-  auto full_of = [&](int i, uint64_t there) { return there == ~0ull && attn_all_seen<KEYS>(p, x.s.first, t0, t1, key_of(i)); };
+  // the place of block i, and which of its keys are there
+  auto place = [&](int i, int u, Places& to) {
+    if constexpr (GROUPS) {
+      const int key = key_of(i) + wave * OWN;
+      const bool wrong = (uint32_t)page >= (uint32_t)p.pages;
+      const bool seen = i < last && key < x.r.hi && (key + OWN > x.r.lo || key < p.sinks);
+      const uint32_t in = wrong || !seen ? 0 : (uint32_t)page * p.page16 + (uint32_t)(key - attn_page_of(p, key) * p.page) * p.row16;
+      to = in + (uint32_t)head * p.head16;
+      if (lane == 0) bad[(i & 7) * 8 + wave] = wrong;
+      return (uint64_t)0;                              // known when all wavefronts have written theirs
+    } else {
+      const int it = *(const int*)(pages + u * 4 * KEYS + lane % KEYS * 4);
+      const uint32_t at = i < last ? attn_place(p, it, key_of(i) + lane % KEYS, head) : kNoRow;
+      to.take(at, wave * OWN);
+      return (uint64_t)__builtin_amdgcn_ballot_w64(at != kNoRow);
+    }
+  };
+  auto keys_there = [&](int i) {                       // GROUPS
+    if (i >= last) return (uint64_t)0;
+    const int kb = key_of(i);
+    uint64_t m = low_bits(x.r.hi - kb) & (~low_bits(x.r.lo - kb) | low_bits(p.sinks - kb));
+    uint64_t wrong = __builtin_amdgcn_ballot_w64(lane < NW && bad[(i & 7) * 8 + (lane & 7)]);
+    for (; wrong; wrong &= wrong - 1) m &= ~(0xFFull << (8 * __builtin_ctzll(wrong)));
+    return m & ALL;
+  };
+  auto request = [&](auto is_k, const Places& from, unsigned char* to) {
+    constexpr bool K = decltype(is_k)::value;
+    to += wave * OFFSET;
+    if constexpr (GROUPS) {
+      const unsigned char* base = (const unsigned char*)(K ? p.k : p.v) + (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)from) * 16;
+      const uint32_t lds = lds_address(to);
+#pragma unroll
+      for (int j = 0; j < Row::N; ++j) to_lds16_from(base, K ? from_k[j] : from_v[j], lds + j * 1024);
+    } else {
+      from.template load<K>(K ? p.k : p.v, wave * OWN, to);
+    }
+  };
+  const std::true_type K_;
+  const std::false_type V_;
+
+  auto full_of = [&](int i, uint64_t there) { return there == ALL && attn_all_seen<KEYS>(p, x.s.first, t0, t1, key_of(i)); };
+  const int tile0 = x.row0 / p.G, tile1 = (x.row0 + x.rows - 1) / p.G;
+  auto edge_of = [&](int i, uint64_t there) { return there != ALL || !attn_all_seen<KEYS>(p, x.s.first, tile0, tile1, key_of(i)); };
+  bool spoilt = false;
   auto mask_of = [&](int i, uint64_t there, int half) {
-    const int64_t* tree = p.tree ? p.tree + (size_t)(x.s.q0 + (has ? t : 0)) * p.tree_words : nullptr;
+    int mine = has ? t : 0;
+    asm volatile("" : "+v"(mine));                     // made here, not kept in registers all along
+    const int64_t* tree = p.tree ? p.tree + (size_t)(x.s.q0 + mine) * p.tree_words : nullptr;
     typename Rows::Mask mask;
-    mask.of[0] = (there & attn_sees(p, x.s.first, t, tree, key_of(i))) >> (32 * half) & 0xFFFFFFFFull;
+    mask.of[0] = (there & attn_sees(p, x.s.first, mine, tree, key_of(i))) >> (32 * half) & 0xFFFFFFFFull;
     return mask;
   };
 
@@ -123,56 +187,90 @@ __global__ __launch_bounds__(64 * TilesCfg<D>::NW) __attribute__((amdgpu_waves_p
     unsigned char* k[AHEAD + 1];                       // keys of blocks i, i + 1 ..
     unsigned char *v0 = smem + (AHEAD + 1) * C::HALF, *v1 = v0 + C::HALF;        // values of blocks i, i + 1
     Places at[AHEAD];                                  // of blocks i + 1 ..
-    uint64_t there[AHEAD + 1];                         // keys of blocks i ..
+    uint64_t there[AHEAD + 1];                         // keys of blocks i .. (GROUPS: of i and i + 1)
     lookup(first, 0);
-    lookup(first + 1, 1);
-    wait_loads<0>();
+    if constexpr (!GROUPS) {
+      lookup(first + 1, 1);
+      wait_loads<0>();
+    }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       k[j] = smem + j * C::HALF;
       Places& to = at[j ? j - 1 : 0];
       there[j] = place(first + j, j & 1, to);
-      to.template load<true>(p.k, wave * OWN, k[j] + wave * OFFSET);
-      if (j == 0) to.template load<false>(p.v, wave * OWN, v0 + wave * OFFSET);
-      lookup(first + j + 2, j & 1);
-      if (j >= 1 && j + 1 < AHEAD) wait_loads<0>();
+      request(K_, to, k[j]);
+      if (j == 0) request(V_, to, v0);
+      if constexpr (GROUPS) {
+        lookup(first + j + 1, 0);
+      } else {
+        lookup(first + j + 2, j & 1);
+        if (j >= 1 && j + 1 < AHEAD) wait_loads<0>();
+      }
     }
     k[AHEAD] = smem + AHEAD * C::HALF;
-    bool some = some_of(first), full = some && full_of(first, there[0]), some1, full1;
     typename Rows::Scores s0, s1;                      // of the two steps of a block (one: s0)
-    typename Rows::Weights w;
+    typename Rows::Keys f;
     float top[1];
     wait_loads<0>();
     there[AHEAD] = place(first + AHEAD, AHEAD & 1, at[AHEAD - 1]);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (some) {
-      a.scores(k[0], s0);
-      if (!full) a.hide(s0, mask_of(first, there[0], 0));
-      a.largest(s0, p.c, top);
+    if constexpr (GROUPS) lookup(first + AHEAD + 1, 0);
+    lds_barrier();
+    if constexpr (GROUPS) there[0] = keys_there(first);
+    bool full = full_of(first, there[0]);
+    auto follow = [&](typename Rows::Scores& s, bool all, int i, uint64_t keys, int half) __attribute__((always_inline)) {
+      if (!all) a.hide(s, mask_of(i, keys, half));
+      a.largest(s, p.c, top);
       a.follow(top);
+    };
+    if (live) {
+      a.read_keys(k[0], f);
+      a.scores_of(f, s0);
+      follow(s0, full, first, there[0], 0);
+      a.read_keys(KEYS == 64 ? k[0] + 64 * D : k[1], f);
     }
-    int i = first, u = AHEAD & 1;
-    // what a block begins with: its values and the next two steps' keys are there, more of both are asked for
-    auto begin = [&]() __attribute__((always_inline)) {
+    int u = AHEAD & 1;
+    for (int i = first; i < last; ++i) {
+      // The block's values and the next two steps' keys are there; more of both are asked for.
       wait_loads<0>();
-      __builtin_amdgcn_s_barrier();                    // everyone's; and block i - 1's are done with
-      asm volatile("" ::: "memory");
-      if (i + 1 < last) at[0].template load<false>(p.v, wave * OWN, v1 + wave * OFFSET);
-      if (i + AHEAD < last) at[AHEAD - 1].template load<true>(p.k, wave * OWN, k[AHEAD] + wave * OFFSET);
-      lookup(i + AHEAD + 2, u);
-      some1 = some_of(i + 1);
-      full1 = some1 && full_of(i + 1, there[1]);
-    };
-    auto next = [&]() __attribute__((always_inline)) { // the places of one block more, while products go on
+      // 0 times an infinity or a NaN would not be 0: in blocks that some row does not see all of, the wavefronts look for such among the values that they
+      // loaded and put zeros there.
+      if (edge_of(i, there[0])) spoilt |= Rows::template clean<Row::N>(v0 + wave * OFFSET, (uint32_t)(there[0] >> (wave * OWN)) & 0xFF);
+      lds_barrier();                                   // everyone's; and block i - 1's are done with
+      if (i + 1 < last) request(V_, at[0], v1);
+      if (i + AHEAD < last) request(K_, at[AHEAD - 1], k[AHEAD]);
+      if constexpr (!GROUPS) lookup(i + AHEAD + 2, u);
+      const uint64_t now = there[0];
+      auto next = [&]() __attribute__((always_inline)) {         // the places of one block more, while products go on
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) there[j] = there[j + 1];
+        for (int j = 0; j < AHEAD; ++j) there[j] = there[j + 1];
 #pragma unroll
-      for (int j = 0; j + 1 < AHEAD; ++j) at[j] = at[j + 1];
-      u ^= 1;
-      there[AHEAD] = place(i + AHEAD + 1, u, at[AHEAD - 1]);
-    };
-    auto end = [&]() __attribute__((always_inline)) {
+        for (int j = 0; j + 1 < AHEAD; ++j) at[j] = at[j + 1];
+        u ^= 1;
+        there[AHEAD] = place(i + AHEAD + 1, u, at[AHEAD - 1]);
+        if constexpr (GROUPS) {
+          lookup(i + AHEAD + 2, 0);
+          there[0] = keys_there(i + 1);
+        }
+      };
+      bool full1;
+      if (!live) {
+        next();
+        full1 = full_of(i + 1, there[0]);
+      } else if constexpr (KEYS == 64) {
+        a.step(s0, v0, f, k[1], p.c, s1);
+        follow(s1, full, i, now, 1);
+        next();
+        full1 = full_of(i + 1, there[0]);
+        a.step(s1, v0 + 64 * D, f, k[1] + 64 * D, p.c, s0);
+        follow(s0, full1, i + 1, there[0], 0);
+      } else {
+        a.step(s0, v0, f, k[2], p.c, s1);
+        next();
+        full1 = full_of(i + 1, there[0]);
+        follow(s1, full1, i + 1, there[0], 0);
+        s0 = s1;
+      }
+      full = full1;
       unsigned char* to = k[0];
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) k[j] = k[j + 1];
@@ -180,54 +278,27 @@ __global__ __launch_bounds__(64 * TilesCfg<D>::NW) __attribute__((amdgpu_waves_p
       to = v0;
       v0 = v1;
       v1 = to;
-      some = some1;
-      full = full1;
-      ++i;
-    };
-    for (;;) {
-      begin();
-      if (full && full1) {                             // all rows see all of this block and of the next
-        typename Rows::Keys f;
-        a.read_keys(KEYS == 64 ? k[0] + 64 * D : k[1], f);
-        do {
-          if constexpr (KEYS == 64) {
-            a.step(s0, v0, f, k[1], p.c, s1, top);
-            next();
-            a.step(s1, v0 + 64 * D, f, k[1] + 64 * D, p.c, s0, top);
-          } else {
-            a.step(s0, v0, f, k[2], p.c, s1, top);
-            next();
-            s0 = s1;
-          }
-          end();
-          begin();                                     // there is a next block
-        } while (full && full1);
-      }
-      const uint64_t now = there[0];
-      next();
-      if (some) {
-        typename Rows::Mask mask = mask_of(i, now, 0);
-        a.weigh(s0, p.c, w);
-        a.add_hidden(v0, w, mask);
-        if constexpr (KEYS == 64) {
-          mask = mask_of(i, now, 1);
-          a.scores(k[0] + 64 * D, s1);
-          a.hide(s1, mask);
-          a.largest(s1, p.c, top);
-          a.follow(top);
-          a.weigh(s1, p.c, w);
-          a.add_hidden(v0 + 64 * D, w, mask);
+    }
+  }
+
+  // Values that are no numbers, where zeros stood in for them and some row sees them: each goes to the rows that do, from the cache itself.
+  if (first < last) {
+    if (lane == 0) dirty[wave] = spoilt;
+    lds_barrier();
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(lane < NW && dirty[lane & 7]) != 0, 0))
+#pragma unroll 1
+      for (int i = first; i < last; ++i) {
+        const int kb = key_of(i), key = kb + lane % KEYS;
+        const uint32_t place = attn_in(p, x.r, key) ? attn_place(p, table[attn_page_of(p, key)], key, head) : kNoRow;
+        uint64_t there = __builtin_amdgcn_ballot_w64(place != kNoRow) & ALL;
+        if (!edge_of(i, there)) continue;
+        const uint64_t sees = attn_sees(p, x.s.first, t, p.tree ? p.tree + (size_t)(x.s.q0 + (has ? t : 0)) * p.tree_words : nullptr, kb);
+#pragma unroll 1
+        for (; there; there &= there - 1) {
+          const int j = __builtin_ctzll(there);
+          a.add_not_finite((const unsigned char*)p.v + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)place, j) * 16, sees >> j & 1);
         }
       }
-      if (some1) {
-        a.scores(k[1], s0);
-        if (!full1) a.hide(s0, mask_of(i + 1, there[0], 0));
-        a.largest(s0, p.c, top);
-        a.follow(top);
-      }
-      end();
-      if (i >= last) break;
-    }
   }
 
   const Halves ls = both_halves(a.l[0]);
@@ -275,12 +346,20 @@ __global__ __launch_bounds__(kJoin) void attn_tiles_join_kernel(const AttnArgs p
                     [&](int row) { return (typename Act::elem*)p.out + row_of(row) * D; });
 }
 
+template <class Act, int D, bool GROUPS>
+static int launch_tiles(const AttnArgs& p, hipStream_t st) {
+  static std::atomic<unsigned long long> raised{0};
+  const int rc = int8_raise_lds(attn_tiles_kernel<Act, D, GROUPS>, raised, TilesCfg<D>::LDS);
+  if (rc != MI_OK) return rc;
+  attn_tiles_kernel<Act, D, GROUPS><<<(unsigned)(p.slots * p.splits * p.Hkv), 64 * TilesCfg<D>::NW, TilesCfg<D>::LDS, st>>>(p);
+  return launch_status();
+}
 template <class Act, int D>
 static int launch(const AttnArgs& p, hipStream_t st) {
-  static std::atomic<unsigned long long> raised{0};
-  const int rc = int8_raise_lds(attn_tiles_kernel<Act, D>, raised, TilesCfg<D>::LDS);
+  // a group's rows: 32-bit distances in bytes
+  const bool groups = p.page % 8 == 0 && p.row16 < 1u << 24;
+  const int rc = groups ? launch_tiles<Act, D, true>(p, st) : launch_tiles<Act, D, false>(p, st);
   if (rc != MI_OK) return rc;
-  attn_tiles_kernel<Act, D><<<(unsigned)(p.slots * p.splits * p.Hkv), 64 * TilesCfg<D>::NW, TilesCfg<D>::LDS, st>>>(p);
   if (p.splits > 1) attn_tiles_join_kernel<Act, D><<<(unsigned)(p.slots * p.Hkv * TilesCfg<D>::NW), kJoin, 0, st>>>(p);
   return launch_status();
 }
