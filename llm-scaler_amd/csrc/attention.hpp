@@ -135,9 +135,12 @@ __device__ const int32_t kNoPage[1] = {-1};
 
 // 16 (4) bytes per lane from memory to LDS, side by side.  As a builtin the compiler waits for all of them in front of every transposing read of
 // LDS, loads for the next block included; here the kernels wait for themselves (wait_loads) and the compiler counts none of them.
-__device__ __forceinline__ uint32_t lds_address(const void* p) {
-  return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
+template <class T> __device__ __forceinline__ __attribute__((address_space(3))) T* in_lds(uint32_t at) {
+  return (__attribute__((address_space(3))) T*)(uintptr_t)at;
 }
+// An address that is the same for all lanes of a wavefront: read by a scalar load, which counts with those of LDS
+template <class T> __device__ __forceinline__ T scalar_load(const T* p) { return *(const __attribute__((address_space(4))) T*)(uintptr_t)p; }
 __device__ __forceinline__ void to_lds16(const void* from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
 }
@@ -161,14 +164,13 @@ struct RowPlaces {
     for (int j = 0; j < N; ++j) of[j] = __shfl(place, first + j * RPI + (int)(threadIdx.x & 63) / CH, 64);
   }
   template <bool IS_K>
-  __device__ __forceinline__ void load(const void* from, int first, const unsigned char* to) const {
+  __device__ __forceinline__ void load(const void* from, int first, uint32_t to) const {     // to: in LDS
     const int lane = threadIdx.x & 63;
-    const uint32_t lds = lds_address(to);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int r = first + j * RPI + lane / CH, chunk = (lane % CH) ^ (IS_K ? k_swizzle<D>(r) : v_swizzle<D>(r));
       const unsigned char* a = of[j] != kNoRow ? (const unsigned char*)from + (uint64_t)of[j] * 16 : (const unsigned char*)kZeroRow;
-      to_lds16(a + chunk * 16, lds + j * 1024);
+      to_lds16(a + chunk * 16, to + j * 1024);
     }
   }
 };
@@ -213,19 +215,18 @@ struct AttnRows {
       q[n][s] = as_v8<v8>(x);
     }
   }
-  // K of 32 keys (from 32 t of the block) and columns 16 ks ..
-  __device__ __forceinline__ v8 k_operand(const unsigned char* k, int t, int ks) const {
-    return as_v8<v8>(*(const u32x4*)(k + ((ka ^ (ks % 8 * 32)) + ks / 8 * 256 + t * 64 * D)));
+  // K of 32 keys (from 32 t of the block at LDS address k) and columns 16 ks ..
+  __device__ __forceinline__ v8 k_operand(uint32_t k, int t, int ks) const {
+    return as_v8<v8>(*in_lds<const u32x4>(k + (ka ^ (ks % 8 * 32)) + ks / 8 * 256 + t * 64 * D));
   }
-  // V^T of 16 keys (from 16 t of the block) and columns 32 d ..: element e is key 4 (lane / 32) + e % 4 + 8 (e / 4)
-  __device__ __forceinline__ v8 v_operand(const unsigned char* v, int t, int d) const {
-    const unsigned char* at = v + ((va ^ ((d & 3) * 64)) + (d >> 2) * 256 + t * 32 * D);
-    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)at);
-    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(at + 16 * D));
+  // V^T of 16 keys (from 16 t of the block at LDS address v) and columns 32 d ..: element e is key 4 (lane / 32) + e % 4 + 8 (e / 4)
+  __device__ __forceinline__ v8 v_operand(uint32_t v, int t, int d) const {
+    const uint32_t at = v + (va ^ ((d & 3) * 64)) + (d >> 2) * 256 + t * 32 * D;
+    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(in_lds<i16x4>(at)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(in_lds<i16x4>(at + 16 * D));
     return __builtin_bit_cast(v8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 
-  __device__ __forceinline__ void scores(const unsigned char* k, Scores& x) const {
+  __device__ __forceinline__ void scores(uint32_t k, Scores& x) const {
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -244,11 +245,11 @@ struct AttnRows {
   struct Keys { v8 k[D / 16]; };
   struct Values { v8 v[DT]; };
   static __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0x40E); }
-  __device__ __forceinline__ void read_keys(const unsigned char* k, Keys& f) const {
+  __device__ __forceinline__ void read_keys(uint32_t k, Keys& f) const {
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) f.k[ks] = k_operand(k, 0, ks);
   }
-  __device__ __forceinline__ void read_values(const unsigned char* v, int t, Values& f) const {
+  __device__ __forceinline__ void read_values(uint32_t v, int t, Values& f) const {
 #pragma unroll
     for (int d = 0; d < DT; ++d) f.v[d] = v_operand(v, t, d);
   }
@@ -257,7 +258,7 @@ struct AttnRows {
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) y.s[0][0] = mfma32(f.k[ks], q[0][ks], y.s[0][0]);
   }
-  __device__ __forceinline__ void step(const Scores& x, const unsigned char* v, Keys& f, const unsigned char* k2, float c, Scores& y) {
+  __device__ __forceinline__ void step(const Scores& x, uint32_t v, Keys& f, uint32_t k2, float c, Scores& y) {
     static_assert(NQ == 1 && KT == 1, "a step of 32 keys");
     Values va, vb;
     Weights w;
@@ -340,7 +341,7 @@ struct AttnRows {
     if constexpr (Act::dt == DT_F16) return __builtin_amdgcn_fdot2(two, one, sum, false);
     else return __builtin_amdgcn_fdot2_f32_bf16(two, one, sum, false);
   }
-  __device__ __forceinline__ void add(const unsigned char* v, const Weights& w) {
+  __device__ __forceinline__ void add(uint32_t v, const Weights& w) {
 #pragma unroll
     for (int t = 0; t < 2 * KT; ++t)
 #pragma unroll
@@ -352,11 +353,11 @@ struct AttnRows {
   }
   // Zeros in place of infinities and NaN in 8 rows of values in LDS; whether there were any in the rows whose bits `there` has
   template <int PIECES>
-  static __device__ __forceinline__ bool clean(unsigned char* v, uint32_t there) {
+  static __device__ __forceinline__ bool clean(uint32_t v, uint32_t there) {
     bool spoilt = false;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
-      u16x8* at = (u16x8*)(v + j * 1024 + (threadIdx.x & 63) * 16);
+      auto* at = in_lds<u16x8>(v + j * 1024 + (threadIdx.x & 63) * 16);
       const u16x8 x = *at, finite = __builtin_elementwise_min(EXPONENT - (x & EXPONENT), (u16x8)1);
       const u32x4 all = __builtin_bit_cast(u32x4, finite);
       const bool found = (all[0] & all[1] & all[2] & all[3]) != 0x00010001u;
@@ -383,7 +384,7 @@ struct AttnRows {
   }
   // The same where some row does not see some key: 0 times an infinity or a NaN there would not be 0, so such values go to the rows that see
   // them by themselves.
-  __device__ __forceinline__ void add_hidden(const unsigned char* v, const Weights& w, const Mask& mask) {
+  __device__ __forceinline__ void add_hidden(uint32_t v, const Weights& w, const Mask& mask) {
     u16x8 one = 1;                                     // 0 where a value was not finite
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -401,7 +402,7 @@ struct AttnRows {
     const u32x4 all = __builtin_bit_cast(u32x4, one);
     if (__builtin_amdgcn_ballot_w64((all[0] & all[1] & all[2] & all[3]) != 0x00010001u)) add_not_finite(v, mask);
   }
-  __device__ __forceinline__ void add_not_finite(const unsigned char* v, const Mask& mask) {
+  __device__ __forceinline__ void add_not_finite(uint32_t v, const Mask& mask) {
     const int h = (threadIdx.x & 63) >> 5;
     typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
     typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
@@ -412,7 +413,7 @@ struct AttnRows {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                  // columns 32 d + 8 i + 4 h ..
-          const u16x4 x = *(const u16x4*)(v + j * 2 * D + ((4 * d + i) ^ v_swizzle<D>(j)) * 16 + h * 8);
+          const u16x4 x = *in_lds<const u16x4>(v + j * 2 * D + ((4 * d + i) ^ v_swizzle<D>(j)) * 16 + h * 8);
           const e4 y = __builtin_bit_cast(e4, x);
 #pragma unroll
           for (int n = 0; n < NQ; ++n)

@@ -135,20 +135,20 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
       a.load_q(0, has ? (const typename Act::elem*)p.q + (x.s.q0 + t) * p.q_token + (y.head * p.G + r - t * p.G) * p.q_head : nullptr);
 
       // block i's keys and values lie in half (i - first) % 2 of the ring, the pages of its keys likewise behind it
-      const unsigned char* pages = smem + C::STAGES * 2 * C::HALF;
+      const uint32_t ring = lds_address(smem), pages = ring + C::STAGES * 2 * C::HALF;
       auto lookup = [&](int i, int u) {
         const int key = attn_key<32>(x.r, i) + (lane & 31);
-        to_lds4(i < last && attn_in(p, x.r, key) ? table + attn_page_of(p, key) : kNoPage, lds_address(pages + u * 256));
+        to_lds4(i < last && attn_in(p, x.r, key) ? table + attn_page_of(p, key) : kNoPage, pages + u * 256);
       };
       auto place = [&](int i, int u) {
-        const int page = *(const int*)(pages + u * 256 + lane * 4);
+        const int page = *in_lds<const int>(pages + u * 256 + lane * 4);
         return i < last ? attn_place(p, page, attn_key<32>(x.r, i) + (lane & 31), y.head) : kNoRow;
       };
       auto request = [&](uint32_t at16, int u) {
         RowPlaces<D, 32> rows;
         rows.take(at16, 0);
-        rows.template load<true>(p.k, 0, smem + u * 2 * C::HALF);
-        rows.template load<false>(p.v, 0, smem + u * 2 * C::HALF + C::HALF);
+        rows.template load<true>(p.k, 0, ring + u * 2 * C::HALF);
+        rows.template load<false>(p.v, 0, ring + u * 2 * C::HALF + C::HALF);
         return (uint32_t)__builtin_amdgcn_ballot_w64(at16 != kNoRow);
       };
       uint32_t there[2];
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
           if (i >= last) break;
           wait_loads<LOADS>();                         // block i is there, and the pages of block i + 2
           __builtin_amdgcn_sched_barrier(0);
-          const unsigned char *k = smem + u * 2 * C::HALF, *v = k + C::HALF;
+          const uint32_t k = ring + u * 2 * C::HALF, v = k + C::HALF;
           const int kb = attn_key<32>(x.r, i);
           const bool full = there[u] == 0xFFFFFFFFu && attn_all_seen<32>(p, x.s.first, t0, t1, kb);
           typename Rows::Scores s;

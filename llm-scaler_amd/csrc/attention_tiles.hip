@@ -106,7 +106,7 @@ void attn_tiles_kernel(const AttnArgs p) {
   // like the keys, a block ahead of what is asked for with them
   using Places = std::conditional_t<GROUPS, uint32_t, RowPlaces<D, OWN>>;
   using Row = RowPlaces<D, OWN>;
-  const unsigned char* pages = smem + C::PAGES + wave * (2 * 4 * KEYS);
+  const uint32_t rings = lds_address(smem), pages = rings + C::PAGES + wave * (2 * 4 * KEYS);
   uint32_t* bad = (uint32_t*)(smem + C::FLAGS);        // [block % 8][wave]: its page is outside the cache
   uint32_t* dirty = bad + 64;                          // [wave]: it put zeros in place of values that some row sees
   uint32_t from_k[Row::N], from_v[Row::N];             // bytes from a group's first place
@@ -117,37 +117,71 @@ void attn_tiles_kernel(const AttnArgs p) {
       from_k[j] = g * p.row16 * 16 + ((lane % Row::CH) ^ k_swizzle<D>(row)) * 16;
       from_v[j] = g * p.row16 * 16 + ((lane % Row::CH) ^ v_swizzle<D>(row)) * 16;
     }
-  int page = -1;                                       // GROUPS: of the block whose places come next
+  // Blocks `inner` .. inner + inners - 1 hold keys that all rows of the tile see; where no page of the call is outside the cache nothing is looked up for
+  // them but the page.
+  const int tile0 = x.row0 / p.G, tile1 = (x.row0 + x.rows - 1) / p.G;
+  int inner = 0, inners = 0;
+  if constexpr (GROUPS) {
+    const int from = max(x.r.lo, p.window ? x.s.first + tile1 - p.window + 1 : 0), to = p.tree ? min(x.r.hi, x.s.first) : min(x.r.hi, x.s.first + tile0 + 1);
+    inner = max(x.r.head + (max(from - x.r.from, 0) + KEYS - 1) / KEYS, first);
+    inners = max(min(x.r.head + (to - x.r.from) / KEYS, last) - inner, 0);
+    if (to <= x.r.from) inners = 0;
+    bool wrong = false;
+    auto scan = [&](int a, int b) {                    // the pages of keys a .. b - 1
+      if (a < b)
+        for (int i = attn_page_of(p, a) + (int)threadIdx.x; i <= attn_page_of(p, b - 1); i += 64 * NW) wrong |= (uint32_t)table[i] >= (uint32_t)p.pages;
+    };
+    scan(first * KEYS, min(min(last, x.r.head) * KEYS, min(p.sinks, x.r.hi)));
+    scan(max(x.r.lo, attn_key<KEYS>(x.r, max(first, x.r.head))), min(x.r.hi, attn_key<KEYS>(x.r, last - 1) + KEYS));
+    wrong = __builtin_amdgcn_ballot_w64(wrong) != 0;
+    if (lane == 0) bad[wave] = wrong;
+    lds_barrier();
+    if (__builtin_amdgcn_ballot_w64(lane < NW && bad[lane & 7])) inners = 0;
+    lds_barrier();
+  }
+  const int inner_key = x.r.from + (inner - x.r.head) * KEYS;
+  auto is_inner = [&](int i) { return GROUPS && (uint32_t)(i - inner) < (uint32_t)inners; };
+  int page = 0;                                        // GROUPS: of the block whose place comes next
   auto lookup = [&](int i, int u) {
     if constexpr (GROUPS) {
+      if (is_inner(i)) {
+        page = scalar_load(table + attn_page_of(p, inner_key + (i - inner) * KEYS + wave * OWN));
+        return;
+      }
       const int key = key_of(i) + wave * OWN;
       const bool seen = i < last && key < x.r.hi && (key + OWN > x.r.lo || key < p.sinks);
       page = 0;
-      if (seen) page = __builtin_amdgcn_readfirstlane(table[attn_page_of(p, key)]);          // a group that nothing sees: some place of the cache
+      if (seen) page = scalar_load(table + attn_page_of(p, key));          // a group that nothing sees: some place of the cache
     } else {
       const int key = key_of(i) + lane % KEYS;
       if (KEYS == 64 || lane < KEYS)
-        to_lds4(i < last && attn_in(p, x.r, key) ? table + attn_page_of(p, key) : kNoPage, lds_address(pages + u * 4 * KEYS));
+        to_lds4(i < last && attn_in(p, x.r, key) ? table + attn_page_of(p, key) : kNoPage, pages + u * 4 * KEYS);
     }
   };
   // the place of block i, and which of its keys are there
   auto place = [&](int i, int u, Places& to) {
     if constexpr (GROUPS) {
+      if (is_inner(i)) {
+        const int key = inner_key + (i - inner) * KEYS + wave * OWN;
+        to = (uint32_t)page * p.page16 + (uint32_t)(key - attn_page_of(p, key) * p.page) * p.row16 + (uint32_t)head * p.head16;
+        return ALL;
+      }
       const int key = key_of(i) + wave * OWN;
       const bool wrong = (uint32_t)page >= (uint32_t)p.pages;
       const bool seen = i < last && key < x.r.hi && (key + OWN > x.r.lo || key < p.sinks);
       const uint32_t in = wrong || !seen ? 0 : (uint32_t)page * p.page16 + (uint32_t)(key - attn_page_of(p, key) * p.page) * p.row16;
       to = in + (uint32_t)head * p.head16;
       if (lane == 0) bad[(i & 7) * 8 + wave] = wrong;
-      return (uint64_t)0;                              // known when all wavefronts have written theirs
+      return ALL;                                      // less what keys_there says when all wavefronts have written theirs
     } else {
-      const int it = *(const int*)(pages + u * 4 * KEYS + lane % KEYS * 4);
+      const int it = *in_lds<const int>(pages + u * 4 * KEYS + lane % KEYS * 4);
       const uint32_t at = i < last ? attn_place(p, it, key_of(i) + lane % KEYS, head) : kNoRow;
       to.take(at, wave * OWN);
       return (uint64_t)__builtin_amdgcn_ballot_w64(at != kNoRow);
     }
   };
   auto keys_there = [&](int i) {                       // GROUPS
+    if (is_inner(i)) return ALL;
     if (i >= last) return (uint64_t)0;
     const int kb = key_of(i);
     uint64_t m = low_bits(x.r.hi - kb) & (~low_bits(x.r.lo - kb) | low_bits(p.sinks - kb));
@@ -155,14 +189,13 @@ void attn_tiles_kernel(const AttnArgs p) {
     for (; wrong; wrong &= wrong - 1) m &= ~(0xFFull << (8 * __builtin_ctzll(wrong)));
     return m & ALL;
   };
-  auto request = [&](auto is_k, const Places& from, unsigned char* to) {
+  auto request = [&](auto is_k, const Places& from, uint32_t to) {
     constexpr bool K = decltype(is_k)::value;
     to += wave * OFFSET;
     if constexpr (GROUPS) {
       const unsigned char* base = (const unsigned char*)(K ? p.k : p.v) + (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)from) * 16;
-      const uint32_t lds = lds_address(to);
 #pragma unroll
-      for (int j = 0; j < Row::N; ++j) to_lds16_from(base, K ? from_k[j] : from_v[j], lds + j * 1024);
+      for (int j = 0; j < Row::N; ++j) to_lds16_from(base, K ? from_k[j] : from_v[j], to + j * 1024);
     } else {
       from.template load<K>(K ? p.k : p.v, wave * OWN, to);
     }
@@ -170,9 +203,8 @@ void attn_tiles_kernel(const AttnArgs p) {
   const std::true_type K_;
   const std::false_type V_;
 
-  auto full_of = [&](int i, uint64_t there) { return there == ALL && attn_all_seen<KEYS>(p, x.s.first, t0, t1, key_of(i)); };
-  const int tile0 = x.row0 / p.G, tile1 = (x.row0 + x.rows - 1) / p.G;
-  auto edge_of = [&](int i, uint64_t there) { return there != ALL || !attn_all_seen<KEYS>(p, x.s.first, tile0, tile1, key_of(i)); };
+  auto full_of = [&](int i, uint64_t there) { return is_inner(i) || (there == ALL && attn_all_seen<KEYS>(p, x.s.first, t0, t1, key_of(i))); };
+  auto edge_of = [&](int i, uint64_t there) { return !is_inner(i) && (there != ALL || !attn_all_seen<KEYS>(p, x.s.first, tile0, tile1, key_of(i))); };
   bool spoilt = false;
   auto mask_of = [&](int i, uint64_t there, int half) {
     int mine = has ? t : 0;
@@ -184,8 +216,8 @@ void attn_tiles_kernel(const AttnArgs p) {
   };
 
   if (first < last) {
-    unsigned char* k[AHEAD + 1];                       // keys of blocks i, i + 1 ..
-    unsigned char *v0 = smem + (AHEAD + 1) * C::HALF, *v1 = v0 + C::HALF;        // values of blocks i, i + 1
+    uint32_t k[AHEAD + 1];                             // where in LDS: keys of blocks i, i + 1 ..
+    uint32_t v0 = rings + (AHEAD + 1) * C::HALF, v1 = v0 + C::HALF;              // values of blocks i, i + 1
     Places at[AHEAD];                                  // of blocks i + 1 ..
     uint64_t there[AHEAD + 1];                         // keys of blocks i .. (GROUPS: of i and i + 1)
     lookup(first, 0);
@@ -195,7 +227,7 @@ void attn_tiles_kernel(const AttnArgs p) {
     }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      k[j] = smem + j * C::HALF;
+      k[j] = rings + j * C::HALF;
       Places& to = at[j ? j - 1 : 0];
       there[j] = place(first + j, j & 1, to);
       request(K_, to, k[j]);
@@ -207,7 +239,7 @@ void attn_tiles_kernel(const AttnArgs p) {
         if (j >= 1 && j + 1 < AHEAD) wait_loads<0>();
       }
     }
-    k[AHEAD] = smem + AHEAD * C::HALF;
+    k[AHEAD] = rings + AHEAD * C::HALF;
     typename Rows::Scores s0, s1;                      // of the two steps of a block (one: s0)
     typename Rows::Keys f;
     float top[1];
@@ -271,7 +303,7 @@ void attn_tiles_kernel(const AttnArgs p) {
         s0 = s1;
       }
       full = full1;
-      unsigned char* to = k[0];
+      uint32_t to = k[0];
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) k[j] = k[j + 1];
       k[AHEAD] = to;
