@@ -53,10 +53,12 @@ static int attn_plan(int T, int B, int Hq, int Hkv, int D, int max_query_len, in
   if (a.tiles) {
     const int R = attn_tile_rows(D);
     const long long slots = (long long)T * G / R + B;
-    if (slots * Hkv >= 1 << 30) return MI_ERR_SHAPE;
+    if (slots * Hkv * (R / kJoinRows) >= 1 << 30) return MI_ERR_SHAPE;
     a.slots = (int)slots;
     // about three workgroups per CU, of 512 keys at least
-    const long long tiles = (((long long)T * G + R - 1) / R) * Hkv;
+    long long tiles = (long long)T * G / R;
+    if (tiles < B) tiles = B;
+    tiles *= Hkv;
     long long s = 3LL * cus() / tiles, most_s = blocks / 8;
     if (s > most_s) s = most_s;
     if (s > 64) s = 64;
@@ -104,6 +106,10 @@ static int run(const AttnArgs& base, const MiPagedCache* cache, int D, float sca
   p.c = scale * 1.4426950408889634f;
   p.rows_from = a.rows_from;
   p.groups = a.groups;
+  const long long most = max_query_len < p.T ? max_query_len : p.T;
+  p.tile_rows = a.tiles || most * p.G > 32 ? 32 : most < 1 ? p.G : (int)(most * p.G);
+  p.many_parts = (long long)a.groups > 16LL * p.B * p.Hkv;
+  p.wide = ((long long)p.T * p.G / 32 + p.B) * p.Hkv * ((long long)p.width * cache->page_size / 32 + 8) >= 1LL << 31;
   p.slots = a.slots;
   p.splits = a.splits;
   if (a.tiles) {

@@ -34,7 +34,8 @@ struct AttnArgs {
   int T, B, Hq, Hkv, G, page, width, pages;
   int window, sinks, tree_words;         // window 0: none
   float c;
-  int groups;                  // rows kernel: workgroups
+  int groups, tile_rows;       // rows kernel: workgroups, rows of a tile at most
+  bool wide, many_parts;       // its work counts 2^31 blocks or more; a tile is in many parts
   int slots, splits;           // tiles kernel
   int rows_from;               // sequences with that many rows (tokens x G) or more belong to the tiles kernel
 };
@@ -427,14 +428,14 @@ struct AttnRows {
 };
 
 // ---- joining parts ------------------------------------------------------------------------------
-// A workgroup of kJoin threads makes `rows` (up to 32) rows of out from `parts` parts of each: sums(i, row) points to the D sums of part i, ml(i, row)
+// A workgroup of THREADS threads makes `rows` rows of out from `parts` parts of each: sums(i, row) points to the D sums of part i, ml(i, row)
 // to its m and l (m = -inf: the part has no sums), to(row) to the row of out.  A thread has four columns of a row; where threads are left over they
 // share a row's parts, and what they have meets in LDS.  All loads of four parts are under way together.
-constexpr int kJoin = 1024;
-template <class Act, int D, class Sums, class Ml, class To>
+constexpr int kJoinRows = 8;                          // of a workgroup
+template <class Act, int D, int THREADS, class Sums, class Ml, class To>
 __device__ __forceinline__ void attn_join(int rows, int parts, Sums sums, Ml ml, To to) {
-  constexpr int Q = D / 4, PLACES = kJoin / Q;         // threads of a row; rows, or shares of rows, at a time
-  __shared__ f32x4 part_o[kJoin];
+  constexpr int Q = D / 4, PLACES = THREADS / Q;         // threads of a row; rows, or shares of rows, at a time
+  __shared__ f32x4 part_o[THREADS];
   __shared__ f32x2 part_ml[PLACES];
   const int col = threadIdx.x % Q * 4, place = threadIdx.x / Q;
   int share = 1;

@@ -30,42 +30,47 @@ __device__ __forceinline__ RowsSeq rows_seq(const AttnArgs& p, int b) {
   x.tiles = rows >= p.rows_from ? 0 : (rows + 31) / 32;
   return x;
 }
-__device__ __forceinline__ long long rows_work(const AttnArgs& p, const RowsSeq& x) { return (long long)x.tiles * p.Hkv * (x.r.blocks + kItem); }
+// Num: int where all work of the call counts less than 2^31 blocks
+template <class Num>
+__device__ __forceinline__ Num rows_work(const AttnArgs& p, const RowsSeq& x) { return (Num)x.tiles * p.Hkv * (x.r.blocks + kItem); }
 
-__device__ __forceinline__ long long shfl64(long long v, int lane) {
+__device__ __forceinline__ int from_lane(int v, int lane) { return __shfl(v, lane, 64); }
+__device__ __forceinline__ long long from_lane(long long v, int lane) {
   return (long long)(uint32_t)__shfl((int)v, lane, 64) | (long long)__shfl((int)(v >> 32), lane, 64) << 32;
 }
 
 // All work of the call, and the share of a workgroup: every wavefront finds it by itself.
-struct RowsPlan { long long incl, before, total, share; int per; };
-__device__ __forceinline__ RowsPlan rows_plan(const AttnArgs& p) {
+template <class Num> struct RowsPlan { Num incl, before, total, share; int per; };
+template <class Num>
+__device__ __forceinline__ RowsPlan<Num> rows_plan(const AttnArgs& p) {
   const int lane = threadIdx.x & 63;
-  RowsPlan a;
+  RowsPlan<Num> a;
   a.per = (p.B + 63) / 64;
-  long long mine = 0;
+  Num mine = 0;
   for (int i = 0; i < a.per; ++i) {
     const int b = lane * a.per + i;
-    if (b < p.B) mine += rows_work(p, rows_seq(p, b));
+    if (b < p.B) mine += rows_work<Num>(p, rows_seq(p, b));
   }
-  long long incl = mine;
-  for (int d = 1; d < 64; d <<= 1) {
-    const long long up = shfl64(incl, lane >= d ? lane - d : lane);
+  Num incl = mine;
+  for (int d = 1; d < 64 && d < p.B; d <<= 1) {
+    const Num up = from_lane(incl, lane >= d ? lane - d : lane);
     if (lane >= d) incl += up;
   }
   a.incl = incl;
   a.before = incl - mine;
-  a.total = shfl64(incl, 63);
+  a.total = from_lane(incl, (p.B - 1) / a.per);        // the last lane with sequences; those behind it have not added all up
   a.share = (a.total + p.groups - 1) / p.groups;
   return a;
 }
 // The sequence with block `at` of the work, and the place of the block in it.  at < total.
-__device__ __forceinline__ void rows_find(const AttnArgs& p, const RowsPlan& a, long long at, int& b, long long& in) {
+template <class Num>
+__device__ __forceinline__ void rows_find(const AttnArgs& p, const RowsPlan<Num>& a, Num at, int& b, Num& in) {
   const int owner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(at < a.incl));
-  long long rest = at - shfl64(a.before, owner);
+  Num rest = at - from_lane(a.before, owner);
   b = owner * a.per;
-  for (;; ++b) {
-    const long long n = rows_work(p, rows_seq(p, b));
-    if (rest < n || b + 1 >= p.B) break;
+  for (; a.per > 1 && b + 1 < p.B; ++b) {
+    const Num n = rows_work<Num>(p, rows_seq(p, b));
+    if (rest < n) break;
     rest -= n;
   }
   in = rest;
@@ -73,11 +78,12 @@ __device__ __forceinline__ void rows_find(const AttnArgs& p, const RowsPlan& a, 
 
 // A tile's place in the work: its sequence's `in`-th unit
 struct RowsItem { int tile, head, rows, unit; };      // unit: of the tile; its first kItem are none of its blocks
-__device__ __forceinline__ RowsItem rows_item(const AttnArgs& p, const RowsSeq& x, long long in) {
+template <class Num>
+__device__ __forceinline__ RowsItem rows_item(const AttnArgs& p, const RowsSeq& x, Num in) {
   const int per = x.r.blocks + kItem;
   const int item = __builtin_amdgcn_readfirstlane((int)(in / per));
   RowsItem y;
-  y.unit = __builtin_amdgcn_readfirstlane((int)(in - (long long)item * per));
+  y.unit = __builtin_amdgcn_readfirstlane((int)(in - (Num)item * per));
   y.tile = item / p.Hkv;
   y.head = item - y.tile * p.Hkv;
   y.rows = min(32, x.s.n * p.G - y.tile * 32);
@@ -92,7 +98,7 @@ __device__ __forceinline__ long long rows_row(const AttnArgs& p, int q0, int til
 template <int D>
 __device__ __forceinline__ i32x4* rows_cuts(const AttnArgs& p) { return (i32x4*)(p.part + (size_t)p.groups * 2 * RowsCfg<D>::PART); }
 
-template <class Act, int D>
+template <class Act, int D, class Num>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2))) void attn_rows_kernel(const AttnArgs p) {
   using C = RowsCfg<D>;
   using Rows = AttnRows<Act, D, 32, 1>;
@@ -100,27 +106,29 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int lane = threadIdx.x;
 
-  const RowsPlan plan = rows_plan(p);
-  long long at = plan.share * blockIdx.x;
-  const long long end = min(at + plan.share, plan.total);
+  const RowsPlan<Num> plan = rows_plan<Num>(p);
+  // shares: all of them may count up to 2^31 and a share more
+  const bool none = plan.share == 0 || (Num)blockIdx.x > plan.total / plan.share;
+  Num at = none ? plan.total : plan.share * (Num)blockIdx.x;
+  const Num end = plan.total - at < plan.share ? plan.total : at + plan.share;
   if (at >= end) {
     if (lane == 0) rows_cuts<D>(p)[blockIdx.x] = i32x4{};
     return;
   }
   int b;
-  long long in;
-  rows_find(p, plan, at, b, in);
+  Num in;
+  rows_find<Num>(p, plan, at, b, in);
   b = __builtin_amdgcn_readfirstlane(b);
 
   for (bool starts = true; at < end; starts = false) {
     const RowsSeq x = rows_seq(p, b);
     const RowsItem y = rows_item(p, x, in);
     if (starts) {                                      // the cut in front of this share is one to join at if it goes through blocks, as the tile's first
-      const long long begin = at - y.unit + kItem, w = blockIdx.x;
+      const Num begin = at - y.unit + kItem, w = blockIdx.x;
       const int parts = at <= begin || (w - 1) * plan.share > begin ? 0 : 1 + (int)((begin + x.r.blocks - 1) / plan.share - (w - 1));
       if (lane == 0) rows_cuts<D>(p)[w] = i32x4{parts, x.s.q0, y.tile, y.head * 64 + y.rows};
     }
-    const int take = __builtin_amdgcn_readfirstlane((int)min((long long)(x.r.blocks + kItem - y.unit), end - at));
+    const int take = __builtin_amdgcn_readfirstlane((int)min((Num)(x.r.blocks + kItem - y.unit), end - at));
     const int first = max(y.unit - kItem, 0), last = y.unit + take - kItem;      // blocks
     at += take;
     in += take;
@@ -220,36 +228,48 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
         }
       }
     }
-    if (in >= rows_work(p, x)) {
+    if (in >= rows_work<Num>(p, x)) {
       in = 0;
       do ++b;
-      while (b + 1 < p.B && at < end && rows_work(p, rows_seq(p, b)) == 0);
+      while (b + 1 < p.B && at < end && rows_work<Num>(p, rows_seq(p, b)) == 0);
     }
   }
 }
 
-// Workgroup w joins the tile that the cut in front of share w + 1 goes through.
-template <class Act, int D>
-__global__ __launch_bounds__(kJoin) void attn_rows_join_kernel(const AttnArgs p) {
+// Workgroup w, y joins rows 8 y .., and every 8 gridDim.y further, of the tile that the cut in front of share w + 1 goes through.
+template <class Act, int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void attn_rows_join_kernel(const AttnArgs p) {
   constexpr int PART = RowsCfg<D>::PART;
   const int w = blockIdx.x + 1;
   const i32x4 cut = rows_cuts<D>(p)[w];
+  const int rows = cut[3] % 64;
   if (!cut[0]) return;
   // the first part is the one that share w - 1 began, the others those that a share continued
   auto part = [&](int i) { return p.part + ((size_t)(w - 1 + i) * 2 + (i == 0)) * PART; };
-  attn_join<Act, D>(cut[3] % 64, cut[0], [&](int i, int row) { return part(i) + row * D; }, [&](int i, int row) { return part(i) + 32 * D + 2 * row; },
-                    [&](int row) { return (typename Act::elem*)p.out + rows_row(p, cut[1], cut[2], cut[3] / 64, row) * D; });
+  for (int row0 = blockIdx.y * kJoinRows; row0 < rows; row0 += gridDim.y * kJoinRows)
+    attn_join<Act, D, THREADS>(
+        min(kJoinRows, rows - row0), cut[0], [&](int i, int row) { return part(i) + (row0 + row) * D; },
+        [&](int i, int row) { return part(i) + 32 * D + 2 * (row0 + row); },
+        [&](int row) { return (typename Act::elem*)p.out + rows_row(p, cut[1], cut[2], cut[3] / 64, row0 + row) * D; });
 }
 
 long long attn_rows_bytes(int groups, int D) { return (long long)groups * (2 * 32 * (D + 2) * 4 + 16); }
 
+template <class Act, int D, class Num>
+static int launch_rows(const AttnArgs& p, hipStream_t st) {
+  static std::atomic<unsigned long long> raised{0};
+  const int rc = int8_raise_lds(attn_rows_kernel<Act, D, Num>, raised, RowsCfg<D>::LDS);
+  if (rc != MI_OK) return rc;
+  attn_rows_kernel<Act, D, Num><<<p.groups, 64, RowsCfg<D>::LDS, st>>>(p);
+  return launch_status();
+}
 template <class Act, int D>
 static int launch(const AttnArgs& p, hipStream_t st) {
-  static std::atomic<unsigned long long> raised{0};
-  const int rc = int8_raise_lds(attn_rows_kernel<Act, D>, raised, RowsCfg<D>::LDS);
-  if (rc != MI_OK) return rc;
-  attn_rows_kernel<Act, D><<<p.groups, 64, RowsCfg<D>::LDS, st>>>(p);
-  if (p.groups > 1) attn_rows_join_kernel<Act, D><<<p.groups - 1, kJoin, 0, st>>>(p);
+  const int rc = p.wide ? launch_rows<Act, D, long long>(p, st) : launch_rows<Act, D, int>(p, st);
+  if (rc != MI_OK || p.groups == 1) return rc;
+  const dim3 grid(p.groups - 1, (p.tile_rows + kJoinRows - 1) / kJoinRows);
+  if (p.many_parts) attn_rows_join_kernel<Act, D, 1024><<<grid, 1024, 0, st>>>(p);
+  else attn_rows_join_kernel<Act, D, 256><<<grid, 256, 0, st>>>(p);
   return launch_status();
 }
 

@@ -362,20 +362,21 @@ void attn_tiles_kernel(const AttnArgs p) {
       *(f32x4*)(to + d * 32 + i * 2) = f32x4{a.o[0][d][i], a.o[0][d][i + 1], a.o[0][d][i + 2], a.o[0][d][i + 3]};
 }
 
-// A workgroup per 32 rows of a slot and kv head.
-template <class Act, int D>
-__global__ __launch_bounds__(kJoin) void attn_tiles_join_kernel(const AttnArgs p) {
+// A workgroup per 8 rows of a slot and kv head.
+template <class Act, int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void attn_tiles_join_kernel(const AttnArgs p) {
   using C = TilesCfg<D>;
-  const int piece = blockIdx.x % C::NW, rest = blockIdx.x / C::NW, head = rest % p.Hkv, slot = rest / p.Hkv;
+  constexpr int PIECES = C::ROWS / kJoinRows;
+  const int row0 = blockIdx.x % PIECES * kJoinRows, rest = blockIdx.x / PIECES, head = rest % p.Hkv, slot = rest / p.Hkv;
   Tile x;
-  if (!tile_at<C::ROWS, C::KEYS>(p, slot, x) || piece * 32 >= x.rows) return;
+  if (!tile_at<C::ROWS, C::KEYS>(p, slot, x) || row0 >= x.rows) return;
   auto row_of = [&](int row) {
-    const int r = x.row0 + piece * 32 + row, t = r / p.G;
+    const int r = x.row0 + row0 + row, t = r / p.G;
     return (long long)(x.s.q0 + t) * p.Hq + head * p.G + r - t * p.G;
   };
-  attn_join<Act, D>(min(32, x.rows - piece * 32), p.splits, [&](int i, int row) { return part_sums(p, D, i, row_of(row)); },
-                    [&](int i, int row) { return part_ml(p, D, i, row_of(row)); },
-                    [&](int row) { return (typename Act::elem*)p.out + row_of(row) * D; });
+  attn_join<Act, D, THREADS>(min(kJoinRows, x.rows - row0), p.splits, [&](int i, int row) { return part_sums(p, D, i, row_of(row)); },
+                             [&](int i, int row) { return part_ml(p, D, i, row_of(row)); },
+                             [&](int row) { return (typename Act::elem*)p.out + row_of(row) * D; });
 }
 
 template <class Act, int D, bool GROUPS>
@@ -392,7 +393,11 @@ static int launch(const AttnArgs& p, hipStream_t st) {
   const bool groups = p.page % 8 == 0 && p.row16 < 1u << 24;
   const int rc = groups ? launch_tiles<Act, D, true>(p, st) : launch_tiles<Act, D, false>(p, st);
   if (rc != MI_OK) return rc;
-  if (p.splits > 1) attn_tiles_join_kernel<Act, D><<<(unsigned)(p.slots * p.Hkv * TilesCfg<D>::NW), kJoin, 0, st>>>(p);
+  if (p.splits > 1) {
+    const unsigned grid = (unsigned)(p.slots * p.Hkv * (TilesCfg<D>::ROWS / kJoinRows));
+    if (p.splits > 16) attn_tiles_join_kernel<Act, D, 1024><<<grid, 1024, 0, st>>>(p);
+    else attn_tiles_join_kernel<Act, D, 256><<<grid, 256, 0, st>>>(p);
+  }
   return launch_status();
 }
 
