@@ -9,7 +9,7 @@ namespace qlin {
 // sequences of both kinds can be in a call both are launched, and each takes its own.
 struct AttnPlan {
   bool rows, tiles;
-  int rows_from, groups, slots, splits;
+  int rows_from, groups, slots, shares;
   long long rows_bytes, tiles_bytes;
 };
 
@@ -43,28 +43,29 @@ static int attn_plan(int T, int B, int Hq, int Hkv, int D, int max_query_len, in
     a.rows = false;
     a.rows_from = 0;
   }
-  const long long blocks = ((long long)(max_seq_len < 1 ? 1 : max_seq_len) + kBlock - 1) / kBlock;
   if (a.rows) {
     const long long full = (long long)cus() * (D == 64 ? 8 : D == 128 ? 4 : 2);  // workgroups that the device holds
-    const long long some = ((long long)T * G / 32 + B) * Hkv * 2 * blocks;
+    const long long some = ((long long)T * G / kFewRows + B) * Hkv * ((max_seq_len < 1 ? 1 : max_seq_len) / 32LL + 1);
     a.groups = (int)(some < full ? some : full);
-    a.rows_bytes = round256(attn_rows_bytes(a.groups, D));
+    a.rows_bytes = round256(attn_parts_bytes(a.groups, D, kFewRows));
   }
   if (a.tiles) {
-    const int R = attn_tile_rows(D);
+    const int R = attn_tile_rows(D), hold = cus() * (D == 64 ? 2 : 1);           // workgroups that the device holds
     const long long slots = (long long)T * G / R + B;
-    if (slots * Hkv * (R / kJoinRows) >= 1 << 30) return MI_ERR_SHAPE;
+    if (slots * Hkv >= 1 << 30) return MI_ERR_SHAPE;
     a.slots = (int)slots;
-    // about three workgroups per CU, of 512 keys at least
+    // What the longer of both ways takes, in blocks of keys per workgroup: a workgroup per tile takes as long as the longest tile, and half as long again
+    // on top of the even share where workgroups follow each other; equal shares have every tile see what its sequence's last token sees, and
+    // a part more to write and read (8 blocks or so each).
     long long tiles = (long long)T * G / R;
     if (tiles < B) tiles = B;
     tiles *= Hkv;
-    long long s = 3LL * cus() / tiles, most_s = blocks / 8;
-    if (s > most_s) s = most_s;
-    if (s > 64) s = 64;
-    a.splits = s < 2 ? 1 : (int)s;
-    if (slots * Hkv * a.splits >= 1LL << 30) a.splits = 1;
-    if (a.splits > 1) a.tiles_bytes = round256((long long)a.splits * T * Hq * (D + 2) * 4);
+    const long long keys = max_seq_len < 1 ? 1 : max_seq_len, seen = keys - (most < keys ? most : keys) / 2;
+    const long long even = tiles * seen / hold, alone = tiles <= hold ? keys : even + keys / 2, shared = tiles * keys / hold + 1024;
+    if (alone > shared) {
+      a.shares = hold;
+      a.tiles_bytes = round256(attn_parts_bytes(a.shares, D, R));
+    }
   }
   return MI_OK;
 }
@@ -108,10 +109,10 @@ static int run(const AttnArgs& base, const MiPagedCache* cache, int D, float sca
   p.groups = a.groups;
   const long long most = max_query_len < p.T ? max_query_len : p.T;
   p.tile_rows = a.tiles || most * p.G > 32 ? 32 : most < 1 ? p.G : (int)(most * p.G);
-  p.many_parts = (long long)a.groups > 16LL * p.B * p.Hkv;
+  p.many_parts = a.tiles || (long long)a.groups > 16LL * p.B * p.Hkv;          // with tiles beside them hardly any sequence is here
   p.wide = ((long long)p.T * p.G / 32 + p.B) * p.Hkv * ((long long)p.width * cache->page_size / 32 + 8) >= 1LL << 31;
   p.slots = a.slots;
-  p.splits = a.splits;
+  p.shares = a.shares;
   if (a.tiles) {
     p.part = (float*)((char*)workspace + a.rows_bytes);
     const int r = launch_attn_tiles(p, D, act_dtype, st);

@@ -34,9 +34,9 @@ struct AttnArgs {
   int T, B, Hq, Hkv, G, page, width, pages;
   int window, sinks, tree_words;         // window 0: none
   float c;
-  int groups, tile_rows;       // rows kernel: workgroups, rows of a tile at most
+  int groups, tile_rows;       // rows kernel: workgroups; rows of a tile, as the caller says
   bool wide, many_parts;       // its work counts 2^31 blocks or more; a tile is in many parts
-  int slots, splits;           // tiles kernel
+  int slots, shares;           // tiles kernel: a workgroup per tile (slots of them), or in that many equal shares
   int rows_from;               // sequences with that many rows (tokens x G) or more belong to the tiles kernel
 };
 
@@ -314,9 +314,12 @@ struct AttnRows {
       const float to = moves ? top[n] : m[n], a = moves ? __builtin_amdgcn_exp2f(m[n] - to) : 1.f;
       l[n] *= a;
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d) {
+        if constexpr (D == 256) asm volatile("" : "+a"(o[n][d]));          // accumulation registers up to here: not all copied in every step
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[n][d][i] *= a;
+        if constexpr (D == 256) asm volatile("" : "+a"(o[n][d]));
+      }
       m[n] = to;
     }
   }
@@ -427,6 +430,118 @@ struct AttnRows {
   }
 };
 
+// ---- equal shares of the work -------------------------------------------------------------------
+// All blocks of KEYS keys of all (sequence, tile of ROWS rows, kv head) in a row, each of these with ITEM blocks more for what beginning it costs, are cut
+// into equal shares, one per workgroup, whatever the sequences' lengths are.  A tile whose blocks all lie in one share is finished there; of the
+// others a workgroup has at most one that it continues and one that it begins: two parts, unscaled fp32 sums with their m and l, which a second launch
+// joins.  FEW: of the sequences with fewer than rows_from rows; otherwise of the others.  Num: int where all work counts less than 2^31 blocks.
+template <int ROWS, int KEYS, int ITEM, bool FEW, class Num>
+struct Shares {
+  // How many tiles a sequence has here, and how many blocks each of them
+  struct Seq { AttnSeq s; AttnRange r; int tiles; };
+  static __device__ __forceinline__ Seq seq(const AttnArgs& p, int b) {
+    Seq x;
+    x.s = attn_seq(p, b);
+    x.r = attn_range<KEYS>(p, x.s, 0, x.s.n - 1);
+    x.r.blocks = max(x.r.blocks, 1);                   // a row that sees nothing is written too
+    const int rows = x.s.n * p.G;
+    x.tiles = FEW == (rows >= p.rows_from) ? 0 : (rows + ROWS - 1) / ROWS;
+    return x;
+  }
+  static __device__ __forceinline__ Num work(const AttnArgs& p, const Seq& x) { return (Num)x.tiles * p.Hkv * (x.r.blocks + ITEM); }
+
+  static __device__ __forceinline__ int from_lane(int v, int lane) { return __shfl(v, lane, 64); }
+  static __device__ __forceinline__ long long from_lane(long long v, int lane) {
+    return (long long)(uint32_t)__shfl((int)v, lane, 64) | (long long)__shfl((int)(v >> 32), lane, 64) << 32;
+  }
+
+  // The same for all lanes: the tiles kernel's addresses have to be scalars, the rows kernel has none to spare.
+  static __device__ __forceinline__ int uniform(int v) { return FEW ? v : __builtin_amdgcn_readfirstlane(v); }
+  static __device__ __forceinline__ long long uniform(long long v) {
+    if (FEW) return v;
+    return (long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) | (long long)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
+  }
+
+  // Every wavefront finds its share by itself.
+  Num incl, before, total, share;                      // work up to, and in front of, this lane's sequences
+  int per;
+  __device__ __forceinline__ void plan(const AttnArgs& p, int groups) {
+    const int lane = threadIdx.x & 63;
+    per = (p.B + 63) / 64;
+    Num mine = 0;
+    for (int i = 0; i < per; ++i) {
+      const int b = lane * per + i;
+      if (b < p.B) mine += work(p, seq(p, b));
+    }
+    incl = mine;
+    for (int d = 1; d < 64 && d < p.B; d <<= 1) {
+      const Num up = from_lane(incl, lane >= d ? lane - d : lane);
+      if (lane >= d) incl += up;
+    }
+    before = incl - mine;
+    total = uniform(from_lane(incl, (p.B - 1) / per)); // the last lane with sequences; those behind it have not added all up
+    share = uniform((total + groups - 1) / groups);
+  }
+  // Blocks begin .. end - 1 of the work are workgroup w's; none: begin = end
+  __device__ __forceinline__ void of(int w, Num& begin, Num& end) const {
+    begin = uniform(share == 0 || (Num)w > total / share ? total : share * (Num)w);
+    end = uniform(total - begin < share ? total : begin + share);
+  }
+  // The sequence with block `at` of the work, and the place of the block in it.  at < total.
+  __device__ __forceinline__ void find(const AttnArgs& p, Num at, int& b, Num& in) const {
+    const int owner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(at < incl));
+    Num rest = at - from_lane(before, owner);
+    b = owner * per;
+    for (; per > 1 && b + 1 < p.B; ++b) {
+      const Num n = work(p, seq(p, b));
+      if (rest < n) break;
+      rest -= n;
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    in = uniform(rest);
+  }
+  struct Item { int tile, head, rows, unit; };         // unit: of the tile; its first ITEM are none of its blocks
+  static __device__ __forceinline__ Item item(const AttnArgs& p, const Seq& x, Num in) {
+    const int each = x.r.blocks + ITEM;
+    const int n = __builtin_amdgcn_readfirstlane((int)(in / each));
+    Item y;
+    y.unit = __builtin_amdgcn_readfirstlane((int)(in - (Num)n * each));
+    y.tile = n / p.Hkv;
+    y.head = n - y.tile * p.Hkv;
+    y.rows = min(ROWS, x.s.n * p.G - y.tile * ROWS);
+    return y;
+  }
+  // How many parts are to be joined at the cut in front of share w, at `at`: those of the tile whose blocks it goes through, if it is the first that does
+  __device__ __forceinline__ int parts_at(int w, Num at, const Seq& x, const Item& y) const {
+    const Num begin = at - y.unit + ITEM;              // of the tile's blocks
+    if (at <= begin || ((Num)w - 1) * share > begin) return 0;
+    return 1 + (int)((begin + x.r.blocks - 1) / share - (w - 1));
+  }
+  // Behind what a workgroup did of a sequence (`in`): on to the next one with work
+  static __device__ __forceinline__ void advance(const AttnArgs& p, const Seq& x, bool more, int& b, Num& in) {
+    if (in < work(p, x)) return;
+    in = 0;
+    do ++b;
+    while (b + 1 < p.B && more && work(p, seq(p, b)) == 0);
+  }
+};
+
+// Parts: two per workgroup, the one that it continues and the one that it begins; ROWS x D sums, then m and l.  Behind all of them, for the cut in front of
+// each share, how many parts are to be joined there (0: none), and the tile.
+template <int D, int ROWS> constexpr int kPart = ROWS * (D + 2);
+template <int D, int ROWS> __device__ __forceinline__ float* attn_part(const AttnArgs& p, int w, bool begins) {
+  return p.part + ((size_t)w * 2 + begins) * kPart<D, ROWS>;
+}
+template <int D, int ROWS> __device__ __forceinline__ i32x4* attn_cuts(const AttnArgs& p, int groups) {
+  return (i32x4*)(p.part + (size_t)groups * 2 * kPart<D, ROWS>);
+}
+constexpr long long attn_parts_bytes(int groups, int D, int rows) { return (long long)groups * (2LL * rows * (D + 2) * 4 + 16); }
+// Row `row` of a sequence's kv head in out
+__device__ __forceinline__ long long attn_row(const AttnArgs& p, int q0, int head, int row) {
+  const int t = row / p.G;
+  return (long long)(q0 + t) * p.Hq + head * p.G + row - t * p.G;
+}
+
 // ---- joining parts ------------------------------------------------------------------------------
 // A workgroup of THREADS threads makes `rows` rows of out from `parts` parts of each: sums(i, row) points to the D sums of part i, ml(i, row)
 // to its m and l (m = -inf: the part has no sums), to(row) to the row of out.  A thread has four columns of a row; where threads are left over they
@@ -507,9 +622,33 @@ __device__ __forceinline__ void attn_join(int rows, int parts, Sums sums, Ml ml,
   }
 }
 
+// Workgroup w, y joins rows 8 y .., and every 8 gridDim.y further, of the tile that the cut in front of share w + 1 goes through.
+template <class Act, int D, int ROWS, int THREADS>
+__global__ __launch_bounds__(THREADS) void attn_join_kernel(const AttnArgs p, int groups) {
+  const int w = blockIdx.x + 1;
+  const i32x4 cut = attn_cuts<D, ROWS>(p, groups)[w];  // parts, first token, tile, kv head and rows
+  const int rows = cut[3] & 511;
+  if (!cut[0]) return;
+  // the first part is the one that share w - 1 began, the others those that a share continued
+  auto part = [&](int i) { return attn_part<D, ROWS>(p, w - 1 + i, i == 0); };
+  for (int row0 = blockIdx.y * kJoinRows; row0 < rows; row0 += gridDim.y * kJoinRows)
+    attn_join<Act, D, THREADS>(
+        min(kJoinRows, rows - row0), cut[0], [&](int i, int row) { return part(i) + (row0 + row) * D; },
+        [&](int i, int row) { return part(i) + ROWS * D + 2 * (row0 + row); },
+        [&](int row) { return (typename Act::elem*)p.out + attn_row(p, cut[1], cut[3] >> 9, cut[2] * ROWS + row0 + row) * D; });
+}
+template <class Act, int D, int ROWS>
+static inline int launch_join(const AttnArgs& p, int groups, int rows, bool many_parts, hipStream_t st) {
+  if (groups == 1) return MI_OK;
+  const dim3 grid(groups - 1, (rows + kJoinRows - 1) / kJoinRows);
+  if (many_parts) attn_join_kernel<Act, D, ROWS, 1024><<<grid, 1024, 0, st>>>(p, groups);
+  else attn_join_kernel<Act, D, ROWS, 256><<<grid, 256, 0, st>>>(p, groups);
+  return launch_status();
+}
+
+constexpr int kFewRows = 32;                          // a tile of the rows kernel
 int launch_attn_rows(const AttnArgs& p, int D, int act_dtype, hipStream_t st);       // and what joins the parts
 int launch_attn_tiles(const AttnArgs& p, int D, int act_dtype, hipStream_t st);
-long long attn_rows_bytes(int groups, int D);
 constexpr int attn_tile_rows(int D) { return D == 256 ? 128 : 256; }
 
 }  // namespace qlin

@@ -6,8 +6,8 @@
 // 256); keys come two blocks ahead (three), values one.  Where pages hold whole groups of 8 places (GROUPS), the keys that a wavefront loads
 // lie on one page: their address is a scalar.
 //
-// Where there are few tiles, their keys are cut into `splits` parts; a second launch joins them.  Tiles of the last tokens, which see
-// the most keys, go first; the kv heads go round the XCDs, so that the tiles of a head share its keys in L2.
+// Long prompts have a workgroup per tile: tiles of the last tokens, which see the most keys, go first, and the kv heads go round the XCDs, so that
+// the tiles of a head share its keys in L2.  Few tokens over long contexts are done in equal shares instead.
 //
 // Bound: the matrix cores; for a few hundred rows HBM.
 #include "attention.hpp"
@@ -65,28 +65,16 @@ __device__ __forceinline__ bool tile_at(const AttnArgs& p, int slot, Tile& x) {
   return true;
 }
 
-// Parts: sums [splits][T Hq][D], then m and l [splits][T Hq][2]
-__device__ __forceinline__ float* part_sums(const AttnArgs& p, int D, int split, long long row) {
-  return p.part + ((long long)split * p.T * p.Hq + row) * D;
-}
-__device__ __forceinline__ float* part_ml(const AttnArgs& p, int D, int split, long long row) {
-  return p.part + (long long)p.splits * p.T * p.Hq * D + ((long long)split * p.T * p.Hq + row) * 2;
-}
-
+// Blocks first .. last - 1 of a tile, by a whole workgroup.  part: where sums, m and l go; null: the rows of out are finished.
 template <class Act, int D, bool GROUPS>
-__global__ __launch_bounds__(64 * TilesCfg<D>::NW) __attribute__((amdgpu_waves_per_eu(TilesCfg<D>::WAVES, TilesCfg<D>::WAVES)))
-void attn_tiles_kernel(const AttnArgs p) {
+__device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int head, int first, int last, float* part) {
   using C = TilesCfg<D>;
   constexpr int KEYS = C::KEYS, NW = C::NW, OWN = KEYS / NW, AHEAD = C::AHEAD;   // OWN: rows of a block that a wavefront loads
   static_assert(OWN == 8 && NW <= 8, "a group of 8 places per wavefront");
   using Rows = AttnRows<Act, D, 32, 1>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv, split = rest % p.splits, slot = p.slots - 1 - rest / p.splits;
-  Tile x;
-  if (!tile_at<C::ROWS, KEYS>(p, slot, x)) return;
   const int32_t* table = p.table + (size_t)x.b * p.width;
-  const int first = (int)((long long)x.r.blocks * split / p.splits), last = (int)((long long)x.r.blocks * (split + 1) / p.splits);
 
   // the wavefront's rows wr0 .. wr1 of the sequence, tokens t0 .. t1
   const int wr0 = x.row0 + wave * 32, wr1 = min(wr0 + 32, x.row0 + x.rows) - 1;
@@ -120,12 +108,13 @@ void attn_tiles_kernel(const AttnArgs p) {
   // Blocks `inner` .. inner + inners - 1 hold keys that all rows of the tile see; where no page of the call is outside the cache nothing is looked up for
   // them but the page.
   const int tile0 = x.row0 / p.G, tile1 = (x.row0 + x.rows - 1) / p.G;
-  int inner = 0, inners = 0;
+  int inner = 0, inners = 0, inners_then = 0;          // then: when all pages are known to be inside
   if constexpr (GROUPS) {
     const int from = max(x.r.lo, p.window ? x.s.first + tile1 - p.window + 1 : 0), to = p.tree ? min(x.r.hi, x.s.first) : min(x.r.hi, x.s.first + tile0 + 1);
     inner = max(x.r.head + (max(from - x.r.from, 0) + KEYS - 1) / KEYS, first);
-    inners = max(min(x.r.head + (to - x.r.from) / KEYS, last) - inner, 0);
-    if (to <= x.r.from) inners = 0;
+    if (to > x.r.from) inners_then = max(min(x.r.head + (to - x.r.from) / KEYS, last) - inner, 0);
+  }
+  auto pages_wrong = [&]() {
     bool wrong = false;
     auto scan = [&](int a, int b) {                    // the pages of keys a .. b - 1
       if (a < b)
@@ -133,12 +122,8 @@ void attn_tiles_kernel(const AttnArgs p) {
     };
     scan(first * KEYS, min(min(last, x.r.head) * KEYS, min(p.sinks, x.r.hi)));
     scan(max(x.r.lo, attn_key<KEYS>(x.r, max(first, x.r.head))), min(x.r.hi, attn_key<KEYS>(x.r, last - 1) + KEYS));
-    wrong = __builtin_amdgcn_ballot_w64(wrong) != 0;
-    if (lane == 0) bad[wave] = wrong;
-    lds_barrier();
-    if (__builtin_amdgcn_ballot_w64(lane < NW && bad[lane & 7])) inners = 0;
-    lds_barrier();
-  }
+    return __builtin_amdgcn_ballot_w64(wrong) != 0;
+  };
   const int inner_key = x.r.from + (inner - x.r.head) * KEYS;
   auto is_inner = [&](int i) { return GROUPS && (uint32_t)(i - inner) < (uint32_t)inners; };
   int page = 0;                                        // GROUPS: of the block whose place comes next
@@ -243,11 +228,18 @@ void attn_tiles_kernel(const AttnArgs p) {
     typename Rows::Scores s0, s1;                      // of the two steps of a block (one: s0)
     typename Rows::Keys f;
     float top[1];
+    if constexpr (GROUPS) {
+      const bool wrong = pages_wrong();
+      if (lane == 0) dirty[wave] = wrong;
+    }
     wait_loads<0>();
     there[AHEAD] = place(first + AHEAD, AHEAD & 1, at[AHEAD - 1]);
     if constexpr (GROUPS) lookup(first + AHEAD + 1, 0);
     lds_barrier();
-    if constexpr (GROUPS) there[0] = keys_there(first);
+    if constexpr (GROUPS) {
+      if (!__builtin_amdgcn_ballot_w64(lane < NW && dirty[lane & 7])) inners = inners_then;
+      there[0] = keys_there(first);
+    }
     bool full = full_of(first, there[0]);
     auto follow = [&](typename Rows::Scores& s, bool all, int i, uint64_t keys, int half) __attribute__((always_inline)) {
       if (!all) a.hide(s, mask_of(i, keys, half));
@@ -313,6 +305,7 @@ void attn_tiles_kernel(const AttnArgs p) {
     }
   }
 
+  wait_loads<0>();                                     // nothing is on its way to LDS any more
   // Values that are no numbers, where zeros stood in for them and some row sees them: each goes to the rows that do, from the cache itself.
   if (first < last) {
     if (lane == 0) dirty[wave] = spoilt;
@@ -336,11 +329,10 @@ void attn_tiles_kernel(const AttnArgs p) {
   const Halves ls = both_halves(a.l[0]);
   const float l = ls.low + ls.high;
   if (!has) return;
-  const long long row = (long long)(x.s.q0 + t) * p.Hq + head * p.G + r - t * p.G;
-  if (p.splits == 1) {
+  if (!part) {
     const float f = l == 0.f ? 0.f : 1.f / l;
     typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
-    typename Act::elem* to = (typename Act::elem*)p.out + row * D + (lane >> 5) * 4;
+    typename Act::elem* to = (typename Act::elem*)p.out + attn_row(p, x.s.q0, head, r) * D + (lane >> 5) * 4;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -352,9 +344,9 @@ void attn_tiles_kernel(const AttnArgs p) {
       }
     return;
   }
-  if (lane < 32) *(f32x2*)part_ml(p, D, split, row) = f32x2{a.m[0], l};
-  if (first == last) return;                           // m = -inf: the sums are not read
-  float* to = part_sums(p, D, split, row) + (lane >> 5) * 4;
+  const int row = r - x.row0;
+  if (lane < 32) *(f32x2*)(part + C::ROWS * D + 2 * row) = f32x2{a.m[0], l};
+  float* to = part + row * D + (lane >> 5) * 4;
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -362,43 +354,71 @@ void attn_tiles_kernel(const AttnArgs p) {
       *(f32x4*)(to + d * 32 + i * 2) = f32x4{a.o[0][d][i], a.o[0][d][i + 1], a.o[0][d][i + 2], a.o[0][d][i + 3]};
 }
 
-// A workgroup per 8 rows of a slot and kv head.
-template <class Act, int D, int THREADS>
-__global__ __launch_bounds__(THREADS) void attn_tiles_join_kernel(const AttnArgs p) {
+template <class Act, int D, bool GROUPS>
+__global__ __launch_bounds__(64 * TilesCfg<D>::NW) __attribute__((amdgpu_waves_per_eu(TilesCfg<D>::WAVES, TilesCfg<D>::WAVES)))
+void attn_tiles_kernel(const AttnArgs p) {
   using C = TilesCfg<D>;
-  constexpr int PIECES = C::ROWS / kJoinRows;
-  const int row0 = blockIdx.x % PIECES * kJoinRows, rest = blockIdx.x / PIECES, head = rest % p.Hkv, slot = rest / p.Hkv;
   Tile x;
-  if (!tile_at<C::ROWS, C::KEYS>(p, slot, x) || row0 >= x.rows) return;
-  auto row_of = [&](int row) {
-    const int r = x.row0 + row0 + row, t = r / p.G;
-    return (long long)(x.s.q0 + t) * p.Hq + head * p.G + r - t * p.G;
-  };
-  attn_join<Act, D, THREADS>(min(kJoinRows, x.rows - row0), p.splits, [&](int i, int row) { return part_sums(p, D, i, row_of(row)); },
-                             [&](int i, int row) { return part_ml(p, D, i, row_of(row)); },
-                             [&](int row) { return (typename Act::elem*)p.out + row_of(row) * D; });
+  if (!tile_at<C::ROWS, C::KEYS>(p, p.slots - 1 - (int)(blockIdx.x / p.Hkv), x)) return;
+  tile_piece<Act, D, GROUPS>(p, x, blockIdx.x % p.Hkv, 0, x.r.blocks, nullptr);
+}
+
+// In equal shares.  All tiles of a sequence have the blocks that any of its tokens sees.
+template <class Act, int D, bool GROUPS>
+__global__ __launch_bounds__(64 * TilesCfg<D>::NW) __attribute__((amdgpu_waves_per_eu(TilesCfg<D>::WAVES, TilesCfg<D>::WAVES)))
+void attn_tiles_shared_kernel(const AttnArgs p) {
+  using C = TilesCfg<D>;
+  constexpr int kItem = 8;
+  using Work = Shares<C::ROWS, C::KEYS, kItem, false, long long>;
+  Work shares;
+  shares.plan(p, p.shares);
+  long long at, end, in;
+  shares.of(blockIdx.x, at, end);
+  i32x4* cut = attn_cuts<D, C::ROWS>(p, p.shares) + blockIdx.x;
+  if (at >= end) {
+    if (threadIdx.x == 0) *cut = i32x4{};
+    return;
+  }
+  int b;
+  shares.find(p, at, b, in);
+  for (bool starts = true; at < end; starts = false) {
+    const typename Work::Seq s = Work::seq(p, b);
+    const typename Work::Item y = Work::item(p, s, in);
+    if (starts && threadIdx.x == 0) *cut = i32x4{shares.parts_at(blockIdx.x, at, s, y), s.s.q0, y.tile, y.head << 9 | y.rows};
+    const int take = __builtin_amdgcn_readfirstlane((int)min((long long)(s.r.blocks + kItem - y.unit), end - at));
+    const int first = max(y.unit - kItem, 0), last = y.unit + take - kItem;
+    at += take;
+    in += take;
+    if (last > first) {
+      const Tile x{s.s, s.r, b, y.tile * C::ROWS, y.rows};
+      const bool whole = first == 0 && last == s.r.blocks;
+      tile_piece<Act, D, GROUPS>(p, x, y.head, first, last, whole ? nullptr : attn_part<D, C::ROWS>(p, blockIdx.x, first == 0));
+      lds_barrier();                                   // before LDS is used for the next tile
+    }
+    Work::advance(p, s, at < end, b, in);
+  }
 }
 
 template <class Act, int D, bool GROUPS>
 static int launch_tiles(const AttnArgs& p, hipStream_t st) {
-  static std::atomic<unsigned long long> raised{0};
-  const int rc = int8_raise_lds(attn_tiles_kernel<Act, D, GROUPS>, raised, TilesCfg<D>::LDS);
-  if (rc != MI_OK) return rc;
-  attn_tiles_kernel<Act, D, GROUPS><<<(unsigned)(p.slots * p.splits * p.Hkv), 64 * TilesCfg<D>::NW, TilesCfg<D>::LDS, st>>>(p);
+  static std::atomic<unsigned long long> raised{0}, raised_shared{0};
+  constexpr int THREADS = 64 * TilesCfg<D>::NW, LDS = TilesCfg<D>::LDS;
+  if (p.shares) {
+    const int rc = int8_raise_lds(attn_tiles_shared_kernel<Act, D, GROUPS>, raised_shared, LDS);
+    if (rc != MI_OK) return rc;
+    attn_tiles_shared_kernel<Act, D, GROUPS><<<p.shares, THREADS, LDS, st>>>(p);
+  } else {
+    const int rc = int8_raise_lds(attn_tiles_kernel<Act, D, GROUPS>, raised, LDS);
+    if (rc != MI_OK) return rc;
+    attn_tiles_kernel<Act, D, GROUPS><<<(unsigned)(p.slots * p.Hkv), THREADS, LDS, st>>>(p);
+  }
   return launch_status();
 }
 template <class Act, int D>
 static int launch(const AttnArgs& p, hipStream_t st) {
-  // a group's rows: 32-bit distances in bytes
-  const bool groups = p.page % 8 == 0 && p.row16 < 1u << 24;
+  const bool groups = p.page % 8 == 0 && p.row16 < 1u << 24;     // a group's rows: 32-bit distances in bytes
   const int rc = groups ? launch_tiles<Act, D, true>(p, st) : launch_tiles<Act, D, false>(p, st);
-  if (rc != MI_OK) return rc;
-  if (p.splits > 1) {
-    const unsigned grid = (unsigned)(p.slots * p.Hkv * (TilesCfg<D>::ROWS / kJoinRows));
-    if (p.splits > 16) attn_tiles_join_kernel<Act, D, 1024><<<grid, 1024, 0, st>>>(p);
-    else attn_tiles_join_kernel<Act, D, 256><<<grid, 256, 0, st>>>(p);
-  }
-  return launch_status();
+  return rc != MI_OK || !p.shares ? rc : launch_join<Act, D, TilesCfg<D>::ROWS>(p, p.shares, TilesCfg<D>::ROWS, false, st);
 }
 
 int launch_attn_tiles(const AttnArgs& p, int D, int act_dtype, hipStream_t st) {
