@@ -439,14 +439,20 @@ template <int ROWS, int KEYS, int ITEM, bool FEW, class Num>
 struct Shares {
   // How many tiles a sequence has here, and how many blocks each of them
   struct Seq { AttnSeq s; AttnRange r; int tiles; };
-  static __device__ __forceinline__ Seq seq(const AttnArgs& p, int b) {
+  static __device__ __forceinline__ Seq seq_of(const AttnArgs& p, const AttnSeq& s) {
     Seq x;
-    x.s = attn_seq(p, b);
+    x.s = s;
     x.r = attn_range<KEYS>(p, x.s, 0, x.s.n - 1);
     x.r.blocks = max(x.r.blocks, 1);                   // a row that sees nothing is written too
     const int rows = x.s.n * p.G;
     x.tiles = FEW == (rows >= p.rows_from) ? 0 : (rows + ROWS - 1) / ROWS;
     return x;
+  }
+  // b the same for all lanes
+  __device__ __forceinline__ Seq seq(const AttnArgs& p, int b) const {
+    if (per > 1) return seq_of(p, attn_seq(p, b));
+    return seq_of(p, {__builtin_amdgcn_readlane(lanes.q0, b), __builtin_amdgcn_readlane(lanes.n, b), __builtin_amdgcn_readlane(lanes.first, b),
+                      __builtin_amdgcn_readlane(lanes.cap, b)});
   }
   static __device__ __forceinline__ Num work(const AttnArgs& p, const Seq& x) { return (Num)x.tiles * p.Hkv * (x.r.blocks + ITEM); }
 
@@ -465,13 +471,17 @@ struct Shares {
   // Every wavefront finds its share by itself.
   Num incl, before, total, share;                      // work up to, and in front of, this lane's sequences
   int per;
+  AttnSeq lanes;                                       // per = 1: this lane's sequence
   __device__ __forceinline__ void plan(const AttnArgs& p, int groups) {
     const int lane = threadIdx.x & 63;
     per = (p.B + 63) / 64;
     Num mine = 0;
+    lanes = AttnSeq{};
     for (int i = 0; i < per; ++i) {
       const int b = lane * per + i;
-      if (b < p.B) mine += work(p, seq(p, b));
+      if (b >= p.B) continue;
+      lanes = attn_seq(p, b);
+      mine += work(p, seq_of(p, lanes));
     }
     incl = mine;
     for (int d = 1; d < 64 && d < p.B; d <<= 1) {
@@ -518,7 +528,7 @@ struct Shares {
     return 1 + (int)((begin + x.r.blocks - 1) / share - (w - 1));
   }
   // Behind what a workgroup did of a sequence (`in`): on to the next one with work
-  static __device__ __forceinline__ void advance(const AttnArgs& p, const Seq& x, bool more, int& b, Num& in) {
+  __device__ __forceinline__ void advance(const AttnArgs& p, const Seq& x, bool more, int& b, Num& in) const {
     if (in < work(p, x)) return;
     in = 0;
     do ++b;

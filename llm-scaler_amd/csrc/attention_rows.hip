@@ -34,7 +34,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
   shares.find(p, at, b, in);
 
   for (bool starts = true; at < end; starts = false) {
-    const typename Work::Seq x = Work::seq(p, b);
+    const typename Work::Seq x = shares.seq(p, b);
     const typename Work::Item y = Work::item(p, x, in);
     if (starts) {
       const int parts = shares.parts_at(blockIdx.x, at, x, y);
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
         }
       }
     }
-    Work::advance(p, x, at < end, b, in);
+    shares.advance(p, x, at < end, b, in);
   }
 }
 

@@ -382,7 +382,7 @@ void attn_tiles_shared_kernel(const AttnArgs p) {
   int b;
   shares.find(p, at, b, in);
   for (bool starts = true; at < end; starts = false) {
-    const typename Work::Seq s = Work::seq(p, b);
+    const typename Work::Seq s = shares.seq(p, b);
     const typename Work::Item y = Work::item(p, s, in);
     if (starts && threadIdx.x == 0) *cut = i32x4{shares.parts_at(blockIdx.x, at, s, y), s.s.q0, y.tile, y.head << 9 | y.rows};
     const int take = __builtin_amdgcn_readfirstlane((int)min((long long)(s.r.blocks + kItem - y.unit), end - at));
@@ -395,7 +395,7 @@ void attn_tiles_shared_kernel(const AttnArgs p) {
       tile_piece<Act, D, GROUPS>(p, x, y.head, first, last, whole ? nullptr : attn_part<D, C::ROWS>(p, blockIdx.x, first == 0));
       lds_barrier();                                   // before LDS is used for the next tile
     }
-    Work::advance(p, s, at < end, b, in);
+    shares.advance(p, s, at < end, b, in);
   }
 }
 

@@ -611,8 +611,7 @@ Span span(const Tensor& t) {                           // from the first byte to
   const char* p = (const char*)t.data_ptr();
   return {p, p + (last + 1) * t.element_size()};
 }
-void attn_apart(const char* who, const Tensor& out, const char* out_name, const Tensor& t, const char* name) {
-  const Span a = span(out), b = span(t);
+void attn_apart(const char* who, const Span& a, const char* out_name, const Span& b, const char* name) {
   REFUSE_UNLESS(!a.from || !b.from || a.from >= b.to || b.from >= a.to, out_name, " must not overlap ", name);
 }
 void attn_device(const char* who, const Tensor& x, const Tensor& t, const char* name) {
@@ -729,17 +728,19 @@ Tensor qk_norm_rope(const Tensor& qkv, const c10::optional<Tensor>& qw, const c1
     int8_device(who, qkv, *slots, "slot_mapping");
     REFUSE_UNLESS(slots->scalar_type() == at::kLong && slots->numel() == T, "slot_mapping must be int64 with T=", T, " entries");
   }
+  const std::pair<Span, const char*> in[] = {{qw.has_value() ? span(*qw) : Span{}, "q_weight"}, {kw.has_value() ? span(*kw) : Span{}, "k_weight"},
+                                            {span(table), "cos_sin"}, {span(positions), "positions"},
+                                            {slots.has_value() ? span(*slots) : Span{}, "slot_mapping"}};
+  const Span rows = span(qkv);
+  Span to[4] = {};
   for (int i = 0; i < 4; ++i) {
     if (!outs[i]) continue;
     attn_apart_inside(who, *outs[i], names[i]);
-    if (!(i == 0 && q_own) && !(i == 1 && k_own)) attn_apart(who, *outs[i], names[i], qkv, "qkv");
-    if (qw.has_value()) attn_apart(who, *outs[i], names[i], *qw, "q_weight");
-    if (kw.has_value()) attn_apart(who, *outs[i], names[i], *kw, "k_weight");
-    attn_apart(who, *outs[i], names[i], table, "cos_sin");
-    attn_apart(who, *outs[i], names[i], positions, "positions");
-    if (slots.has_value()) attn_apart(who, *outs[i], names[i], *slots, "slot_mapping");
+    to[i] = span(*outs[i]);
+    if (!(i == 0 && q_own) && !(i == 1 && k_own)) attn_apart(who, to[i], names[i], rows, "qkv");
+    for (const auto& t : in) attn_apart(who, to[i], names[i], t.first, t.second);
     for (int j = 0; j < i; ++j)                        // keys and values against each other: in paged_cache
-      if (outs[j] && !(i == 1 && j == 0 && q_own && k_own) && !(i == 3 && j == 2)) attn_apart(who, *outs[i], names[i], *outs[j], names[j]);
+      if (!(i == 1 && j == 0 && q_own && k_own) && !(i == 3 && j == 2)) attn_apart(who, to[i], names[i], to[j], names[j]);
   }
   if (!T) return q;
   const On on(qkv);
@@ -780,12 +781,13 @@ AttnCall attn_call(const char* who, const Tensor& q, const Tensor& kc, const Ten
   int8_aligned(who, out, "output");
   REFUSE_UNLESS(scale > 0 && scale < 1e30, "scale must be positive, got ", scale);
   REFUSE_UNLESS(max_query_len >= 0 && max_seq_len >= 0, "max_query_len and max_seq_len must not be negative");
-  attn_apart(who, out, "output", q, "query");
-  attn_apart(who, out, "output", kc, "key_cache");
-  attn_apart(who, out, "output", vc, "value_cache");
-  attn_apart(who, out, "output", table, "block_table");
-  attn_apart(who, out, "output", seq, "seq_lens");
-  attn_apart(who, out, "output", cu, "cu_seqlens_q");
+  const Span to = span(out);
+  attn_apart(who, to, "output", span(q), "query");
+  attn_apart(who, to, "output", span(kc), "key_cache");
+  attn_apart(who, to, "output", span(vc), "value_cache");
+  attn_apart(who, to, "output", span(table), "block_table");
+  attn_apart(who, to, "output", span(seq), "seq_lens");
+  attn_apart(who, to, "output", span(cu), "cu_seqlens_q");
   a.T = (int)T;
   a.B = (int)B;
   a.Hq = (int)Hq;
@@ -825,7 +827,7 @@ Tensor tree_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const
   REFUSE_UNLESS(mask.scalar_type() == at::kLong && mask.dim() == 2 && mask.size(0) == a.T && mask.size(1) >= 1 && mask.size(1) <= 1 << 20,
                 "tree_mask must be int64 [T, words], got ", mask.scalar_type(), " ", mask.sizes());
   REFUSE_UNLESS(max_query_len <= 64 * mask.size(1), "tree_mask has ", mask.size(1), " words for up to ", max_query_len, " drafted tokens");
-  attn_apart(who, out, "output", mask, "tree_mask");
+  attn_apart(who, span(out), "output", span(mask), "tree_mask");
   if (!a.T || !a.B) return out;
   const On on(q);
   long long bytes = 0;
