@@ -20,7 +20,7 @@ namespace qlin {
 
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) short i16x4;
-typedef __attribute__((ext_vector_type(8))) short i16x8;
+typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
 
 struct AttnArgs {
   const void *q, *k, *v;
@@ -101,20 +101,21 @@ __device__ __forceinline__ uint32_t attn_place(const AttnArgs& p, int page, int 
   return (uint32_t)page * p.page16 + (uint32_t)(key - attn_page_of(p, key) * p.page) * p.row16 + (uint32_t)head * p.head16;
 }
 
-// Bit i: a token sees key kb + i.  The token stands at place s.first + t (negative: before the cache's start), its tree bits in `tree`.
+// Bit i: a token sees key kb + i.  The token stands at place first + t (negative: before the cache's start), its tree bits in `tree`.
 __device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
-__device__ __forceinline__ uint64_t attn_sees(const AttnArgs& p, int first, int t, const int64_t* tree, int kb) {
+__device__ __forceinline__ uint32_t low_bits32(int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1; }
+__device__ __forceinline__ uint32_t attn_sees(const AttnArgs& p, int first, int t, const int64_t* tree, int kb) {
   if (p.tree) {
     const int at = kb - first;                         // the drafted token of key kb
-    if (at <= -64) return ~0ull;
-    auto word = [&](int w) { return w >= 0 && w < p.tree_words ? (uint64_t)tree[w] : 0ull; };
-    if (at < 0) return low_bits(-at) | word(0) << -at;
-    const int w = at >> 6, by = at & 63;
-    return word(w) >> by | (by ? word(w + 1) << (64 - by) : 0ull);
+    if (at <= -32) return ~0u;
+    auto word = [&](int w) { return w < 2 * p.tree_words ? ((const uint32_t*)tree)[w] : 0u; };
+    if (at < 0) return low_bits32(-at) | word(0) << -at;
+    const int w = at >> 5, by = at & 31;
+    return word(w) >> by | (by ? word(w + 1) << (32 - by) : 0u);
   }
   const int place = first + t;
-  uint64_t m = low_bits(place - kb + 1);
-  if (p.window) m &= ~low_bits(place - p.window + 1 - kb) | low_bits(p.sinks - kb);
+  uint32_t m = low_bits32(place - kb + 1);
+  if (p.window) m &= ~low_bits32(place - p.window + 1 - kb) | low_bits32(p.sinks - kb);
   return m;
 }
 // Whether every token from t0 to t1 sees all of the N keys from kb on
@@ -177,256 +178,205 @@ struct RowPlaces {
 };
 
 // ---- the rows of a wavefront ------------------------------------------------------------------
-// 32 NQ rows over blocks of N keys, a step at a time: scores (K Q^T), their maximum, weights (exp), and the product with V.
-template <class Act, int D, int N, int NQ>
+// 32 rows over steps of 32 keys: scores (K Q^T), their maximum, weights (exp), and the product with V.
+template <class Act, int D>
 struct AttnRows {
   using v8 = typename Act::v8;
   typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
-  static constexpr int DT = D / 32, KT = N / 32;
+  typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
+  static constexpr int DT = D / 32;
   static constexpr float kRaise = 7.f;
   static constexpr unsigned short EXPONENT = Act::dt == DT_F16 ? 0x7C00 : 0x7F80;
-  struct Scores { f32x16 s[NQ][KT]; };                 // s[n][t][i]: key 32 t + 8 (i / 4) + 4 (lane / 32) + i % 4, row 32 n + lane % 32
-  struct Weights { v8 p[NQ][2 * KT]; };                // p[n][t][e]: key 16 t + 8 (e / 4) + 4 (lane / 32) + e % 4
-  struct Mask { uint64_t of[NQ]; };                    // bit i: row 32 n + lane % 32 sees key i; null where a key is not there
+  struct Weights { v8 p[2]; };                         // p[t][e]: key 16 t + 8 (e / 4) + 4 (lane / 32) + e % 4 of row lane % 32
+  // Operands whose reads of LDS go out long before their products: they stay on their side of a `pin`, everything else may move.
+  struct Keys { v8 k[D / 16]; };
+  struct Values { v8 v[DT]; };
+  static __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0x40E); }
 
-  v8 q[NQ][D / 16];
-  f32x16 o[NQ][DT];            // o[n][t][i]: column 32 t + 8 (i / 4) + 4 (lane / 32) + i % 4
-  float m[NQ], l[NQ];          // m: what a row's exponents are taken from, at most 8 below the largest; l: of this lane's keys
-  int ka, va;                  // where this lane reads K and V of a block
+  v8 q[D / 16];
+  f32x16 o[DT];                // o[t][i]: column 32 t + 8 (i / 4) + 4 (lane / 32) + i % 4 of row lane % 32
+  float m, l;                  // m: what a row's exponents are taken from, at most 8 below the largest; l: of this lane's keys
+  int ka, va;                  // where this lane reads K and V of a step
 
   __device__ __forceinline__ void start() {
     const int lane = threadIdx.x & 63, h = lane >> 5, i = lane & 15;
+    m = -__builtin_inff();
+    l = 0.f;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      m[n] = -__builtin_inff();
-      l[n] = 0.f;
-#pragma unroll
-      for (int t = 0; t < DT; ++t) o[n][t] = f32x16{};
-    }
+    for (int t = 0; t < DT; ++t) o[t] = f32x16{};
     ka = (lane & 31) * 2 * D + ((h ^ k_swizzle<D>(lane & 31)) * 16);
     // keys 4 h + i / 4, columns 16 (lane / 16 % 2) + 4 (i % 4)
     va = (4 * h + (i >> 2)) * 2 * D + (((2 * (lane >> 4 & 1) + (i >> 1 & 1)) ^ v_swizzle<D>(i >> 2)) * 16) + (i & 1) * 8;
   }
-  __device__ __forceinline__ void load_q(int n, const void* row) {         // null: zeros
+  __device__ __forceinline__ void load_q(const void* row) {      // null: zeros
     const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
       u32x4 x = {};
       if (row) x = *(const u32x4*)((const unsigned char*)row + s * 32 + h * 16);
-      q[n][s] = as_v8<v8>(x);
+      q[s] = as_v8<v8>(x);
     }
   }
-  // K of 32 keys (from 32 t of the block at LDS address k) and columns 16 ks ..
-  __device__ __forceinline__ v8 k_operand(uint32_t k, int t, int ks) const {
-    return as_v8<v8>(*in_lds<const u32x4>(k + (ka ^ (ks % 8 * 32)) + ks / 8 * 256 + t * 64 * D));
+  // K of the 32 keys at LDS address k, columns 16 ks ..
+  __device__ __forceinline__ v8 k_operand(uint32_t k, int ks) const {
+    return as_v8<v8>(*in_lds<const u32x4>(k + (ka ^ (ks % 8 * 32)) + ks / 8 * 256));
   }
-  // V^T of 16 keys (from 16 t of the block at LDS address v) and columns 32 d ..: element e is key 4 (lane / 32) + e % 4 + 8 (e / 4)
+  // V^T of 16 keys (from 16 t of those at LDS address v) and columns 32 d ..: element e is key 4 (lane / 32) + e % 4 + 8 (e / 4)
   __device__ __forceinline__ v8 v_operand(uint32_t v, int t, int d) const {
     const uint32_t at = v + (va ^ ((d & 3) * 64)) + (d >> 2) * 256 + t * 32 * D;
     const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(in_lds<i16x4>(at)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(in_lds<i16x4>(at + 16 * D));
     return __builtin_bit_cast(v8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   }
-
-  __device__ __forceinline__ void scores(uint32_t k, Scores& x) const {
-#pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-      for (int t = 0; t < KT; ++t) x.s[n][t] = f32x16{};
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        const v8 a = k_operand(k, t, ks);
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) x.s[n][t] = mfma32(a, q[n][ks], x.s[n][t]);
-      }
-  }
-  // A step of the tiles kernel: weights of the scores x, the product with their values, and the next step's scores y.  Reads of LDS go out long before
-  // their products, keys a step ahead (f: the next step's, then those at k2), values while the scores are made: they stay on their side of a `pin`.
-  struct Keys { v8 k[D / 16]; };
-  struct Values { v8 v[DT]; };
-  static __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0x40E); }
   __device__ __forceinline__ void read_keys(uint32_t k, Keys& f) const {
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) f.k[ks] = k_operand(k, 0, ks);
+    for (int ks = 0; ks < D / 16; ++ks) f.k[ks] = k_operand(k, ks);
   }
   __device__ __forceinline__ void read_values(uint32_t v, int t, Values& f) const {
 #pragma unroll
     for (int d = 0; d < DT; ++d) f.v[d] = v_operand(v, t, d);
   }
-  __device__ __forceinline__ void scores_of(const Keys& f, Scores& y) const {
-    y.s[0][0] = f32x16{};
+
+  // Scores: element i is key 8 (i / 4) + 4 (lane / 32) + i % 4 of row lane % 32
+  __device__ __forceinline__ f32x16 scores(const Keys& f) const {
+    f32x16 x = {};
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) y.s[0][0] = mfma32(f.k[ks], q[0][ks], y.s[0][0]);
+    for (int ks = 0; ks < D / 16; ++ks) x = mfma32(f.k[ks], q[ks], x);
+    return x;
   }
-  __device__ __forceinline__ void step(const Scores& x, uint32_t v, Keys& f, uint32_t k2, float c, Scores& y) {
-    static_assert(NQ == 1 && KT == 1, "a step of 32 keys");
+  // -inf where the row does not see the key.  mask: bit i of this lane's row, null where a key is not there
+  __device__ __forceinline__ void hide(f32x16& x, uint32_t mask) const {
+    const uint32_t bits = mask >> (4 * ((threadIdx.x & 63) >> 5));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t sees = (uint32_t)((int32_t)(bits << (31 - 8 * (i / 4) - i % 4)) >> 31);
+      const float s = x[i];                            // its own variable: a bit cast of an element is one of element 0
+      x[i] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, s) & sees) | (0xFF800000u & ~sees));
+    }
+  }
+  // Makes m fit the scores x.  Sums move to a new m only where an exponent would pass it by 8.  Weights are 2^kRaise times as large, up to 2^15, so that
+  // in fp16 those of a long tail keep their bits (half of the smallest number is 2^-32 of the largest weight).
+  __device__ __forceinline__ void follow(const f32x16& x, float c) {
+    float mx = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+    const Halves y = both_halves(mx);
+    const float top = fmaxf(y.low, y.high) * c;
+    const bool moves = top > m + 8.f;                  // row by row: a row's bits depend on no other row
+    if (!__builtin_amdgcn_ballot_w64(moves)) return;
+    const float to = moves ? top : m, a = moves ? __builtin_amdgcn_exp2f(m - to) : 1.f;
+    l *= a;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      if constexpr (D == 256) asm volatile("" : "+a"(o[d]));     // accumulation registers up to here: not all copied in every step
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] *= a;
+      if constexpr (D == 256) asm volatile("" : "+a"(o[d]));
+    }
+    m = to;
+  }
+  __device__ __forceinline__ void weigh(const f32x16& x, float c, Weights& w) {
+    const float top = m == -__builtin_inff() ? 0.f : m - kRaise;           // first: a row that has seen nothing yet
+    typedef __attribute__((ext_vector_type(2))) typename Act::elem e2;
+    const e2 one = {(typename Act::elem)1.f, (typename Act::elem)1.f};
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w.p[t][e] = Act::from_f32(__builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * t + e], c, -top)));
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const e2 two = {w.p[t][e], w.p[t][e + 1]};
+        if constexpr (Act::dt == DT_F16) sum = __builtin_amdgcn_fdot2(two, one, sum, false);
+        else sum = __builtin_amdgcn_fdot2_f32_bf16(two, one, sum, false);
+      }
+    }
+    l += sum;
+  }
+  // A step of the tiles kernel: weights of the scores x, the product with their values, and the next step's scores.  f: the next step's keys, then
+  // those at k2; the values are read while the scores are made.
+  __device__ __forceinline__ f32x16 step(const f32x16& x, uint32_t v, Keys& f, uint32_t k2, float c) {
     Values va, vb;
     Weights w;
     read_values(v, 0, va);
     pin();
-    scores_of(f, y);
+    const f32x16 y = scores(f);
     read_values(v, 1, vb);
     pin();
     weigh(x, c, w);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[0][d] = mfma32(va.v[d], w.p[0][0], o[0][d]);
+    for (int d = 0; d < DT; ++d) o[d] = mfma32(va.v[d], w.p[0], o[d]);
     read_keys(k2, f);
     pin();
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[0][d] = mfma32(vb.v[d], w.p[0][1], o[0][d]);
-  }
-  __device__ __forceinline__ void hide(Scores& x, const Mask& mask) const {
-    const int h = (threadIdx.x & 63) >> 5;
-#pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        const uint32_t bits = (uint32_t)(mask.of[n] >> (32 * t)) >> (4 * h);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t sees = (uint32_t)((int32_t)(bits << (31 - 8 * (i / 4) - i % 4)) >> 31);
-          const float s = x.s[n][t][i];                // its own variable: a bit cast of an element is one of element 0
-          x.s[n][t][i] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, s) & sees) | (0xFF800000u & ~sees));
-        }
-      }
-  }
-  // c times the largest score of a row
-  __device__ __forceinline__ void largest(const Scores& x, float c, float (&top)[NQ]) const {
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float mx = x.s[n][0][0];
-#pragma unroll
-      for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x.s[n][t][i]);
-      const Halves y = both_halves(mx);
-      top[n] = fmaxf(y.low, y.high) * c;
-    }
-  }
-  // Sums move to a new m only where an exponent would pass it by 8.  Weights are 2^kRaise times as large, up to 2^15, so that in fp16 those of a
-  // long tail keep their bits (half of the smallest number is 2^-32 of the largest weight).
-  __device__ __forceinline__ void follow(const float (&top)[NQ]) {
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const bool moves = top[n] > m[n] + 8.f;          // row by row: a row's bits depend on no other row
-      if (!__builtin_amdgcn_ballot_w64(moves)) continue;
-      const float to = moves ? top[n] : m[n], a = moves ? __builtin_amdgcn_exp2f(m[n] - to) : 1.f;
-      l[n] *= a;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        if constexpr (D == 256) asm volatile("" : "+a"(o[n][d]));          // accumulation registers up to here: not all copied in every step
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[n][d][i] *= a;
-        if constexpr (D == 256) asm volatile("" : "+a"(o[n][d]));
-      }
-      m[n] = to;
-    }
-  }
-  __device__ __forceinline__ void weigh(const Scores& x, float c, Weights& w) {
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const float top = m[n] == -__builtin_inff() ? 0.f : m[n] - kRaise;   // first: a row that has seen nothing yet
-      float sum = 0.f;
-#pragma unroll
-      for (int t = 0; t < 2 * KT; ++t) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          w.p[n][t][e] = Act::from_f32(__builtin_amdgcn_exp2f(__builtin_fmaf(x.s[n][t / 2][8 * (t % 2) + e], c, -top)));
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) sum = add_two(w.p[n][t], e, sum);
-      }
-      l[n] += sum;
-    }
-  }
-  static __device__ __forceinline__ float add_two(v8 p, int e, float sum) {
-    typedef __attribute__((ext_vector_type(2))) typename Act::elem e2;
-    const e2 two = {p[e], p[e + 1]}, one = {(typename Act::elem)1.f, (typename Act::elem)1.f};
-    if constexpr (Act::dt == DT_F16) return __builtin_amdgcn_fdot2(two, one, sum, false);
-    else return __builtin_amdgcn_fdot2_f32_bf16(two, one, sum, false);
+    for (int d = 0; d < DT; ++d) o[d] = mfma32(vb.v[d], w.p[1], o[d]);
+    return y;
   }
   __device__ __forceinline__ void add(uint32_t v, const Weights& w) {
 #pragma unroll
-    for (int t = 0; t < 2 * KT; ++t)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const v8 a = v_operand(v, t, d);
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) o[n][d] = mfma32(a, w.p[n][t], o[n][d]);
-      }
+      for (int d = 0; d < DT; ++d) o[d] = mfma32(v_operand(v, t, d), w.p[t], o[d]);
   }
-  // Zeros in place of infinities and NaN in 8 rows of values in LDS; whether there were any in the rows whose bits `there` has
+
+  // Infinities and NaN among values that a row does not see: 0 times them would not be 0.  They give way to zeros, and go to the rows that see them by
+  // themselves.
+  //
+  // The rows kernel: while the values are read
+  __device__ __forceinline__ void add_hidden(uint32_t v, const Weights& w, uint32_t mask) {
+    u16x8 one = 1;                                     // 0 where a value was not finite
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const u16x8 x = __builtin_bit_cast(u16x8, v_operand(v, t, d)), finite = are_finite(x);
+        one &= finite;
+        o[d] = mfma32(__builtin_bit_cast(v8, x & (0 - finite)), w.p[t], o[d]);
+      }
+    }
+    if (!__builtin_amdgcn_ballot_w64(any_not(one))) return;
+#pragma unroll 1
+    for (int j = 0; j < 32; ++j)
+      add_not_finite(mask >> j & 1, [&](int column) {
+        return *in_lds<const u16x4>(v + j * 2 * D + ((column >> 3) ^ v_swizzle<D>(j)) * 16 + (column & 7) * 2);
+      });
+  }
+  // The tiles kernel: zeros in 8 rows of values in LDS, and whether there were any in the rows whose bits `there` has; the values themselves from the
+  // cache at the end
   template <int PIECES>
   static __device__ __forceinline__ bool clean(uint32_t v, uint32_t there) {
     bool spoilt = false;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
       auto* at = in_lds<u16x8>(v + j * 1024 + (threadIdx.x & 63) * 16);
-      const u16x8 x = *at, finite = __builtin_elementwise_min(EXPONENT - (x & EXPONENT), (u16x8)1);
-      const u32x4 all = __builtin_bit_cast(u32x4, finite);
-      const bool found = (all[0] & all[1] & all[2] & all[3]) != 0x00010001u;
+      const u16x8 x = *at, finite = are_finite(x);
+      const bool found = any_not(finite);
       if (!__builtin_amdgcn_ballot_w64(found)) continue;
       *at = x & (0 - finite);
       spoilt |= found && there >> (j * (512 / D) + (threadIdx.x & 63) / (D / 8)) & 1;
     }
     return __builtin_amdgcn_ballot_w64(spoilt) != 0;
   }
-  // The infinities and NaN of a row of values in memory, where this lane's row sees it
-  __device__ __forceinline__ void add_not_finite(const unsigned char* v, bool sees) {
+  // The infinities and NaN of a row of values, four columns from `column` on at a time, where this lane's row sees it
+  template <class Read>
+  __device__ __forceinline__ void add_not_finite(bool sees, Read read) {
     const int h = (threadIdx.x & 63) >> 5;
-    typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
-    typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {                    // columns 32 d + 8 i + 4 h ..
-        const u16x4 x = *(const u16x4*)(v + (32 * d + 8 * i + 4 * h) * 2);
-        const e4 y = __builtin_bit_cast(e4, x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[0][d][4 * i + e] += sees && (x[e] & EXPONENT) == EXPONENT ? Act::to_f32(y[e]) : 0.f;
-      }
-  }
-  // The same where some row does not see some key: 0 times an infinity or a NaN there would not be 0, so such values go to the rows that see
-  // them by themselves.
-  __device__ __forceinline__ void add_hidden(uint32_t v, const Weights& w, const Mask& mask) {
-    u16x8 one = 1;                                     // 0 where a value was not finite
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int t = 0; t < 2 * KT; ++t) {
-        const u16x8 x = __builtin_bit_cast(u16x8, v_operand(v, t, d));
-        const u16x8 finite = __builtin_elementwise_min(EXPONENT - (x & EXPONENT), (u16x8)1);
-        one &= finite;
-        const v8 a = __builtin_bit_cast(v8, x & (0 - finite));
+      for (int i = 0; i < 4; ++i) {
+        const u16x4 x = read(32 * d + 8 * i + 4 * h);
+        const e4 y = __builtin_bit_cast(e4, x);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) o[n][d] = mfma32(a, w.p[n][t], o[n][d]);
+        for (int e = 0; e < 4; ++e) o[d][4 * i + e] += sees && (x[e] & EXPONENT) == EXPONENT ? Act::to_f32(y[e]) : 0.f;
       }
     }
-    const u32x4 all = __builtin_bit_cast(u32x4, one);
-    if (__builtin_amdgcn_ballot_w64((all[0] & all[1] & all[2] & all[3]) != 0x00010001u)) add_not_finite(v, mask);
   }
-  __device__ __forceinline__ void add_not_finite(uint32_t v, const Mask& mask) {
-    const int h = (threadIdx.x & 63) >> 5;
-    typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
-    typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
-#pragma unroll 1
-    for (int j = 0; j < N; ++j) {
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {                  // columns 32 d + 8 i + 4 h ..
-          const u16x4 x = *in_lds<const u16x4>(v + j * 2 * D + ((4 * d + i) ^ v_swizzle<D>(j)) * 16 + h * 8);
-          const e4 y = __builtin_bit_cast(e4, x);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              o[n][d][4 * i + e] += (mask.of[n] >> j & 1) && (x[e] & EXPONENT) == EXPONENT ? Act::to_f32(y[e]) : 0.f;
-        }
-      }
-    }
+  static __device__ __forceinline__ u16x8 are_finite(u16x8 x) { return __builtin_elementwise_min(EXPONENT - (x & EXPONENT), (u16x8)1); }
+  static __device__ __forceinline__ bool any_not(u16x8 ones) {
+    const u32x4 x = __builtin_bit_cast(u32x4, ones);
+    return (x[0] & x[1] & x[2] & x[3]) != 0x00010001u;
   }
 };
 

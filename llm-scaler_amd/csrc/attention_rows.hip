@@ -15,7 +15,7 @@ template <int D> struct RowsCfg {
 template <class Act, int D, class Num>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, D == 256 ? 1 : 2))) void attn_rows_kernel(const AttnArgs p) {
   using C = RowsCfg<D>;
-  using Rows = AttnRows<Act, D, 32, 1>;
+  using Rows = AttnRows<Act, D>;
   constexpr int LOADS = 2 * C::HALF / 1024, kItem = 3;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int lane = threadIdx.x;
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
       const int t0 = y.tile * 32 / p.G, t1 = (y.tile * 32 + y.rows - 1) / p.G;
       Rows a;
       a.start();
-      a.load_q(0, has ? (const typename Act::elem*)p.q + (x.s.q0 + t) * p.q_token + (y.head * p.G + r - t * p.G) * p.q_head : nullptr);
+      a.load_q(has ? (const typename Act::elem*)p.q + (x.s.q0 + t) * p.q_token + (y.head * p.G + r - t * p.G) * p.q_head : nullptr);
 
       // block i's keys and values lie in half (i - first) % 2 of the ring, the pages of its keys likewise behind it
       const uint32_t ring = lds_address(smem), pages = ring + C::STAGES * 2 * C::HALF;
@@ -88,17 +88,16 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
           const uint32_t k = ring + u * 2 * C::HALF, v = k + C::HALF;
           const int kb = attn_key<32>(x.r, i);
           const bool full = there[u] == 0xFFFFFFFFu && attn_all_seen<32>(p, x.s.first, t0, t1, kb);
-          typename Rows::Scores s;
+          typename Rows::Keys f;
           typename Rows::Weights w;
-          typename Rows::Mask mask;
-          float top[1];
-          a.scores(k, s);
+          uint32_t mask = there[u];
+          a.read_keys(k, f);
+          f32x16 s = a.scores(f);
           if (!full) {
-            mask.of[0] = there[u] & attn_sees(p, x.s.first, t, tree, kb);
+            mask &= attn_sees(p, x.s.first, t, tree, kb);
             a.hide(s, mask);
           }
-          a.largest(s, p.c, top);
-          a.follow(top);
+          a.follow(s, p.c);
           a.weigh(s, p.c, w);
           if (full) a.add(v, w);
           else a.add_hidden(v, w, mask);
@@ -111,7 +110,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
       }
       wait_loads<0>();                                 // the ring is filled anew for the next tile
 
-      const Halves ls = both_halves(a.l[0]);
+      const Halves ls = both_halves(a.l);
       const float l = ls.low + ls.high;
       if (has) {
         const int h = lane >> 5;
@@ -125,18 +124,18 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
             for (int j = 0; j < 16; j += 4) {
               e4 z;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) z[e] = Act::from_f32(a.o[0][d][j + e] * f);
+              for (int e = 0; e < 4; ++e) z[e] = Act::from_f32(a.o[d][j + e] * f);
               *(e4*)(to + d * 32 + j * 2) = z;
             }
         } else {
           float* part = attn_part<D, kFewRows>(p, blockIdx.x, first == 0);
-          if (h == 0) *(f32x2*)(part + 32 * D + 2 * lane) = f32x2{a.m[0], l};
+          if (h == 0) *(f32x2*)(part + 32 * D + 2 * lane) = f32x2{a.m, l};
 #pragma unroll
           for (int d = 0; d < D / 32; ++d)
 #pragma unroll
             for (int j = 0; j < 16; j += 4)
               *(f32x4*)(part + (lane & 31) * D + h * 4 + d * 32 + j * 2) =
-                  f32x4{a.o[0][d][j], a.o[0][d][j + 1], a.o[0][d][j + 2], a.o[0][d][j + 3]};
+                  f32x4{a.o[d][j], a.o[d][j + 1], a.o[d][j + 2], a.o[d][j + 3]};
         }
       }
     }

@@ -71,7 +71,7 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
   using C = TilesCfg<D>;
   constexpr int KEYS = C::KEYS, NW = C::NW, OWN = KEYS / NW, AHEAD = C::AHEAD;   // OWN: rows of a block that a wavefront loads
   static_assert(OWN == 8 && NW <= 8, "a group of 8 places per wavefront");
-  using Rows = AttnRows<Act, D, 32, 1>;
+  using Rows = AttnRows<Act, D>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int32_t* table = p.table + (size_t)x.b * p.width;
@@ -84,7 +84,7 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
   const bool has = r <= wr1;
   Rows a;
   a.start();
-  a.load_q(0, has ? (const typename Act::elem*)p.q + (x.s.q0 + t) * p.q_token + (head * p.G + r - t * p.G) * p.q_head : nullptr);
+  a.load_q(has ? (const typename Act::elem*)p.q + (x.s.q0 + t) * p.q_token + (head * p.G + r - t * p.G) * p.q_head : nullptr);
 
   auto key_of = [&](int i) { return attn_key<KEYS>(x.r, i); };
   constexpr uint64_t ALL = KEYS == 64 ? ~0ull : (1ull << (KEYS % 64)) - 1;
@@ -195,9 +195,7 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
     int mine = has ? t : 0;
     asm volatile("" : "+v"(mine));                     // made here, not kept in registers all along
     const int64_t* tree = p.tree ? p.tree + (size_t)(x.s.q0 + mine) * p.tree_words : nullptr;
-    typename Rows::Mask mask;
-    mask.of[0] = (there & attn_sees(p, x.s.first, mine, tree, key_of(i))) >> (32 * half) & 0xFFFFFFFFull;
-    return mask;
+    return (uint32_t)(there >> (32 * half)) & attn_sees(p, x.s.first, mine, tree, key_of(i) + 32 * half);
   };
 
   if (first < last) {
@@ -225,9 +223,8 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
       }
     }
     k[AHEAD] = rings + AHEAD * C::HALF;
-    typename Rows::Scores s0, s1;                      // of the two steps of a block (one: s0)
+    f32x16 s0, s1;                                     // scores of the two steps of a block (one: s0)
     typename Rows::Keys f;
-    float top[1];
     if constexpr (GROUPS) {
       const bool wrong = pages_wrong();
       if (lane == 0) dirty[wave] = wrong;
@@ -241,14 +238,13 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
       there[0] = keys_there(first);
     }
     bool full = full_of(first, there[0]);
-    auto follow = [&](typename Rows::Scores& s, bool all, int i, uint64_t keys, int half) __attribute__((always_inline)) {
+    auto follow = [&](f32x16& s, bool all, int i, uint64_t keys, int half) __attribute__((always_inline)) {
       if (!all) a.hide(s, mask_of(i, keys, half));
-      a.largest(s, p.c, top);
-      a.follow(top);
+      a.follow(s, p.c);
     };
     if (live) {
       a.read_keys(k[0], f);
-      a.scores_of(f, s0);
+      s0 = a.scores(f);
       follow(s0, full, first, there[0], 0);
       a.read_keys(KEYS == 64 ? k[0] + 64 * D : k[1], f);
     }
@@ -281,18 +277,17 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
         next();
         full1 = full_of(i + 1, there[0]);
       } else if constexpr (KEYS == 64) {
-        a.step(s0, v0, f, k[1], p.c, s1);
+        s1 = a.step(s0, v0, f, k[1], p.c);
         follow(s1, full, i, now, 1);
         next();
         full1 = full_of(i + 1, there[0]);
-        a.step(s1, v0 + 64 * D, f, k[1] + 64 * D, p.c, s0);
+        s0 = a.step(s1, v0 + 64 * D, f, k[1] + 64 * D, p.c);
         follow(s0, full1, i + 1, there[0], 0);
       } else {
-        a.step(s0, v0, f, k[2], p.c, s1);
+        s0 = a.step(s0, v0, f, k[2], p.c);
         next();
         full1 = full_of(i + 1, there[0]);
-        follow(s1, full1, i + 1, there[0], 0);
-        s0 = s1;
+        follow(s0, full1, i + 1, there[0], 0);
       }
       full = full1;
       uint32_t to = k[0];
@@ -317,16 +312,18 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
         const uint32_t place = attn_in(p, x.r, key) ? attn_place(p, table[attn_page_of(p, key)], key, head) : kNoRow;
         uint64_t there = __builtin_amdgcn_ballot_w64(place != kNoRow) & ALL;
         if (!edge_of(i, there)) continue;
-        const uint64_t sees = attn_sees(p, x.s.first, t, p.tree ? p.tree + (size_t)(x.s.q0 + (has ? t : 0)) * p.tree_words : nullptr, kb);
+        const int64_t* tree = p.tree ? p.tree + (size_t)(x.s.q0 + (has ? t : 0)) * p.tree_words : nullptr;
+        const uint64_t sees = attn_sees(p, x.s.first, t, tree, kb) | (uint64_t)attn_sees(p, x.s.first, t, tree, kb + 32) << 32;
 #pragma unroll 1
         for (; there; there &= there - 1) {
           const int j = __builtin_ctzll(there);
-          a.add_not_finite((const unsigned char*)p.v + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)place, j) * 16, sees >> j & 1);
+          const unsigned char* v = (const unsigned char*)p.v + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)place, j) * 16;
+          a.add_not_finite(sees >> j & 1, [&](int column) { return *(const u16x4*)(v + column * 2); });
         }
       }
   }
 
-  const Halves ls = both_halves(a.l[0]);
+  const Halves ls = both_halves(a.l);
   const float l = ls.low + ls.high;
   if (!has) return;
   if (!part) {
@@ -339,19 +336,19 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
       for (int i = 0; i < 16; i += 4) {
         e4 y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = Act::from_f32(a.o[0][d][i + e] * f);
+        for (int e = 0; e < 4; ++e) y[e] = Act::from_f32(a.o[d][i + e] * f);
         *(e4*)(to + d * 32 + i * 2) = y;
       }
     return;
   }
   const int row = r - x.row0;
-  if (lane < 32) *(f32x2*)(part + C::ROWS * D + 2 * row) = f32x2{a.m[0], l};
+  if (lane < 32) *(f32x2*)(part + C::ROWS * D + 2 * row) = f32x2{a.m, l};
   float* to = part + row * D + (lane >> 5) * 4;
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
     for (int i = 0; i < 16; i += 4)
-      *(f32x4*)(to + d * 32 + i * 2) = f32x4{a.o[0][d][i], a.o[0][d][i + 1], a.o[0][d][i + 2], a.o[0][d][i + 3]};
+      *(f32x4*)(to + d * 32 + i * 2) = f32x4{a.o[d][i], a.o[d][i + 1], a.o[d][i + 2], a.o[d][i + 3]};
 }
 
 template <class Act, int D, bool GROUPS>
