@@ -719,7 +719,8 @@ int mi_qk_norm_rope(const void* qkv, long long qkv_stride, const void* q_weight,
  * fp32; the weights are rounded to the activations' type in front of their product with the values; one rounding at the end.  What lies in
  * places that a token does not see does not reach it, infinities and NaN included.
  * query [T, num_heads, head_dim] with strides (multiples of 8), out contiguous; head_dim 64, 128 or 256; T num_heads below 2^28;
- * table_width x page_size below 2^30; scale > 0.  max_query_len and max_seq_len, the largest n and seq_lens, choose kernels and splits only:
+ * table_width x page_size below 2^30; B num_kv_heads below 2^22 where sequences of more than 32 rows can be (n num_heads / num_kv_heads);
+ * scale > 0.  cu_seqlens_q ascends (where it does not, out is not defined, and nothing outside is read or written).  max_query_len and max_seq_len, the largest n and seq_lens, choose kernels and splits only:
  * results are right for any values, up to the order of sums.  The workspace (mi_paged_attention_workspace bytes for the same arguments; 16-byte
  * aligned) must stay untouched until the stream has passed the call; 0 bytes: none.
  * In place of eagle_ops::page_attn_decode and of the sdp kernels of prompts (V/csrc/eagle, V/csrc/xpu). */

@@ -54,7 +54,7 @@ static int attn_plan(int T, int B, int Hq, int Hkv, int D, int max_query_len, in
   if (a.tiles) {
     const int R = attn_tile_rows(D), hold = cus() * (D == 64 ? 2 : 1);           // workgroups that the device holds
     const long long slots = (long long)T * G / R + B;
-    if (slots * Hkv >= 1 << 30) return MI_ERR_SHAPE;
+    if (slots * Hkv >= (1LL << 32) / (2 * R)) return MI_ERR_SHAPE;               // a grid holds less than 2^32 threads
     a.slots = (int)slots;
     // What the longer of both ways takes, in blocks of keys per workgroup: a workgroup per tile takes as long as the longest tile, and half as long again
     // on top of the even share where workgroups follow each other; equal shares have every tile see what its sequence's last token sees, and
@@ -112,7 +112,7 @@ static int run(const AttnArgs& base, const MiPagedCache* cache, int D, float sca
   const long long most = max_query_len < p.T ? max_query_len : p.T;
   p.tile_rows = a.tiles || most * p.G > 32 ? 32 : most < 1 ? p.G : (int)(most * p.G);
   p.many_parts = a.tiles || (long long)a.groups > 16LL * p.B * p.Hkv;          // with tiles beside them hardly any sequence is here
-  p.wide = ((long long)p.T * p.G / 32 + p.B) * p.Hkv * ((long long)p.width * cache->page_size / 32 + 8) >= 1LL << 31;
+  p.wide = ((long long)p.T * p.G / 32 + p.B) * p.Hkv * ((long long)p.width * cache->page_size / 32 + 8) >= 1LL << 30;
   p.slots = a.slots;
   p.shares = a.shares;
   if (a.tiles) {

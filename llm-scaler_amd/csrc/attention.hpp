@@ -35,7 +35,7 @@ struct AttnArgs {
   int window, sinks, tree_words;         // window 0: none
   float c;
   int groups, tile_rows;       // rows kernel: workgroups; rows of a tile, as the caller says
-  bool wide, many_parts;       // its work counts 2^31 blocks or more; a tile is in many parts
+  bool wide, many_parts;       // its work may count 2^30 blocks or more; a tile is in many parts
   int slots, shares;           // tiles kernel: a workgroup per tile (slots of them), or in that many equal shares
   int rows_from;               // sequences with that many rows (tokens x G) or more belong to the tiles kernel
 };
@@ -384,7 +384,7 @@ struct AttnRows {
 // All blocks of KEYS keys of all (sequence, tile of ROWS rows, kv head) in a row, each of these with ITEM blocks more for what beginning it costs, are cut
 // into equal shares, one per workgroup, whatever the sequences' lengths are.  A tile whose blocks all lie in one share is finished there; of the
 // others a workgroup has at most one that it continues and one that it begins: two parts, unscaled fp32 sums with their m and l, which a second launch
-// joins.  FEW: of the sequences with fewer than rows_from rows; otherwise of the others.  Num: int where all work counts less than 2^31 blocks.
+// joins.  FEW: of the sequences with fewer than rows_from rows; otherwise of the others.  Num: int where all work counts less than 2^30 blocks.
 template <int ROWS, int KEYS, int ITEM, bool FEW, class Num>
 struct Shares {
   // How many tiles a sequence has here, and how many blocks each of them
@@ -426,10 +426,12 @@ struct Shares {
     const int lane = threadIdx.x & 63;
     per = (p.B + 63) / 64;
     Num mine = 0;
+    bool wrong = false;                                // sequences that overlap: their work has no bound
     lanes = AttnSeq{};
     for (int i = 0; i < per; ++i) {
       const int b = lane * per + i;
       if (b >= p.B) continue;
+      wrong |= p.cu[b] > p.cu[b + 1];
       lanes = attn_seq(p, b);
       mine += work(p, seq_of(p, lanes));
     }
@@ -440,6 +442,7 @@ struct Shares {
     }
     before = incl - mine;
     total = uniform(from_lane(incl, (p.B - 1) / per)); // the last lane with sequences; those behind it have not added all up
+    if (__builtin_amdgcn_ballot_w64(wrong)) total = 0;
     share = uniform((total + groups - 1) / groups);
   }
   // Blocks begin .. end - 1 of the work are workgroup w's; none: begin = end

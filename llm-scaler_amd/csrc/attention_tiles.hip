@@ -162,7 +162,7 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
       const int it = *in_lds<const int>(pages + u * 4 * KEYS + lane % KEYS * 4);
       const uint32_t at = i < last ? attn_place(p, it, key_of(i) + lane % KEYS, head) : kNoRow;
       to.take(at, wave * OWN);
-      return (uint64_t)__builtin_amdgcn_ballot_w64(at != kNoRow);
+      return (uint64_t)__builtin_amdgcn_ballot_w64(at != kNoRow) & ALL;
     }
   };
   auto keys_there = [&](int i) {                       // GROUPS

@@ -35,7 +35,12 @@ def test_workspace():
                 dict(T=1 << 25), dict(B=1 << 24), dict(Hq=1 << 17), dict(T=2**31 - 1, Hq=65536, Hkv=1)):
         assert _size(**bad)[0] == -2, bad
     assert capi.lib().mi_paged_attention_workspace(1, 1, 1, 1, 64, 1, 1, None) == -1
-    assert _size(T=2**31 - 1, B=1, Hq=1, Hkv=1)[0] == -2 and _size(T=(1 << 28) - 1, B=(1 << 24) - 1, Hq=1, Hkv=1, mq=2**31 - 1, mk=2**31 - 1)[0] == 0
+    assert _size(T=2**31 - 1, B=1, Hq=1, Hkv=1)[0] == -2 and _size(T=(1 << 28) - 1, B=1, Hq=1, Hkv=1, mq=2**31 - 1, mk=2**31 - 1)[0] == 0
+    # a grid holds less than 2^32 threads: a workgroup per tile and kv head, 512 threads each (256 with heads of 256), and a tile or more per sequence
+    for D, most in ((64, 1 << 23), (128, 1 << 23), (256, 1 << 24)):
+        many = dict(T=most // 8, Hq=8, Hkv=8, D=D, mq=100)
+        assert _size(B=most // 8 - most // 64, **many)[0] == 0 and _size(B=most // 8, **many)[0] == -2
+        assert _size(**dict(many, B=most // 8, mq=1))[0] == 0           # single tokens: a fixed number of workgroups
 
 
 @pytest.mark.parametrize("tree", [False, True])

@@ -42,7 +42,7 @@ def _both(v, dev, seed, lens, news, Hq, Hkv, D, page, dt, window=-1, sinks=0, wo
 
 
 # lengths around a step of 32, a block of 64 and the shares of the workgroups; unused places of the batch; groups that do not divide 32
-SINGLE = [([1], 1, 1), ([2, 33], 4, 2), ([31, 32, 33, 63, 64, 65], 8, 1), ([700], 32, 8), ([0, 5, 0, 129], 6, 2), ([1000, 1, 257], 12, 4), ([4097], 16, 1),
+SINGLE = [([1], 1, 1), ([2, 33], 4, 2), ([31, 32, 33, 63, 64, 65], 8, 1), ([700], 32, 8), ([0, 5, 0, 129], 6, 2), ([1000, 1, 257], 15, 5), ([4097], 16, 1),
           ([64] * 70, 4, 4), ([300, 2000] * 40, 5, 1), ([130, 0, 64], 32, 1), ([77], 33, 1), ([500, 90], 80, 2)]
 
 
@@ -137,25 +137,27 @@ def test_rows_behind_the_last_sequence_stay(v, dev, n, splits):
     _check(out[:2 * n], *R.attention(q, kc, vc, table, lens, news, 0.1))
 
 
+# [2600]: few tokens over a long context, in shares of its keys
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("dt", DTS)
 @pytest.mark.parametrize("kind", ["prompt", "window", "tree"])
-def test_what_a_token_does_not_see_reaches_nothing(v, dev, D, dt, kind):
+@pytest.mark.parametrize("L,page", [(150, 16), (2600, 16), (2600, 12)])
+def test_what_a_token_does_not_see_reaches_nothing(v, dev, D, dt, kind, L, page):
     """Infinities and NaN in keys and values that some tokens of a tile see and others do not: the others' rows keep their bits."""
-    lens, news, words = [150, 90], [70, 20], 2 if kind == "tree" else 0
+    lens, news, words = [L, 90], [70, 20], 2 if kind == "tree" else 0
     window, sinks = (40, 3) if kind == "window" else (-1, 0)
-    case = R.make(dev, D, lens, news, 4, 2, D, 16, dt, words)
+    case = R.make(dev, D, lens, news, 4, 2, D, page, dt, words)
     clean = _run(v, case, lens, news, D, window, sinks)
     q, kc, vc, table, seq, cu, masks = case
     for value in (float("inf"), float("-inf"), float("nan")):
         for cache in (1, 2):
             dirty = list(case)
             dirty[cache] = case[cache].clone()
-            j = 130                                     # of sequence 0, a key of the call's own tokens
-            dirty[cache][table[0, j // 16].long(), j % 16, 0, 5] = value
+            j = L - 20                                  # of sequence 0, a key of the call's own tokens
+            dirty[cache][table[0, j // page].long(), j % page, 0, 5] = value
             out = _run(v, dirty, lens, news, D, window, sinks)
-            place = torch.arange(80, 150, device=dev)
-            see = R.visible("causal" if masks is None else "tree", place, 150, 70, window, sinks, None if masks is None else masks[:70])[:, j]
+            place = torch.arange(L - 70, L, device=dev)
+            see = R.visible("causal" if masks is None else "tree", place, L, 70, window, sinks, None if masks is None else masks[:70])[:, j]
             rows = torch.zeros(90, 4, dtype=torch.bool, device=dev)
             rows[:70, :2] = see[:, None]                # heads 0 and 1 read kv head 0
             assert see.any() and not see.all()
@@ -167,6 +169,71 @@ def test_what_a_token_does_not_see_reaches_nothing(v, dev, D, dt, kind):
             else:                                       # a key: a score of -inf takes the key out, any other makes the row NaN
                 lost = q[rows][:, 5].double() * value != float("-inf")
                 assert torch.equal(out[rows].isnan().all(1), lost) and torch.equal(out[rows].isnan().any(1), lost)
+
+
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (300, 0), (700, 40), (1200, 129), (64, 1)])
+@pytest.mark.parametrize("D,page", [(64, 16), (64, 5), (128, 64), (128, 12), (256, 16), (256, 3)])
+def test_few_tokens_over_long_contexts(v, dev, window, sinks, D, page):
+    """Equal shares of the keys: tiles that end inside a share, sequences without tokens or with a single one between them, pages outside the cache."""
+    lens, news = [2600, 30, 1500, 700, 2100, 64], [40, 30, 1, 0, 61, 3]
+    case = R.make(dev, window + D, lens, news, 16, 2, D, page, torch.bfloat16)
+    _check(_run(v, case, lens, news, D, window, sinks), *R.attention(*case[:4], lens, news, D ** -0.5, window, sinks))
+    table, pages = case[3], case[1].shape[0]
+    for b, key, bad in ((0, 1, -1), (0, 2500, pages), (2, 1499, -7), (4, 2040, 2 ** 31 - 1), (4, 1024, -2 ** 31)):
+        table[b, key // page] = bad
+    _check(_run(v, case, lens, news, D, window, sinks), *R.attention(*case[:4], lens, news, D ** -0.5, window, sinks))
+
+
+@pytest.mark.parametrize("longest", [150, 2300])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_batches_of_more_sequences_than_lanes(v, dev, longest, D):
+    lens = [(37 * i) % 140 for i in range(150)] + [longest, 100]
+    news = [min(L, (1, 0, 40, 3)[i % 4]) for i, L in enumerate(lens)]
+    _both(v, dev, longest + D, lens, news, 4, 2, D, 16, torch.float16)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(300, 1), (129, 1), (514, 2)])
+def test_groups_larger_than_a_tile(v, dev, Hq, Hkv):
+    for D in (64, 256):
+        _both(v, dev, Hq + D, [70, 200], [1, 3], Hq, Hkv, D, 16, torch.bfloat16)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_tables_of_many_places(v, dev, D):
+    """A table that could hold so many keys that their blocks are counted in 64 bits; all but the first columns are never used."""
+    lens, news = [100, 1, 1030, 0] * 16, [1] * 64
+    case = list(R.make(dev, D, lens, news, 8, 4, D, 512, torch.bfloat16))
+    wide = torch.full((64, (1 << 28) // 512), -1, dtype=torch.int32, device=dev)
+    wide[:, :case[3].shape[1]] = case[3]
+    out = _run(v, case[:3] + [wide] + case[4:], lens, news, D)
+    _check(out, *R.attention(*case[:4], lens, news, D ** -0.5))
+
+
+@pytest.mark.parametrize("n,L", [(1, 900), (40, 300), (40, 2600)])
+def test_starts_that_do_not_ascend_stay_inside(v, dev, n, L):
+    lens, news = [L, 90, L], [n, n, n]
+    q, kc, vc, table, seq, cu, _ = R.make(dev, n, lens, news, 8, 2, 128, 16, torch.bfloat16)
+    for starts in ([0, 3 * n, 0, 3 * n], [2 * n, n, 0, 0], [-5, n, 2 * n, 10 ** 9], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 0]):
+        around = torch.full((5 * n, 8, 128), 3.0, dtype=q.dtype, device=dev)
+        out = around[n:4 * n]
+        v.paged_attention(q, kc, vc, table, seq, torch.tensor(starts, dtype=torch.int32, device=dev), out, 0.1, -1, 0, n, L)
+        assert (around[:n] == 3).all() and (around[4 * n:] == 3).all()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_two_streams_at_once(v, dev, n):
+    lens, news = [5000, 300], [n, n]
+    cases = [R.make(dev, s, lens, news, 8, 2, 128, 16, torch.bfloat16) for s in range(2)]
+    alone = [_run(v, c, lens, news, 128) for c in cases]
+    outs = [[torch.empty_like(alone[0]) for _ in range(10)] for _ in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for i in range(10):
+        for s, c, o in zip(streams, cases, outs):
+            with torch.cuda.stream(s):
+                _run(v, c, lens, news, 128, out=o[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, a) for a, many in zip(alone, outs) for o in many)
 
 
 def test_pages_outside_the_cache_are_not_seen(v, dev):
