@@ -219,12 +219,12 @@ struct AttnRows {
   }
   // K of the 32 keys at LDS address k, columns 16 ks ..
   __device__ __forceinline__ v8 k_operand(uint32_t k, int ks) const {
-    return as_v8<v8>(*in_lds<const u32x4>(k + (ka ^ (ks % 8 * 32)) + ks / 8 * 256));
+    return as_v8<v8>(in_lds<const u32x4>(k + (ka ^ (ks % 8 * 32)))[ks / 8 * 16]);
   }
   // V^T of 16 keys (from 16 t of those at LDS address v) and columns 32 d ..: element e is key 4 (lane / 32) + e % 4 + 8 (e / 4)
   __device__ __forceinline__ v8 v_operand(uint32_t v, int t, int d) const {
-    const uint32_t at = v + (va ^ ((d & 3) * 64)) + (d >> 2) * 256 + t * 32 * D;
-    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(in_lds<i16x4>(at)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(in_lds<i16x4>(at + 16 * D));
+    auto* at = in_lds<i16x4>(v + (va ^ ((d & 3) * 64))) + (d >> 2) * 32 + t * 4 * D;       // one address and distances known to the instruction
+    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at + 2 * D);
     return __builtin_bit_cast(v8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   }
   __device__ __forceinline__ void read_keys(uint32_t k, Keys& f) const {
@@ -253,14 +253,18 @@ struct AttnRows {
       x[i] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, s) & sees) | (0xFF800000u & ~sees));
     }
   }
-  // Makes m fit the scores x.  Sums move to a new m only where an exponent would pass it by 8.  Weights are 2^kRaise times as large, up to 2^15, so that
-  // in fp16 those of a long tail keep their bits (half of the smallest number is 2^-32 of the largest weight).
-  __device__ __forceinline__ void follow(const f32x16& x, float c) {
+  // The largest of a row's scores
+  static __device__ __forceinline__ float largest(const f32x16& x) {
     float mx = x[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
     const Halves y = both_halves(mx);
-    const float top = fmaxf(y.low, y.high) * c;
+    return fmaxf(y.low, y.high);
+  }
+  // Makes m fit scores up to most.  Sums move to a new m only where an exponent would pass it by 8.  Weights are 2^kRaise times as large, up to 2^15, so that
+  // in fp16 those of a long tail keep their bits (half of the smallest number is 2^-32 of the largest weight).
+  __device__ __forceinline__ void follow(float most, float c) {
+    const float top = most * c;
     const bool moves = top > m + 8.f;                  // row by row: a row's bits depend on no other row
     if (!__builtin_amdgcn_ballot_w64(moves)) return;
     const float to = moves ? top : m, a = moves ? __builtin_amdgcn_exp2f(m - to) : 1.f;
@@ -292,9 +296,9 @@ struct AttnRows {
     }
     l += sum;
   }
-  // A step of the tiles kernel: weights of the scores x, the product with their values, and the next step's scores.  f: the next step's keys, then
+  // A step of the tiles kernel: weights of the scores x, the product with their values, and the next step's scores with their largest.  f: the next step's keys, then
   // those at k2; the values are read while the scores are made.
-  __device__ __forceinline__ f32x16 step(const f32x16& x, uint32_t v, Keys& f, uint32_t k2, float c) {
+  __device__ __forceinline__ f32x16 step(const f32x16& x, uint32_t v, Keys& f, uint32_t k2, float c, float& most) {
     Values va, vb;
     Weights w;
     read_values(v, 0, va);
@@ -306,6 +310,7 @@ struct AttnRows {
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = mfma32(va.v[d], w.p[0], o[d]);
     read_keys(k2, f);
+    most = largest(y);
     pin();
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = mfma32(vb.v[d], w.p[1], o[d]);

@@ -97,7 +97,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
             mask &= attn_sees(p, x.s.first, t, tree, kb);
             a.hide(s, mask);
           }
-          a.follow(s, p.c);
+          a.follow(a.largest(s), p.c);
           a.weigh(s, p.c, w);
           if (full) a.add(v, w);
           else a.add_hidden(v, w, mask);

@@ -127,9 +127,9 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
   const int inner_key = x.r.from + (inner - x.r.head) * KEYS;
   auto is_inner = [&](int i) { return GROUPS && (uint32_t)(i - inner) < (uint32_t)inners; };
   int page = 0;                                        // GROUPS: of the block whose place comes next
-  auto lookup = [&](int i, int u) {
+  auto lookup = [&](int i, int u, bool known = false) {
     if constexpr (GROUPS) {
-      if (is_inner(i)) {
+      if (known || is_inner(i)) {
         page = scalar_load(table + attn_page_of(p, inner_key + (i - inner) * KEYS + wave * OWN));
         return;
       }
@@ -144,9 +144,9 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
     }
   };
   // the place of block i, and which of its keys are there
-  auto place = [&](int i, int u, Places& to) {
+  auto place = [&](int i, int u, Places& to, bool known = false) {
     if constexpr (GROUPS) {
-      if (is_inner(i)) {
+      if (known || is_inner(i)) {
         const int key = inner_key + (i - inner) * KEYS + wave * OWN;
         to = (uint32_t)page * p.page16 + (uint32_t)(key - attn_page_of(p, key) * p.page) * p.row16 + (uint32_t)head * p.head16;
         return ALL;
@@ -238,18 +238,53 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
       there[0] = keys_there(first);
     }
     bool full = full_of(first, there[0]);
+    float most;                                        // the largest of the scores that were made last
     auto follow = [&](f32x16& s, bool all, int i, uint64_t keys, int half) __attribute__((always_inline)) {
-      if (!all) a.hide(s, mask_of(i, keys, half));
-      a.follow(s, p.c);
+      if (!all) {
+        a.hide(s, mask_of(i, keys, half));
+        most = a.largest(s);
+      }
+      a.follow(most, p.c);
     };
     if (live) {
       a.read_keys(k[0], f);
       s0 = a.scores(f);
+      most = a.largest(s0);
       follow(s0, full, first, there[0], 0);
       a.read_keys(KEYS == 64 ? k[0] + 64 * D : k[1], f);
     }
+    auto turn = [&]() __attribute__((always_inline)) { // the rings
+      uint32_t to = k[0];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) k[j] = k[j + 1];
+      k[AHEAD] = to;
+      to = v0;
+      v0 = v1;
+      v1 = to;
+    };
     int u = AHEAD & 1;
     for (int i = first; i < last; ++i) {
+      if constexpr (GROUPS)
+        // All blocks that are loaded or looked up meanwhile are inner ones: the same without a question.
+        for (; live && i >= inner && i + AHEAD + 2 < inner + inners; ++i) {
+          wait_loads<0>();
+          lds_barrier();
+          request(V_, at[0], v1);
+          request(K_, at[AHEAD - 1], k[AHEAD]);
+#pragma unroll
+          for (int j = 0; j + 1 < AHEAD; ++j) at[j] = at[j + 1];
+          place(i + AHEAD + 1, 0, at[AHEAD - 1], true);
+          lookup(i + AHEAD + 2, 0, true);
+          if constexpr (KEYS == 64) {
+            s1 = a.step(s0, v0, f, k[1], p.c, most);
+            a.follow(most, p.c);
+            s0 = a.step(s1, v0 + 64 * D, f, k[1] + 64 * D, p.c, most);
+          } else {
+            s0 = a.step(s0, v0, f, k[2], p.c, most);
+          }
+          a.follow(most, p.c);
+          turn();
+        }
       // The block's values and the next two steps' keys are there; more of both are asked for.
       wait_loads<0>();
       // 0 times an infinity or a NaN would not be 0: in blocks that some row does not see all of, the wavefronts look for such among the values that they
@@ -277,26 +312,20 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
         next();
         full1 = full_of(i + 1, there[0]);
       } else if constexpr (KEYS == 64) {
-        s1 = a.step(s0, v0, f, k[1], p.c);
+        s1 = a.step(s0, v0, f, k[1], p.c, most);
         follow(s1, full, i, now, 1);
         next();
         full1 = full_of(i + 1, there[0]);
-        s0 = a.step(s1, v0 + 64 * D, f, k[1] + 64 * D, p.c);
+        s0 = a.step(s1, v0 + 64 * D, f, k[1] + 64 * D, p.c, most);
         follow(s0, full1, i + 1, there[0], 0);
       } else {
-        s0 = a.step(s0, v0, f, k[2], p.c);
+        s0 = a.step(s0, v0, f, k[2], p.c, most);
         next();
         full1 = full_of(i + 1, there[0]);
         follow(s0, full1, i + 1, there[0], 0);
       }
       full = full1;
-      uint32_t to = k[0];
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) k[j] = k[j + 1];
-      k[AHEAD] = to;
-      to = v0;
-      v0 = v1;
-      v1 = to;
+      turn();
     }
   }
 
