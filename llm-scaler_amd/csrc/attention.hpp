@@ -183,6 +183,7 @@ template <class Act, int D>
 struct AttnRows {
   using v8 = typename Act::v8;
   typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
+  typedef __attribute__((ext_vector_type(8))) short i16x8;
   typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
   static constexpr int DT = D / 32;
   static constexpr float kRaise = 7.f;
@@ -328,18 +329,18 @@ struct AttnRows {
   //
   // The rows kernel: while the values are read
   __device__ __forceinline__ void add_hidden(uint32_t v, const Weights& w, uint32_t mask) {
-    u16x8 one = 1;                                     // 0 where a value was not finite
+    u16x8 all = 0xFFFF;                                // 0 where a value was not finite
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const u16x8 x = __builtin_bit_cast(u16x8, v_operand(v, t, d)), finite = are_finite(x);
-        one &= finite;
-        o[d] = mfma32(__builtin_bit_cast(v8, x & (0 - finite)), w.p[t], o[d]);
+        all &= finite;
+        o[d] = mfma32(__builtin_bit_cast(v8, x & finite), w.p[t], o[d]);
       }
     }
-    if (!__builtin_amdgcn_ballot_w64(any_not(one))) return;
+    if (!__builtin_amdgcn_ballot_w64(any_not(all))) return;
 #pragma unroll 1
     for (int j = 0; j < 32; ++j)
       add_not_finite(mask >> j & 1, [&](int column) {
@@ -357,7 +358,7 @@ struct AttnRows {
       const u16x8 x = *at, finite = are_finite(x);
       const bool found = any_not(finite);
       if (!__builtin_amdgcn_ballot_w64(found)) continue;
-      *at = x & (0 - finite);
+      *at = x & finite;
       spoilt |= found && there >> (j * (512 / D) + (threadIdx.x & 63) / (D / 8)) & 1;
     }
     return __builtin_amdgcn_ballot_w64(spoilt) != 0;
@@ -378,10 +379,13 @@ struct AttnRows {
       }
     }
   }
-  static __device__ __forceinline__ u16x8 are_finite(u16x8 x) { return __builtin_elementwise_min(EXPONENT - (x & EXPONENT), (u16x8)1); }
+  // All ones where a number is finite: the difference of its exponent and the largest one is below zero
+  static __device__ __forceinline__ u16x8 are_finite(u16x8 x) {
+    return __builtin_bit_cast(u16x8, __builtin_bit_cast(i16x8, (x & EXPONENT) - EXPONENT) >> 15);
+  }
   static __device__ __forceinline__ bool any_not(u16x8 ones) {
     const u32x4 x = __builtin_bit_cast(u32x4, ones);
-    return (x[0] & x[1] & x[2] & x[3]) != 0x00010001u;
+    return (x[0] & x[1] & x[2] & x[3]) != 0xFFFFFFFFu;
   }
 };
 
