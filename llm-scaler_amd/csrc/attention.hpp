@@ -130,7 +130,7 @@ __device__ const u32x4 kZeroRow[64] = {};             // what a key that nothing
 
 // 16-byte chunk c of key row r lies at place c ^ swizzle of its row: eight lanes that read a column of K rows at a time, and the four rows of 64
 // bytes that a transposing read of V takes, find different banks.
-template <int D> __device__ __forceinline__ int k_swizzle(int r) { return r & (D / 8 < 16 ? D / 8 - 1 : 15); }
+template <int D> __device__ __forceinline__ int k_swizzle(int r) { return D == 64 ? r >> 1 & 7 : r & 15; }
 template <int D> __device__ __forceinline__ int v_swizzle(int r) { return D == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2; }
 
 __device__ const int32_t kNoPage[1] = {-1};
