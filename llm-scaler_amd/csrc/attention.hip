@@ -6,7 +6,8 @@
 namespace qlin {
 
 // Which kernels a call runs.  Up to 32 rows (tokens x heads of a group) per sequence go to the rows kernel, more to the tiles kernel; where
-// sequences of both kinds can be in a call both are launched, and each takes its own.
+// sequences of both kinds can be in a call both are launched, and each takes its own.  32 and 48 rows by the rows kernel and by tiles, 8 kv heads of 128:
+// one sequence of 1000 keys 14.2 and 23.7, 15.9 and 24.8 us; 16 of 4000 59 and 53, 66 and 55; 4 of 30000 118 and 109, 207 and 111.
 struct AttnPlan {
   bool rows, tiles;
   int rows_from, groups, slots, shares;
@@ -58,12 +59,13 @@ static int attn_plan(int T, int B, int Hq, int Hkv, int D, int max_query_len, in
     a.slots = (int)slots;
     // What the longer of both ways takes, in blocks of keys per workgroup: a workgroup per tile takes as long as the longest tile, and half as long again
     // on top of the even share where workgroups follow each other; equal shares have every tile see what its sequence's last token sees, and
-    // a part more to write and read (8 blocks or so each).
+    // parts to write and read.  One and four sequences of 1000 keys, 48 rows, heads of 128: 25.1 and 25.4 us by tiles, 16.4 and 17.7 in shares; four of
+    // 500 with 256 rows 25.5 and 26.9, 16 of 700 with 48 20.8 and 26.2; heads of 64, four of 1000: 20.5 and 21.1.
     long long tiles = (long long)T * G / R;
     if (tiles < B) tiles = B;
     tiles *= Hkv;
     const long long keys = max_seq_len < 1 ? 1 : max_seq_len, seen = keys - (most < keys ? most : keys) / 2;
-    const long long even = tiles * seen / hold, alone = tiles <= hold ? keys : even + keys / 2, shared = tiles * keys / hold + 1024;
+    const long long even = tiles * seen / hold, alone = tiles <= hold ? keys : even + keys / 2, shared = tiles * keys / hold + (D == 64 ? 1024 : 560);
     if (alone > shared) {
       a.shares = hold;
       a.tiles_bytes = round256(attn_parts_bytes(a.shares, D, R));

@@ -297,8 +297,8 @@ struct AttnRows {
     }
     l += sum;
   }
-  // A step of the tiles kernel: weights of the scores x, the product with their values, and the next step's scores with their largest.  f: the next step's keys, then
-  // those at k2; the values are read while the scores are made.
+  // A step of the tiles kernel: weights of the scores x, the product with their values, and the next step's scores with their largest.  f: the next
+  // step's keys, then those at k2; the values are read while the scores are made.
   __device__ __forceinline__ f32x16 step(const f32x16& x, uint32_t v, Keys& f, uint32_t k2, float c, float& most) {
     Values va, vb;
     Weights w;

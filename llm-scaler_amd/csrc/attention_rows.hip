@@ -2,8 +2,7 @@
 // 32 keys at a time, with its loads two steps ahead.
 //
 // A wavefront needs no barrier, and eight (four, two with heads of 64, 128, 256) fill a CU's LDS with loads under way.  Equal shares: whatever the
-// lengths, all wavefronts end together (sequences of 1 to 8192 keys; a workgroup per tile and a fixed number of parts took 1.2 to 1.5 times as long for trees over
-// long contexts).
+// lengths, all wavefronts end together (a workgroup per tile and a fixed number of parts took 1.2 to 1.5 times as long for trees over long contexts).
 //
 // Bound: HBM.  Two sequences of 131072 keys, 8 kv heads of 128: 1.07 GB in 205 us (5.2 TB/s) and 10 to join the parts; 64 sequences of up to 8192:
 // 260 MB in 45 us (5.8 TB/s) and 7.  Short calls: two launches, of which the second waits for the first
