@@ -109,6 +109,7 @@ static int run(const AttnArgs& base, const MiPagedCache* cache, int D, float sca
   divide_by((uint32_t)p.page, p.page_mul, p.page_shift);
   p.G = p.Hq / p.Hkv;
   p.c = scale * 1.4426950408889634f;
+  p.far = 1024.f / p.c;
   p.rows_from = a.rows_from;
   p.groups = a.groups;
   const long long most = max_query_len < p.T ? max_query_len : p.T;

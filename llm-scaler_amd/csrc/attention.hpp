@@ -1,9 +1,9 @@
 // Attention over a paged cache: what its two kernels share.
 //
-//   o_i = sum_j p_ij v_j,   p_ij = 2^(c s_ij - m_i) / l_i,   s_ij = q_i . k_j,   c = scale log2(e)
+//   o_i = sum_j p_ij v_j,   p_ij = 2^(c (s_ij - m_i)) / l_i,   s_ij = q_i . k_j,   c = scale log2(e)
 //
-// in one pass over the keys: m follows the largest c s of a row, l is the running sum, and both o and l are multiplied by
-// 2^(m_old - m_new) where m moves.  s, m, l and o are fp32; p is rounded to the type of the values in front of its product with
+// in one pass over the keys: m follows the largest s of a row, l is the running sum, and both o and l are multiplied by
+// 2^(c (m_old - m_new)) where m moves.  s, m, l and o are fp32; p is rounded to the type of the values in front of its product with
 // them (off by half a step of a 16-bit number, below the output's rounding, as v_j is already such a number), and l sums the rounded p.
 //
 // The rows of a kv head are (token, head of the group) pairs of a sequence, token first: row r is head r % G of token r / G.  A wavefront holds 32
@@ -33,7 +33,7 @@ struct AttnArgs {
   uint32_t page_mul, page_shift;         // key / page
   int T, B, Hq, Hkv, G, page, width, pages;
   int window, sinks, tree_words;         // window 0: none
-  float c;
+  float c, far;                // far: 2^10 / c
   int groups, tile_rows;       // rows kernel: workgroups; rows of a tile, as the caller says
   bool wide, many_parts;       // its work may count 2^30 blocks or more; a tile is in many parts
   int slots, shares;           // tiles kernel: a workgroup per tile (slots of them), or in that many equal shares
@@ -178,6 +178,16 @@ struct RowPlaces {
 };
 
 // ---- the rows of a wavefront ------------------------------------------------------------------
+// Exponents of the weights: fma(c, s, raise - c m), one instruction, while c |m| < 2^10; raise - c m is then rounded by 2^-15 at most, the same for all
+// weights that go by this m.  Of a larger one the last place is worth whole units in the end: there the scores give way to s - m, exact where it matters,
+// and the exponent is fma(c, s - m, raise).  Those rows keep their m apart, so that others pay nothing for them (with a comparison more in every step
+// 695 against 680 us for chunks of heads of 256, 410 against 405 for a prompt in a window with heads of 64).
+// The raise: m may lag, so the largest weight of a row is 2^raise to 2^(raise + 8).  fp16: up to 2^15, so that the weights of a long tail keep
+// their bits (half of the smallest number is 2^-32 of the largest weight).
+template <class Act> constexpr float attn_raise = 7.f;
+// What sums that go by m are multiplied by where they go by `to` >= m; 0 from m = -inf
+__device__ __forceinline__ float attn_moved(const AttnArgs& p, float m, float to) { return __builtin_amdgcn_exp2f((m - to) * p.c); }
+
 // 32 rows over steps of 32 keys: scores (K Q^T), their maximum, weights (exp), and the product with V.
 template <class Act, int D>
 struct AttnRows {
@@ -186,7 +196,7 @@ struct AttnRows {
   typedef __attribute__((ext_vector_type(8))) short i16x8;
   typedef __attribute__((ext_vector_type(4))) typename Act::elem e4;
   static constexpr int DT = D / 32;
-  static constexpr float kRaise = 7.f;
+  static constexpr float kRaise = attn_raise<Act>;
   static constexpr unsigned short EXPONENT = Act::dt == DT_F16 ? 0x7C00 : 0x7F80;
   struct Weights { v8 p[2]; };                         // p[t][e]: key 16 t + 8 (e / 4) + 4 (lane / 32) + e % 4 of row lane % 32
   // Operands whose reads of LDS go out long before their products: they stay on their side of a `pin`, everything else may move.
@@ -196,13 +206,15 @@ struct AttnRows {
 
   v8 q[D / 16];
   f32x16 o[DT];                // o[t][i]: column 32 t + 8 (i / 4) + 4 (lane / 32) + i % 4 of row lane % 32
-  float m, l;                  // m: what a row's exponents are taken from, at most 8 below the largest; l: of this lane's keys
+  float m, l;                  // m: the score that a row's exponents are taken from, at most 8 / c below the largest; l: of this lane's keys
+  float apart;                 // m where c |m| is 2^10 or more; m is -inf there, as where a row has seen nothing yet
   int ka, va;                  // where this lane reads K and V of a step
 
   __device__ __forceinline__ void start() {
     const int lane = threadIdx.x & 63, h = lane >> 5, i = lane & 15;
     m = -__builtin_inff();
     l = 0.f;
+    apart = m;
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = f32x16{};
     ka = (lane & 31) * 2 * D + ((h ^ k_swizzle<D>(lane & 31)) * 16);
@@ -262,32 +274,40 @@ struct AttnRows {
     const Halves y = both_halves(mx);
     return fmaxf(y.low, y.high);
   }
-  // Makes m fit scores up to most.  Sums move to a new m only where an exponent would pass it by 8.  Weights are 2^kRaise times as large, up to 2^15, so that
-  // in fp16 those of a long tail keep their bits (half of the smallest number is 2^-32 of the largest weight).
-  __device__ __forceinline__ void follow(float most, float c) {
-    const float top = most * c;
-    const bool moves = top > m + 8.f;                  // row by row: a row's bits depend on no other row
-    if (!__builtin_amdgcn_ballot_w64(moves)) return;
-    const float to = moves ? top : m, a = moves ? __builtin_amdgcn_exp2f(m - to) : 1.f;
-    l *= a;
+  __device__ __forceinline__ float reference() const { return m == -__builtin_inff() ? apart : m; }
+  // Makes m fit the scores x, most their largest.  Sums move to a new m only where an exponent would pass it by 8.
+  __device__ __forceinline__ void follow(const AttnArgs& p, f32x16& x, float most) {
+    if (!__builtin_amdgcn_ballot_w64((most - m) * p.c > 8.f)) return;         // m = -inf: all that is seen
+    const float from = reference();
+    const bool moves = (most - from) * p.c > 8.f;      // row by row: a row's bits depend on no other row
+    if (__builtin_amdgcn_ballot_w64(moves)) {
+      const float to = moves ? most : from, a = moves ? attn_moved(p, from, to) : 1.f;
+      l *= a;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      if constexpr (D == 256) asm volatile("" : "+a"(o[d]));     // accumulation registers up to here: not all copied in every step
+      for (int d = 0; d < DT; ++d) {
+        if constexpr (D == 256) asm volatile("" : "+a"(o[d]));   // accumulation registers up to here: not all copied in every step
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[d][i] *= a;
-      if constexpr (D == 256) asm volatile("" : "+a"(o[d]));
+        for (int i = 0; i < 16; ++i) o[d][i] *= a;
+        if constexpr (D == 256) asm volatile("" : "+a"(o[d]));
+      }
+      const bool far = fabsf(to) >= p.far && to != -__builtin_inff();
+      m = far ? -__builtin_inff() : to;
+      apart = far ? to : -__builtin_inff();
     }
-    m = to;
+    if (!__builtin_amdgcn_ballot_w64(apart != -__builtin_inff())) return;
+    const float by = apart == -__builtin_inff() ? 0.f : apart;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] -= by;
   }
-  __device__ __forceinline__ void weigh(const f32x16& x, float c, Weights& w) {
-    const float top = m == -__builtin_inff() ? 0.f : m - kRaise;           // first: a row that has seen nothing yet
+  __device__ __forceinline__ void weigh(const AttnArgs& p, const f32x16& x, Weights& w) {
+    const float add = fabsf(m) >= p.far ? kRaise : __builtin_fmaf(-m, p.c, kRaise);
     typedef __attribute__((ext_vector_type(2))) typename Act::elem e2;
     const e2 one = {(typename Act::elem)1.f, (typename Act::elem)1.f};
     float sum = 0.f;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w.p[t][e] = Act::from_f32(__builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * t + e], c, -top)));
+      for (int e = 0; e < 8; ++e) w.p[t][e] = Act::from_f32(__builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * t + e], p.c, add)));
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         const e2 two = {w.p[t][e], w.p[t][e + 1]};
@@ -299,7 +319,7 @@ struct AttnRows {
   }
   // A step of the tiles kernel: weights of the scores x, the product with their values, and the next step's scores with their largest.  f: the next
   // step's keys, then those at k2; the values are read while the scores are made.
-  __device__ __forceinline__ f32x16 step(const f32x16& x, uint32_t v, Keys& f, uint32_t k2, float c, float& most) {
+  __device__ __forceinline__ f32x16 step(const AttnArgs& p, const f32x16& x, uint32_t v, Keys& f, uint32_t k2, float& most) {
     Values va, vb;
     Weights w;
     read_values(v, 0, va);
@@ -307,7 +327,7 @@ struct AttnRows {
     const f32x16 y = scores(f);
     read_values(v, 1, vb);
     pin();
-    weigh(x, c, w);
+    weigh(p, x, w);
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = mfma32(va.v[d], w.p[0], o[d]);
     read_keys(k2, f);
@@ -520,7 +540,7 @@ __device__ __forceinline__ long long attn_row(const AttnArgs& p, int q0, int hea
 // share a row's parts, and what they have meets in LDS.  All loads of four parts are under way together.
 constexpr int kJoinRows = 8;                          // of a workgroup
 template <class Act, int D, int THREADS, class Sums, class Ml, class To>
-__device__ __forceinline__ void attn_join(int rows, int parts, Sums sums, Ml ml, To to) {
+__device__ __forceinline__ void attn_join(const AttnArgs& p, int rows, int parts, Sums sums, Ml ml, To to) {
   constexpr int Q = D / 4, PLACES = THREADS / Q;         // threads of a row; rows, or shares of rows, at a time
   __shared__ f32x4 part_o[THREADS];
   __shared__ f32x2 part_ml[PLACES];
@@ -552,12 +572,12 @@ __device__ __forceinline__ void attn_join(int rows, int parts, Sums sums, Ml ml,
           for (int j = 0; j < 4; ++j) sum += a[j][1];
           continue;
         }
-        const float f = __builtin_amdgcn_exp2f(m - top);
+        const float f = attn_moved(p, m, top);
         sum *= f;
         o *= f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float g = __builtin_amdgcn_exp2f(a[j][0] - top);
+          const float g = attn_moved(p, a[j][0], top);
           sum += g * a[j][1];
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] += a[j][0] == -__builtin_inff() ? 0.f : g * x[j][e];
@@ -572,12 +592,12 @@ __device__ __forceinline__ void attn_join(int rows, int parts, Sums sums, Ml ml,
       if (who == 0 && row < rows) {
         float top = m;
         for (int j = 1; j < share; ++j) top = fmaxf(top, part_ml[place + j][0]);
-        float f = top == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - top);
+        float f = top == -__builtin_inff() ? 1.f : attn_moved(p, m, top);
         sum *= f;
         o *= f;
         for (int j = 1; j < share; ++j) {
           const f32x2 b = part_ml[place + j];
-          f = top == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(b[0] - top);
+          f = top == -__builtin_inff() ? 1.f : attn_moved(p, b[0], top);
           sum += f * b[1];
           o += f * part_o[threadIdx.x + j * Q];
         }
@@ -605,7 +625,7 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(const AttnArgs p, in
   auto part = [&](int i) { return attn_part<D, ROWS>(p, w - 1 + i, i == 0); };
   for (int row0 = blockIdx.y * kJoinRows; row0 < rows; row0 += gridDim.y * kJoinRows)
     attn_join<Act, D, THREADS>(
-        min(kJoinRows, rows - row0), cut[0], [&](int i, int row) { return part(i) + (row0 + row) * D; },
+        p, min(kJoinRows, rows - row0), cut[0], [&](int i, int row) { return part(i) + (row0 + row) * D; },
         [&](int i, int row) { return part(i) + ROWS * D + 2 * (row0 + row); },
         [&](int row) { return (typename Act::elem*)p.out + attn_row(p, cut[1], cut[3] >> 9, cut[2] * ROWS + row0 + row) * D; });
 }

@@ -102,8 +102,8 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
             mask &= attn_sees(p, x.s.first, t, tree, kb);
             a.hide(s, mask);
           }
-          a.follow(a.largest(s), p.c);
-          a.weigh(s, p.c, w);
+          a.follow(p, s, a.largest(s));
+          a.weigh(p, s, w);
           if (full) a.add(v, w);
           else a.add_hidden(v, w, mask);
           __builtin_amdgcn_sched_barrier(0);
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1
             }
         } else {
           float* part = attn_part<D, kFewRows>(p, blockIdx.x, first == 0);
-          if (h == 0) *(f32x2*)(part + 32 * D + 2 * lane) = f32x2{a.m, l};
+          if (h == 0) *(f32x2*)(part + 32 * D + 2 * lane) = f32x2{a.reference(), l};
 #pragma unroll
           for (int d = 0; d < D / 32; ++d)
 #pragma unroll

@@ -247,7 +247,7 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
         a.hide(s, mask_of(i, keys, half));
         most = a.largest(s);
       }
-      a.follow(most, p.c);
+      a.follow(p, s, most);
     };
     if (live) {
       a.read_keys(k[0], f);
@@ -279,13 +279,13 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
           place(i + AHEAD + 1, 0, at[AHEAD - 1], true);
           lookup(i + AHEAD + 2, 0, true);
           if constexpr (KEYS == 64) {
-            s1 = a.step(s0, v0, f, k[1], p.c, most);
-            a.follow(most, p.c);
-            s0 = a.step(s1, v0 + 64 * D, f, k[1] + 64 * D, p.c, most);
+            s1 = a.step(p, s0, v0, f, k[1], most);
+            a.follow(p, s1, most);
+            s0 = a.step(p, s1, v0 + 64 * D, f, k[1] + 64 * D, most);
           } else {
-            s0 = a.step(s0, v0, f, k[2], p.c, most);
+            s0 = a.step(p, s0, v0, f, k[2], most);
           }
-          a.follow(most, p.c);
+          a.follow(p, s0, most);
           turn();
         }
       // The block's values and the next two steps' keys are there; more of both are asked for.
@@ -315,14 +315,14 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
         next();
         full1 = full_of(i + 1, there[0]);
       } else if constexpr (KEYS == 64) {
-        s1 = a.step(s0, v0, f, k[1], p.c, most);
+        s1 = a.step(p, s0, v0, f, k[1], most);
         follow(s1, full, i, now, 1);
         next();
         full1 = full_of(i + 1, there[0]);
-        s0 = a.step(s1, v0 + 64 * D, f, k[1] + 64 * D, p.c, most);
+        s0 = a.step(p, s1, v0 + 64 * D, f, k[1] + 64 * D, most);
         follow(s0, full1, i + 1, there[0], 0);
       } else {
-        s0 = a.step(s0, v0, f, k[2], p.c, most);
+        s0 = a.step(p, s0, v0, f, k[2], most);
         next();
         full1 = full_of(i + 1, there[0]);
         follow(s0, full1, i + 1, there[0], 0);
@@ -374,7 +374,7 @@ __device__ __forceinline__ void tile_piece(const AttnArgs& p, const Tile& x, int
     return;
   }
   const int row = r - x.row0;
-  if (lane < 32) *(f32x2*)(part + C::ROWS * D + 2 * row) = f32x2{a.m, l};
+  if (lane < 32) *(f32x2*)(part + C::ROWS * D + 2 * row) = f32x2{a.reference(), l};
   float* to = part + row * D + (lane >> 5) * 4;
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
