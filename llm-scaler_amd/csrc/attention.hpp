@@ -183,8 +183,9 @@ struct RowPlaces {
 // and the exponent is fma(c, s - m, raise).  Those rows keep their m apart, so that others pay nothing for them (with a comparison more in every step
 // 695 against 680 us for chunks of heads of 256, 410 against 405 for a prompt in a window with heads of 64).
 // The raise: m may lag, so the largest weight of a row is 2^raise to 2^(raise + 8).  fp16: up to 2^15, so that the weights of a long tail keep
-// their bits (half of the smallest number is 2^-32 of the largest weight).
-template <class Act> constexpr float attn_raise = 7.f;
+// their bits (half of the smallest number is 2^-32 of the largest weight).  bf16, whose values reach as far as the sums: up to 1, so that no sum is
+// larger than the formula's.
+template <class Act> constexpr float attn_raise = Act::dt == DT_F16 ? 7.f : -8.f;
 // What sums that go by m are multiplied by where they go by `to` >= m; 0 from m = -inf
 __device__ __forceinline__ float attn_moved(const AttnArgs& p, float m, float to) { return __builtin_amdgcn_exp2f((m - to) * p.c); }
 

@@ -86,3 +86,34 @@ def test_scores_of_2_to_the_30(v, dev, lens, news, D, page, dt, kind):
             k[:L // 3, :, 0], k[L // 3:2 * L // 3, :, 0] = -32768.0, 0.0
         kc[_keys(case, b, L)] = k.to(dt).to(dev)
     _check(_run(v, case, lens, news, 1 / 64), *_exact_scores(case, lens, news, 1 / 64))
+
+
+# one or few keys per row; a prompt whose first tokens see few; long contexts
+LARGE = [([1, 2, 3, 70], [1, 1, 1, 1], 126), ([70, 1, 33], [70, 1, 33], 119), ([300, 100], [70, 100], 117), ([2600, 1500], [40, 61], 114),
+         ([2600, 40, 9000], [40, 1, 1], 112)]
+
+
+@pytest.mark.parametrize("lens,news,size", LARGE)
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 12), (256, 16)])
+def test_values_of_any_size(v, dev, lens, news, size, D, page):
+    """bf16 values of 2^size (what keeps a sum of them under weights of 1 finite), and of 2^-size: exponents of fp32."""
+    for exponent in (size, -size):
+        case = R.make(dev, D + size, lens, news, 4, 2, D, page, torch.bfloat16)
+        case[2].copy_((case[2].double().clamp(-3.9, 3.9) * 2.0 ** exponent).bfloat16())
+        _check(_run(v, case, lens, news, D ** -0.5), *R.attention(*case[:4], lens, news, D ** -0.5))
+
+
+@pytest.mark.parametrize("n", [1, 70])
+def test_a_rising_maximum_under_large_values(v, dev, n):
+    """Scores that rise by less than what moves the maximum, one key after the other: weights far above the first one's."""
+    lens, news, D = [200], [n], 64
+    case = R.make(dev, n, lens, news, 1, 1, D, 16, torch.bfloat16)
+    q, kc, vc = case[:3]
+    q.zero_()
+    q[..., 0] = 8.0
+    k = torch.zeros(200, 1, D)
+    k[:, 0, 0] = torch.where(torch.arange(200) < 120, 0.0, 5.0)       # 2^7.2 of the first ones' weight
+    at = _keys(case, 0, 200)
+    kc[at] = k.bfloat16().to(dev)
+    vc[at] = torch.full_like(vc[at], 2.0 ** 120)
+    _check(_run(v, case, lens, news, D ** -0.5), *R.attention(*case[:4], lens, news, D ** -0.5))
