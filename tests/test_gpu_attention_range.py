@@ -117,3 +117,20 @@ def test_a_rising_maximum_under_large_values(v, dev, n):
     kc[at] = k.bfloat16().to(dev)
     vc[at] = torch.full_like(vc[at], 2.0 ** 120)
     _check(_run(v, case, lens, news, D ** -0.5), *R.attention(*case[:4], lens, news, D ** -0.5))
+
+
+@pytest.mark.parametrize("score", [14.75, 15.25, 16.75])
+@pytest.mark.parametrize("n", [1, 40])
+def test_tails_of_subnormal_weights(v, dev, n, score):
+    """One key far above 100000 others, which have 2^-21.3, 2^-22 and 2^-24.2 of its weight: in fp16 subnormal (2^-14.3, 2^-15, 2^-17.2) as they are
+    raised by 2^7.  Together they count for 2^-4.7, 2^-5.4 and 2^-7.6, twice that in the result: more than the tolerance, where a product or the sum of the
+    weights lost them."""
+    L, D = 100000, 64
+    q, kc, vc, table, seq, cu, _ = case = R.make(dev, 1, [L], [n], 1, 1, D, 64, torch.float16)
+    q.zero_()
+    q[..., 0] = 8.0
+    at = _keys(case, 0, L)
+    k, val = torch.zeros(L, 1, D, dtype=torch.float16, device=dev), torch.ones(L, 1, D, dtype=torch.float16, device=dev)
+    k[5, 0, 0], val[5] = score, -1.0
+    kc[at], vc[at] = k, val
+    _check(_run(v, case, [L], [n], D ** -0.5), *R.attention(*case[:4], [L], [n], D ** -0.5))
