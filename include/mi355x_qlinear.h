@@ -722,10 +722,13 @@ int mi_qk_norm_rope(const void* qkv, long long qkv_stride, const void* q_weight,
  * table_width x page_size below 2^30; B num_kv_heads below 2^22 where sequences of more than 32 rows can be (n num_heads / num_kv_heads);
  * scale > 0.  cu_seqlens_q ascends (where it does not, out is not defined, and nothing outside is read or written).  max_query_len and max_seq_len, the largest n and seq_lens, choose kernels and splits only:
  * results are right for any values, up to the order of sums.  The workspace (mi_paged_attention_workspace bytes for the same arguments; 16-byte
- * aligned) must stay untouched until the stream has passed the call; 0 bytes: none.
+ * aligned) must stay untouched until the stream has passed the call; 0 bytes: none.  It is enough for a call with any window;
+ * mi_paged_attention_window_workspace says what one with these window and sinks uses, which is often less.
  * In place of eagle_ops::page_attn_decode and of the sdp kernels of prompts (V/csrc/eagle, V/csrc/xpu). */
 int mi_paged_attention_workspace(int T, int B, int num_heads, int num_kv_heads, int head_dim, int max_query_len, int max_seq_len,
                                  long long* bytes);
+int mi_paged_attention_window_workspace(int T, int B, int num_heads, int num_kv_heads, int head_dim, int window, int sinks, int max_query_len,
+                                        int max_seq_len, long long* bytes);
 int mi_paged_attention_ws(const void* query, long long token_stride, long long head_stride, const MiPagedCache* cache,
                           const int32_t* block_table, int table_width, const int32_t* seq_lens, const int32_t* cu_seqlens_q, void* out,
                           void* workspace, long long workspace_bytes, int T, int B, int num_heads, int num_kv_heads, int head_dim,

@@ -28,13 +28,17 @@ static int cus() {
 
 static long long round256(long long v) { return (v + 255) / 256 * 256; }
 
-static int attn_plan(int T, int B, int Hq, int Hkv, int D, int max_query_len, int max_seq_len, AttnPlan& a) {
+// window 0: none
+static int attn_plan(int T, int B, int Hq, int Hkv, int D, int max_query_len, int max_seq_len, long long window, long long sinks, AttnPlan& a) {
   if (D != 64 && D != 128 && D != 256) return MI_ERR_SHAPE;
   if (T < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || max_query_len < 0 || max_seq_len < 0) return MI_ERR_SHAPE;
   if ((long long)T * Hq >= 1 << 28 || B >= 1 << 24 || Hq > 1 << 16) return MI_ERR_SHAPE;
   const int G = Hq / Hkv, most = max_query_len < T ? max_query_len : T;
   a = AttnPlan{};
   if (!T || !B) return MI_OK;
+  // keys that `tokens` tokens side by side see
+  const long long keys = max_seq_len < 1 ? 1 : max_seq_len;
+  auto reach = [&](long long tokens) { return window && window + sinks + tokens < keys ? window + sinks + tokens : keys; };
   a.rows = a.tiles = true;
   a.rows_from = 33;
   if ((long long)most * G <= 32) {
@@ -48,7 +52,7 @@ static int attn_plan(int T, int B, int Hq, int Hkv, int D, int max_query_len, in
     const long long full = (long long)cus() * (D == 64 ? 8 : D == 128 ? 4 : 2);  // workgroups that the device holds
     // shares of two blocks at least: more of one block each make the joining longer (17.8 -> 15.4 us for 8 tiles of 908 keys)
     const long long tiles = ((long long)T * G / kFewRows < B ? B : (long long)T * G / kFewRows) * Hkv;
-    const long long some = tiles * ((max_seq_len < 1 ? 1 : max_seq_len) / 32LL + 4) / 2 + 1;
+    const long long some = tiles * (reach(kFewRows) / 32 + 4) / 2 + 1;
     a.groups = (int)(some < full ? some : full);
     a.rows_bytes = round256(attn_parts_bytes(a.groups, D, kFewRows));
   }
@@ -60,12 +64,14 @@ static int attn_plan(int T, int B, int Hq, int Hkv, int D, int max_query_len, in
     // What the longer of both ways takes, in blocks of keys per workgroup: a workgroup per tile takes as long as the longest tile, and half as long again
     // on top of the even share where workgroups follow each other; equal shares have every tile see what its sequence's last token sees, and
     // parts to write and read.  One and four sequences of 1000 keys, 48 rows, heads of 128: 25.1 and 25.4 us by tiles, 16.4 and 17.7 in shares; four of
-    // 500 with 256 rows 25.5 and 26.9, 16 of 700 with 48 20.8 and 26.2; heads of 64, four of 1000: 20.5 and 21.1.
+    // 500 with 256 rows 25.5 and 26.9, 16 of 700 with 48 20.8 and 26.2; heads of 64, four of 1000: 20.5 and 21.1.  In a window a tile
+    // sees little of that: 2048 tokens at the end of 65536 in one of 1024, 64 heads of 128: 111 and 289 us; a prompt of 6000 in one of 512, 8 heads: 31
+    // and 245.
     long long tiles = (long long)T * G / R;
     if (tiles < B) tiles = B;
     tiles *= Hkv;
-    const long long keys = max_seq_len < 1 ? 1 : max_seq_len, seen = keys - (most < keys ? most : keys) / 2;
-    const long long even = tiles * seen / hold, alone = tiles <= hold ? keys : even + keys / 2, shared = tiles * keys / hold + (D == 64 ? 1024 : 560);
+    const long long tile = reach(R / G + 1), half = keys - (most < keys ? most : keys) / 2, seen = half < tile ? half : tile;    // of a tile: the most, the mean
+    const long long even = tiles * seen / hold, alone = tiles <= hold ? tile : even + tile / 2, shared = tiles * reach(most) / hold + (D == 64 ? 1024 : 560);
     if (alone > shared) {
       a.shares = hold;
       a.tiles_bytes = round256(attn_parts_bytes(a.shares, D, R));
@@ -73,6 +79,21 @@ static int attn_plan(int T, int B, int Hq, int Hkv, int D, int max_query_len, in
   }
   return MI_OK;
 }
+
+// A window takes no more workspace than the call would without one.
+static int attn_plan_within(int T, int B, int Hq, int Hkv, int D, int max_query_len, int max_seq_len, int window, int sinks, AttnPlan& a) {
+  AttnPlan whole;
+  const int rc = attn_plan(T, B, Hq, Hkv, D, max_query_len, max_seq_len, 0, 0, whole);
+  if (rc != MI_OK || !window) {
+    a = whole;
+    return rc;
+  }
+  const int r = attn_plan(T, B, Hq, Hkv, D, max_query_len, max_seq_len, window, sinks, a);
+  if (!whole.shares) a.shares = 0, a.tiles_bytes = 0;
+  return r;
+}
+// window of a call: 1 and more, or -1: none.  0: none, as no place is 2^30 from another
+static int window_of(int window) { return window < 0 || window >= 1 << 30 ? 0 : window; }
 
 // key / d for keys below 2^30: (umulhi(key, mul) + key) >> shift
 static void divide_by(uint32_t d, uint32_t& mul, uint32_t& shift) {
@@ -86,7 +107,7 @@ static int run(const AttnArgs& base, const MiPagedCache* cache, int D, float sca
   AttnArgs p = base;
   if (act_dtype != DT_F16 && act_dtype != DT_BF16) return MI_ERR_ARG;
   AttnPlan a;
-  const int rc = attn_plan(p.T, p.B, p.Hq, p.Hkv, D, max_query_len, max_seq_len, a);
+  const int rc = attn_plan_within(p.T, p.B, p.Hq, p.Hkv, D, max_query_len, max_seq_len, p.window, p.sinks, a);
   if (rc != MI_OK) return rc;
   if (!a.rows && !a.tiles) return MI_OK;
   if (!cache || !p.q || !p.out || !p.seq_lens || !p.cu || !cache->key || !cache->value || !(scale > 0.f) || scale > 3e38f) return MI_ERR_ARG;
@@ -140,7 +161,17 @@ int mi_paged_attention_workspace(int T, int B, int num_heads, int num_kv_heads, 
                                  long long* bytes) {
   if (!bytes) return MI_ERR_ARG;
   AttnPlan a;
-  const int rc = attn_plan(T, B, num_heads, num_kv_heads, head_dim, max_query_len, max_seq_len, a);
+  const int rc = attn_plan(T, B, num_heads, num_kv_heads, head_dim, max_query_len, max_seq_len, 0, 0, a);
+  if (rc == MI_OK) *bytes = a.rows_bytes + a.tiles_bytes;
+  return rc;
+}
+
+int mi_paged_attention_window_workspace(int T, int B, int num_heads, int num_kv_heads, int head_dim, int window, int sinks, int max_query_len,
+                                        int max_seq_len, long long* bytes) {
+  if (!bytes) return MI_ERR_ARG;
+  if ((window < 1 && window != -1) || sinks < 0) return MI_ERR_SHAPE;
+  AttnPlan a;
+  const int rc = attn_plan_within(T, B, num_heads, num_kv_heads, head_dim, max_query_len, max_seq_len, window_of(window), sinks, a);
   if (rc == MI_OK) *bytes = a.rows_bytes + a.tiles_bytes;
   return rc;
 }
@@ -163,7 +194,7 @@ int mi_paged_attention_ws(const void* query, long long token_stride, long long h
   p.B = B;
   p.Hq = num_heads;
   p.Hkv = num_kv_heads;
-  p.window = window < 0 || window >= 1 << 30 ? 0 : window;       // no place is that far from another
+  p.window = window_of(window);
   p.sinks = sinks;
   return run(p, cache, head_dim, scale, max_query_len, max_seq_len, workspace, workspace_bytes, act_dtype, (hipStream_t)stream);
 }

@@ -798,8 +798,8 @@ AttnCall attn_call(const char* who, const Tensor& q, const Tensor& kc, const Ten
   a.keys = (int)std::min<int64_t>(max_seq_len, INT_MAX);
   return a;
 }
-Tensor attn_workspace(const Tensor& q, const AttnCall& a, long long& bytes) {
-  CALL(mi_paged_attention_workspace, a.T, a.B, a.Hq, a.Hkv, a.D, a.longest, a.keys, &bytes);
+Tensor attn_workspace(const Tensor& q, const AttnCall& a, int window, int sinks, long long& bytes) {
+  CALL(mi_paged_attention_window_workspace, a.T, a.B, a.Hq, a.Hkv, a.D, window, sinks, a.longest, a.keys, &bytes);
   return bytes ? buffer(q, bytes) : Tensor();
 }
 
@@ -812,10 +812,11 @@ Tensor paged_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, cons
   if (!a.T || !a.B) return out;
   const On on(q);
   long long bytes = 0;
-  const Tensor ws = attn_workspace(q, a, bytes);
+  const int w = (int)std::min<int64_t>(window, INT_MAX), first = (int)std::min<int64_t>(sinks, INT_MAX);
+  const Tensor ws = attn_workspace(q, a, w, first, bytes);
   CALL(mi_paged_attention_ws, q.data_ptr(), stride_of(q, 0), stride_of(q, 1), &a.cache, table.data_ptr<int>(), a.width, seq.data_ptr<int>(),
-       cu.data_ptr<int>(), out.data_ptr(), int8_buffer(ws), bytes, a.T, a.B, a.Hq, a.Hkv, a.D, (float)scale,
-       (int)std::min<int64_t>(window, INT_MAX), (int)std::min<int64_t>(sinks, INT_MAX), a.longest, a.keys, act(q), on.stream);
+       cu.data_ptr<int>(), out.data_ptr(), int8_buffer(ws), bytes, a.T, a.B, a.Hq, a.Hkv, a.D, (float)scale, w, first,
+       a.longest, a.keys, act(q), on.stream);
   return out;
 }
 
@@ -831,7 +832,7 @@ Tensor tree_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const
   if (!a.T || !a.B) return out;
   const On on(q);
   long long bytes = 0;
-  const Tensor ws = attn_workspace(q, a, bytes);
+  const Tensor ws = attn_workspace(q, a, -1, 0, bytes);
   CALL(mi_tree_attention_ws, q.data_ptr(), stride_of(q, 0), stride_of(q, 1), &a.cache, table.data_ptr<int>(), a.width, seq.data_ptr<int>(),
        cu.data_ptr<int>(), mask.data_ptr<int64_t>(), (int)mask.size(1), out.data_ptr(), int8_buffer(ws), bytes, a.T, a.B, a.Hq, a.Hkv, a.D,
        (float)scale, a.longest, a.keys, act(q), on.stream);
