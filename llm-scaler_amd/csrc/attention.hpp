@@ -630,12 +630,11 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(const AttnArgs p, in
         [&](int i, int row) { return part(i) + ROWS * D + 2 * (row0 + row); },
         [&](int row) { return (typename Act::elem*)p.out + attn_row(p, cut[1], cut[3] >> 9, cut[2] * ROWS + row0 + row) * D; });
 }
-template <class Act, int D, int ROWS>
-static inline int launch_join(const AttnArgs& p, int groups, int rows, bool many_parts, hipStream_t st) {
+template <class Act, int D, int ROWS, int THREADS>
+static inline int launch_join(const AttnArgs& p, int groups, int rows, hipStream_t st) {
   if (groups == 1) return MI_OK;
   const dim3 grid(groups - 1, (rows + kJoinRows - 1) / kJoinRows);
-  if (many_parts) attn_join_kernel<Act, D, ROWS, 1024><<<grid, 1024, 0, st>>>(p, groups);
-  else attn_join_kernel<Act, D, ROWS, 256><<<grid, 256, 0, st>>>(p, groups);
+  attn_join_kernel<Act, D, ROWS, THREADS><<<grid, THREADS, 0, st>>>(p, groups);
   return launch_status();
 }
 

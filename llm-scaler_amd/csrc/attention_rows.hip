@@ -159,7 +159,8 @@ static int launch_rows(const AttnArgs& p, hipStream_t st) {
 template <class Act, int D>
 static int launch(const AttnArgs& p, hipStream_t st) {
   const int rc = p.wide ? launch_rows<Act, D, long long>(p, st) : launch_rows<Act, D, int>(p, st);
-  return rc != MI_OK ? rc : launch_join<Act, D, kFewRows>(p, p.groups, p.tile_rows, p.many_parts, st);
+  if (rc != MI_OK) return rc;
+  return p.many_parts ? launch_join<Act, D, kFewRows, 1024>(p, p.groups, p.tile_rows, st) : launch_join<Act, D, kFewRows, 256>(p, p.groups, p.tile_rows, st);
 }
 
 int launch_attn_rows(const AttnArgs& p, int D, int act_dtype, hipStream_t st) {

@@ -447,7 +447,7 @@ template <class Act, int D>
 static int launch(const AttnArgs& p, hipStream_t st) {
   const bool groups = p.page % 8 == 0 && p.row16 < 1u << 24;     // a group's rows: 32-bit distances in bytes
   const int rc = groups ? launch_tiles<Act, D, true>(p, st) : launch_tiles<Act, D, false>(p, st);
-  return rc != MI_OK || !p.shares ? rc : launch_join<Act, D, TilesCfg<D>::ROWS>(p, p.shares, TilesCfg<D>::ROWS, false, st);
+  return rc != MI_OK || !p.shares ? rc : launch_join<Act, D, TilesCfg<D>::ROWS, 256>(p, p.shares, TilesCfg<D>::ROWS, st);
 }
 
 int launch_attn_tiles(const AttnArgs& p, int D, int act_dtype, hipStream_t st) {
