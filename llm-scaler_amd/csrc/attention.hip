@@ -6,8 +6,12 @@
 namespace qlin {
 
 // Which kernels a call runs.  Up to 32 rows (tokens x heads of a group) per sequence go to the rows kernel, more to the tiles kernel; where
-// sequences of both kinds can be in a call both are launched, and each takes its own.  32 and 48 rows by the rows kernel and by tiles, 8 kv heads of 128:
-// one sequence of 1000 keys 14.2 and 23.7, 15.9 and 24.8 us; 16 of 4000 59 and 53, 66 and 55; 4 of 30000 118 and 109, 207 and 111.
+// sequences of both kinds can be in a call both are launched, and each takes its own.  Measured at 16, 32 and 48 rows, 8 kv heads, us by the rows kernel
+// and by tiles:
+//   heads of 64    1 sequence of 1000 keys 12.1 / 19.3, 12.3 / 19.4, 13.8 / 20.5; 4 of 1000 14.3 / 19.6, 17.2 / 19.8, 18.9 / 21.0; 4 of 30000 59 / 61, 65 / 61, 104 / 60
+//   heads of 128   1 of 1000 14.3 / 15.4, 14.8 / 16.7, 15.8 / 17.0; 4 of 1000 17.4 / 17.2, 21.5 / 17.3, 22.0 / 18.5; 4 of 30000 114 / 110, 121 / 113, 211 / 114
+//   heads of 256   1 of 1000 20.7 / 21.7, 21.8 / 23.1, 24.5 / 24.6; 4 of 1000 27.6 / 24.2, 29.3 / 24.9, 31.5 / 26.5; 4 of 30000 201 / 191, 201 / 192, 359 / 192
+// One bound for all: at 32 rows it is the better side by up to a third for short calls and heads of 64, and the worse by up to a fifth between.
 struct AttnPlan {
   bool rows, tiles;
   int rows_from, groups, slots, shares;
