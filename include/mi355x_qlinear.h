@@ -703,7 +703,7 @@ typedef struct {
  * activations' type): (a, b) -> (a cos - b sin, b cos + a sin) for the pairs (i, i + rot / 2), or (2 i, 2 i + 1) if interleaved; fp32, one
  * rounding.  Queries go to q_out, keys to k_out (NULL: nowhere), keys and the untouched values to slot slots[t] of the cache (NULL: nowhere).
  * A slot outside the cache is not written; a position outside the table gives NaN.  q_out may be qkv's own query columns and k_out its key
- * columns; otherwise nothing overlaps.  Slots of a call differ.  head_dim 64, 128 or 256; rot a multiple of 16.  One launch.
+ * columns, or both columns of another array; otherwise nothing overlaps.  Slots of a call differ.  head_dim 64, 128 or 256; rot a multiple of 16.  One launch.
  * In place of esimd_qkv_split_norm_rope (V/csrc/xpu/torch_extension.cc), with a paged cache behind it. */
 int mi_qk_norm_rope(const void* qkv, long long qkv_stride, const void* q_weight, const void* k_weight, const void* cos_sin, int table_f32,
                     const int64_t* positions, void* q_out, long long q_token_stride, long long q_head_stride, void* k_out,

@@ -614,6 +614,21 @@ Span span(const Tensor& t) {                           // from the first byte to
 void attn_apart(const char* who, const Span& a, const char* out_name, const Span& b, const char* name) {
   REFUSE_UNLESS(!a.from || !b.from || a.from >= b.to || b.from >= a.to, out_name, " must not overlap ", name);
 }
+// As above; tensors of T rows may also be columns of one array: the same stride, and no row reaches one of the other's, here or in the next row.
+void attn_apart_rows(const char* who, const Tensor& out, const Span& a, const char* out_name, const Tensor& t, const Span& b, const char* name) {
+  if (!a.from || !b.from || a.from >= b.to || b.from >= a.to) return;
+  auto extent = [](const Tensor& x) {                  // bytes of a row
+    int64_t last = 0;
+    for (int64_t d = 1; d < x.dim(); ++d) last += (x.size(d) - 1) * x.stride(d);
+    return (last + 1) * x.element_size();
+  };
+  bool columns = out.size(0) > 1 && out.stride(0) == t.stride(0) && out.stride(0) > 0;
+  if (columns) {
+    const int64_t step = out.stride(0) * out.element_size(), behind = ((b.from - a.from) % step + step) % step;
+    columns = behind >= extent(out) && behind + extent(t) <= step;
+  }
+  REFUSE_UNLESS(columns, out_name, " must not overlap ", name);
+}
 void attn_device(const char* who, const Tensor& x, const Tensor& t, const char* name) {
   REFUSE_UNLESS(t.is_cuda() && t.device() == x.device(), name, " must be on the same ROCm device as the input, got ", t.device());
 }
@@ -737,10 +752,11 @@ Tensor qk_norm_rope(const Tensor& qkv, const c10::optional<Tensor>& qw, const c1
     if (!outs[i]) continue;
     attn_apart_inside(who, *outs[i], names[i]);
     to[i] = span(*outs[i]);
-    if (!(i == 0 && q_own) && !(i == 1 && k_own)) attn_apart(who, to[i], names[i], rows, "qkv");
+    if (i == 0 ? !q_own : i == 1 && !k_own) attn_apart_rows(who, *outs[i], to[i], names[i], qkv, rows, "qkv");
+    if (i >= 2) attn_apart(who, to[i], names[i], rows, "qkv");
     for (const auto& t : in) attn_apart(who, to[i], names[i], t.first, t.second);
-    for (int j = 0; j < i; ++j)                        // keys and values against each other: in paged_cache
-      if (!(i == 1 && j == 0 && q_own && k_own) && !(i == 3 && j == 2)) attn_apart(who, to[i], names[i], to[j], names[j]);
+    if (i == 1) attn_apart_rows(who, *outs[1], to[1], names[1], q, to[0], names[0]);
+    for (int j = 0; i >= 2 && j < 2; ++j) attn_apart(who, to[i], names[i], to[j], names[j]);       // keys and values against each other: in paged_cache
   }
   if (!T) return q;
   const On on(qkv);
