@@ -75,12 +75,22 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const RopeArgs p) {
   load8(x + second, b);
   const Elem* w = (const Elem*)(is_q ? p.qw : p.kw);
   if (w) {
-    float sum = 0.f;
+    auto squares = [&]() {
+      float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += a[i] * a[i] + b[i] * b[i];
+      for (int i = 0; i < 8; ++i) sum += a[i] * a[i] + b[i] * b[i];
 #pragma unroll
-    for (int d = 1; d < L; d <<= 1) sum += __shfl_xor(sum, d, 64);
-    const float f = 1.f / sqrtf(sum * (1.f / D) + p.eps);
+      for (int d = 1; d < L; d <<= 1) sum += __shfl_xor(sum, d, 64);
+      return sum;
+    };
+    float sum = squares(), eps = p.eps;
+    if (sum == __builtin_inff()) {                     // bf16 from 1e18 on: the same for all lanes of a head
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] *= 0x1p-68f, b[i] *= 0x1p-68f;    // x 2^-68: the norm takes it out again; eps, 2^-136 of itself, no longer counts
+      sum = squares();
+      eps = 0.f;
+    }
+    const float f = 1.f / sqrtf(sum * (1.f / D) + eps);
     float wa[8], wb[8];
     load8(w + first, wa);
     load8(w + second, wb);

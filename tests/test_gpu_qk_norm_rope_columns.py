@@ -61,3 +61,22 @@ def test_columns_that_meet_are_refused(v, dev):
                     (dict(q=wide[:10].as_strided((T, HQ, D), (8 * D, D, 1)), k=_columns(wide, HQ, HKV)), "overlap q_out")):
         with pytest.raises(RuntimeError, match=why):
             call(**kw)
+
+
+@pytest.mark.parametrize("head", [64, 128, 256])
+def test_norm_of_elements_whose_squares_pass_fp32(v, dev, head):
+    """bf16 rows from 1e15 to the type's largest number, beside rows of one: normed like any other; an infinity stays NaN."""
+    g = torch.Generator().manual_seed(head)
+    x = torch.randn(6, 4 * head, generator=g).double()
+    x *= torch.tensor([1.0, 1e15, 1e19, 1e30, 8e37, 1.0])[:, None].double()
+    x = x.clamp(-3.3e38, 3.3e38).bfloat16().to(dev)
+    x[5, head + 3] = float("inf")
+    q, k = (torch.empty(6, h, head, dtype=x.dtype, device=dev) for h in (2, 1))
+    w = [(1 + 0.3 * torch.randn(head, generator=g)).bfloat16().to(dev) for _ in range(2)]
+    v.qk_norm_rope(x, w[0], w[1], torch.empty(4, 0, device=dev), torch.zeros(6, dtype=torch.int64, device=dev), q, k, None, None, None, 1e-6)
+    heads = x.double().view(6, 4, head)
+    assert q[5, 1].isnan()[3] and not q[5, 0].isnan().any()
+    for got, part, weight in ((q[:5], heads[:5, :2], w[0]), (k, heads[:, 2:3], w[1])):
+        ref = part / torch.sqrt(part.pow(2).mean(-1, keepdim=True) + 1e-6) * weight.double()
+        # one rounding to bf16, and 28 steps of fp32 as for rows of ordinary size
+        assert ((got.double() - ref).abs() <= (2.0 ** -8 * (1 + 2.0 ** -10) + 28 * 2.0 ** -24) * ref.abs() + 1e-40).all()
