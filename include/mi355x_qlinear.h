@@ -717,7 +717,9 @@ int mi_qk_norm_rope(const void* qkv, long long qkv_stride, const void* q_weight,
  *   out = sum_j softmax_j(scale q . k_j) v_j.
  * A token that sees nothing gets zeros.  Keys behind the table's end or on a page outside the cache are not seen.  Scores, softmax and sums in
  * fp32; the weights are rounded to the activations' type in front of their product with the values; one rounding at the end.  What lies in
- * places that a token does not see does not reach it, infinities and NaN included.
+ * places that a token does not see does not reach it, infinities and NaN included; an infinity among values that it sees leaves that column infinite
+ * or NaN.  Scores that fit fp32 and finite values may be of any size (as long as the values' sum under weights of up to 1 fits
+ * fp32).
  * query [T, num_heads, head_dim] with strides (multiples of 8), out contiguous; head_dim 64, 128 or 256; T num_heads below 2^28;
  * table_width x page_size below 2^30; B num_kv_heads below 2^22 where sequences of more than 32 rows can be (n num_heads / num_kv_heads);
  * scale > 0.  cu_seqlens_q ascends (where it does not, out is not defined, and nothing outside is read or written).  max_query_len and max_seq_len, the largest n and seq_lens, choose kernels and splits only:

@@ -4,9 +4,11 @@
 // A wavefront needs no barrier, and eight (four, two with heads of 64, 128, 256) fill a CU's LDS with loads under way.  Equal shares: whatever the
 // lengths, all wavefronts end together (a workgroup per tile and a fixed number of parts took 1.2 to 1.5 times as long for trees over long contexts).
 //
-// Bound: HBM.  Two sequences of 131072 keys, 8 kv heads of 128: 1.07 GB in 205 us (5.2 TB/s) and 10 to join the parts; 64 sequences of up to 8192:
-// 260 MB in 45 us (5.8 TB/s) and 7.  Short calls: two launches, of which the second waits for the first
-// (8 and 3 us for a sequence of 700).
+// Bound: HBM.  Two sequences of 131072 keys, 8 kv heads of 128: 1.07 GB in 204 us (5.3 TB/s) and 10 to join the parts; 64 sequences of up to 8192:
+// 260 MB in 56 us (4.6 TB/s) and 7.  Heads of 256, two wavefronts per CU: 1.07 GB in 185 us and 9, 130 MB of 64 sequences in 34 (3.8 TB/s) and 15.
+// Short calls: two launches, of which the second waits for the first (8 and 4 us for a sequence of 700).
+// 28, 43 and 91 scalar registers (heads of 64, 128, 256) lie in lanes of vector registers: of the shares, read again between tiles, and of the edges, read in the
+// loop (0, 7 and up to 20 reads per two steps).
 #include "attention.hpp"
 
 namespace qlin {

@@ -9,10 +9,11 @@
 // Long prompts have a workgroup per tile: tiles of the last tokens, which see the most keys, go first, and the kv heads go round the XCDs, so that
 // the tiles of a head share its keys in L2.  Few tokens over long contexts are done in equal shares instead.
 //
-// Bound: what a wavefront can issue beside the matrix instructions.  8192 tokens, 32 heads of 128 over 8: 553 us, 0.99 PFLOP/s, matrix pipe 49 % busy
-// at 2.1 GHz (power); chunks, 16 heads of 256 over 2: 690 us, 0.86 PFLOP/s, 42 %; a window of 1024, 64 heads of 64 over 8: 405 us, 0.66 PFLOP/s, 36 %,
-// vector instructions 74 % (the exponentials alone take as long as both products).  Keys and values a block further ahead change nothing (699 against 694 us,
-// 560 against 556), nor does an order of instructions laid down by hand (696), nor four wavefronts with 64 rows each (copies between register files).
+// Bound: what a wavefront can issue beside the matrix instructions.  8192 tokens, 32 heads of 128 over 8: 560 us, 0.98 PFLOP/s, matrix pipe 47 % busy
+// at 2.1 GHz (power); chunks, 16 heads of 256 over 2: 684 us, 0.87 PFLOP/s, 43 %; a window of 1024, 64 heads of 64 over 8: 413 us, 0.65 PFLOP/s, 35 %,
+// vector instructions 73 % (the exponentials alone take as long as both products; 12 registers are put aside around the loop).  Each compared on one card, keys and
+// values a block further ahead change nothing (699 against 694 us for the chunks, 560 against 556 for the prompt), nor does an order of instructions
+// laid down by hand (696 against 694), nor four wavefronts with 64 rows each (copies between register files).
 #include "attention.hpp"
 
 #include <type_traits>
@@ -392,7 +393,8 @@ void attn_tiles_kernel(const AttnArgs p) {
   tile_piece<Act, D, GROUPS>(p, x, blockIdx.x % p.Hkv, 0, x.r.blocks, nullptr);
 }
 
-// In equal shares.  All tiles of a sequence have the blocks that any of its tokens sees.
+// In equal shares.  All tiles of a sequence have the blocks that any of its tokens sees.  66 to 71 scalar registers lie in lanes of vector registers: the
+// shares' counts, read again between tiles, none in the loop over inner blocks.
 template <class Act, int D, bool GROUPS>
 __global__ __launch_bounds__(64 * TilesCfg<D>::NW) __attribute__((amdgpu_waves_per_eu(TilesCfg<D>::WAVES, TilesCfg<D>::WAVES)))
 void attn_tiles_shared_kernel(const AttnArgs p) {
