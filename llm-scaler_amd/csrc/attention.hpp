@@ -182,7 +182,7 @@ struct RowPlaces {
 };
 
 // ---- the rows of a wavefront ------------------------------------------------------------------
-// Exponents of the weights: fma(c, s, raise - c m), one instruction, while c |m| < 2^10; raise - c m is then rounded by 2^-15 at most, the same for all
+// Exponents of the weights: fma(c, s, raise - c m), one instruction, while c |m| < 2^10; raise - c m is then rounded by 2^-14 at most, the same for all
 // weights that go by this m.  Of a larger one the last place is worth whole units in the end: there the scores give way to s - m, exact where it matters,
 // and the exponent is fma(c, s - m, raise).  Those rows keep their m apart, so that others pay nothing for them (with a comparison more in every step
 // 695 against 680 us for chunks of heads of 256, 410 against 405 for a prompt in a window with heads of 64).
